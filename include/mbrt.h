@@ -404,6 +404,74 @@ MBRT_API int mbrt_attention_ex(const void* q, const void* k, const void* v, int 
                                int gate_is_logit, void* out, int out_dtype, float scale, int p_precision,
                                mbrt_stream_t stream);
 
+/* ---- transformer layer: products, head norms, windowed attention --------------------- */
+
+/* Linear layer: out[r, n] = act(sum_k x[r, k] weight[n, k] + bias[n]) + residual[r, n] for x
+ * [rows, in_features] and weight [out_features, in_features] of one dtype (F32/F16/BF16), bias
+ * [out_features] and residual [rows, out_features] of any of the three, each NULL for none, and out
+ * [rows, out_features] of any.  Row strides in elements; x, weight and residual may have any from
+ * 0 on, out at least out_features; rows at any alignment (16-byte ones are read faster).  Sums and
+ * the epilogue are f32, with one rounding on the store; the activations are mbrt_bias_act's, and an
+ * F32 operand's products are F32 products.  out may be residual (same dtype, same rows): the residual
+ * stream updated in place.  in_features 0 leaves act(bias) + residual.  No workspace, no atomics.
+ * The projections that the reference's model calls (linear*, src/mbr_cuda_tile.cu:712-3790,
+ * 7586-7949), with the epilogues they end in and the residual add behind them. */
+MBRT_API int mbrt_linear(const void* x, int dtype, int64_t x_row_stride, const void* weight,
+                         int64_t weight_row_stride, const void* bias, int bias_dtype, const void* residual,
+                         int residual_dtype, int64_t residual_row_stride, void* out, int out_dtype,
+                         int64_t out_row_stride, int64_t rows, int64_t in_features, int64_t out_features, int act,
+                         mbrt_stream_t stream);
+
+/* Split of a fused qkv projection with an RMS norm of every query and key head and the rotary
+ * rotation in one pass.  qkv holds, per token, H query heads, H_kv key heads and H_kv value heads of D
+ * elements side by side (token n of batch b at qkv + b*qkv_batch_stride + n*qkv_token_stride).  A query
+ * head x becomes x * scale * q_gamma / sqrt(sum x^2 + eps) (mbrt_rms_norm over D), its pairs (2i, 2i+1) are
+ * then rotated as by mbrt_rotary_inplace with row pos0 + n of the tables [n_pos, D/2]; key heads
+ * likewise with k_gamma; value heads are copied.  f32 throughout, one rounding on the store.
+ * Head h of token (b, n) goes to q + b*q_batch_stride + h*q_head_stride + n*q_token_stride, keys and
+ * values likewise by the kv strides: any order, padded rows or a cache's rows, which are
+ * written only where a token goes.  v NULL leaves the values where they are.  Outputs must not overlap
+ * qkv, except that q and k may be their own places in it (same dtype): the projection normed and
+ * rotated in place.  qkv and outputs F32/F16/BF16, gammas and tables F32/BF16; even D up to 65536;
+ * requires pos0 + N <= n_pos.
+ * Beside mbrt_split_qkv_heads_rotary, for models that norm their heads. */
+MBRT_API int mbrt_split_qkv_norm_rotary(const void* qkv, int qkv_dtype, int64_t qkv_batch_stride,
+                                        int64_t qkv_token_stride, const void* q_gamma, const void* k_gamma,
+                                        int gamma_dtype, const void* cos_table, const void* sin_table,
+                                        int trig_dtype, int64_t n_pos, int64_t pos0, void* q, void* k, void* v,
+                                        int out_dtype, int64_t q_batch_stride, int64_t q_head_stride,
+                                        int64_t q_token_stride, int64_t kv_batch_stride, int64_t kv_head_stride,
+                                        int64_t kv_token_stride, int64_t B, int64_t N, int64_t H, int64_t H_kv,
+                                        int64_t D, float scale, float eps, mbrt_stream_t stream);
+
+/* Attention through a sliding window with sinks: the query at position p of batch entry b sees key j iff
+ *   j < len_b,   j <= p + right,   and   j >= p - left  or  j < sinks,
+ * and out = softmax over the keys it sees of scale * q.k, times v (zeros where it sees none; hidden keys and
+ * values may hold anything).  left or right -1: no limit; right 0 is causal.  Query i stands at
+ * position q_start + i, or, with q_start -1, len_b - n_q + i (the queries are the last of the keys: streaming,
+ * one token against a cache).  len_b = key_lens[b] (device, clamped to 0 .. n_k), or n_k where key_lens is
+ * NULL; keys from len_b on are never read.  H query heads share H_kv key heads, H / H_kv neighbours each.
+ * q, k, v BF16 or F16 with head_dim 32, 64 or 128; strides (batch, head, row) in elements, multiples of
+ * 8, k and v strided alike; q, k, v, out 16-byte aligned.  out F32/F16/BF16 by its own strides (multiples of 8), rows
+ * written only for the n_q queries.  scale > 0, or 0 for 1/sqrt(head_dim).  gate [B, n_q, H] (F32/F16/BF16, NULL for
+ * none) multiplies each head's output by sigmoid(gate), or by gate itself when !gate_is_logit, before
+ * the one rounding on the store.  f32 softmax and sums, probabilities as sums of two 2-byte values
+ * (three where BF16 heads go to an F32 out), beside which the inputs' own rounding is what is left.  A few queries against many keys are shared out over the keys and joined through
+ * `workspace` (mbrt_attention_window_workspace_bytes of the same sizes; 0 bytes: may be NULL), in a fixed order:
+ * results do not change from call to call.  Calls that overlap need workspaces of their own.
+ * Beside mbrt_attention_ex, for songs longer than a chunk and for streaming. */
+MBRT_API int64_t mbrt_attention_window_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int64_t n_q, int64_t n_k,
+                                                       int64_t head_dim, int64_t left, int64_t right,
+                                                       int64_t sinks);
+MBRT_API int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t H,
+                                   int64_t H_kv, int64_t n_q, int64_t n_k, int64_t head_dim, int64_t q_batch_stride,
+                                   int64_t q_head_stride, int64_t q_row_stride, int64_t kv_batch_stride,
+                                   int64_t kv_head_stride, int64_t kv_row_stride, int64_t left, int64_t right,
+                                   int64_t sinks, int64_t q_start, const int32_t* key_lens, const void* gate,
+                                   int gate_dtype, int gate_is_logit, void* out, int out_dtype,
+                                   int64_t out_batch_stride, int64_t out_head_stride, int64_t out_row_stride,
+                                   float scale, void* workspace, int64_t workspace_bytes, mbrt_stream_t stream);
+
 /* ---- STFT / iSTFT (n_fft = win_length = 2048) --------------------------------- */
 
 /* Hann window of `size` f32 samples, 0.5 (1 - cos(2 pi n / size)) in f32; size 1 gives

@@ -62,6 +62,9 @@ KERNEL_SOURCES = [
     "k_rotary.hip",
     "k_band.hip",
     "k_attention.hip",
+    "k_linear.hip",
+    "k_qkv_norm.hip",
+    "k_window.hip",
     "k_stft.hip",
     "k_chunk.hip",
     "host_tables.cpp",
@@ -74,6 +77,9 @@ KERNEL_SOURCES = [
 # result (a NaN score still reaches the output through exp2 and the P V product).
 EXTRA_FLAGS = {
     "k_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-Xarch_device", "-fno-honor-nans"],
+    # accumulators in ordinary VGPRs here too; NaN keeps its meaning (rows with one are looked for)
+    "k_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "k_window.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 TENSOR_SOURCES = [

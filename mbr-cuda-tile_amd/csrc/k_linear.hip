@@ -1,0 +1,548 @@
+// Linear layer with its epilogue: out[r, n] = act(sum_k x[r, k] w[n, k] + bias[n]) + residual[r, n],
+// the projections of the band-split transformer (src/mbr_cuda_tile.cu:712-3790) with the epilogues they
+// end in there (bias, GELU, sigmoid, tanh) and the residual add.
+//
+// Both operands hold their contraction index last, so a 16-byte piece of a row of either is what one
+// lane feeds to a matrix instruction: lane l = (g = l / 16, c = l % 16) takes bytes 16 g .. of a 64-byte
+// piece of row c.  For 2-byte types that is one v_mfma_f32_16x16x32 (k = 8 g + j); for f32 four
+// v_mfma_f32_16x16x4_f32, the j-th over the j-th element of every lane's four (k = 4 g + j): any order of the
+// contraction serves if both operands have the same.  Sums are f32; the epilogue works in f32 and rounds once,
+// on its store.
+//
+// Three forms, by shape (choose() below): tiles of 128 x 128 or 64 x 64 through LDS, and strips of 16 rows of
+// the longer operand against all of a short one (few rows, or few output columns).
+#include "abi_common.hpp"
+
+#include <algorithm>
+
+namespace mbrt {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kStepBytes = 128;          // of every row, per step of the tile kernel
+constexpr int kBufferDword3 = 0x00020000;  // raw buffer resource: 32-bit data format, no swizzle, no stride
+
+struct LinArgs {
+    const char* x;
+    const char* w;
+    const void* bias;
+    const void* res;
+    void* out;
+    int64_t xs, ws, rs, os;  // row strides: bytes (x, w), elements (residual, out)
+    int64_t M;
+    int N, K;
+    int bdt, rdt, odt, act;
+    uint32_t ntiles;         // tiles along N
+    int split;               // strips: waves that share a strip's K
+};
+
+// 16 bytes per lane from base + off + step straight to lds + 16 lane.  Not a template: the builtin's operands must not
+// depend on one, or the host pass drops the kernel that holds it.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t base, char* lds, uint32_t off, int step) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_void*)lds, 16, off, step, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (DT == BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else if constexpr (DT == F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    } else {
+        const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[j], fb[j], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// The 16 bytes of a row of K elements that start at byte kb, zeros behind its end; at any alignment
+// (ALIGNED: of 16 bytes, where the piece is whole).
+template <int DT, bool ALIGNED>
+__device__ __forceinline__ u32x4 row_piece(const char* row, int64_t kb, int K) {
+    constexpr int S = DT == F32 ? 4 : 2, VE = 16 / S;
+    const int64_t left = (int64_t)K * S - kb;
+    if (left >= 16) {
+        if constexpr (ALIGNED) return *reinterpret_cast<const u32x4*>(row + kb);
+        else return ld_any<0, S>(row + kb);
+    }
+    u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < VE - 1; ++j) {
+        if (left > (int64_t)j * S) {
+            if constexpr (S == 4) v[j] = reinterpret_cast<const uint32_t*>(row + kb)[j];
+            else v[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row + kb)[j] << (16 * (j & 1));
+        }
+    }
+    return v;
+}
+
+// f32 results take the library's erfc and tanh, 2-byte ones the short forms that bias_act uses for them (errors of
+// 1.5e-7 and less beside their half steps of 2^-9 and 2^-12).
+template <int NV>
+__device__ __forceinline__ void activate(float (&v)[NV], int act, bool f32_out) {
+    if (act == MBRT_ACT_GELU_REF || act == MBRT_ACT_GELU_STD) {
+        const bool ref = act == MBRT_ACT_GELU_REF;
+        const float s = ref ? 1.0f : 0.70710678118654752440f;
+        if (f32_out) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = 0.5f * v[i] * erfcf(-v[i] * s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = 0.5f * v[i] * one_plus_erf_as(v[i] * s);
+        }
+    } else if (act == MBRT_ACT_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = sigmoidf(v[i]);
+    } else if (act == MBRT_ACT_TANH) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = tanhf(v[i]);
+    }
+}
+
+// NV consecutive elements at p[e], e on, as f32: 16 bytes at a time at any alignment.
+template <int NV>
+__device__ __forceinline__ void load_run(const void* p, int dt, int64_t e, float (&f)[NV]) {
+    static_assert(NV % 4 == 0 || NV == 1, "whole pieces, or one element");
+    if constexpr (NV == 1) {
+        f[0] = load1(p, dt, e);
+    } else if (dt == F32) {
+        const char* b = reinterpret_cast<const char*>(p) + 4 * e;
+#pragma unroll
+        for (int q = 0; q < NV / 4; ++q) {
+            const f32x4 t = __builtin_bit_cast(f32x4, ld_any<0, 4>(b + 16 * q));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[4 * q + i] = t[i];
+        }
+    } else {
+        const char* b = reinterpret_cast<const char*>(p) + 2 * e;
+        if constexpr (NV % 8 == 0) {
+#pragma unroll
+            for (int q = 0; q < NV / 8; ++q) {
+                const u32x4 t = ld_any<0, 2>(b + 16 * q);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (dt == BF16) {
+                        f[8 * q + 2 * i] = bf16_lo(t[i]);
+                        f[8 * q + 2 * i + 1] = bf16_hi(t[i]);
+                    } else {
+                        const f32x2 h = unpack_f16x2(t[i]);
+                        f[8 * q + 2 * i] = h.x;
+                        f[8 * q + 2 * i + 1] = h.y;
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) f[i] = load1(p, dt, e + i);
+        }
+    }
+}
+template <int NV>
+__device__ __forceinline__ void store_run(void* p, int dt, int64_t e, const float (&f)[NV]) {
+    static_assert(NV % 4 == 0 || NV == 1, "whole pieces, or one element");
+    if constexpr (NV == 1) {
+        store1(p, dt, e, f[0]);
+    } else if (dt == F32) {
+        char* b = reinterpret_cast<char*>(p) + 4 * e;
+#pragma unroll
+        for (int q = 0; q < NV / 4; ++q)
+            st_any<0, 4>(b + 16 * q, u32x4{__float_as_uint(f[4 * q]), __float_as_uint(f[4 * q + 1]),
+                                           __float_as_uint(f[4 * q + 2]), __float_as_uint(f[4 * q + 3])});
+    } else if constexpr (NV % 8 == 0) {
+        char* b = reinterpret_cast<char*>(p) + 2 * e;
+#pragma unroll
+        for (int q = 0; q < NV / 8; ++q) {
+            u32x4 t;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                t[i] = dt == BF16 ? pack_bf16x2(f[8 * q + 2 * i], f[8 * q + 2 * i + 1])
+                                  : pack_f16x2(f[8 * q + 2 * i], f[8 * q + 2 * i + 1]);
+            st_any<0, 2>(b + 16 * q, t);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store1(p, dt, e + i, f[i]);
+    }
+}
+
+// The epilogue of NV consecutive columns n .. of row m (n a multiple of NV; columns past N and rows past M
+// are not stored).  bias[] holds the columns' bias.
+template <bool ACT, int NV>
+__device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int n, float (&v)[NV], const float (&bias)[NV]) {
+    if (m >= a.M || n >= a.N) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] += bias[i];
+    if constexpr (ACT) activate<NV>(v, a.act, a.odt == F32);
+    const bool whole = n + NV <= a.N;
+    if (a.res != nullptr) {
+        float r[NV];
+        const int64_t e = m * a.rs + n;
+        if (whole) {
+            load_run<NV>(a.res, a.rdt, e, r);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += r[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (n + i < a.N) v[i] += load1(a.res, a.rdt, e + i);
+        }
+    }
+    const int64_t e = m * a.os + n;
+    if (whole) {
+        store_run<NV>(a.out, a.odt, e, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (n + i < a.N) store1(a.out, a.odt, e + i, v[i]);
+    }
+}
+
+template <int NV>
+__device__ __forceinline__ void load_bias(const LinArgs& a, int n, float (&b)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) b[i] = a.bias != nullptr && n + i < a.N ? load1(a.bias, a.bdt, n + i) : 0.0f;
+}
+
+// Tile form: WM x WN waves, each with MI x NI blocks of 16 x 16, one step of 128 bytes of K at a time, two steps'
+// tiles in LDS.  An LDS row is 8 pieces of 16 bytes; piece j of a row stands at j ^ key(row), which makes the
+// eight rows that neighbouring lanes read fall on different banks.  w is the A operand: a lane's four results of a
+// block are four columns of one row of out, and block ni takes the columns 4 NI q + 4 ni + j (q = c / 4, j = c % 4) of the
+// wave's, so that a lane ends with 4 NI columns in a row.
+// DIRECT: rows are 16-byte aligned, and whole steps go from global memory straight into LDS.
+template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, bool ACT>
+__global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
+    constexpr int NW = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16;
+    constexpr int S = DT == F32 ? 4 : 2;
+    constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW;  // 1 KB loads per wave and step
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads per wave");
+    __shared__ __attribute__((aligned(16))) char s0[(BM + BN) * kStepBytes];
+    __shared__ __attribute__((aligned(16))) char s1[(BM + BN) * kStepBytes];
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int w = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wm = w / WN, wn = w % WN;
+    // column tiles of one row tile are neighbours, on one XCD: x is read once into its L2
+    const uint32_t tile = xcd_tile(blockIdx.x, gridDim.x);
+    const int64_t m0 = (int64_t)(tile / a.ntiles) * BM;
+    const int n0 = (int)(tile % a.ntiles) * BN;
+    const char* xb = a.x + m0 * a.xs;
+    const char* wb = a.w + (int64_t)n0 * a.ws;
+    const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
+    const int64_t kbytes = (int64_t)a.K * S;
+    const int steps = (int)((kbytes + kStepBytes - 1) / kStepBytes);
+    const int whole = DIRECT ? (int)(kbytes / kStepBytes) : 0;  // steps loaded straight into LDS
+
+    // lane i of load u covers LDS row 8 (LX w + u) + i / 8, place i % 8; rows past the end repeat the last one
+    int xr[LX], wr[LW];
+    uint32_t xo[LX], wo[LW];  // within the step: byte offset of the lane's piece from xb, wb (DIRECT)
+    auto key_x = [](int r) { return r & 7; };
+    auto key_w = [](int r) { return (r & 3) | (((r / (4 * NI)) & 1) << 2); };
+#pragma unroll
+    for (int u = 0; u < LX; ++u) {
+        const int r = 8 * (LX * w + u) + (lane >> 3);
+        xr[u] = min(r, mrows - 1);
+        xo[u] = (uint32_t)xr[u] * (uint32_t)a.xs + 16u * ((lane & 7) ^ key_x(r));
+    }
+#pragma unroll
+    for (int u = 0; u < LW; ++u) {
+        const int r = 8 * (LW * w + u) + (lane >> 3);
+        wr[u] = min(r, nrows - 1);
+        wo[u] = (uint32_t)wr[u] * (uint32_t)a.ws + 16u * ((lane & 7) ^ key_w(r));
+    }
+    const __amdgpu_buffer_rsrc_t xres = __builtin_amdgcn_make_buffer_rsrc((void*)xb, (short)0, -1, kBufferDword3);
+    const __amdgpu_buffer_rsrc_t wres = __builtin_amdgcn_make_buffer_rsrc((void*)wb, (short)0, -1, kBufferDword3);
+    auto load_direct = [&](int kt, char* d) {
+#pragma unroll
+        for (int u = 0; u < LX; ++u)
+            load_to_lds(xres, d + 1024 * (LX * w + u), xo[u], kt * kStepBytes);
+#pragma unroll
+        for (int u = 0; u < LW; ++u)
+            load_to_lds(wres, d + BM * kStepBytes + 1024 * (LW * w + u), wo[u], kt * kStepBytes);
+    };
+    u32x4 px[LX], pw[LW];
+    auto load_regs = [&](int kt) {
+#pragma unroll
+        for (int u = 0; u < LX; ++u) {
+            const int r = 8 * (LX * w + u) + (lane >> 3);
+            px[u] = row_piece<DT, DIRECT>(xb + xr[u] * a.xs, (int64_t)kt * kStepBytes + 16 * ((lane & 7) ^ key_x(r)), a.K);
+        }
+#pragma unroll
+        for (int u = 0; u < LW; ++u) {
+            const int r = 8 * (LW * w + u) + (lane >> 3);
+            pw[u] = row_piece<DT, DIRECT>(wb + wr[u] * a.ws, (int64_t)kt * kStepBytes + 16 * ((lane & 7) ^ key_w(r)), a.K);
+        }
+    };
+    auto put_regs = [&](char* d) {
+#pragma unroll
+        for (int u = 0; u < LX; ++u) *reinterpret_cast<u32x4*>(d + 1024 * (LX * w + u) + 16 * lane) = px[u];
+#pragma unroll
+        for (int u = 0; u < LW; ++u)
+            *reinterpret_cast<u32x4*>(d + BM * kStepBytes + 1024 * (LW * w + u) + 16 * lane) = pw[u];
+    };
+
+    f32x4 acc[MI][NI];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    const int xrow = (wm * MI * 16 + c) * kStepBytes;
+    const int wrow = BM * kStepBytes + (wn * NI * 16 + 4 * NI * (c >> 2) + (c & 3)) * kStepBytes;
+    auto compute = [&](const char* d) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int piece = 16 * ((4 * s + g) ^ (c & 7));
+            u32x4 xf[MI], wf[NI];
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi) xf[mi] = *reinterpret_cast<const u32x4*>(d + xrow + mi * 16 * kStepBytes + piece);
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) wf[ni] = *reinterpret_cast<const u32x4*>(d + wrow + ni * 4 * kStepBytes + piece);
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = mma<DT>(wf[ni], xf[mi], acc[mi][ni]);
+        }
+    };
+    // Step kt sits in d; the next one is loaded into dn meanwhile.  The two buffers are separate objects and the
+    // loop is unrolled by two, so that the compiler sees that loads in flight into one do not touch the other.
+    auto step = [&](int kt, const char* d, char* dn) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of the step have landed
+        __syncthreads();                     // every wave's have, and none still reads dn
+        const bool next = kt + 1 < steps, direct = DIRECT && kt + 1 < whole;
+        if (direct) load_direct(kt + 1, dn);
+        else if (next) load_regs(kt + 1);
+        compute(d);
+        if (next && !direct) put_regs(dn);
+    };
+    if (DIRECT && whole > 0) {
+        load_direct(0, s0);
+    } else {
+        load_regs(0);
+        put_regs(s0);
+    }
+    for (int kt = 0; kt < steps; kt += 2) {
+        step(kt, s0, s1);
+        if (kt + 1 < steps) step(kt + 1, s1, s0);
+    }
+
+    const int n = n0 + wn * NI * 16 + 4 * NI * g;
+    float bias[4 * NI];
+    load_bias<4 * NI>(a, n, bias);
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+        float v[4 * NI];
+#pragma unroll
+        for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * ni + i] = acc[mi][ni][i];
+        finish<ACT, 4 * NI>(a, m0 + wm * MI * 16 + mi * 16 + c, n, v, bias);
+    }
+}
+
+// Strip form: a wave takes 16 rows of the longer operand and every row of the shorter (16 R at most), straight from
+// global memory into the matrix instructions.  `split` waves of a block share a strip's K, two 64-byte pieces at
+// a time in turn, and are added through LDS in wave order.
+// WIDE: strips of w against few rows of x (a lane ends with 4 columns of a row); else strips of x against few
+// columns (4 rows of a column).
+template <int DT, int R, bool WIDE, bool ALIGNED>
+__global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
+    constexpr int S = DT == F32 ? 4 : 2;
+    extern __shared__ f32x4 part[];  // [strips of the block][split - 1][R][64]
+    const int lane = threadIdx.x % 64, g = lane / 16, c = lane % 16;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int ks = w % a.split, strip = w / a.split;
+    const int64_t p0 = ((int64_t)blockIdx.x * (blockDim.x / 64 / a.split) + strip) * 16;
+    const int64_t P = WIDE ? a.N : a.M;
+    const int Q = WIDE ? (int)a.M : a.N;
+    const char* pb = (WIDE ? a.w : a.x) + min(p0 + c, P - 1) * (WIDE ? a.ws : a.xs);
+    const char* qb[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) qb[r] = (WIDE ? a.x : a.w) + (int64_t)min(16 * r + c, Q - 1) * (WIDE ? a.xs : a.ws);
+    const int64_t kbytes = (int64_t)a.K * S;
+    const int pairs = (int)((kbytes + 127) / 128);
+
+    f32x4 acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int U = R >= 4 ? 2 : 4;  // pairs in flight
+    for (int t0 = ks; t0 < pairs; t0 += U * a.split) {
+        u32x4 pf[U][2], qf[U][2][R];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int t = t0 + u * a.split;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int64_t kb = (int64_t)t * 128 + 64 * s + 16 * g;
+                pf[u][s] = row_piece<DT, ALIGNED>(pb, kb, a.K);
+#pragma unroll
+                for (int r = 0; r < R; ++r) qf[u][s][r] = row_piece<DT, ALIGNED>(qb[r], kb, a.K);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int r = 0; r < R; ++r) acc[r] = mma<DT>(pf[u][s], qf[u][s][r], acc[r]);
+    }
+    if (a.split > 1) {
+        f32x4* mine = part + (int64_t)strip * (a.split - 1) * R * 64;
+        if (ks > 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) mine[((ks - 1) * R + r) * 64 + lane] = acc[r];
+        }
+        __syncthreads();
+        if (ks > 0) return;
+        for (int k = 0; k < a.split - 1; ++k)
+#pragma unroll
+            for (int r = 0; r < R; ++r) acc[r] += mine[(k * R + r) * 64 + lane];
+    }
+    if constexpr (WIDE) {
+        const int n = (int)min<int64_t>(p0 + 4 * g, P);
+        float bias[4];
+        load_bias<4>(a, n, bias);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float v[4] = {acc[r][0], acc[r][1], acc[r][2], acc[r][3]};
+            finish<true, 4>(a, 16 * r + c, n, v, bias);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float bias[1];
+            load_bias<1>(a, 16 * r + c, bias);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[1] = {acc[r][i]};
+                finish<true, 1>(a, p0 + 4 * g + i, 16 * r + c, v, bias);
+            }
+        }
+    }
+}
+
+// K of nothing: act(bias) + residual, one thread per element.
+__global__ __launch_bounds__(256) void linear_empty_kernel(LinArgs a) {
+    const int64_t total = a.M * a.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / a.N;
+        const int n = (int)(i - m * a.N);
+        float v[1] = {0.0f}, bias[1];
+        load_bias<1>(a, n, bias);
+        finish<true, 1>(a, m, n, v, bias);
+    }
+}
+
+template <int DT, int R>
+void launch_strip(const LinArgs& a, bool wide, bool al, unsigned blocks, unsigned threads, size_t lds, hipStream_t st) {
+    if (wide && al) hipLaunchKernelGGL((linear_strip_kernel<DT, R, true, true>), dim3(blocks), dim3(threads), lds, st, a);
+    else if (wide) hipLaunchKernelGGL((linear_strip_kernel<DT, R, true, false>), dim3(blocks), dim3(threads), lds, st, a);
+    else if (al) hipLaunchKernelGGL((linear_strip_kernel<DT, R, false, true>), dim3(blocks), dim3(threads), lds, st, a);
+    else hipLaunchKernelGGL((linear_strip_kernel<DT, R, false, false>), dim3(blocks), dim3(threads), lds, st, a);
+}
+
+template <int DT, int WM, int WN, int MI, int NI>
+void launch_tile(const LinArgs& a, bool direct, unsigned tiles, hipStream_t st) {
+    const dim3 grid(tiles), block(WM * WN * 64);
+    const bool act = a.act != MBRT_ACT_NONE;
+    if (direct && act) hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, true, true>), grid, block, 0, st, a);
+    else if (direct) hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, true, false>), grid, block, 0, st, a);
+    else if (act) hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, false, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, false, false>), grid, block, 0, st, a);
+}
+
+template <int DT>
+int launch(LinArgs& a, bool al, hipStream_t st) {
+    const int64_t es = DT == F32 ? 4 : 2, cus = cu_count();
+    const bool wide = a.M <= a.N;
+    const int64_t shorter = wide ? a.M : a.N, longer = wide ? a.N : a.M;
+    if (shorter <= 64) {
+        const int R = shorter <= 16 ? 1 : shorter <= 32 ? 2 : 4;
+        const int64_t strips = ceil_div(longer, 16), pairs = ceil_div(a.K * es, 128);
+        int split = 1;
+        while (split < 16 && 2 * split <= pairs && strips * split < 8 * cus) split *= 2;
+        a.split = split;
+        const int per_block = std::max(1, 4 / split);
+        const int64_t blocks = ceil_div(strips, per_block);
+        if (blocks >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many rows");
+        const size_t lds = (size_t)per_block * (split - 1) * R * 1024;
+        const unsigned threads = per_block * split * 64;
+        if (R == 1) launch_strip<DT, 1>(a, wide, al, (unsigned)blocks, threads, lds, st);
+        else if (R == 2) launch_strip<DT, 2>(a, wide, al, (unsigned)blocks, threads, lds, st);
+        else launch_strip<DT, 4>(a, wide, al, (unsigned)blocks, threads, lds, st);
+        return MBRT_OK;
+    }
+    // 32-bit offsets within a tile
+    const bool direct = al && a.xs < (int64_t(1) << 22) && a.ws < (int64_t(1) << 22);
+    const bool big = ceil_div(a.M, 128) * ceil_div(a.N, 128) >= cus;
+    const int64_t bm = big ? 128 : 64;
+    a.ntiles = (uint32_t)ceil_div(a.N, bm);
+    const int64_t tiles = ceil_div(a.M, bm) * a.ntiles;
+    if (tiles >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many tiles");
+    if (big) launch_tile<DT, 2, 2, 4, 4>(a, direct, (unsigned)tiles, st);
+    else launch_tile<DT, 2, 2, 2, 2>(a, direct, (unsigned)tiles, st);
+    return MBRT_OK;
+}
+
+}  // namespace
+}  // namespace mbrt
+
+using namespace mbrt;
+
+extern "C" {
+
+int mbrt_linear(const void* x, int dtype, int64_t x_row_stride, const void* weight, int64_t weight_row_stride,
+                const void* bias, int bias_dtype, const void* residual, int residual_dtype,
+                int64_t residual_row_stride, void* out, int out_dtype, int64_t out_row_stride, int64_t rows,
+                int64_t in_features, int64_t out_features, int act, mbrt_stream_t stream) {
+    const char* op = "mbrt_linear";
+    MBRT_REQUIRE_FLOAT_DT(dtype, op);
+    MBRT_REQUIRE_FLOAT_DT(out_dtype, op);
+    MBRT_REQUIRE(!bias || is_float_dt(bias_dtype), MBRT_E_UNSUPPORTED_DTYPE, "%s: bias dtype %d", op, bias_dtype);
+    MBRT_REQUIRE(!residual || is_float_dt(residual_dtype), MBRT_E_UNSUPPORTED_DTYPE, "%s: residual dtype %d", op,
+                 residual_dtype);
+    MBRT_REQUIRE(act >= MBRT_ACT_NONE && act <= MBRT_ACT_TANH, MBRT_E_INVALID_ARG, "%s: unknown activation %d", op, act);
+    MBRT_REQUIRE(rows >= 0 && in_features >= 0 && out_features >= 0, MBRT_E_SHAPE, "%s: negative size", op);
+    if (rows == 0 || out_features == 0) return MBRT_OK;
+    const int64_t es = dt_size(dtype), lim = int64_t(1) << 28;
+    MBRT_REQUIRE(rows < (int64_t(1) << 40) && in_features < lim && out_features < lim, MBRT_E_SHAPE,
+                 "%s: size beyond 2^28 features or 2^40 rows", op);
+    MBRT_REQUIRE(x_row_stride >= 0 && weight_row_stride >= 0 && (!residual || residual_row_stride >= 0) &&
+                     (out_row_stride >= out_features || rows == 1),
+                 MBRT_E_SHAPE, "%s: negative row stride, or rows of out that overlap", op);
+    MBRT_REQUIRE(out && (in_features == 0 || (x && weight)), MBRT_E_INVALID_ARG, "%s: NULL pointer", op);
+    MBRT_REQUIRE(aligned(x, es) && aligned(weight, es) && aligned(out, dt_size(out_dtype)) &&
+                     (!bias || aligned(bias, dt_size(bias_dtype))) &&
+                     (!residual || aligned(residual, dt_size(residual_dtype))),
+                 MBRT_E_ALIGN, "%s: pointer not aligned to its elements", op);
+    LinArgs a{};
+    a.x = static_cast<const char*>(x);
+    a.w = static_cast<const char*>(weight);
+    a.bias = bias;
+    a.res = residual;
+    a.out = out;
+    a.xs = x_row_stride * es;
+    a.ws = weight_row_stride * es;
+    a.rs = residual_row_stride;
+    a.os = out_row_stride;
+    a.M = rows;
+    a.N = (int)out_features;
+    a.K = (int)in_features;
+    a.bdt = bias_dtype;
+    a.rdt = residual_dtype;
+    a.odt = out_dtype;
+    a.act = act;
+    hipStream_t st = as_stream(stream);
+    if (in_features == 0) {
+        hipLaunchKernelGGL(linear_empty_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(rows * out_features, 256), 1 << 16)),
+                           dim3(256), 0, st, a);
+        return check_launch(op);
+    }
+    const bool al = aligned(x, 16) && aligned(weight, 16) && a.xs % 16 == 0 && a.ws % 16 == 0;
+    const int status = dtype == F32 ? launch<F32>(a, al, st) : dtype == BF16 ? launch<BF16>(a, al, st) : launch<F16>(a, al, st);
+    return status == MBRT_OK ? check_launch(op) : status;
+}
+
+}  // extern "C"

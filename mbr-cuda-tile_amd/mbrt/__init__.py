@@ -373,6 +373,83 @@ def attention_bnhd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch
     return out
 
 
+# ---- transformer layer ----------------------------------------------------------------------
+
+def _new(shape, dtype, device, stream) -> torch.Tensor:
+    """Memory for a call on `stream`: taken from that stream's own, so that nothing still running
+    elsewhere uses it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
+           act: int = ACT_NONE, residual: torch.Tensor | None = None, out_dtype=None, stream=None) -> torch.Tensor:
+    """act(x weight^T + bias) + residual, rounded once.  x [.., K] and weight [N, K] of one dtype, bias [N],
+    residual and out [.., N], each f32, f16 or bf16; rows at any stride and alignment, the last dim
+    contiguous.  out may be residual itself.  out_dtype defaults to x's."""
+    if out is None:
+        out = _new((*x.shape[:-1], weight.shape[0]), out_dtype or x.dtype, x.device, stream)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("linear: out and out_dtype disagree")
+    _n.linear(x, weight, bias, out, act, residual, _h(stream))
+    return out
+
+
+def split_qkv_norm_rotary(qkv: torch.Tensor, q_gamma: torch.Tensor, k_gamma: torch.Tensor, cos: torch.Tensor,
+                          sin: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None, heads: int,
+                          kv_heads: int | None = None, scale: float | None = None, eps: float = 1e-12, pos0: int = 0,
+                          stream=None) -> None:
+    """Heads of qkv [B, N, (H + 2 H_kv) D] into q [B, H, N, D] and k, v [B, H_kv, N, D], views of any strides
+    with a unit last dim (k and v strided alike).  Query and key heads are RMS-normed (x * scale * gamma /
+    sqrt(sum x^2 + eps), scale sqrt(D) by default) and rotated by rows pos0 .. of cos, sin [n_pos, D/2].  v None
+    leaves the values in qkv; q and k may be their own places in qkv."""
+    _n.split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v, heads, heads if kv_heads is None else kv_heads,
+                             -1.0 if scale is None else scale, eps, pos0, _h(stream))
+
+
+def attention_window_workspace_bytes(B: int, heads: int, kv_heads: int, n_q: int, n_k: int, dim_head: int,
+                                     left: int | None = None, right: int | None = None, sinks: int = 0) -> int:
+    n = int(_abi.lib().mbrt_attention_window_workspace_bytes(B, heads, kv_heads, n_q, n_k, dim_head,
+                                                             -1 if left is None else left,
+                                                             -1 if right is None else right, sinks))
+    if n < 0:
+        raise ValueError("attention_window_workspace_bytes: sizes out of range")
+    return n
+
+
+def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor | None = None,
+                     left: int | None = None, right: int | None = None, sinks: int = 0, q_start: int | None = None,
+                     key_lens: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                     gate_is_logit: bool = True, scale: float = 0.0, out_dtype=None,
+                     workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Attention of q [B, N_q, H, D] over the keys within `left` positions before and `right` after each query, and
+    the first `sinks` keys (as far as `right` lets them be seen), for k, v [B, N_k, H_kv, D] bf16 or f16, D 32, 64
+    or 128; views of any strides that are multiples of 8 with a unit last dim, k and v strided alike.  None: no limit.
+    Query i stands at position q_start + i, by default at the end of its keys (key_lens [B] int32, or all N_k).
+    out [B, N_q, H, D] (q's dtype by default); gate [B, N_q, H] multiplies each head by its sigmoid (or itself).
+    workspace: attention_window_workspace_bytes of the same sizes, allocated here when None."""
+    if out is None:
+        out = _new(q.shape, out_dtype or q.dtype, q.device, stream)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("attention_window: out and out_dtype disagree")
+    for name, x in (("left", left), ("right", right), ("q_start", q_start)):
+        if x is not None and x < 0:
+            raise ValueError(f"attention_window: {name} is None or at least 0")
+    if workspace is None and q.dim() == 4 and k.dim() == 4:
+        need = int(_abi.lib().mbrt_attention_window_workspace_bytes(
+            q.shape[0], q.shape[2], k.shape[2], q.shape[1], k.shape[1], q.shape[3], -1 if left is None else left,
+            -1 if right is None else right, sinks))
+        if need > 0:
+            workspace = _new(need, torch.uint8, q.device, stream)
+    _n.attention_window(q, k, v, out, -1 if left is None else left, -1 if right is None else right, sinks,
+                        -1 if q_start is None else q_start, key_lens, gate, gate_is_logit, scale, workspace, _h(stream))
+    return out
+
+
 N_FFT = 2048
 
 

@@ -104,6 +104,10 @@ SIGNATURES: dict[str, list] = {
     "mbrt_attention": [P, P, P, I, P, I, L, L, L, L, Fl, P],
     "mbrt_attention_strided": [P, P, P, I, L, L, L, L, L, L, L, L, L, L, L, P, P, I, P, I, I, P, I, Fl, P],
     "mbrt_attention_ex": [P, P, P, I, L, L, L, L, L, L, L, L, L, L, L, P, P, I, P, I, I, P, I, Fl, I, P],
+    "mbrt_linear": [P, I, L, P, L, P, I, P, I, L, P, I, L, L, L, L, I, P],
+    "mbrt_split_qkv_norm_rotary": [P, I, L, L, P, P, I, P, P, I, L, L, P, P, P, I, *[L] * 6, *[L] * 5, Fl, Fl, P],
+    "mbrt_attention_window_workspace_bytes": [L] * 9,
+    "mbrt_attention_window": [P, P, P, I, *[L] * 6, *[L] * 6, *[L] * 4, P, P, I, I, P, I, L, L, L, Fl, P, L, P],
     "mbrt_hann_window": [P, L, P],
     "mbrt_stft_num_frames": [L, L, I],
     "mbrt_stft": [P, P, P, L, L, L, L, L, L, I, I, P],
@@ -121,6 +125,7 @@ SIGNATURES: dict[str, list] = {
 _RESTYPE = {
     "mbrt_last_error": C.c_char_p,
     "mbrt_get_arith_flags": C.c_uint32,
+    "mbrt_attention_window_workspace_bytes": C.c_int64,
     "mbrt_stft_num_frames": C.c_int64,
     "mbrt_istft_output_length": C.c_int64,
     "mbrt_istft_workspace_bytes": C.c_int64,

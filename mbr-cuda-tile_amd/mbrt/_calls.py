@@ -173,6 +173,115 @@ def attention_ex(q, k, v, sizes, strides, cos, sin, gate, gate_is_logit, out, sc
               _s(stream))
 
 
+def _gpu(*ts):
+    """The device of these tensors, which a call is made on."""
+    ts = [t for t in ts if t is not None]
+    for t in ts:
+        if t.device.type != "cuda" or t.device != ts[0].device:
+            raise ValueError("mbrt: expected tensors on one GPU")
+    return torch.cuda.device(ts[0].device)
+
+
+def _unit_last(*ts):
+    for t in ts:
+        if t is not None and t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError("mbrt: expected a contiguous last dim")
+
+
+def _row_stride(t):
+    """The one stride between the rows of [.., n] (0 where there is one row)."""
+    span, stride = 1, 0
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] == 1:
+            continue
+        if t.numel() and span > 1 and t.stride(d) != span * stride:
+            raise ValueError("linear: the rows of a tensor lie at more than one stride")
+        if span == 1:
+            stride = t.stride(d)
+        span *= t.shape[d]
+    return stride
+
+
+def linear(x, weight, bias, out, act, residual, stream):
+    _tensors(x, weight, out, *(t for t in (bias, residual) if t is not None))
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[1] != x.shape[-1]:
+        raise ValueError("linear: expected x [.., K] and weight [N, K]")
+    N, K = weight.shape
+    if x.dtype != weight.dtype:
+        raise ValueError("linear: x and weight differ in dtype")
+    want = x.shape[:-1] + (N,)
+    if out.shape != want or residual is not None and residual.shape != want:
+        raise ValueError("linear: expected out and residual [.., N]")
+    if bias is not None and bias.shape != (N,):
+        raise ValueError("linear: expected bias [N]")
+    _unit_last(x, weight, out, residual, bias)
+    rows = 1
+    for s in x.shape[:-1]:
+        rows *= s
+    ws = weight.stride(0) if N > 1 else 0
+    os = _row_stride(out) if rows > 1 else N
+    args = (_p(x), _dt(x), _row_stride(x), _p(weight), ws, _p(bias), _dt(bias, _abi.F32), _p(residual),
+            _dt(residual, _abi.F32), 0 if residual is None else _row_stride(residual), _p(out), _dt(out), os, rows, K, N,
+            act)
+    with _gpu(x, weight, bias, residual, out):
+        _abi.call("mbrt_linear", *args, _s(stream))
+
+
+def split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v, heads, kv_heads, scale, eps, pos0, stream):
+    _tensors(qkv, q_gamma, k_gamma, cos, sin, q, k, *(t for t in (v,) if t is not None))
+    if qkv.dim() != 3 or heads < 1 or kv_heads < 1 or qkv.shape[2] % (heads + 2 * kv_heads):
+        raise ValueError("split_qkv_norm_rotary: expected qkv [B, N, (H + 2 H_kv) D]")
+    B, N, width = qkv.shape
+    D = width // (heads + 2 * kv_heads)
+    if q.shape != (B, heads, N, D) or k.shape != (B, kv_heads, N, D) or v is not None and v.shape != k.shape:
+        raise ValueError("split_qkv_norm_rotary: expected q [B, H, N, D] and k, v [B, H_kv, N, D]")
+    if q.dtype != k.dtype or v is not None and v.dtype != k.dtype:
+        raise ValueError("split_qkv_norm_rotary: q, k and v differ in dtype")
+    if v is not None and v.stride() != k.stride():
+        raise ValueError("split_qkv_norm_rotary: k and v must be strided alike")
+    if q_gamma.shape != (D,) or k_gamma.shape != (D,) or q_gamma.dtype != k_gamma.dtype:
+        raise ValueError("split_qkv_norm_rotary: expected gammas [D] of one dtype")
+    if cos.dim() != 2 or cos.shape[1] != D // 2 or sin.shape != cos.shape or sin.dtype != cos.dtype:
+        raise ValueError("split_qkv_norm_rotary: expected cos, sin [n_pos, D/2] of one dtype")
+    _contig(q_gamma, k_gamma, cos, sin)
+    _unit_last(qkv, q, k, v)
+    args = (_p(qkv), _dt(qkv), qkv.stride(0), qkv.stride(1), _p(q_gamma), _p(k_gamma), _dt(q_gamma), _p(cos), _p(sin),
+            _dt(cos), cos.shape[0], pos0, _p(q), _p(k), _p(v), _dt(q), *q.stride()[:3], *k.stride()[:3], B, N, heads,
+            kv_heads, D, D ** 0.5 if _float(scale) < 0 else _float(scale), _float(eps))
+    with _gpu(qkv, q_gamma, k_gamma, cos, sin, q, k, v):
+        _abi.call("mbrt_split_qkv_norm_rotary", *args, _s(stream))
+
+
+def attention_window(q, k, v, out, left, right, sinks, q_start, key_lens, gate, gate_is_logit, scale, workspace,
+                     stream):
+    _tensors(q, k, v, out, *(t for t in (key_lens, gate, workspace) if t is not None))
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("attention_window: expected q [B, N_q, H, D] and k, v [B, N_k, H_kv, D]")
+    B, nq, H, D = q.shape
+    nk, KV = k.shape[1], k.shape[2]
+    if k.shape != (B, nk, KV, D) or v.shape != k.shape:
+        raise ValueError("attention_window: expected q [B, N_q, H, D] and k, v [B, N_k, H_kv, D]")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("attention_window: q, k and v differ in dtype")
+    if v.stride() != k.stride():
+        raise ValueError("attention_window: k and v must be strided alike")
+    if out.shape != q.shape:
+        raise ValueError("attention_window: expected out [B, N_q, H, D]")
+    if key_lens is not None and (key_lens.shape != (B,) or key_lens.dtype != torch.int32):
+        raise ValueError("attention_window: expected key_lens [B] int32")
+    if gate is not None and gate.shape != (B, nq, H):
+        raise ValueError("attention_window: expected gate [B, N_q, H]")
+    _unit_last(q, k, v, out)
+    _contig(key_lens, gate, workspace)
+    qs, ks, os = q.stride(), k.stride(), out.stride()
+    args = (_p(q), _p(k), _p(v), _dt(q), B, H, KV, nq, nk, D, qs[0], qs[2], qs[1], ks[0], ks[2], ks[1], left, right,
+            sinks, q_start, _p(key_lens), _p(gate), _dt(gate, _abi.F32), int(bool(gate_is_logit)), _p(out), _dt(out),
+            os[0], os[2], os[1], _float(scale), _p(workspace),
+            0 if workspace is None else workspace.numel() * workspace.element_size())
+    with _gpu(q, k, v, out, key_lens, gate, workspace):
+        _abi.call("mbrt_attention_window", *args, _s(stream))
+
+
 def stft(x, window, hop, center, normalized, out, n_fft, win_length, stream):
     _tensors(x, window, out)
     _contig(x, window, out)

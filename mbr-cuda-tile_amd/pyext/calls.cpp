@@ -16,7 +16,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+
+#include <cmath>
 
 #include <vector>
 
@@ -351,6 +354,145 @@ MBRT_PY(attention_ex) {
     END_HANDLE_TH_ERRORS
 }
 
+// The device of these tensors, which a call is made on.
+at::Device gpu(std::initializer_list<const at::Tensor*> ts) {
+    const at::Device dev = (*ts.begin())->device();
+    for (const at::Tensor* t : ts)
+        if (t->defined() && (!t->is_cuda() || t->device() != dev)) raise(PyExc_ValueError, "mbrt: expected tensors on one GPU");
+    return dev;
+}
+
+void unit_last(std::initializer_list<const at::Tensor*> ts) {
+    for (const at::Tensor* t : ts)
+        if (t->defined() && t->dim() && t->size(-1) > 1 && t->stride(-1) != 1)
+            raise(PyExc_ValueError, "mbrt: expected a contiguous last dim");
+}
+
+// The one stride between the rows of [.., n] (0 where there is one row).
+int64_t row_stride(const at::Tensor& t) {
+    int64_t span = 1, stride = 0;
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (t.numel() && span > 1 && t.stride(d) != span * stride)
+            raise(PyExc_ValueError, "linear: the rows of a tensor lie at more than one stride");
+        if (span == 1) stride = t.stride(d);
+        span *= t.size(d);
+    }
+    return stride;
+}
+
+// linear(x, weight, bias | None, out, act, residual | None, stream)
+MBRT_PY(linear) {
+    HANDLE_TH_ERRORS
+    count(n, 7);
+    const at::Tensor &x = tensor(a[0]), &w = tensor(a[1]), &out = tensor(a[3]);
+    const at::Tensor b = tensor_or_none(a[2]), res = tensor_or_none(a[5]);
+    if (x.dim() < 1 || w.dim() != 2 || w.size(1) != x.size(-1))
+        raise(PyExc_ValueError, "linear: expected x [.., K] and weight [N, K]");
+    const int64_t N = w.size(0), K = w.size(1);
+    if (x.scalar_type() != w.scalar_type()) raise(PyExc_ValueError, "linear: x and weight differ in dtype");
+    auto fits = [&](const at::Tensor& t) {
+        if (t.dim() != x.dim() || t.size(-1) != N) return false;
+        for (int64_t d = 0; d < x.dim() - 1; ++d)
+            if (t.size(d) != x.size(d)) return false;
+        return true;
+    };
+    if (!fits(out) || (res.defined() && !fits(res))) raise(PyExc_ValueError, "linear: expected out and residual [.., N]");
+    if (b.defined() && (b.dim() != 1 || b.size(0) != N)) raise(PyExc_ValueError, "linear: expected bias [N]");
+    unit_last({&x, &w, &out, &res, &b});
+    int64_t rows = 1;
+    for (int64_t d = 0; d < x.dim() - 1; ++d) rows *= x.size(d);
+    const int64_t xs = row_stride(x), ws = N > 1 ? w.stride(0) : 0, os = rows > 1 ? row_stride(out) : N;
+    const int64_t rs = res.defined() ? row_stride(res) : 0;
+    const int dt = dtype_code(x), bd = dtype_or(b, MBRT_F32), rd = dtype_or(res, MBRT_F32), od = dtype_code(out);
+    const int act = (int)integer(a[4]);
+    void *xp = ptr(x), *wp = ptr(w), *bp = ptr(b), *rp = ptr(res), *op = ptr(out);
+    const c10::DeviceGuard guard(gpu({&x, &w, &b, &res, &out}));
+    const mbrt_stream_t st = stream(a[6]);
+    return call("mbrt_linear",
+                [&] { return mbrt_linear(xp, dt, xs, wp, ws, bp, bd, rp, rd, rs, op, od, os, rows, K, N, act, st); });
+    END_HANDLE_TH_ERRORS
+}
+
+// split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v | None, heads, kv_heads, scale (< 0: sqrt(D)), eps,
+//                       pos0, stream)
+MBRT_PY(split_qkv_norm_rotary) {
+    HANDLE_TH_ERRORS
+    count(n, 14);
+    const at::Tensor &qkv = tensor(a[0]), &qg = tensor(a[1]), &kg = tensor(a[2]), &c = tensor(a[3]), &s = tensor(a[4]);
+    const at::Tensor &q = tensor(a[5]), &k = tensor(a[6]);
+    const at::Tensor v = tensor_or_none(a[7]);
+    const int64_t H = integer(a[8]), KV = integer(a[9]);
+    if (qkv.dim() != 3 || H < 1 || KV < 1 || qkv.size(2) % (H + 2 * KV))
+        raise(PyExc_ValueError, "split_qkv_norm_rotary: expected qkv [B, N, (H + 2 H_kv) D]");
+    const int64_t B = qkv.size(0), N = qkv.size(1), D = qkv.size(2) / (H + 2 * KV);
+    auto is = [&](const at::Tensor& t, int64_t h) {
+        return t.dim() == 4 && t.size(0) == B && t.size(1) == h && t.size(2) == N && t.size(3) == D;
+    };
+    if (!is(q, H) || !is(k, KV) || (v.defined() && !is(v, KV)))
+        raise(PyExc_ValueError, "split_qkv_norm_rotary: expected q [B, H, N, D] and k, v [B, H_kv, N, D]");
+    if (q.scalar_type() != k.scalar_type() || (v.defined() && v.scalar_type() != k.scalar_type()))
+        raise(PyExc_ValueError, "split_qkv_norm_rotary: q, k and v differ in dtype");
+    if (v.defined() && v.strides() != k.strides())
+        raise(PyExc_ValueError, "split_qkv_norm_rotary: k and v must be strided alike");
+    if (qg.dim() != 1 || qg.size(0) != D || kg.sizes() != qg.sizes() || kg.scalar_type() != qg.scalar_type())
+        raise(PyExc_ValueError, "split_qkv_norm_rotary: expected gammas [D] of one dtype");
+    if (c.dim() != 2 || c.size(1) != D / 2 || s.sizes() != c.sizes() || s.scalar_type() != c.scalar_type())
+        raise(PyExc_ValueError, "split_qkv_norm_rotary: expected cos, sin [n_pos, D/2] of one dtype");
+    contig({&qg, &kg, &c, &s});
+    unit_last({&qkv, &q, &k, &v});
+    const int dt = dtype_code(qkv), gd = dtype_code(qg), td = dtype_code(c), od = dtype_code(q);
+    const double sc = number(a[10]);
+    const float scale = (float)(sc < 0 ? std::sqrt((double)D) : sc), eps = (float)number(a[11]);
+    const int64_t pos0 = integer(a[12]), n_pos = c.size(0);
+    const int64_t z[8] = {qkv.stride(0), qkv.stride(1), q.stride(0), q.stride(1), q.stride(2),
+                          k.stride(0), k.stride(1), k.stride(2)};
+    void *xp = ptr(qkv), *qgp = ptr(qg), *kgp = ptr(kg), *cp = ptr(c), *sp = ptr(s), *qp = ptr(q), *kp = ptr(k), *vp = ptr(v);
+    const c10::DeviceGuard guard(gpu({&qkv, &qg, &kg, &c, &s, &q, &k, &v}));
+    const mbrt_stream_t st = stream(a[13]);
+    return call("mbrt_split_qkv_norm_rotary", [&] {
+        return mbrt_split_qkv_norm_rotary(xp, dt, z[0], z[1], qgp, kgp, gd, cp, sp, td, n_pos, pos0, qp, kp, vp, od, z[2],
+                                          z[3], z[4], z[5], z[6], z[7], B, N, H, KV, D, scale, eps, st);
+    });
+    END_HANDLE_TH_ERRORS
+}
+
+// attention_window(q, k, v, out, left, right, sinks, q_start, key_lens | None, gate | None, gate_is_logit, scale,
+//                  workspace | None, stream), -1 for no limit and for queries at the end
+MBRT_PY(attention_window) {
+    HANDLE_TH_ERRORS
+    count(n, 14);
+    const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]), &v = tensor(a[2]), &out = tensor(a[3]);
+    const at::Tensor lens = tensor_or_none(a[8]), gate = tensor_or_none(a[9]), ws = tensor_or_none(a[12]);
+    if (q.dim() != 4 || k.dim() != 4 || k.size(0) != q.size(0) || k.size(3) != q.size(3) || v.sizes() != k.sizes())
+        raise(PyExc_ValueError, "attention_window: expected q [B, N_q, H, D] and k, v [B, N_k, H_kv, D]");
+    const int64_t B = q.size(0), nq = q.size(1), H = q.size(2), D = q.size(3), nk = k.size(1), KV = k.size(2);
+    if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
+        raise(PyExc_ValueError, "attention_window: q, k and v differ in dtype");
+    if (v.strides() != k.strides()) raise(PyExc_ValueError, "attention_window: k and v must be strided alike");
+    if (out.sizes() != q.sizes()) raise(PyExc_ValueError, "attention_window: expected out [B, N_q, H, D]");
+    if (lens.defined() && (lens.dim() != 1 || lens.size(0) != B || lens.scalar_type() != at::kInt))
+        raise(PyExc_ValueError, "attention_window: expected key_lens [B] int32");
+    if (gate.defined() && (gate.dim() != 3 || gate.size(0) != B || gate.size(1) != nq || gate.size(2) != H))
+        raise(PyExc_ValueError, "attention_window: expected gate [B, N_q, H]");
+    unit_last({&q, &k, &v, &out});
+    contig({&lens, &gate, &ws});
+    const int dt = dtype_code(q), gd = dtype_or(gate, MBRT_F32), od = dtype_code(out), logit = truth(a[10]);
+    const int64_t left = integer(a[4]), right = integer(a[5]), sinks = integer(a[6]), start = integer(a[7]);
+    const float scale = (float)number(a[11]);
+    const int64_t bytes = ws.defined() ? ws.numel() * (int64_t)ws.element_size() : 0;
+    void *qp = ptr(q), *kp = ptr(k), *vp = ptr(v), *op = ptr(out), *gp = ptr(gate), *wp = ptr(ws);
+    const int32_t* lp = static_cast<const int32_t*>(ptr(lens));
+    const c10::DeviceGuard guard(gpu({&q, &k, &v, &out, &lens, &gate, &ws}));
+    const mbrt_stream_t st = stream(a[13]);
+    return call("mbrt_attention_window", [&] {
+        return mbrt_attention_window(qp, kp, vp, dt, B, H, KV, nq, nk, D, q.stride(0), q.stride(2), q.stride(1),
+                                     k.stride(0), k.stride(2), k.stride(1), left, right, sinks, start, lp, gp, gd, logit,
+                                     op, od, out.stride(0), out.stride(2), out.stride(1), scale, wp, bytes, st);
+    });
+    END_HANDLE_TH_ERRORS
+}
+
 // stft(x [B, L], window, hop, center, normalized, out, n_fft, win_length, stream)
 MBRT_PY(stft) {
     HANDLE_TH_ERRORS
@@ -420,6 +562,7 @@ PyMethodDef kMethods[] = {
     MBRT_DEF(init), MBRT_DEF(fill), MBRT_DEF(strided_copy), MBRT_DEF(pad), MBRT_DEF(cat), MBRT_DEF(rms_norm),
     MBRT_DEF(residual_add_rms_norm), MBRT_DEF(bias_act), MBRT_DEF(glu), MBRT_DEF(gate_merge), MBRT_DEF(softmax),
     MBRT_DEF(split_qkv_rotary), MBRT_DEF(attention_ex), MBRT_DEF(stft), MBRT_DEF(istft), MBRT_DEF(chunk_accumulate),
+    MBRT_DEF(linear), MBRT_DEF(split_qkv_norm_rotary), MBRT_DEF(attention_window),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_mbrt_calls", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
