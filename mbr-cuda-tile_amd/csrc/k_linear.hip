@@ -9,7 +9,7 @@
 // contraction serves if both operands have the same.  Sums are f32; the epilogue works in f32 and rounds once,
 // on its store.
 //
-// Three forms, by shape (choose() below): tiles of 128 x 128 or 64 x 64 through LDS, and strips of 16 rows of
+// Three forms, by shape (launch() below): tiles of 64 x 64 up to 128 x 192 through LDS, and strips of 16 rows of
 // the longer operand against all of a short one (few rows, or few output columns).
 #include "abi_common.hpp"
 
@@ -22,7 +22,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kStepBytes = 128;          // of every row, per step of the tile kernel
+constexpr int kStepBytes = 128;            // of every row, per step of the tile form
 constexpr int kBufferDword3 = 0x00020000;  // raw buffer resource: 32-bit data format, no swizzle, no stride
 
 struct LinArgs {
@@ -43,6 +43,17 @@ struct LinArgs {
 // depend on one, or the host pass drops the kernel that holds it.
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t base, char* lds, uint32_t off, int step) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_void*)lds, 16, off, step, 0, 0);
+}
+
+// Until this wave's loads have landed and its LDS accesses are done (vmcnt and lgkmcnt 0).
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0070); }
+
+// A barrier without the fence of __syncthreads(), which would wait for every load under way: LDS accesses stay
+// on their side of it, and the caller has waited for its own.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 template <int DT>
@@ -80,6 +91,19 @@ __device__ __forceinline__ u32x4 row_piece(const char* row, int64_t kb, int K) {
     return v;
 }
 
+// x Phi = max(x, 0) - |x| erfc(|z|) / 2, z = s x, by Abramowitz & Stegun 7.1.26 as in one_plus_erf_as (halved
+// coefficients): 12 operations and two transcendental ones.
+__device__ __forceinline__ float gelu_short(float x, float s) {
+    const float az = fabsf(x) * s;
+    const float t = fast_rcp(fmaf(0.3275911f, az, 1.0f));
+    float p = fmaf(0.5307027145f, t, -0.7265760135f);
+    p = fmaf(p, t, 0.7107068705f);
+    p = fmaf(p, t, -0.142248368f);
+    p = fmaf(p, t, 0.127414796f);
+    p *= t * __builtin_amdgcn_exp2f(az * (az * -1.44269504088896341f));
+    return fmaf(-fabsf(x), p, fmaxf(x, 0.0f));
+}
+
 // f32 results take the library's erfc and tanh, 2-byte ones the short forms that bias_act uses for them (errors of
 // 1.5e-7 and less beside their half steps of 2^-9 and 2^-12).
 template <int NV>
@@ -92,7 +116,7 @@ __device__ __forceinline__ void activate(float (&v)[NV], int act, bool f32_out) 
             for (int i = 0; i < NV; ++i) v[i] = 0.5f * v[i] * erfcf(-v[i] * s);
         } else {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = 0.5f * v[i] * one_plus_erf_as(v[i] * s);
+            for (int i = 0; i < NV; ++i) v[i] = gelu_short(v[i], s);
         }
     } else if (act == MBRT_ACT_SIGMOID) {
 #pragma unroll
@@ -141,7 +165,7 @@ __device__ __forceinline__ void load_run(const void* p, int dt, int64_t e, float
         }
     }
 }
-template <int NV>
+template <int NT, int NV>
 __device__ __forceinline__ void store_run(void* p, int dt, int64_t e, const float (&f)[NV]) {
     static_assert(NV % 4 == 0 || NV == 1, "whole pieces, or one element");
     if constexpr (NV == 1) {
@@ -150,7 +174,7 @@ __device__ __forceinline__ void store_run(void* p, int dt, int64_t e, const floa
         char* b = reinterpret_cast<char*>(p) + 4 * e;
 #pragma unroll
         for (int q = 0; q < NV / 4; ++q)
-            st_any<0, 4>(b + 16 * q, u32x4{__float_as_uint(f[4 * q]), __float_as_uint(f[4 * q + 1]),
+            st_any<NT, 4>(b + 16 * q, u32x4{__float_as_uint(f[4 * q]), __float_as_uint(f[4 * q + 1]),
                                            __float_as_uint(f[4 * q + 2]), __float_as_uint(f[4 * q + 3])});
     } else if constexpr (NV % 8 == 0) {
         char* b = reinterpret_cast<char*>(p) + 2 * e;
@@ -161,7 +185,7 @@ __device__ __forceinline__ void store_run(void* p, int dt, int64_t e, const floa
             for (int i = 0; i < 4; ++i)
                 t[i] = dt == BF16 ? pack_bf16x2(f[8 * q + 2 * i], f[8 * q + 2 * i + 1])
                                   : pack_f16x2(f[8 * q + 2 * i], f[8 * q + 2 * i + 1]);
-            st_any<0, 2>(b + 16 * q, t);
+            st_any<NT, 2>(b + 16 * q, t);
         }
     } else {
 #pragma unroll
@@ -171,7 +195,7 @@ __device__ __forceinline__ void store_run(void* p, int dt, int64_t e, const floa
 
 // The epilogue of NV consecutive columns n .. of row m (n a multiple of NV; columns past N and rows past M
 // are not stored).  bias[] holds the columns' bias.
-template <bool ACT, int NV>
+template <bool ACT, int NT, int NV>
 __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int n, float (&v)[NV], const float (&bias)[NV]) {
     if (m >= a.M || n >= a.N) return;
 #pragma unroll
@@ -193,7 +217,7 @@ __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int n, float
     }
     const int64_t e = m * a.os + n;
     if (whole) {
-        store_run<NV>(a.out, a.odt, e, v);
+        store_run<NT, NV>(a.out, a.odt, e, v);
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -207,20 +231,26 @@ __device__ __forceinline__ void load_bias(const LinArgs& a, int n, float (&b)[NV
     for (int i = 0; i < NV; ++i) b[i] = a.bias != nullptr && n + i < a.N ? load1(a.bias, a.bdt, n + i) : 0.0f;
 }
 
-// Tile form: WM x WN waves, each with MI x NI blocks of 16 x 16, one step of 128 bytes of K at a time, two steps'
-// tiles in LDS.  An LDS row is 8 pieces of 16 bytes; piece j of a row stands at j ^ key(row), which makes the
-// eight rows that neighbouring lanes read fall on different banks.  w is the A operand: a lane's four results of a
-// block are four columns of one row of out, and block ni takes the columns 4 NI q + 4 ni + j (q = c / 4, j = c % 4) of the
-// wave's, so that a lane ends with 4 NI columns in a row.
-// DIRECT: rows are 16-byte aligned, and whole steps go from global memory straight into LDS.
-template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, bool ACT>
+// Tile form: WM x WN waves, each with MI x NI blocks of 16 x 16.  K goes by in steps of 128 bytes of every row, in
+// two LDS buffers: the next step's tiles are on their way while one is computed.  An LDS row is 8 pieces of 16 bytes; piece
+// j of a row stands at j ^ key(row), which makes the eight rows that neighbouring lanes read fall on different banks.  w is
+// the A operand: a lane's four results of a block are four columns of one row of out, and two blocks 2 p, 2 p + 1 take
+// the columns 32 p + 8 q + 4 (ni % 2) + j (q = c / 4, j = c % 4) of the wave's, so that a lane ends with 8 columns in a
+// row, and a store of 16 bytes per lane fills 64 bytes in a row of out.
+// DIRECT: rows are 16-byte aligned, and whole steps go from global memory straight into LDS.  NT: out is stored past the
+// caches: a large one would push x and w out of them.
+__device__ __forceinline__ int key_x(int r) { return r & 7; }
+__device__ __forceinline__ int key_w(int r) { return (r & 3) | (((r >> 3) & 1) << 2); }
+
+template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, int NT, bool ACT>
 __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
     constexpr int NW = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16;
     constexpr int S = DT == F32 ? 4 : 2;
-    constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW;  // 1 KB loads per wave and step
-    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole loads per wave");
-    __shared__ __attribute__((aligned(16))) char s0[(BM + BN) * kStepBytes];
-    __shared__ __attribute__((aligned(16))) char s1[(BM + BN) * kStepBytes];
+    constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW;  // loads of 1 KB, 8 rows, per wave and step
+    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NI % 2 == 0, "whole loads per wave, blocks in pairs");
+    constexpr int SB = kStepBytes, kBuf = (BM + BN) * SB;
+    __shared__ __attribute__((aligned(16))) char s0[kBuf];
+    __shared__ __attribute__((aligned(16))) char s1[kBuf];
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int w = __builtin_amdgcn_readfirstlane(tid / 64);
     const int wm = w / WN, wn = w % WN;
@@ -232,55 +262,47 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
     const char* wb = a.w + (int64_t)n0 * a.ws;
     const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
     const int64_t kbytes = (int64_t)a.K * S;
-    const int steps = (int)((kbytes + kStepBytes - 1) / kStepBytes);
-    const int whole = DIRECT ? (int)(kbytes / kStepBytes) : 0;  // steps loaded straight into LDS
+    const int steps = (int)((kbytes + SB - 1) / SB);
+    const int whole = DIRECT ? (int)(kbytes / SB) : 0;  // steps loaded straight into LDS
 
     // lane i of load u covers LDS row 8 (LX w + u) + i / 8, place i % 8; rows past the end repeat the last one
     int xr[LX], wr[LW];
     uint32_t xo[LX], wo[LW];  // within the step: byte offset of the lane's piece from xb, wb (DIRECT)
-    auto key_x = [](int r) { return r & 7; };
-    auto key_w = [](int r) { return (r & 3) | (((r / (4 * NI)) & 1) << 2); };
 #pragma unroll
     for (int u = 0; u < LX; ++u) {
-        const int r = 8 * (LX * w + u) + (lane >> 3);
+        const int r = 8 * (LX * w + u) + lane / 8;
         xr[u] = min(r, mrows - 1);
-        xo[u] = (uint32_t)xr[u] * (uint32_t)a.xs + 16u * ((lane & 7) ^ key_x(r));
+        xo[u] = (uint32_t)xr[u] * (uint32_t)a.xs + 16u * ((lane % 8) ^ key_x(r));
     }
 #pragma unroll
     for (int u = 0; u < LW; ++u) {
-        const int r = 8 * (LW * w + u) + (lane >> 3);
+        const int r = 8 * (LW * w + u) + lane / 8;
         wr[u] = min(r, nrows - 1);
-        wo[u] = (uint32_t)wr[u] * (uint32_t)a.ws + 16u * ((lane & 7) ^ key_w(r));
+        wo[u] = (uint32_t)wr[u] * (uint32_t)a.ws + 16u * ((lane % 8) ^ key_w(r));
     }
     const __amdgpu_buffer_rsrc_t xres = __builtin_amdgcn_make_buffer_rsrc((void*)xb, (short)0, -1, kBufferDword3);
     const __amdgpu_buffer_rsrc_t wres = __builtin_amdgcn_make_buffer_rsrc((void*)wb, (short)0, -1, kBufferDword3);
     auto load_direct = [&](int kt, char* d) {
 #pragma unroll
-        for (int u = 0; u < LX; ++u)
-            load_to_lds(xres, d + 1024 * (LX * w + u), xo[u], kt * kStepBytes);
+        for (int u = 0; u < LX; ++u) load_to_lds(xres, d + 1024 * (LX * w + u), xo[u], kt * SB);
 #pragma unroll
-        for (int u = 0; u < LW; ++u)
-            load_to_lds(wres, d + BM * kStepBytes + 1024 * (LW * w + u), wo[u], kt * kStepBytes);
+        for (int u = 0; u < LW; ++u) load_to_lds(wres, d + BM * SB + 1024 * (LW * w + u), wo[u], kt * SB);
     };
+    // a step that is cut by the end of the rows, or of rows at other alignments: through registers
     u32x4 px[LX], pw[LW];
     auto load_regs = [&](int kt) {
 #pragma unroll
-        for (int u = 0; u < LX; ++u) {
-            const int r = 8 * (LX * w + u) + (lane >> 3);
-            px[u] = row_piece<DT, DIRECT>(xb + xr[u] * a.xs, (int64_t)kt * kStepBytes + 16 * ((lane & 7) ^ key_x(r)), a.K);
-        }
+        for (int u = 0; u < LX; ++u)
+            px[u] = row_piece<DT, DIRECT>(xb + xr[u] * a.xs, (int64_t)kt * SB + 16 * ((lane % 8) ^ key_x(8 * (LX * w + u) + lane / 8)), a.K);
 #pragma unroll
-        for (int u = 0; u < LW; ++u) {
-            const int r = 8 * (LW * w + u) + (lane >> 3);
-            pw[u] = row_piece<DT, DIRECT>(wb + wr[u] * a.ws, (int64_t)kt * kStepBytes + 16 * ((lane & 7) ^ key_w(r)), a.K);
-        }
+        for (int u = 0; u < LW; ++u)
+            pw[u] = row_piece<DT, DIRECT>(wb + wr[u] * a.ws, (int64_t)kt * SB + 16 * ((lane % 8) ^ key_w(8 * (LW * w + u) + lane / 8)), a.K);
     };
     auto put_regs = [&](char* d) {
 #pragma unroll
         for (int u = 0; u < LX; ++u) *reinterpret_cast<u32x4*>(d + 1024 * (LX * w + u) + 16 * lane) = px[u];
 #pragma unroll
-        for (int u = 0; u < LW; ++u)
-            *reinterpret_cast<u32x4*>(d + BM * kStepBytes + 1024 * (LW * w + u) + 16 * lane) = pw[u];
+        for (int u = 0; u < LW; ++u) *reinterpret_cast<u32x4*>(d + BM * SB + 1024 * (LW * w + u) + 16 * lane) = pw[u];
     };
 
     f32x4 acc[MI][NI];
@@ -289,137 +311,166 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
 #pragma unroll
         for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int xrow = (wm * MI * 16 + c) * kStepBytes;
-    const int wrow = BM * kStepBytes + (wn * NI * 16 + 4 * NI * (c >> 2) + (c & 3)) * kStepBytes;
+    const int xrow = (wm * MI * 16 + c) * SB;
+    const int wrow = BM * SB + (wn * NI * 16 + 8 * (c >> 2) + (c & 3)) * SB;
     auto compute = [&](const char* d) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < SB / 64; ++s) {
             const int piece = 16 * ((4 * s + g) ^ (c & 7));
             u32x4 xf[MI], wf[NI];
 #pragma unroll
-            for (int mi = 0; mi < MI; ++mi) xf[mi] = *reinterpret_cast<const u32x4*>(d + xrow + mi * 16 * kStepBytes + piece);
+            for (int mi = 0; mi < MI; ++mi) xf[mi] = *reinterpret_cast<const u32x4*>(d + xrow + mi * 16 * SB + piece);
 #pragma unroll
-            for (int ni = 0; ni < NI; ++ni) wf[ni] = *reinterpret_cast<const u32x4*>(d + wrow + ni * 4 * kStepBytes + piece);
+            for (int ni = 0; ni < NI; ++ni) wf[ni] = *reinterpret_cast<const u32x4*>(d + wrow + (32 * (ni / 2) + 4 * (ni % 2)) * SB + piece);
 #pragma unroll
             for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
                 for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = mma<DT>(wf[ni], xf[mi], acc[mi][ni]);
         }
     };
-    // Step kt sits in d; the next one is loaded into dn meanwhile.  The two buffers are separate objects and the
-    // loop is unrolled by two, so that the compiler sees that loads in flight into one do not touch the other.
-    auto step = [&](int kt, const char* d, char* dn) {
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of the step have landed
-        __syncthreads();                     // every wave's have, and none still reads dn
-        const bool next = kt + 1 < steps, direct = DIRECT && kt + 1 < whole;
-        if (direct) load_direct(kt + 1, dn);
-        else if (next) load_regs(kt + 1);
-        compute(d);
-        if (next && !direct) put_regs(dn);
-    };
-    if (DIRECT && whole > 0) {
-        load_direct(0, s0);
+    if constexpr (DIRECT) {
+        // The column tiles of one row tile run side by side and read the same rows of x.  Where they are few, each begins at
+        // another step and goes round, so that together they have more of the rows on their way from memory at
+        // once (bf16 [48060, 1536] -> 384, two tiles: 97 -> 93 us); many of them run apart by themselves, and going round
+        // then costs reuse ([4096, 4096] -> 4096: 127 -> 146).
+        const int first = a.ntiles <= 4 ? (int)((int64_t)(tile % a.ntiles) * whole / a.ntiles) : 0;
+        auto at = [&](int kt) { return kt + first < whole ? kt + first : kt + first - whole; };
+        // Step kt sits in d, the next one goes to dn, which held step kt - 1.  The buffers are separate objects and the
+        // loop is unrolled by two, so that the compiler sees that loads in flight into one do not touch the other.
+        auto step = [&](int kt, const char* d, char* dn) {
+            wait_loads();
+            lds_barrier();  // every wave's loads have landed, and none still reads dn
+            if (kt + 1 < whole) load_direct(at(kt + 1), dn);
+            compute(d);
+        };
+        if (whole > 0) load_direct(at(0), s0);
+        for (int kt = 0; kt < whole; kt += 2) {
+            step(kt, s0, s1);
+            if (kt + 1 < whole) step(kt + 1, s1, s0);
+        }
+        if (steps > whole) {
+            load_regs(whole);
+            __syncthreads();  // none still reads s0
+            put_regs(s0);
+            __syncthreads();
+            compute(s0);
+        }
     } else {
+        // through registers: the next step's loads are issued before a step is computed and written to LDS after it
         load_regs(0);
         put_regs(s0);
-    }
-    for (int kt = 0; kt < steps; kt += 2) {
-        step(kt, s0, s1);
-        if (kt + 1 < steps) step(kt + 1, s1, s0);
+        for (int kt = 0; kt < steps; kt += 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (kt + i < steps) {
+                    __syncthreads();  // the step is in LDS, and none still reads the other buffer
+                    const bool next = kt + i + 1 < steps;
+                    if (next) load_regs(kt + i + 1);
+                    compute(i == 0 ? s0 : s1);
+                    if (next) put_regs(i == 0 ? s1 : s0);
+                }
+            }
+        }
     }
 
-    const int n = n0 + wn * NI * 16 + 4 * NI * g;
-    float bias[4 * NI];
-    load_bias<4 * NI>(a, n, bias);
+    const int n = n0 + wn * NI * 16 + 8 * g;
+    float bias[NI / 2][8];
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-        float v[4 * NI];
+    for (int p = 0; p < NI / 2; ++p) load_bias<8>(a, n + 32 * p, bias[p]);
 #pragma unroll
-        for (int ni = 0; ni < NI; ++ni)
+    for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * ni + i] = acc[mi][ni][i];
-        finish<ACT, 4 * NI>(a, m0 + wm * MI * 16 + mi * 16 + c, n, v, bias);
-    }
+        for (int p = 0; p < NI / 2; ++p) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = acc[mi][2 * p + i / 4][i % 4];
+            finish<ACT, NT, 8>(a, m0 + wm * MI * 16 + mi * 16 + c, n + 32 * p, v, bias[p]);
+        }
 }
 
-// Strip form: a wave takes 16 rows of the longer operand and every row of the shorter (16 R at most), straight from
-// global memory into the matrix instructions.  `split` waves of a block share a strip's K, two 64-byte pieces at
-// a time in turn, and are added through LDS in wave order.
-// WIDE: strips of w against few rows of x (a lane ends with 4 columns of a row); else strips of x against few
-// columns (4 rows of a column).
+// Strip form: a wave takes 16 rows of one operand and 16 R of the other, straight from global memory into the matrix
+// instructions; `split` waves of a block share the K of one such piece, 128 bytes of every row at a time in turn, and are
+// added through LDS in wave order.  Nothing but the loads' latency, once or twice, stands between a small call's launch and
+// its stores.
+// WIDE: strips of w (16 columns of out) against groups of 16 R rows of x; else strips of x against groups of 16 R columns.
+// The groups of one strip are neighbours.
 template <int DT, int R, bool WIDE, bool ALIGNED>
 __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
     constexpr int S = DT == F32 ? 4 : 2;
-    extern __shared__ f32x4 part[];  // [strips of the block][split - 1][R][64]
+    extern __shared__ f32x4 part[];  // [strips of the block][split][R][64]
     const int lane = threadIdx.x % 64, g = lane / 16, c = lane % 16;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int ks = w % a.split, strip = w / a.split;
-    const int64_t p0 = ((int64_t)blockIdx.x * (blockDim.x / 64 / a.split) + strip) * 16;
-    const int64_t P = WIDE ? a.N : a.M;
-    const int Q = WIDE ? (int)a.M : a.N;
-    const char* pb = (WIDE ? a.w : a.x) + min(p0 + c, P - 1) * (WIDE ? a.ws : a.xs);
+    const int64_t p0 = ((int64_t)(blockIdx.x / a.ntiles) * (blockDim.x / 64 / a.split) + strip) * 16;
+    const int64_t q0 = (int64_t)(blockIdx.x % a.ntiles) * 16 * R;
+    const int64_t P = WIDE ? a.N : a.M, Q = WIDE ? a.M : a.N;
+    const char* pb = (WIDE ? a.w : a.x) + min(p0 + c, P - 1) * (WIDE ? a.ws : a.xs) + 16 * g;
     const char* qb[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) qb[r] = (WIDE ? a.x : a.w) + (int64_t)min(16 * r + c, Q - 1) * (WIDE ? a.xs : a.ws);
+    for (int r = 0; r < R; ++r) qb[r] = (WIDE ? a.x : a.w) + min(q0 + 16 * r + c, Q - 1) * (WIDE ? a.xs : a.ws) + 16 * g;
     const int64_t kbytes = (int64_t)a.K * S;
-    const int pairs = (int)((kbytes + 127) / 128);
+    const int whole = (int)(kbytes / 128);
 
     f32x4 acc[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int U = R >= 4 ? 2 : 4;  // pairs in flight
-    for (int t0 = ks; t0 < pairs; t0 += U * a.split) {
+    // U pieces of 128 bytes, all loads before the first product (a lane's loads are whole: no checks)
+    auto pieces = [&](auto count, int t0) {
+        constexpr int U = decltype(count)::value;
         u32x4 pf[U][2], qf[U][2][R];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int t = t0 + u * a.split;
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const int64_t kb = (int64_t)t * 128 + 64 * s + 16 * g;
-                pf[u][s] = row_piece<DT, ALIGNED>(pb, kb, a.K);
+                const int64_t kb = (int64_t)(t0 + u * a.split) * 128 + 64 * s;
+                pf[u][s] = ALIGNED ? *reinterpret_cast<const u32x4*>(pb + kb) : ld_any<0, S>(pb + kb);
 #pragma unroll
-                for (int r = 0; r < R; ++r) qf[u][s][r] = row_piece<DT, ALIGNED>(qb[r], kb, a.K);
+                for (int r = 0; r < R; ++r) qf[u][s][r] = ALIGNED ? *reinterpret_cast<const u32x4*>(qb[r] + kb) : ld_any<0, S>(qb[r] + kb);
             }
-        }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int r = 0; r < R; ++r) acc[r] = mma<DT>(pf[u][s], qf[u][s][r], acc[r]);
-    }
-    if (a.split > 1) {
-        f32x4* mine = part + (int64_t)strip * (a.split - 1) * R * 64;
-        if (ks > 0) {
+                for (int r = 0; r < R; ++r)
+                    acc[r] = WIDE ? mma<DT>(pf[u][s], qf[u][s][r], acc[r]) : mma<DT>(qf[u][s][r], pf[u][s], acc[r]);
+    };
+    constexpr int U = R >= 4 ? 2 : R == 2 ? 3 : 6;
+    int t0 = ks;
+    for (; t0 + (U - 1) * a.split < whole; t0 += U * a.split) pieces(std::integral_constant<int, U>(), t0);
+    for (; t0 < whole; t0 += a.split) pieces(std::integral_constant<int, 1>(), t0);
+    if (t0 == whole && kbytes > (int64_t)whole * 128) {  // this wave's turn at the piece that the rows' end cuts
 #pragma unroll
-            for (int r = 0; r < R; ++r) mine[((ks - 1) * R + r) * 64 + lane] = acc[r];
-        }
-        __syncthreads();
-        if (ks > 0) return;
-        for (int k = 0; k < a.split - 1; ++k)
+        for (int s = 0; s < 2; ++s) {
+            const int64_t kb = (int64_t)whole * 128 + 64 * s + 16 * g;
+            const u32x4 pf = row_piece<DT, ALIGNED>(pb - 16 * g, kb, a.K);
 #pragma unroll
-            for (int r = 0; r < R; ++r) acc[r] += mine[(k * R + r) * 64 + lane];
-    }
-    if constexpr (WIDE) {
-        const int n = (int)min<int64_t>(p0 + 4 * g, P);
-        float bias[4];
-        load_bias<4>(a, n, bias);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float v[4] = {acc[r][0], acc[r][1], acc[r][2], acc[r][3]};
-            finish<true, 4>(a, 16 * r + c, n, v, bias);
-        }
-    } else {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float bias[1];
-            load_bias<1>(a, 16 * r + c, bias);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v[1] = {acc[r][i]};
-                finish<true, 1>(a, p0 + 4 * g + i, 16 * r + c, v, bias);
+            for (int r = 0; r < R; ++r) {
+                const u32x4 qf = row_piece<DT, ALIGNED>(qb[r] - 16 * g, kb, a.K);
+                acc[r] = WIDE ? mma<DT>(pf, qf, acc[r]) : mma<DT>(qf, pf, acc[r]);
             }
         }
+    }
+    // w is the A operand: a lane holds four columns of one row
+    auto finish_block = [&](int r, const f32x4& s) {
+        const int64_t n = min<int64_t>(WIDE ? p0 + 4 * g : q0 + 16 * r + 4 * g, a.N);
+        float bias[4], v[4] = {s[0], s[1], s[2], s[3]};
+        load_bias<4>(a, (int)n, bias);
+        finish<true, 0, 4>(a, WIDE ? q0 + 16 * r + c : p0 + c, (int)n, v, bias);
+    };
+    if (a.split == 1) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) finish_block(r, acc[r]);
+        return;
+    }
+    f32x4* all = part + (int64_t)strip * a.split * R * 64 + lane;
+#pragma unroll
+    for (int r = 0; r < R; ++r) all[(ks * R + r) * 64] = acc[r];
+    __syncthreads();
+    for (int r = ks; r < R; r += a.split) {
+        f32x4 s = all[r * 64];
+        for (int k = 1; k < a.split; ++k) s += all[(k * R + r) * 64];
+        finish_block(r, s);
     }
 }
 
@@ -431,7 +482,7 @@ __global__ __launch_bounds__(256) void linear_empty_kernel(LinArgs a) {
         const int n = (int)(i - m * a.N);
         float v[1] = {0.0f}, bias[1];
         load_bias<1>(a, n, bias);
-        finish<true, 1>(a, m, n, v, bias);
+        finish<true, 0, 1>(a, m, n, v, bias);
     }
 }
 
@@ -443,14 +494,18 @@ void launch_strip(const LinArgs& a, bool wide, bool al, unsigned blocks, unsigne
     else hipLaunchKernelGGL((linear_strip_kernel<DT, R, false, false>), dim3(blocks), dim3(threads), lds, st, a);
 }
 
-template <int DT, int WM, int WN, int MI, int NI>
-void launch_tile(const LinArgs& a, bool direct, unsigned tiles, hipStream_t st) {
-    const dim3 grid(tiles), block(WM * WN * 64);
-    const bool act = a.act != MBRT_ACT_NONE;
-    if (direct && act) hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, true, true>), grid, block, 0, st, a);
-    else if (direct) hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, true, false>), grid, block, 0, st, a);
-    else if (act) hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, false, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, false, false>), grid, block, 0, st, a);
+template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, int NT>
+int launch_tile(LinArgs& a, hipStream_t st) {
+    constexpr int BM = WM * MI * 16, BN = WN * NI * 16;
+    a.ntiles = (uint32_t)ceil_div(a.N, BN);
+    const int64_t tiles = ceil_div(a.M, BM) * a.ntiles;
+    if (tiles >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many tiles");
+    const dim3 grid((unsigned)tiles), block(WM * WN * 64);
+    if (a.act != MBRT_ACT_NONE)
+        hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, DIRECT, NT, true>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, DIRECT, NT, false>), grid, block, 0, st, a);
+    return MBRT_OK;
 }
 
 template <int DT>
@@ -458,17 +513,24 @@ int launch(LinArgs& a, bool al, hipStream_t st) {
     const int64_t es = DT == F32 ? 4 : 2, cus = cu_count();
     const bool wide = a.M <= a.N;
     const int64_t shorter = wide ? a.M : a.N, longer = wide ? a.N : a.M;
-    if (shorter <= 64) {
-        const int R = shorter <= 16 ? 1 : shorter <= 32 ? 2 : 4;
-        const int64_t strips = ceil_div(longer, 16), pairs = ceil_div(a.K * es, 128);
-        int split = 1;
-        while (split < 16 && 2 * split <= pairs && strips * split < 8 * cus) split *= 2;
-        a.split = split;
-        const int per_block = std::max(1, 4 / split);
-        const int64_t blocks = ceil_div(strips, per_block);
+    const int64_t strips = ceil_div(longer, 16);
+    // Strips, where one operand is short, or where tiles would leave CUs idle; of as few rows per wave as there are CUs
+    // for.  Rows at odd alignments, which tiles take through registers step by step, go in strips up to twice as
+    // far, spread eight times as wide.  us, tiles and strips: bf16 [200, 1536] -> 384 8.5 and 7.0, f32 31 and 11.3; [120,
+    // 1536] -> 384 9.0 and 5.8, f32 31 and 8.2; [801, 384] -> 384 4.6 and 7.0; [801, 118] -> 384 6.2 and 5.0, f32 7.0 and 5.2.
+    if (shorter <= 64 || strips * ceil_div(shorter, 64) <= (al ? 1 : 2) * cus) {
+        int R = shorter <= 16 ? 1 : shorter <= 32 ? 2 : 4;
+        while (R > 1 && strips * ceil_div(shorter, 8 * R) <= (al ? 1 : 8) * cus) R /= 2;
+        const int64_t groups = ceil_div(shorter, 16 * R), pairs = ceil_div(a.K * es, 128);
+        // waves to a strip's K: as many as find room side by side, each with the same number of turns
+        const int64_t room = std::max<int64_t>(1, std::min<int64_t>(16, 8 * cus / (strips * groups)));
+        a.split = (int)ceil_div(pairs, ceil_div(pairs, room));
+        a.ntiles = (uint32_t)groups;
+        const int per_block = std::max(1, 4 / a.split);
+        const int64_t blocks = ceil_div(strips, per_block) * groups;
         if (blocks >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many rows");
-        const size_t lds = (size_t)per_block * (split - 1) * R * 1024;
-        const unsigned threads = per_block * split * 64;
+        const size_t lds = a.split == 1 ? 0 : (size_t)per_block * a.split * R * 1024;
+        const unsigned threads = per_block * a.split * 64;
         if (R == 1) launch_strip<DT, 1>(a, wide, al, (unsigned)blocks, threads, lds, st);
         else if (R == 2) launch_strip<DT, 2>(a, wide, al, (unsigned)blocks, threads, lds, st);
         else launch_strip<DT, 4>(a, wide, al, (unsigned)blocks, threads, lds, st);
@@ -476,14 +538,16 @@ int launch(LinArgs& a, bool al, hipStream_t st) {
     }
     // 32-bit offsets within a tile
     const bool direct = al && a.xs < (int64_t(1) << 22) && a.ws < (int64_t(1) << 22);
-    const bool big = ceil_div(a.M, 128) * ceil_div(a.N, 128) >= cus;
-    const int64_t bm = big ? 128 : 64;
-    a.ntiles = (uint32_t)ceil_div(a.N, bm);
-    const int64_t tiles = ceil_div(a.M, bm) * a.ntiles;
-    if (tiles >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many tiles");
-    if (big) launch_tile<DT, 2, 2, 4, 4>(a, direct, (unsigned)tiles, st);
-    else launch_tile<DT, 2, 2, 2, 2>(a, direct, (unsigned)tiles, st);
-    return MBRT_OK;
+    // Large tiles, two workgroups to a CU, once there are enough of them; of two heights the one whose rounds over the
+    // CUs take fewer rows (the larger at a tie, for its reuse).  bf16 us, 96 and 128 rows: [48060, 384] -> 1536, 8 and 6
+    // rounds, 79 and 70; [48060, 1536] -> 384, 2 and 2 rounds, 93 and 95; [48060, 512] -> 384 43 and 51; [4096, 4096]
+    // -> 4096, 2 and 2, 127 and 137.
+    auto rounds = [&](int64_t bm, int64_t bn) { return ceil_div(ceil_div(a.M, bm) * ceil_div(a.N, bn), 2 * cus); };
+    const bool big = ceil_div(a.M, 96) * ceil_div(a.N, 192) >= cus;
+    if (!direct) return big ? launch_tile<DT, 2, 2, 4, 4, false, 2>(a, st) : launch_tile<DT, 2, 2, 2, 2, false, 0>(a, st);
+    if (!big) return launch_tile<DT, 2, 2, 2, 2, true, 0>(a, st);
+    return 96 * rounds(96, 192) < 128 * rounds(128, 192) ? launch_tile<DT, 2, 2, 3, 6, true, 2>(a, st)
+                                                         : launch_tile<DT, 2, 2, 4, 6, true, 2>(a, st);
 }
 
 }  // namespace
