@@ -37,6 +37,8 @@ struct LinArgs {
     int bdt, rdt, odt, act;
     uint32_t ntiles;         // tiles along N
     int split;               // strips: waves that share a strip's K
+    int per_block;           // strips of a block
+    FastDiv groups, splits;  // ntiles and split
 };
 
 // 16 bytes per lane from base + off + step straight to lds + 16 lane.  Not a template: the builtin's operands must not
@@ -193,13 +195,43 @@ __device__ __forceinline__ void store_run(void* p, int dt, int64_t e, const floa
     }
 }
 
-// The epilogue of NV consecutive columns n .. of row m (n a multiple of NV; columns past N and rows past M
-// are not stored).  bias[] holds the columns' bias.
-template <bool ACT, int NT, int NV>
-__device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int n, float (&v)[NV], const float (&bias)[NV]) {
-    if (m >= a.M || n >= a.N) return;
+// The bias of NV consecutive columns n .. as it stands in memory, turned into f32 where it is used, so that nothing waits
+// for it before (columns past N: the last one's; they are not stored).
+template <int NV>
+struct Bias {
+    uint32_t w[NV];
+    __device__ __forceinline__ void load(const LinArgs& a, int n) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] += bias[i];
+        for (int i = 0; i < NV; ++i) w[i] = 0;
+        if (a.bias == nullptr) return;
+        if (a.bdt == F32) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) w[i] = reinterpret_cast<const uint32_t*>(a.bias)[min(n + i, a.N - 1)];
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) w[i] = reinterpret_cast<const uint16_t*>(a.bias)[min(n + i, a.N - 1)];
+        }
+    }
+    __device__ __forceinline__ void add_to(const LinArgs& a, float (&v)[NV]) const {
+        if (a.bias == nullptr) return;
+        if (a.bdt == F32) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += __uint_as_float(w[i]);
+        } else if (a.bdt == BF16) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += bf16_lo(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += (float)__builtin_bit_cast(_Float16, (uint16_t)w[i]);
+        }
+    }
+};
+
+// The epilogue of NV consecutive columns n .. of row m (columns past N and rows past M are not stored).
+template <bool ACT, int NT, int NV>
+__device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int n, float (&v)[NV], const Bias<NV>& bias) {
+    if (m >= a.M || n >= a.N) return;
+    bias.add_to(a, v);
     if constexpr (ACT) activate<NV>(v, a.act, a.odt == F32);
     const bool whole = n + NV <= a.N;
     if (a.res != nullptr) {
@@ -223,12 +255,6 @@ __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int n, float
         for (int i = 0; i < NV; ++i)
             if (n + i < a.N) store1(a.out, a.odt, e + i, v[i]);
     }
-}
-
-template <int NV>
-__device__ __forceinline__ void load_bias(const LinArgs& a, int n, float (&b)[NV]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) b[i] = a.bias != nullptr && n + i < a.N ? load1(a.bias, a.bdt, n + i) : 0.0f;
 }
 
 // Tile form: WM x WN waves, each with MI x NI blocks of 16 x 16.  K goes by in steps of 128 bytes of every row, in
@@ -256,8 +282,10 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
     const int wm = w / WN, wn = w % WN;
     // column tiles of one row tile are neighbours, on one XCD: x is read once into its L2
     const uint32_t tile = xcd_tile(blockIdx.x, gridDim.x);
-    const int64_t m0 = (int64_t)(tile / a.ntiles) * BM;
-    const int n0 = (int)(tile % a.ntiles) * BN;
+    uint32_t mt, nt;
+    fdivmod(tile, a.groups, mt, nt);
+    const int64_t m0 = (int64_t)mt * BM;
+    const int n0 = (int)nt * BN;
     const char* xb = a.x + m0 * a.xs;
     const char* wb = a.w + (int64_t)n0 * a.ws;
     const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
@@ -333,7 +361,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
         // another step and goes round, so that together they have more of the rows on their way from memory at
         // once (bf16 [48060, 1536] -> 384, two tiles: 97 -> 93 us); many of them run apart by themselves, and going round
         // then costs reuse ([4096, 4096] -> 4096: 127 -> 146).
-        const int first = a.ntiles <= 4 ? (int)((int64_t)(tile % a.ntiles) * whole / a.ntiles) : 0;
+        const int first = a.ntiles <= 4 ? (int)(nt * (uint32_t)whole / a.ntiles) : 0;
         auto at = [&](int kt) { return kt + first < whole ? kt + first : kt + first - whole; };
         // Step kt sits in d, the next one goes to dn, which held step kt - 1.  The buffers are separate objects and the
         // loop is unrolled by two, so that the compiler sees that loads in flight into one do not touch the other.
@@ -374,9 +402,9 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
     }
 
     const int n = n0 + wn * NI * 16 + 8 * g;
-    float bias[NI / 2][8];
+    Bias<8> bias[NI / 2];
 #pragma unroll
-    for (int p = 0; p < NI / 2; ++p) load_bias<8>(a, n + 32 * p, bias[p]);
+    for (int p = 0; p < NI / 2; ++p) bias[p].load(a, n + 32 * p);
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
@@ -400,9 +428,11 @@ __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
     extern __shared__ f32x4 part[];  // [strips of the block][split][R][64]
     const int lane = threadIdx.x % 64, g = lane / 16, c = lane % 16;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int ks = w % a.split, strip = w / a.split;
-    const int64_t p0 = ((int64_t)(blockIdx.x / a.ntiles) * (blockDim.x / 64 / a.split) + strip) * 16;
-    const int64_t q0 = (int64_t)(blockIdx.x % a.ntiles) * 16 * R;
+    uint32_t strip, kw, sb, group;
+    fdivmod((uint32_t)w, a.splits, strip, kw);
+    fdivmod(blockIdx.x, a.groups, sb, group);
+    const int ks = (int)kw;
+    const int64_t p0 = ((int64_t)sb * a.per_block + strip) * 16, q0 = (int64_t)group * 16 * R;
     const int64_t P = WIDE ? a.N : a.M, Q = WIDE ? a.M : a.N;
     const char* pb = (WIDE ? a.w : a.x) + min(p0 + c, P - 1) * (WIDE ? a.ws : a.xs) + 16 * g;
     const char* qb[R];
@@ -410,6 +440,11 @@ __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
     for (int r = 0; r < R; ++r) qb[r] = (WIDE ? a.x : a.w) + min(q0 + 16 * r + c, Q - 1) * (WIDE ? a.xs : a.ws) + 16 * g;
     const int64_t kbytes = (int64_t)a.K * S;
     const int whole = (int)(kbytes / 128);
+    // w is the A operand: a lane ends with four columns n .. of one row of each block; the bias of the first block that
+    // this wave finishes is on its way beside the rows
+    auto column = [&](int r) { return (int)min<int64_t>(WIDE ? p0 + 4 * g : q0 + 16 * r + 4 * g, a.N); };
+    Bias<4> bias;
+    bias.load(a, column(a.split == 1 ? 0 : min(ks, R - 1)));
 
     f32x4 acc[R];
 #pragma unroll
@@ -451,16 +486,16 @@ __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
             }
         }
     }
-    // w is the A operand: a lane holds four columns of one row
     auto finish_block = [&](int r, const f32x4& s) {
-        const int64_t n = min<int64_t>(WIDE ? p0 + 4 * g : q0 + 16 * r + 4 * g, a.N);
-        float bias[4], v[4] = {s[0], s[1], s[2], s[3]};
-        load_bias<4>(a, (int)n, bias);
-        finish<true, 0, 4>(a, WIDE ? q0 + 16 * r + c : p0 + c, (int)n, v, bias);
+        float v[4] = {s[0], s[1], s[2], s[3]};
+        finish<true, 0, 4>(a, WIDE ? q0 + 16 * r + c : p0 + c, column(r), v, bias);
     };
     if (a.split == 1) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) finish_block(r, acc[r]);
+        for (int r = 0; r < R; ++r) {
+            if (r > 0 && !WIDE) bias.load(a, column(r));
+            finish_block(r, acc[r]);
+        }
         return;
     }
     f32x4* all = part + (int64_t)strip * a.split * R * 64 + lane;
@@ -470,6 +505,7 @@ __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
     for (int r = ks; r < R; r += a.split) {
         f32x4 s = all[r * 64];
         for (int k = 1; k < a.split; ++k) s += all[(k * R + r) * 64];
+        if (r > ks && !WIDE) bias.load(a, column(r));
         finish_block(r, s);
     }
 }
@@ -480,8 +516,9 @@ __global__ __launch_bounds__(256) void linear_empty_kernel(LinArgs a) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t m = i / a.N;
         const int n = (int)(i - m * a.N);
-        float v[1] = {0.0f}, bias[1];
-        load_bias<1>(a, n, bias);
+        float v[1] = {0.0f};
+        Bias<1> bias;
+        bias.load(a, n);
         finish<true, 0, 1>(a, m, n, v, bias);
     }
 }
@@ -498,6 +535,7 @@ template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, int NT>
 int launch_tile(LinArgs& a, hipStream_t st) {
     constexpr int BM = WM * MI * 16, BN = WN * NI * 16;
     a.ntiles = (uint32_t)ceil_div(a.N, BN);
+    a.groups = make_fastdiv(a.ntiles);
     const int64_t tiles = ceil_div(a.M, BM) * a.ntiles;
     if (tiles >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many tiles");
     const dim3 grid((unsigned)tiles), block(WM * WN * 64);
@@ -527,6 +565,9 @@ int launch(LinArgs& a, bool al, hipStream_t st) {
         a.split = (int)ceil_div(pairs, ceil_div(pairs, room));
         a.ntiles = (uint32_t)groups;
         const int per_block = std::max(1, 4 / a.split);
+        a.per_block = per_block;
+        a.groups = make_fastdiv((uint32_t)groups);
+        a.splits = make_fastdiv((uint32_t)a.split);
         const int64_t blocks = ceil_div(strips, per_block) * groups;
         if (blocks >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many rows");
         const size_t lds = a.split == 1 ? 0 : (size_t)per_block * a.split * R * 1024;

@@ -17,6 +17,7 @@
 #include <torch/csrc/utils/object_ptr.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -354,13 +355,24 @@ MBRT_PY(attention_ex) {
     END_HANDLE_TH_ERRORS
 }
 
-// The device of these tensors, which a call is made on.
-at::Device gpu(std::initializer_list<const at::Tensor*> ts) {
-    const at::Device dev = (*ts.begin())->device();
-    for (const at::Tensor* t : ts)
-        if (t->defined() && (!t->is_cuda() || t->device() != dev)) raise(PyExc_ValueError, "mbrt: expected tensors on one GPU");
-    return dev;
-}
+// A call on the device of these tensors, which becomes the current one where it is not.
+class OnDevice {
+public:
+    explicit OnDevice(std::initializer_list<const at::Tensor*> ts) : dev_((*ts.begin())->device()) {
+        for (const at::Tensor* t : ts)
+            if (t->defined() && (!t->is_cuda() || t->device() != dev_))
+                raise(PyExc_ValueError, "mbrt: expected tensors on one GPU");
+        if (dev_.index() != c10::hip::current_device()) guard_.reset_device(dev_);
+    }
+    mbrt_stream_t stream(PyObject* o) const {
+        if (o == Py_None) return c10::hip::getCurrentHIPStream(dev_.index()).stream();
+        return reinterpret_cast<mbrt_stream_t>(static_cast<uintptr_t>(integer(o)));
+    }
+
+private:
+    at::Device dev_;
+    c10::OptionalDeviceGuard guard_;
+};
 
 void unit_last(std::initializer_list<const at::Tensor*> ts) {
     for (const at::Tensor* t : ts)
@@ -407,8 +419,8 @@ MBRT_PY(linear) {
     const int dt = dtype_code(x), bd = dtype_or(b, MBRT_F32), rd = dtype_or(res, MBRT_F32), od = dtype_code(out);
     const int act = (int)integer(a[4]);
     void *xp = ptr(x), *wp = ptr(w), *bp = ptr(b), *rp = ptr(res), *op = ptr(out);
-    const c10::DeviceGuard guard(gpu({&x, &w, &b, &res, &out}));
-    const mbrt_stream_t st = stream(a[6]);
+    const OnDevice on({&x, &w, &b, &res, &out});
+    const mbrt_stream_t st = on.stream(a[6]);
     return call("mbrt_linear",
                 [&] { return mbrt_linear(xp, dt, xs, wp, ws, bp, bd, rp, rd, rs, op, od, os, rows, K, N, act, st); });
     END_HANDLE_TH_ERRORS
@@ -448,8 +460,8 @@ MBRT_PY(split_qkv_norm_rotary) {
     const int64_t z[8] = {qkv.stride(0), qkv.stride(1), q.stride(0), q.stride(1), q.stride(2),
                           k.stride(0), k.stride(1), k.stride(2)};
     void *xp = ptr(qkv), *qgp = ptr(qg), *kgp = ptr(kg), *cp = ptr(c), *sp = ptr(s), *qp = ptr(q), *kp = ptr(k), *vp = ptr(v);
-    const c10::DeviceGuard guard(gpu({&qkv, &qg, &kg, &c, &s, &q, &k, &v}));
-    const mbrt_stream_t st = stream(a[13]);
+    const OnDevice on({&qkv, &qg, &kg, &c, &s, &q, &k, &v});
+    const mbrt_stream_t st = on.stream(a[13]);
     return call("mbrt_split_qkv_norm_rotary", [&] {
         return mbrt_split_qkv_norm_rotary(xp, dt, z[0], z[1], qgp, kgp, gd, cp, sp, td, n_pos, pos0, qp, kp, vp, od, z[2],
                                           z[3], z[4], z[5], z[6], z[7], B, N, H, KV, D, scale, eps, st);
@@ -483,8 +495,8 @@ MBRT_PY(attention_window) {
     const int64_t bytes = ws.defined() ? ws.numel() * (int64_t)ws.element_size() : 0;
     void *qp = ptr(q), *kp = ptr(k), *vp = ptr(v), *op = ptr(out), *gp = ptr(gate), *wp = ptr(ws);
     const int32_t* lp = static_cast<const int32_t*>(ptr(lens));
-    const c10::DeviceGuard guard(gpu({&q, &k, &v, &out, &lens, &gate, &ws}));
-    const mbrt_stream_t st = stream(a[13]);
+    const OnDevice on({&q, &k, &v, &out, &lens, &gate, &ws});
+    const mbrt_stream_t st = on.stream(a[13]);
     return call("mbrt_attention_window", [&] {
         return mbrt_attention_window(qp, kp, vp, dt, B, H, KV, nq, nk, D, q.stride(0), q.stride(2), q.stride(1),
                                      k.stride(0), k.stride(2), k.stride(1), left, right, sinks, start, lp, gp, gd, logit,
