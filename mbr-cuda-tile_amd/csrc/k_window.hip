@@ -6,8 +6,7 @@
 // Query rows: the H / H_kv query heads that share a key head are rows of one matrix, row r = (query r / G, head
 // r % G), so that each key and value is read once for all of them.
 // Keys: what the rows of a tile may see is one list, the sinks before the window and then the window's keys lo .. hi
-// of all its rows: t -> j = t < s ? t : lo + t - s, with s <= lo, which loads by rows and never touches a
-// key outside.  Whatever stands in keys that no row of the tile sees (NaN behind a sequence's end) is not read.
+// of all its rows: t -> j = t < s ? t : lo + t - s, with s <= lo.  No key outside is read.  Whatever stands in keys that no row of the tile sees (NaN behind a sequence's end) is not read.
 //
 // Per 32 keys, with v_mfma_f32_16x16x32 (lane l = (g, c): A[c][8 g + j], B[8 g + j][c], C[4 g + i][c]):
 //   S^T = K Q^T      A = K rows, B = the wave's 16 query rows: lane (g, c) holds S^T[key 16 kb + 4 g + i][row c].
@@ -16,8 +15,17 @@
 //   O^T += V^T P^T   B = P^T from the S^T registers: slot j of lane group g is key 4 g + j, or 16 + 4 g + j - 4 from
 //                    j = 4 on; A = V^T by LDS transpose reads.  P enters as a sum of two or three values of the
 //                    2-byte type (split_p), so that only the inputs' and the output's own rounding is left.
-// A-row 4 q + j of block db of four is column 64 (db / 4) + 16 q + 4 (db % 4) + j, so that a lane ends with 16
-// neighbouring columns of its row (of two blocks for D = 32: 8 q + 4 db + j, 8 columns).
+// Lane (g, c) ends with columns 16 db + 4 g .. + 3 of row c.
+//
+// What bounds it (MI355X, us; rocprofv3 counters in profiles/counters_window.md): bf16 [60, 801], 8 heads of 64 through 101
+// keys and 8 sinks, 57.8; its loads and stores alone take 43 (197 MB at 4.6 TB/s), the rest is the softmax's VALU work, which
+// hides behind them only in part (a wave's step of 64 keys: 24 MFMAs of 16 clocks, about 170 VALU instructions of 4 and 16
+// exponentials of 16, and 16 KB of LDS reads).  f16 [2, 16389], 8 heads over 2 of 128 through 1024 keys, 210: 134 GFLOP, half as
+// many again for the second part of p; 2052 workgroups on 512 places, so five rounds where four and a bit would do.
+// One step over 64 keys at a time, priorities around the MFMAs and row sums by the matrix unit gained nothing
+// over steps of 32, none and VALU sums; skipping steps that are hidden from a wave cost as much in register copies as it
+// saved; transpose reads by the compiler's builtin, which it can place early, 71 -> 64 at 32 rows per wave; addresses of a
+// tile from one scalar base and a layout without bank conflicts 290 -> 267 at f16 [2, 16389] with 16 rows per wave.
 //
 // A value that a row does not see but another row of its tile does enters the product with weight 0.  Where that
 // value is infinite or NaN the product is NaN; a row that ends with anything not finite is computed again from the
@@ -36,6 +44,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLazy = 8.0f;  // log2 units the running max may outgrow the exponent's reference
+constexpr int kBufferDword3 = 0x00020000;  // raw buffer resource: 32-bit data format, no swizzle, no stride
 constexpr int kTile = 64;      // keys per LDS tile
 constexpr int kChunk = 32;     // keys per arithmetic step
 
@@ -71,7 +80,8 @@ __device__ __forceinline__ Span make_span(const WinArgs& a, int b, int qa, int q
     p.start = a.start >= 0 ? a.start : p.len - a.nq;
     p.hi = a.right < 0 ? p.len - 1 : min(p.len - 1, p.start + qb + a.right);
     p.lo = a.left < 0 ? 0 : max(0, p.start + qa - a.left);
-    p.s = max(0, min(min(a.sinks, p.lo), p.hi + 1));
+    p.s = a.left < 0 ? 0 : max(0, min(a.sinks, p.hi + 1));
+    p.lo = max(p.lo, p.s);
     p.count = p.s + max(0, p.hi - p.lo + 1);
     return p;
 }
@@ -117,56 +127,32 @@ __device__ __forceinline__ float elem(const uint16_t* p, int64_t i) {
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
-// K and V tiles in LDS: rows of D 2-byte elements in 16-byte pieces, piece j of row r at j ^ swz(r): eight
-// neighbouring rows' pieces j fall on different banks (rows of 64 bytes: two rows to a line of banks).
+// K and V tiles in LDS: rows of D 2-byte elements in 16-byte pieces, piece j of row r at j ^ swz(r).  Eight neighbouring
+// rows' pieces j (K fragments) fall on different banks, and so do the pieces 2 i, 2 i + 1 of four (V's transpose
+// reads).  Rows of 64 bytes: two rows to a line of banks.
 template <int D>
-__device__ __forceinline__ int swz(int r) { return D >= 64 ? (r & 7) : ((r >> 1) & 3); }
+__device__ __forceinline__ int swz(int r) {
+    return D >= 64 ? (((r & 3) << 1) | ((r >> 2) & 1)) : ((r & 2) | ((r >> 2) & 1));
+}
 
-// Transpose reads of V^T fragments for 32 keys: rows r and r + 16 (HI bytes further) at NB addresses.
-template <int HI, int NB>
-__device__ __forceinline__ void lds_read_vt(const uint32_t (&ad)[NB], uint32_t off, u32x4 (&va)[NB]) {
-    static_assert(NB == 4 || NB == 2, "blocks per group");
-    u32x2 r[2 * NB];
-    if constexpr (NB == 4) {
-        asm volatile(
-            "ds_read_b64_tr_b16 %0, %8\n\t"
-            "ds_read_b64_tr_b16 %1, %8 offset:%[hi]\n\t"
-            "ds_read_b64_tr_b16 %2, %9\n\t"
-            "ds_read_b64_tr_b16 %3, %9 offset:%[hi]\n\t"
-            "ds_read_b64_tr_b16 %4, %10\n\t"
-            "ds_read_b64_tr_b16 %5, %10 offset:%[hi]\n\t"
-            "ds_read_b64_tr_b16 %6, %11\n\t"
-            "ds_read_b64_tr_b16 %7, %11 offset:%[hi]\n\t"
-            "s_waitcnt lgkmcnt(0)"
-            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-            : "v"(ad[0] + off), "v"(ad[1] + off), "v"(ad[2] + off), "v"(ad[3] + off), [hi] "n"(HI)
-            : "memory");
-    } else {
-        asm volatile(
-            "ds_read_b64_tr_b16 %0, %4\n\t"
-            "ds_read_b64_tr_b16 %1, %4 offset:%[hi]\n\t"
-            "ds_read_b64_tr_b16 %2, %5\n\t"
-            "ds_read_b64_tr_b16 %3, %5 offset:%[hi]\n\t"
-            "s_waitcnt lgkmcnt(0)"
-            : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
-            : "v"(ad[0] + off), "v"(ad[1] + off), [hi] "n"(HI)
-            : "memory");
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i) va[i] = u32x4{r[2 * i].x, r[2 * i].y, r[2 * i + 1].x, r[2 * i + 1].y};
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+// A V^T fragment of 32 keys by two transpose reads: rows r and r + 16 (32 D bytes further).
+template <int D>
+__device__ __forceinline__ u32x4 lds_read_vt(const char* p) {
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)p));
+    const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p + 32 * D)));
+    return u32x4{a.x, a.y, b.x, b.y};
 }
 
 // 16 bytes per lane from the lane's own p straight to lds + 16 lane.  Not a template: the builtin's operands must not
 // depend on one, or the host pass drops the kernel that holds it.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t base, char* lds, uint32_t off) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (lds_void*)lds, 16, off, 0, 0, 0);
+}
 __device__ __forceinline__ void load_to_lds(const uint16_t* p, char* lds) {
     __builtin_amdgcn_global_load_lds((global_void*)p, (lds_void*)lds, 16, 0, 0);
 }
-
-template <int D>
-struct Cols {
-    static constexpr int NB = D >= 64 ? 4 : 2;      // blocks of a group: a lane holds 4 NB neighbouring columns of each
-    static constexpr int NG = D / (16 * NB);        // groups of 16 NB columns
-};
 
 // Running state of a wave's 16 QS rows.
 template <int D, int QS>
@@ -184,129 +170,151 @@ struct State {
     }
 };
 
-// The rows a wave works on: each lane's row c of each sub-block x, and the wave's first and last position.
+// The rows a wave works on, in the list's places t: the window of the lane's row c of each sub-block x is first ..
+// first + n - 1, behind the sinks; it sees sink t (< s) iff t <= jhi.  From all0 to all1 every row of the wave sees every
+// key; sinks from sink1 on are seen by none.
 template <int QS>
 struct Rows {
-    int jlo[QS], jhi[QS];  // window of the lane's row
-    int pa, pb;
+    int first[QS], n[QS], jhi[QS];
+    int all0, all1, sink1;
 };
 
 template <int QS>
 __device__ __forceinline__ Rows<QS> make_rows(const WinArgs& a, const Span& sp, int r0, int c) {
     Rows<QS> rw;
+    const int off = sp.s - sp.lo;  // t of key j behind the sinks: j + off
 #pragma unroll
     for (int x = 0; x < QS; ++x) {
         const int p = sp.start + (int)fdiv((uint32_t)min(r0 + 16 * x + c, a.rows - 1), a.gdiv);
-        rw.jlo[x] = a.left < 0 ? 0 : p - a.left;
-        rw.jhi[x] = a.right < 0 ? sp.len - 1 : min(sp.len - 1, p + a.right);
+        const int jlo = a.left < 0 ? sp.lo : max(sp.lo, p - a.left);
+        rw.jhi[x] = a.right < 0 ? sp.hi : min(sp.hi, p + a.right);
+        rw.first[x] = jlo + off;
+        rw.n[x] = max(0, rw.jhi[x] - jlo + 1);
     }
-    rw.pa = sp.start + (int)fdiv((uint32_t)min(r0, a.rows - 1), a.gdiv);
-    rw.pb = sp.start + (int)fdiv((uint32_t)min(r0 + 16 * QS - 1, a.rows - 1), a.gdiv);
+    const int pa = sp.start + (int)fdiv((uint32_t)min(r0, a.rows - 1), a.gdiv);
+    const int pb = sp.start + (int)fdiv((uint32_t)min(r0 + 16 * QS - 1, a.rows - 1), a.gdiv);
+    const int hia = a.right < 0 ? sp.hi : min(sp.hi, pa + a.right), hib = a.right < 0 ? sp.hi : min(sp.hi, pb + a.right);
+    rw.all0 = (a.left < 0 ? sp.lo : max(sp.lo, pb - a.left)) + off;
+    rw.all1 = hia + 1 + off;
+    rw.sink1 = min(sp.s, hib + 1);
     return rw;
 }
 
-// Whether the 32 keys from t0 on are hidden from every row of the wave.
-template <int QS>
-__device__ __forceinline__ bool all_hidden(const WinArgs& a, const Span& sp, const Rows<QS>& rw, int t0) {
-    if (t0 >= sp.count) return true;
-    const int ja = sp.key(t0), jb = sp.key(min(t0 + kChunk, sp.count) - 1);
-    return (a.right >= 0 && ja > rw.pb + a.right) || (a.left >= 0 && jb < rw.pa - a.left && ja >= a.sinks);
-}
-// Whether any of them is hidden from any.
-template <int QS>
-__device__ __forceinline__ bool any_hidden(const WinArgs& a, const Span& sp, const Rows<QS>& rw, int t0) {
-    if (t0 + kChunk > sp.count) return true;
-    const int ja = sp.key(t0), jb = sp.key(t0 + kChunk - 1);
-    return (a.right >= 0 && jb > rw.pa + a.right) || (a.left >= 0 && ja < rw.pb - a.left && jb >= a.sinks);
-}
-
-// One step over the 32 keys from t0 on.  kf[kb][s]: K[16 kb + c][32 s + 8 g ..]; vad: the lane's transpose
-// addresses of the V tile's row 0, voff the byte offset of the step's first row.
-template <int DT, int D, int QS, int NP>
-__device__ __forceinline__ void attend(const WinArgs& a, const Span& sp, const Rows<QS>& rw, int t0,
-                                       const u32x4 (&kf)[2][D / 32], const u32x4 (&qf)[QS][D / 32],
-                                       const uint32_t (&vad)[Cols<D>::NG][Cols<D>::NB], uint32_t voff, int g,
-                                       State<D, QS>& st) {
-    f32x4 s[QS][2];
+// One step over the 32 NC keys from t0 on.  kf(kb, s): K[16 kb + c][32 s + 8 g ..]; vad: the lane's transpose addresses
+// from the step's first V row.
+template <int DT, int D, int QS, int NP, int NC, class KF>
+__device__ __forceinline__ void attend(const WinArgs& a, const Span& sp, const Rows<QS>& rw, int t0, KF kf,
+                                       const u32x4 (&qf)[QS][D / 32], const char* vtile, const uint32_t (&vad)[D / 16],
+                                       int g, State<D, QS>& st) {
+    constexpr int KB = 2 * NC;
+    f32x4 s[QS][KB];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int x = 0; x < QS; ++x) s[x][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+            const u32x4 k = kf(kb, e);
+#pragma unroll
+            for (int x = 0; x < QS; ++x) s[x][kb] = mma<DT>(k, qf[x][e], s[x][kb]);
+        }
+    }
+    // Keys hidden from some row: before its window, behind it, or (both at once) in a step that holds sinks, which a row
+    // sees up to jhi.  k = 16 kb + i is the key's place from t0 + 4 g on.
+    if (t0 < rw.sink1) {
 #pragma unroll
         for (int x = 0; x < QS; ++x) {
-            s[x][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const int lo = rw.first[x] - (t0 + 4 * g), hi = lo + rw.n[x], sink = min(sp.s, rw.jhi[x] + 1) - (t0 + 4 * g);
 #pragma unroll
-            for (int e = 0; e < D / 32; ++e) s[x][kb] = mma<DT>(kf[kb][e], qf[x][e], s[x][kb]);
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = 16 * kb + i;
+                    s[x][kb][i] = (bool)(((int)(k >= lo) & (int)(k < hi)) | (int)(k < sink)) ? s[x][kb][i] : -INFINITY;
+                }
         }
-    if (any_hidden<QS>(a, sp, rw, t0)) {
+    } else {
+        if (t0 < rw.all0) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+            for (int x = 0; x < QS; ++x) {
+                const int lo = rw.first[x] - (t0 + 4 * g);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int j = sp.key(t0 + 16 * kb + 4 * g + i);
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int x = 0; x < QS; ++x)
-                    if (j > rw.jhi[x] || (j < rw.jlo[x] && j >= a.sinks)) s[x][kb][i] = -INFINITY;
+                    for (int i = 0; i < 4; ++i) s[x][kb][i] = 16 * kb + i < lo ? -INFINITY : s[x][kb][i];
             }
+        }
+        if (t0 + kChunk * NC > rw.all1) {
+#pragma unroll
+            for (int x = 0; x < QS; ++x) {
+                const int hi = rw.first[x] + rw.n[x] - (t0 + 4 * g);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[x][kb][i] = 16 * kb + i >= hi ? -INFINITY : s[x][kb][i];
+            }
+        }
     }
-    u32x4 pp[QS][NP];
+    float mx[QS];
+    bool grown = false;
 #pragma unroll
     for (int x = 0; x < QS; ++x) {
-        float mx = s[x][0][0];
+        mx[x] = s[x][0][0];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[x][kb][i]);
-        if (__builtin_amdgcn_ballot_w64(mx * a.sl2 > st.m[x] + kLazy) != 0) {
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) * a.sl2;
-            const float mn = mx > st.m[x] + kLazy ? mx : st.m[x];
+            for (int i = 0; i < 4; ++i) mx[x] = fmaxf(mx[x], s[x][kb][i]);
+        grown = grown || mx[x] * a.sl2 > st.m[x] + kLazy;
+    }
+    if (__builtin_amdgcn_ballot_w64(grown) != 0) {
+#pragma unroll
+        for (int x = 0; x < QS; ++x) {
+            float top = fmaxf(mx[x], __shfl_xor(mx[x], 16));
+            top = fmaxf(top, __shfl_xor(top, 32)) * a.sl2;
+            const float mn = top > st.m[x] + kLazy ? top : st.m[x];
             const float alpha = __builtin_amdgcn_exp2f(st.m[x] - mn);
             st.l[x] *= alpha;
 #pragma unroll
             for (int db = 0; db < D / 16; ++db) st.o[x][db] *= alpha;
             st.m[x] = mn;
         }
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[x][kb][i], a.sl2, -st.m[x]));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[x][kb][i + 1], a.sl2, -st.m[x]));
-                st.l[x] += p0 + p1;
-                uint32_t parts[NP];
-                split_p<DT, NP>(p0, p1, parts);
-#pragma unroll
-                for (int n = 0; n < NP; ++n) pp[x][n][2 * kb + i / 2] = parts[n];
-            }
     }
 #pragma unroll
-    for (int gr = 0; gr < Cols<D>::NG; ++gr) {
-        u32x4 va[Cols<D>::NB];
-        lds_read_vt<32 * D, Cols<D>::NB>(vad[gr], voff, va);
+    for (int cc = 0; cc < NC; ++cc) {
+        u32x4 pp[QS][NP];
 #pragma unroll
-        for (int i = 0; i < Cols<D>::NB; ++i)
+        for (int x = 0; x < QS; ++x)
 #pragma unroll
-            for (int x = 0; x < QS; ++x) {
-                f32x4& o = st.o[x][gr * Cols<D>::NB + i];
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int n = 0; n < NP; ++n) o = mma<DT>(va[i], pp[x][n], o);
-            }
+                for (int i = 0; i < 4; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[x][2 * cc + kb][i], a.sl2, -st.m[x]));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[x][2 * cc + kb][i + 1], a.sl2, -st.m[x]));
+                    st.l[x] += p0 + p1;
+                    uint32_t parts[NP];
+                    split_p<DT, NP>(p0, p1, parts);
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) pp[x][n][2 * kb + i / 2] = parts[n];
+                }
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) {
+            const u32x4 va = lds_read_vt<D>(vtile + 2 * D * kChunk * cc + vad[db]);
+#pragma unroll
+            for (int x = 0; x < QS; ++x)
+#pragma unroll
+                for (int n = 0; n < NP; ++n) st.o[x][db] = mma<DT>(va, pp[x][n], st.o[x][db]);
+        }
     }
 }
 
-// The lane's transpose addresses of a V tile: lane (g, c) points to row 4 g + c / 4, columns 16 NB gr + 4 NB (c % 4)
-// + 4 i .. + 3, and receives, for column 16 NB gr + 4 NB (c / 4) + 4 i + c % 4, the four rows 4 g ...
+// The lane's transpose addresses of a V tile, from its first row: lane (g, c) points to row 4 g + c / 4, columns 16 db +
+// 4 (c % 4) .. + 3, and receives column 16 db + c of the rows 4 g .. 4 g + 3.
 template <int D>
-__device__ __forceinline__ void v_addresses(const void* tile, int g, int c, uint32_t (&vad)[Cols<D>::NG][Cols<D>::NB]) {
-    constexpr int NB = Cols<D>::NB;
+__device__ __forceinline__ void v_addresses(int g, int c, uint32_t (&vad)[D / 16]) {
     const int row = 4 * g + (c >> 2);
-    const uint32_t base = lds_addr(reinterpret_cast<const char*>(tile)) + 2 * D * row;
 #pragma unroll
-    for (int gr = 0; gr < Cols<D>::NG; ++gr)
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int col = 16 * NB * gr + 4 * NB * (c & 3) + 4 * i;
-            vad[gr][i] = base + 16 * ((col >> 3) ^ swz<D>(row)) + 2 * (col & 7);
-        }
+    for (int db = 0; db < D / 16; ++db)
+        vad[db] = 2 * D * row + 16 * ((2 * db + ((c & 3) >> 1)) ^ swz<D>(row)) + 8 * (c & 1);
 }
 
 __device__ __forceinline__ float gate_of(const WinArgs& a, int b, int qi, int h) {
@@ -369,15 +377,32 @@ __device__ __forceinline__ void store_row_alone(const WinArgs& a, int b, int kv,
     if (D > 64) store1(a.out, a.odt, e + lane + 64, y[1] * gv);
 }
 
-// NV neighbouring columns at element e (a multiple of 8 elements, out 16-byte aligned).
-template <int NV>
-__device__ __forceinline__ void store_cols(void* out, int dt, int64_t e, const float (&f)[NV]) {
+// A row's D columns from its four lanes: lane g holds columns 16 db + 4 g .. + 3.  f32: 16 bytes each.  2-byte types: the
+// lanes of a pair (g, g ^ 1) exchange halves, so that each stores 8 columns of one of two blocks, 16 bytes; `store` is
+// uniform within a pair.
+template <int D>
+__device__ __forceinline__ void store_row(const WinArgs& a, int64_t e, const f32x4 (&o)[D / 16], float f, int g, bool store) {
+    if (a.odt == F32) {
+        if (!store) return;
 #pragma unroll
-    for (int i = 0; i < NV / 8; ++i) {
-        float t[8];
+        for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(a.out) + e + 16 * db + 4 * g) = o[db] * f;
+        return;
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = f[8 * i + j];
-        store8(out, dt, e + 8 * i, t);
+    for (int p = 0; p < D / 32; ++p) {
+        u32x2 w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x4 v = o[2 * p + i] * f;
+            w[i] = a.odt == BF16 ? u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
+                                 : u32x2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
+        }
+        const bool odd = g & 1;
+        const u32x2 give = odd ? w[0] : w[1];
+        const u32x2 got = {(uint32_t)__shfl_xor((int)give.x, 16), (uint32_t)__shfl_xor((int)give.y, 16)};
+        const u32x4 v = odd ? u32x4{got.x, got.y, w[1].x, w[1].y} : u32x4{w[0].x, w[0].y, got.x, got.y};
+        if (store)
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(a.out) + e + 16 * (2 * p + (g & 1)) + 8 * (g >> 1)));
     }
 }
 
@@ -388,7 +413,6 @@ template <int DT, int D, int QS, int NP>
 __global__ __launch_bounds__(256) void window_tile_kernel(WinArgs a) {
     constexpr int kRow = 2 * D, CH = D / 8;            // bytes and pieces of a key row
     constexpr int RPL = 1024 / kRow, LD = kTile / RPL / 4;  // rows per load instruction; loads per wave, tile and tensor
-    constexpr int NB = Cols<D>::NB, NG = Cols<D>::NG;
     __shared__ __attribute__((aligned(16))) char k0[kTile * kRow];
     __shared__ __attribute__((aligned(16))) char v0[kTile * kRow];
     __shared__ __attribute__((aligned(16))) char k1[kTile * kRow];
@@ -419,7 +443,25 @@ __global__ __launch_bounds__(256) void window_tile_kernel(WinArgs a) {
 
     const uint16_t* kb_ = a.k + b * a.kv_bs + kv * a.kv_hs;
     const uint16_t* vb_ = a.v + b * a.kv_bs + kv * a.kv_hs;
+    // Lane offsets within a tile of neighbouring keys: such a tile's rows are one scalar base and these.
+    uint32_t loff[LD];
+#pragma unroll
+    for (int u = 0; u < LD; ++u) {
+        const int r = (w * LD + u) * RPL + lane / CH;
+        loff[u] = 2u * ((uint32_t)r * (uint32_t)a.kv_ns + 8u * ((lane % CH) ^ swz<D>(r)));
+    }
     auto load_tile = [&](int t0, char* kd, char* vd) {
+        if (t0 >= sp.s && t0 + kTile <= sp.count && a.kv_ns < (1 << 24)) {  // 32-bit offsets
+            const int64_t first = (int64_t)(sp.lo + t0 - sp.s) * a.kv_ns;
+            const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc((void*)(kb_ + first), (short)0, -1, kBufferDword3);
+            const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc((void*)(vb_ + first), (short)0, -1, kBufferDword3);
+#pragma unroll
+            for (int u = 0; u < LD; ++u) {
+                load_to_lds(krs, kd + 1024 * (w * LD + u), loff[u]);
+                load_to_lds(vrs, vd + 1024 * (w * LD + u), loff[u]);
+            }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < LD; ++u) {
             const int r = (w * LD + u) * RPL + lane / CH;
@@ -428,25 +470,16 @@ __global__ __launch_bounds__(256) void window_tile_kernel(WinArgs a) {
             load_to_lds(vb_ + at, vd + 1024 * (w * LD + u));
         }
     };
+    uint32_t vad[D / 16];
+    v_addresses<D>(g, c, vad);
     auto step = [&](int t0, const char* ks, const char* vs, char* kn, char* vn) {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile has landed
         __syncthreads();                     // every wave's has, and none still reads the other buffers
         if (t0 + kTile < sp.count) load_tile(t0 + kTile, kn, vn);
-        if (r0 >= a.rows) return;
-        uint32_t vad[NG][NB];
-        v_addresses<D>(vs, g, c, vad);
-#pragma unroll
-        for (int hh = 0; hh < kTile / kChunk; ++hh) {
-            const int t = t0 + hh * kChunk;
-            if (all_hidden<QS>(a, sp, rw, t)) continue;
-            u32x4 kf[2][D / 32];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int s = 0; s < D / 32; ++s)
-                    kf[kb][s] = *reinterpret_cast<const u32x4*>(ks + (hh * kChunk + 16 * kb + c) * kRow + 16 * ((4 * s + g) ^ swz<D>(c)));
-            attend<DT, D, QS, NP>(a, sp, rw, t, kf, qf, vad, hh * kChunk * kRow, g, st);
-        }
+        auto kf = [&](int kb, int s) {
+            return *reinterpret_cast<const u32x4*>(ks + (16 * kb + c) * kRow + 16 * ((4 * s + g) ^ swz<D>(c)));
+        };
+        attend<DT, D, QS, NP, kTile / kChunk>(a, sp, rw, t0, kf, qf, vs, vad, g, st);
     };
     if (sp.count > 0) load_tile(0, k0, v0);
     for (int t0 = 0; t0 < sp.count; t0 += 2 * kTile) {
@@ -471,18 +504,7 @@ __global__ __launch_bounds__(256) void window_tile_kernel(WinArgs a) {
         rows_bad |= rows_bad >> 32;
         rows_bad = (rows_bad | (rows_bad >> 16)) & 0xffff;
         const float gv = gate_of(a, b, qi, h);
-        if (r < a.rows && ((rows_bad >> c) & 1) == 0) {
-            const int64_t e = b * a.o_bs + h * a.o_hs + qi * a.o_ns;
-#pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-                float f[4 * NB];
-#pragma unroll
-                for (int i = 0; i < NB; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) f[4 * i + j] = st.o[x][gr * NB + i][j] * inv * gv;
-                store_cols<4 * NB>(a.out, a.odt, e + 16 * NB * gr + 4 * NB * g, f);
-            }
-        }
+        store_row<D>(a, b * a.o_bs + h * a.o_hs + qi * a.o_ns, st.o[x], inv * gv, g, r < a.rows && ((rows_bad >> c) & 1) == 0);
         while (rows_bad != 0) {
             const int rc = __builtin_ctzll(rows_bad);
             rows_bad &= rows_bad - 1;
@@ -496,16 +518,17 @@ __global__ __launch_bounds__(256) void window_tile_kernel(WinArgs a) {
 // A block holds 16 rows and a share of their key list; its waves take 32 keys at a time in turn, each with its own
 // V tile in LDS, and are joined through LDS.  With more than one share the block leaves its rows' (m, l, O) in the
 // workspace for window_join_kernel: part[(b, kv, tile, row of 16)][split][D + 2].
+constexpr int kSplitWaves = 8;
 template <int DT, int D, int NP>
-__global__ __launch_bounds__(512) void window_split_kernel(WinArgs a) {
+__global__ __launch_bounds__(kSplitWaves * 64) void window_split_kernel(WinArgs a) {
     constexpr int kRow = 2 * D, CH = D / 8;
     constexpr int RPL = 1024 / kRow, LD = kChunk / RPL;
-    constexpr int NB = Cols<D>::NB, NG = Cols<D>::NG;
     constexpr int kPart = D + 2;
     // V tiles while the keys are read, then the waves' rows: [wave][16][D + 2] f32
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
-    const int w = __builtin_amdgcn_readfirstlane(tid / 64), nw = blockDim.x / 64;
+    const int w = __builtin_amdgcn_readfirstlane(tid / 64);
+    constexpr int nw = kSplitWaves;
     const uint32_t split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
     const uint32_t bkv = tile / a.qtiles;
     uint32_t b, kv;
@@ -529,8 +552,8 @@ __global__ __launch_bounds__(512) void window_split_kernel(WinArgs a) {
     const uint16_t* kb_ = a.k + b * a.kv_bs + kv * a.kv_hs;
     const uint16_t* vb_ = a.v + b * a.kv_bs + kv * a.kv_hs;
     char* vt = lds + w * kChunk * kRow;
-    uint32_t vad[NG][NB];
-    v_addresses<D>(vt, g, c, vad);
+    uint32_t vad[D / 16];
+    v_addresses<D>(g, c, vad);
     for (int i = sa + w; i < sb; i += nw) {
         const int t0 = i * kChunk;
 #pragma unroll
@@ -548,7 +571,7 @@ __global__ __launch_bounds__(512) void window_split_kernel(WinArgs a) {
         }
         wait_vmcnt<0>();
         asm volatile("" ::: "memory");
-        attend<DT, D, 1, NP>(a, sp, rw, t0, kf, qf, vad, 0, g, st);
+        attend<DT, D, 1, NP, 1>(a, sp, rw, t0, [&](int kb, int s) { return kf[kb][s]; }, qf, vt, vad, g, st);
     }
 
     // the waves' rows, joined: m, l and O of each, the four lanes of a row holding its columns
@@ -558,11 +581,9 @@ __global__ __launch_bounds__(512) void window_split_kernel(WinArgs a) {
     __syncthreads();  // the V tiles are done with
     float* mine = reinterpret_cast<float*>(lds) + (w * 16 + c) * kPart;
 #pragma unroll
-    for (int gr = 0; gr < NG; ++gr)
+    for (int db = 0; db < D / 16; ++db)
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mine[16 * NB * gr + 4 * NB * g + 4 * i + j] = st.o[0][gr * NB + i][j];
+        for (int j = 0; j < 4; ++j) mine[16 * db + 4 * g + j] = st.o[0][db][j];
     if (g == 0) {
         mine[D] = st.m[0];
         mine[D + 1] = l;
@@ -603,70 +624,102 @@ __global__ __launch_bounds__(512) void window_split_kernel(WinArgs a) {
     }
 }
 
-// One block per query row: its waves take the shares in turn.
+// One block per query row; each wave joins its shares (64 at most: splits <= kJoinWaves * 64), with every load on its way at
+// once, and the first one joins the waves.
+constexpr int kJoinWaves = 8;
 template <int DT, int D>
-__global__ __launch_bounds__(512) void window_join_kernel(WinArgs a) {
+__global__ __launch_bounds__(kJoinWaves * 64) void window_join_kernel(WinArgs a) {
     constexpr int kPart = D + 2;
-    __shared__ float part[8][kPart];
-    const int lane = threadIdx.x % 64, w = threadIdx.x / 64, nw = blockDim.x / 64;
+    __shared__ float part[kJoinWaves][kPart];
+    const int lane = threadIdx.x % 64, w = threadIdx.x / 64;
     const uint32_t bkv = blockIdx.x / a.rows;
     const int r = (int)(blockIdx.x % a.rows);
     uint32_t b, kv;
     fdivmod(bkv, a.kvdiv, b, kv);
-    const float* p = a.ws + (int64_t)blockIdx.x * a.splits * kPart;
-    float m = -FLT_MAX;
-    for (uint32_t i = lane; i < a.splits; i += 64) m = fmaxf(m, p[i * kPart + D]);
+    const int per = ((int)a.splits + kJoinWaves - 1) / kJoinWaves, mine = min(per, (int)a.splits - w * per);
+    const float* p = a.ws + ((int64_t)blockIdx.x * a.splits + w * per) * kPart;
+    float m = -FLT_MAX, l = 0.0f, o[2] = {0.0f, 0.0f};
+    if (lane < mine) {
+        m = p[lane * kPart + D];
+        l = p[lane * kPart + D + 1];
+    }
+    float top = m;
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x));
-    float l = 0.0f, o[2] = {0.0f, 0.0f};
-    for (uint32_t i = w; i < a.splits; i += nw) {
-        const float* q = p + i * kPart;
-        const float f = __builtin_amdgcn_exp2f(q[D] - m);
-        l += q[D + 1] * f;
-        if (lane < D) o[0] += q[lane] * f;
-        if (D > 64) o[1] += q[lane + 64] * f;
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    const float f = lane < mine ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
+    l *= f;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+    for (int i0 = 0; i0 < mine; i0 += 8) {  // a lane's weight is 0 from share `mine` on
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float fi = __shfl(f, i0 + u);
+            const float* q = p + min(i0 + u, mine - 1) * kPart;
+            if (lane < D) o[0] += q[lane] * fi;
+            if (D > 64) o[1] += q[lane + 64] * fi;
+        }
     }
     if (lane < D) part[w][lane] = o[0];
     if (D > 64) part[w][lane + 64] = o[1];
-    if (lane == 0) part[w][D] = l;
+    if (lane == 0) {
+        part[w][D] = top;
+        part[w][D + 1] = l;
+    }
     __syncthreads();
     if (w > 0) return;
-    for (int i = 1; i < nw; ++i) {
-        l += part[i][D];
-        if (lane < D) o[0] += part[i][lane];
-        if (D > 64) o[1] += part[i][lane + 64];
+    m = -FLT_MAX;
+#pragma unroll
+    for (int i = 0; i < kJoinWaves; ++i) m = fmaxf(m, part[i][D]);
+    l = o[0] = o[1] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kJoinWaves; ++i) {
+        const float g = __builtin_amdgcn_exp2f(part[i][D] - m);
+        l += part[i][D + 1] * g;
+        if (lane < D) o[0] += part[i][lane] * g;
+        if (D > 64) o[1] += part[i][lane + 64] * g;
     }
     if (__builtin_amdgcn_ballot_w64(not_finite(l) || not_finite(o[0]) || not_finite(o[1])) != 0) {
         store_row_alone<DT, D>(a, b, kv, r);
         return;
     }
     const int qi = (int)fdiv((uint32_t)r, a.gdiv), h = kv * (int)a.gdiv.d + r - qi * (int)a.gdiv.d;
-    const float f = (l == 0.0f ? 0.0f : 1.0f / l) * gate_of(a, b, qi, h);
+    const float q = (l == 0.0f ? 0.0f : 1.0f / l) * gate_of(a, b, qi, h);
     const int64_t e = b * a.o_bs + h * a.o_hs + qi * a.o_ns;
-    if (lane < D) store1(a.out, a.odt, e + lane, o[0] * f);
-    if (D > 64) store1(a.out, a.odt, e + lane + 64, o[1] * f);
+    if (lane < D) store1(a.out, a.odt, e + lane, o[0] * q);
+    if (D > 64) store1(a.out, a.odt, e + lane + 64, o[1] * q);
 }
 
 // ---- choice of the form ------------------------------------------------------------------------------
 
 struct Plan {
     bool few;        // window_split_kernel
-    int waves;       // its waves per block
-    int64_t splits;  // its shares of the key list
+    int qs;          // window_tile_kernel: 16-row blocks per wave
+    int64_t splits;  // window_split_kernel: shares of the key list
 };
 
-Plan make_plan(int64_t B, int64_t H, int64_t KV, int64_t nq, int64_t nk, int64_t left, int64_t right, int64_t sinks) {
+// Few rows (of one tile of 16, or of some while the tiles of 64 would leave CUs idle before long lists) go to the kernel that
+// shares out the keys, a workgroup of 8 waves per CU at least, each with 16 steps of 32 keys or more: one token against
+// [1, 200003] keys of 2 heads 28.8 us; twice the shares 33.5, the join then taking longer; 60 x 8 heads of 805 keys 22.0 with
+// one share each, 26 with three shares of 4 waves.
+// Of 128 columns, 32 rows per wave use each fragment read from LDS twice, which pays where lists are long and the larger
+// tiles still fill the CUs: [2, 16389] f16 over 1024 keys 259 -> 216 us, [16, 801] bf16 over all 109 -> 103; over 300 keys [30, 801]
+// 90 -> 92, over 100 72 -> 76.  Of 64 columns they gain nothing: [60, 801] over all keys 162 -> 160, over 101 60 -> 69.
+Plan make_plan(int64_t B, int64_t H, int64_t KV, int64_t nq, int64_t nk, int64_t D, int64_t left, int64_t right,
+               int64_t sinks) {
     Plan p{};
     const int64_t cus = cu_count(), rows = nq * (H / KV);
     // the most keys that a tile of rows may see
     int64_t span = nk;
     if (left >= 0 && right >= 0) span = std::min(nk, sinks + left + right + std::min<int64_t>(nq, 64));
     p.few = rows <= 16 || (rows <= 256 && B * KV * ceil_div(rows, 64) < cus && span > 1024);
-    if (!p.few) return p;
+    p.qs = D == 128 && span >= 512 && B * KV * ceil_div(rows, 128) >= 2 * cus ? 2 : 1;
     const int64_t tiles = B * KV * ceil_div(rows, 16), steps = ceil_div(span, kChunk);
-    p.waves = 4;
-    p.splits = std::max<int64_t>(1, std::min(ceil_div(4 * cus, tiles), steps / 8));
+    p.splits = p.few ? std::max<int64_t>(1, std::min<int64_t>(std::min(cus / tiles, steps / 16), kJoinWaves * 64)) : 1;
     return p;
+}
+
+int64_t workspace_bytes_of(const Plan& p, int64_t B, int64_t H, int64_t nq, int64_t D) {
+    return p.splits > 1 ? B * H * nq * p.splits * (D + 2) * 4 : 0;
 }
 
 bool sizes_ok(int64_t B, int64_t H, int64_t KV, int64_t nq, int64_t nk, int64_t D, int64_t sinks) {
@@ -687,8 +740,8 @@ int64_t mbrt_attention_window_workspace_bytes(int64_t B, int64_t H, int64_t H_kv
                                               int64_t head_dim, int64_t left, int64_t right, int64_t sinks) {
     if (!sizes_ok(B, H, H_kv, n_q, n_k, head_dim, sinks)) return -1;
     if (B == 0 || n_q == 0) return 0;
-    const Plan p = make_plan(B, H, H_kv, n_q, n_k, left, right, std::min(sinks, n_k));
-    return p.few && p.splits > 1 ? B * H * n_q * p.splits * (head_dim + 2) * 4 : 0;
+    const Plan p = make_plan(B, H, H_kv, n_q, n_k, head_dim, left, right, std::min(sinks, n_k));
+    return workspace_bytes_of(p, B, H, n_q, head_dim);
 }
 
 int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t H, int64_t H_kv,
@@ -720,8 +773,8 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
                            kv_row_stride, out_batch_stride, out_head_stride, out_row_stride};
     for (int i = 0; i < 9; ++i)
         MBRT_REQUIRE(st[i] >= 0 && st[i] % 8 == 0, MBRT_E_ALIGN, "%s: strides must be non-negative multiples of 8", op);
-    const Plan plan = make_plan(B, H, H_kv, n_q, n_k, left, right, std::min(sinks, n_k));
-    const int64_t need = mbrt_attention_window_workspace_bytes(B, H, H_kv, n_q, n_k, head_dim, left, right, sinks);
+    const Plan plan = make_plan(B, H, H_kv, n_q, n_k, head_dim, left, right, std::min(sinks, n_k));
+    const int64_t need = workspace_bytes_of(plan, B, H, n_q, head_dim);
     MBRT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 4)), MBRT_E_INVALID_ARG,
                  "%s: workspace of %lld bytes, %lld needed", op, (long long)(workspace ? workspace_bytes : 0),
                  (long long)need);
@@ -761,20 +814,26 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
     a.splits = (uint32_t)plan.splits;
     hipStream_t stm = as_stream(stream);
     const int64_t bkv = B * H_kv;
-    a.qtiles = (uint32_t)ceil_div(a.rows, plan.few ? 16 : 64);
-    const int64_t blocks = bkv * a.qtiles * (plan.few ? plan.splits : 1);
+    a.qtiles = (uint32_t)ceil_div(a.rows, plan.few ? 16 : 64 * plan.qs);
+    const int64_t blocks = bkv * a.qtiles * plan.splits;
     MBRT_REQUIRE(blocks < kMaxGridX && bkv * a.rows < kMaxGridX, MBRT_E_SHAPE, "%s: too many tiles", op);
     auto launch = [&](auto dt, auto dim, auto parts) {
         constexpr int DTv = decltype(dt)::value, Dv = decltype(dim)::value, NP = decltype(parts)::value;
         if (!plan.few) {
+            if constexpr (Dv == 128) {
+                if (plan.qs == 2) {
+                    hipLaunchKernelGGL((window_tile_kernel<DTv, Dv, 2, NP>), dim3((unsigned)blocks), dim3(256), 0, stm, a);
+                    return;
+                }
+            }
             hipLaunchKernelGGL((window_tile_kernel<DTv, Dv, 1, NP>), dim3((unsigned)blocks), dim3(256), 0, stm, a);
             return;
         }
-        const size_t lds = (size_t)plan.waves * 16 * (Dv + 2) * 4;  // the joined rows; the V tiles need less
+        const size_t lds = (size_t)kSplitWaves * 16 * (Dv + 2) * 4;  // the joined rows; the V tiles need less
         static_assert(kChunk * 2 * Dv <= 16 * (Dv + 2) * 4, "V tile within the rows' space");
-        hipLaunchKernelGGL((window_split_kernel<DTv, Dv, NP>), dim3((unsigned)blocks), dim3(plan.waves * 64), lds, stm, a);
+        hipLaunchKernelGGL((window_split_kernel<DTv, Dv, NP>), dim3((unsigned)blocks), dim3(kSplitWaves * 64), lds, stm, a);
         if (plan.splits > 1)
-            hipLaunchKernelGGL((window_join_kernel<DTv, Dv>), dim3((unsigned)(bkv * a.rows)), dim3(512), 0, stm, a);
+            hipLaunchKernelGGL((window_join_kernel<DTv, Dv>), dim3((unsigned)(bkv * a.rows)), dim3(kJoinWaves * 64), 0, stm, a);
     };
     auto by_dim = [&](auto dt, auto parts) {
         if (head_dim == 32) launch(dt, std::integral_constant<int, 32>(), parts);
