@@ -127,12 +127,13 @@ __device__ __forceinline__ float elem(const uint16_t* p, int64_t i) {
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
-// K and V tiles in LDS: rows of D 2-byte elements in 16-byte pieces, piece j of row r at j ^ swz(r).  Eight neighbouring
-// rows' pieces j (K fragments) fall on different banks, and so do the pieces 2 i, 2 i + 1 of four (V's transpose
-// reads).  Rows of 64 bytes: two rows to a line of banks.
+// K and V tiles in LDS: rows of D 2-byte elements in 16-byte pieces, piece j of row r at j ^ swz(r).  The banks are 256
+// bytes wide; an access of 16 bytes per lane goes by lanes 0-3, 12-15, 20-23, 24-27 (and the complement) at a time, one of 8
+// bytes by 32 lanes.  These keys keep both the K fragments (16 rows' pieces j, j ^ 1) and V's transpose reads (8 rows' pieces 2 i,
+// 2 i + 1) on different banks: no conflicts counted.
 template <int D>
 __device__ __forceinline__ int swz(int r) {
-    return D >= 64 ? (((r & 3) << 1) | ((r >> 2) & 1)) : ((r & 2) | ((r >> 2) & 1));
+    return D == 128 ? ((r & 7) << 1) : D == 64 ? (r & 7) : (-(r >> 2) & 3);
 }
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(256) void window_tile_kernel(WinArgs a) {
         __syncthreads();                     // every wave's has, and none still reads the other buffers
         if (t0 + kTile < sp.count) load_tile(t0 + kTile, kn, vn);
         auto kf = [&](int kb, int s) {
-            return *reinterpret_cast<const u32x4*>(ks + (16 * kb + c) * kRow + 16 * ((4 * s + g) ^ swz<D>(c)));
+            return *reinterpret_cast<const u32x4*>(ks + (16 * kb + c) * kRow + 16 * ((4 * s + g) ^ swz<D>(16 * kb + c)));
         };
         attend<DT, D, QS, NP, kTile / kChunk>(a, sp, rw, t0, kf, qf, vs, vad, g, st);
     };
