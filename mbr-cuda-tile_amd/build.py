@@ -63,6 +63,8 @@ KERNEL_SOURCES = [
     "k_band.hip",
     "k_attention.hip",
     "k_linear.hip",
+    "k_linear_bf16.hip",
+    "k_linear_f16.hip",
     "k_qkv_norm.hip",
     "k_window.hip",
     "k_stft.hip",
@@ -77,8 +79,8 @@ KERNEL_SOURCES = [
 # result (a NaN score still reaches the output through exp2 and the P V product).
 EXTRA_FLAGS = {
     "k_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-Xarch_device", "-fno-honor-nans"],
-    # accumulators in ordinary VGPRs here too; NaN keeps its meaning (rows with one are looked for)
-    "k_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    # accumulators in ordinary VGPRs here too
+    **{f"k_linear{t}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for t in ("", "_bf16", "_f16")},
     "k_window.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

@@ -1,0 +1,6 @@
+// The linear layer's kernels for bf16 operands (linear.hpp).
+#include "linear.hpp"
+
+namespace mbrt {
+template int launch_linear<BF16>(LinArgs& a, bool al, hipStream_t st);
+}  // namespace mbrt
