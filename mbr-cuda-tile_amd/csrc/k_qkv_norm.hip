@@ -192,6 +192,11 @@ int mbrt_split_qkv_norm_rotary(const void* qkv, int qkv_dtype, int64_t qkv_batch
                            kv_batch_stride, kv_head_stride, kv_token_stride};
     for (int i = 0; i < 8; ++i) MBRT_REQUIRE(st[i] >= 0, MBRT_E_SHAPE, "%s: negative stride", op);
     MBRT_REQUIRE(B < (int64_t(1) << 31) && N < (int64_t(1) << 31), MBRT_E_SHAPE, "%s: dimension beyond 2^31", op);
+    for (int i = 0; i < 2; ++i) {  // q, then k and v
+        const int64_t* s = st + 2 + 3 * i;
+        MBRT_REQUIRE((B <= 1 || s[0] > 0) && ((i ? H_kv : H) == 1 || s[1] > 0) && (N <= 1 || s[2] > 0), MBRT_E_SHAPE,
+                     "%s: heads of an output overlap", op);
+    }
     if (B == 0 || N == 0) return MBRT_OK;
     MBRT_REQUIRE(qkv && q && k && q_gamma && k_gamma && cos_table && sin_table, MBRT_E_INVALID_ARG, "%s: NULL pointer",
                  op);

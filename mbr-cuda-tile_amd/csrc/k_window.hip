@@ -354,6 +354,10 @@ __device__ __forceinline__ void row_alone(const WinArgs& a, int b, int kv, int r
         const float s = score(sp.key(t) * a.kv_ns), mn = fmaxf(m, s);
         l = l * __builtin_amdgcn_exp2f(m - mn) + __builtin_amdgcn_exp2f(s - mn);
         m = mn;
+        if (not_finite(l)) {  // a score that is NaN or +infinite: so is every weight
+            y[0] = y[1] = l;
+            return;
+        }
     }
     // weights that add up to 1, so that no sum outgrows the values
     for (int t = 0; t < sp.count; ++t) {
@@ -361,6 +365,10 @@ __device__ __forceinline__ void row_alone(const WinArgs& a, int b, int kv, int r
         const float p = __builtin_amdgcn_exp2f(score(at) - m) / l;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += in ? p * elem<DT>(v, at + lane + 64 * e) : 0.0f;
+        bool open = false;  // a column that more keys can still change
+#pragma unroll
+        for (int e = 0; e < E; ++e) open = open || (in && !isnan(acc[e]));
+        if (__builtin_amdgcn_ballot_w64(open) == 0) break;
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) y[e] = e < E ? acc[e < E ? e : 0] : 0.0f;
@@ -774,6 +782,8 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
                            kv_row_stride, out_batch_stride, out_head_stride, out_row_stride};
     for (int i = 0; i < 9; ++i)
         MBRT_REQUIRE(st[i] >= 0 && st[i] % 8 == 0, MBRT_E_ALIGN, "%s: strides must be non-negative multiples of 8", op);
+    MBRT_REQUIRE((B == 1 || out_batch_stride > 0) && (H == 1 || out_head_stride > 0) && (n_q == 1 || out_row_stride > 0),
+                 MBRT_E_SHAPE, "%s: rows of out overlap", op);
     const Plan plan = make_plan(B, H, H_kv, n_q, n_k, head_dim, left, right, std::min(sinks, n_k));
     const int64_t need = workspace_bytes_of(plan, B, H, n_q, head_dim);
     MBRT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 4)), MBRT_E_INVALID_ARG,

@@ -407,8 +407,11 @@ def split_qkv_norm_rotary(qkv: torch.Tensor, q_gamma: torch.Tensor, k_gamma: tor
     with a unit last dim (k and v strided alike).  Query and key heads are RMS-normed (x * scale * gamma /
     sqrt(sum x^2 + eps), scale sqrt(D) by default) and rotated by rows pos0 .. of cos, sin [n_pos, D/2].  v None
     leaves the values in qkv; q and k may be their own places in qkv."""
-    _n.split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v, heads, heads if kv_heads is None else kv_heads,
-                             -1.0 if scale is None else scale, eps, pos0, _h(stream))
+    if kv_heads is None:
+        kv_heads = heads
+    if scale is None:
+        scale = (qkv.shape[-1] // max(heads + 2 * kv_heads, 1)) ** 0.5
+    _n.split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v, heads, kv_heads, scale, eps, pos0, _h(stream))
 
 
 def attention_window_workspace_bytes(B: int, heads: int, kv_heads: int, n_q: int, n_k: int, dim_head: int,

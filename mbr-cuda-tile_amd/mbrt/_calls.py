@@ -247,7 +247,7 @@ def split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v, heads, kv_he
     _unit_last(qkv, q, k, v)
     args = (_p(qkv), _dt(qkv), qkv.stride(0), qkv.stride(1), _p(q_gamma), _p(k_gamma), _dt(q_gamma), _p(cos), _p(sin),
             _dt(cos), cos.shape[0], pos0, _p(q), _p(k), _p(v), _dt(q), *q.stride()[:3], *k.stride()[:3], B, N, heads,
-            kv_heads, D, D ** 0.5 if _float(scale) < 0 else _float(scale), _float(eps))
+            kv_heads, D, _float(scale), _float(eps))
     with _gpu(qkv, q_gamma, k_gamma, cos, sin, q, k, v):
         _abi.call("mbrt_split_qkv_norm_rotary", *args, _s(stream))
 

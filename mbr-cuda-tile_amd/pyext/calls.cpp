@@ -20,7 +20,6 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
-#include <cmath>
 
 #include <vector>
 
@@ -426,7 +425,7 @@ MBRT_PY(linear) {
     END_HANDLE_TH_ERRORS
 }
 
-// split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v | None, heads, kv_heads, scale (< 0: sqrt(D)), eps,
+// split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v | None, heads, kv_heads, scale, eps,
 //                       pos0, stream)
 MBRT_PY(split_qkv_norm_rotary) {
     HANDLE_TH_ERRORS
@@ -454,8 +453,7 @@ MBRT_PY(split_qkv_norm_rotary) {
     contig({&qg, &kg, &c, &s});
     unit_last({&qkv, &q, &k, &v});
     const int dt = dtype_code(qkv), gd = dtype_code(qg), td = dtype_code(c), od = dtype_code(q);
-    const double sc = number(a[10]);
-    const float scale = (float)(sc < 0 ? std::sqrt((double)D) : sc), eps = (float)number(a[11]);
+    const float scale = (float)number(a[10]), eps = (float)number(a[11]);
     const int64_t pos0 = integer(a[12]), n_pos = c.size(0);
     const int64_t z[8] = {qkv.stride(0), qkv.stride(1), q.stride(0), q.stride(1), q.stride(2),
                           k.stride(0), k.stride(1), k.stride(2)};

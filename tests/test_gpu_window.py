@@ -150,6 +150,33 @@ def test_hidden_from_some_rows_only(dev, fill):
             ref.check(got_f, torch.where(finite[..., None], want, 0.0), torch.where(finite[..., None], bound, 1.0), which)
 
 
+def test_everything_nan_ends_early(dev):
+    """Rows that see NaN at once are NaN without a walk over their keys: 64 million query-key pairs here."""
+    import mbrt
+
+    q, k, v = _qkv(2, 1, 8000, 8000, 1, 1, 64, BF16)
+    for t in (q, k, v):
+        kept = t.clone()
+        t.fill_(float("nan"))
+        got = mbrt.attention_window(q, k, v, right=0)
+        torch.cuda.synchronize()
+        assert bool(torch.isnan(got).all())
+        t.copy_(kept)
+
+
+@pytest.mark.parametrize("nq", [1, 30])
+def test_one_column_of_a_value_is_nan(dev, nq):
+    """The other columns, and rows that do not see it, keep their values."""
+    import mbrt
+
+    for D in (32, 128):
+        q, k, v = _qkv(8, 1, nq, 80, 2, 2, D, F16)
+        v[0, 70, 1, 3] = float("nan")
+        got = mbrt.attention_window(q, k, v, left=40, right=0).cpu()
+        want, bound = ref.window(q, k, v, F16, left=40, right=0)
+        ref.check(got, want, bound, "one column")
+
+
 def test_large_scores_and_values(dev):
     """Scores far apart, values near the type's largest: the running maximum and sum must carry them."""
     import mbrt

@@ -52,6 +52,8 @@ def test_split_qkv_norm_rotary_arguments(lib):
         assert call(pos0=pos0, n_pos=n_pos) == SHAPE
         assert "positions" in _err(lib)
     assert call(st=(640, -64, 64, 640, 64, 64)) == SHAPE and call(ns=-1) == SHAPE
+    assert call(st=(640, 64, 0, 640, 64, 64)) == SHAPE and "overlap" in _err(lib)
+    assert call(st=(640, 64, 64, 640, 64, 0)) == SHAPE
     for name in ("qkv", "q", "k", "qg", "kg", "c", "s"):
         assert call(**{name: None}) == ARG
         assert call(**{name: P + 1}) == ALIGN
@@ -78,6 +80,7 @@ def test_attention_window_arguments(lib):
         assert call(**{name: P + 8}) == ALIGN
     assert call(lens=P + 2) == ALIGN and call(gate=P + 2) == ALIGN
     assert call(qs=(25600, 64, 260)) == ALIGN and call(ks=(12800, 4, 128)) == ALIGN and call(os=(25600, 64, -256)) == ALIGN
+    assert call(os=(25600, 0, 256)) == SHAPE and call(os=(25600, 64, 0)) == SHAPE and "overlap" in _err(lib)
     need = lib.mbrt_attention_window_workspace_bytes(1, 4, 2, 1, 50000, 64, -1, 0, 0)
     assert need > 0
     long = dict(nq=1, nk=50000, left=-1, right=0, qs=(256, 64, 256), os=(256, 64, 256))
