@@ -565,6 +565,7 @@ __global__ __launch_bounds__(kSplitWaves * 64) void window_split_kernel(WinArgs 
     v_addresses<D>(g, c, vad);
     for (int i = sa + w; i < sb; i += nw) {
         const int t0 = i * kChunk;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's reads of the V tile are done
 #pragma unroll
         for (int u = 0; u < LD; ++u) {
             const int r = u * RPL + lane / CH;
@@ -707,9 +708,13 @@ struct Plan {
 };
 
 // Few rows (of one tile of 16, or of some while the tiles of 64 would leave CUs idle before long lists) go to the kernel that
-// shares out the keys, a workgroup of 8 waves per CU at least, each with 16 steps of 32 keys or more: one token against
-// [1, 200003] keys of 2 heads 28.8 us; twice the shares 33.5, the join then taking longer; 60 x 8 heads of 805 keys 22.0 with
-// one share each, 26 with three shares of 4 waves.
+// shares out the keys, 8 waves to a share.  What bounds a share is what one CU can read (16 waves to it gain nothing: 805 keys
+// of 64 columns 7.1 us with 8, 7.5 with 16); what a second one costs is the join's launch.  So a list is shared out from 32
+// pieces on, of 32 keys and 64 columns each (8 KB of keys and values), 5 to a share, over at most a workgroup per CU, and shorter ones
+// than 64 pieces only where there are 4 shares or more to it.  us, one share and shared out: 16 lists of 25 pieces 7.3 and
+// 8.7, of 38 9.3 and 8.7, of 50 11.9 and 9.4, of 63 13.4 and 9.6; 80 lists of 38 9.7 and 11.0; 120 of 50 14.5
+// and 14.8, of 58 17.5 and 16.8.
+// One token against [1, 200003] keys of 2 heads 24.7 with a workgroup per CU; with two each, the join taking longer, 33.5.
 // Of 128 columns, 32 rows per wave use each fragment read from LDS twice, which pays where lists are long and the larger
 // tiles still fill the CUs: [2, 16389] f16 over 1024 keys 259 -> 216 us, [16, 801] bf16 over all 109 -> 103; over 300 keys [30, 801]
 // 90 -> 92, over 100 72 -> 76.  Of 64 columns they gain nothing: [60, 801] over all keys 162 -> 160, over 101 60 -> 69.
@@ -719,11 +724,12 @@ Plan make_plan(int64_t B, int64_t H, int64_t KV, int64_t nq, int64_t nk, int64_t
     const int64_t cus = cu_count(), rows = nq * (H / KV);
     // the most keys that a tile of rows may see
     int64_t span = nk;
-    if (left >= 0 && right >= 0) span = std::min(nk, sinks + left + right + std::min<int64_t>(nq, 64));
+    if (left >= 0 && right >= 0) span = std::min(nk, sinks + std::min(left, nk) + std::min(right, nk) + std::min<int64_t>(nq, 64));
     p.few = rows <= 16 || (rows <= 256 && B * KV * ceil_div(rows, 64) < cus && span > 1024);
     p.qs = D == 128 && span >= 512 && B * KV * ceil_div(rows, 128) >= 2 * cus ? 2 : 1;
-    const int64_t tiles = B * KV * ceil_div(rows, 16), steps = ceil_div(span, kChunk);
-    p.splits = p.few ? std::max<int64_t>(1, std::min<int64_t>(std::min(cus / tiles, steps / 16), kJoinWaves * 64)) : 1;
+    const int64_t tiles = B * KV * ceil_div(rows, 16), pieces = ceil_div(span, kChunk) * D / 64;
+    const int64_t shares = std::min<int64_t>(std::min(cus / tiles, ceil_div(pieces, 5)), kJoinWaves * 64);
+    p.splits = p.few && pieces >= (shares >= 4 ? 32 : 64) && shares > 1 ? shares : 1;
     return p;
 }
 
