@@ -2,9 +2,26 @@
 #include "linear.hpp"
 
 namespace mbrt {
-template int launch_linear<F32>(LinArgs& a, bool al, hipStream_t st);
-extern template int launch_linear<BF16>(LinArgs& a, bool al, hipStream_t st);
-extern template int launch_linear<F16>(LinArgs& a, bool al, hipStream_t st);
+namespace {
+
+// K of nothing: act(bias) + residual, one thread per element.
+__global__ __launch_bounds__(256) void linear_empty_kernel(LinArgs a) {
+    const int64_t total = a.M * a.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / a.N;
+        const int n = (int)(i - m * a.N);
+        float v[1] = {0.0f};
+        Bias<1> bias;
+        bias.load(a, n);
+        finish<true, 0, 1>(a, m, n, v, bias);
+    }
+}
+
+}  // namespace
+
+template int launch_linear<F32>(LinArgs& a, int align, hipStream_t st);
+extern template int launch_linear<BF16>(LinArgs& a, int align, hipStream_t st);
+extern template int launch_linear<F16>(LinArgs& a, int align, hipStream_t st);
 }  // namespace mbrt
 
 using namespace mbrt;
@@ -58,10 +75,13 @@ int mbrt_linear(const void* x, int dtype, int64_t x_row_stride, const void* weig
                            dim3(256), 0, st, a);
         return check_launch(op);
     }
-    const bool al = aligned(x, 16) && aligned(weight, 16) && a.xs % 16 == 0 && a.ws % 16 == 0;
-    const int status = dtype == F32    ? launch_linear<F32>(a, al, st)
-                       : dtype == BF16 ? launch_linear<BF16>(a, al, st)
-                                       : launch_linear<F16>(a, al, st);
+    auto rows_at = [&](int64_t bytes) {
+        return aligned(x, bytes) && aligned(weight, bytes) && a.xs % bytes == 0 && a.ws % bytes == 0;
+    };
+    const int align = rows_at(16) ? 16 : rows_at(4) ? 4 : 2;
+    const int status = dtype == F32    ? launch_linear<F32>(a, align, st)
+                       : dtype == BF16 ? launch_linear<BF16>(a, align, st)
+                                       : launch_linear<F16>(a, align, st);
     return status == MBRT_OK ? check_launch(op) : status;
 }
 

@@ -2,5 +2,5 @@
 #include "linear.hpp"
 
 namespace mbrt {
-template int launch_linear<BF16>(LinArgs& a, bool al, hipStream_t st);
+template int launch_linear<BF16>(LinArgs& a, int align, hipStream_t st);
 }  // namespace mbrt

@@ -35,9 +35,9 @@ struct LinArgs {
     FastDiv groups, splits;  // ntiles and split
 };
 
-// The linear layer for operands of one dtype; al: rows are 16-byte aligned.  Instantiated in a source file per dtype.
+// The linear layer for operands of one dtype; align: all rows of x and w begin at multiples of it, 16, 4 or 2 bytes.  Instantiated in a source file per dtype.
 template <int DT>
-int launch_linear(LinArgs& a, bool al, hipStream_t st);
+int launch_linear(LinArgs& a, int align, hipStream_t st);
 
 namespace {
 
@@ -79,20 +79,52 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     }
 }
 
-// The 16 bytes of a row of K elements that start at byte kb, zeros behind its end; at any alignment
-// (ALIGNED: of 16 bytes, where the piece is whole).
-template <int DT, bool ALIGNED>
+// 16 bytes of a row at a multiple of A bytes: 16, 4 or 2.  Loads at odd multiples of 2 are several times slower than others,
+// so with A = 2 they come as the 20 bytes around them, moved down: the dwords at both ends hold an element of the 16 bytes
+// each, and nothing outside these dwords is read ([48060, 385] -> 8 25.8 -> 14.4 us, [60, 385] -> 1536 7.9 -> 4.7; with A = 4
+// the fifth dword costs: [20000, 500] -> 48 15.3 -> 25.7).
+template <int A>
+__device__ __forceinline__ u32x4 load_row(const char* p) {
+    if constexpr (A == 16) {
+        return *reinterpret_cast<const u32x4*>(p);
+    } else if constexpr (A == 4) {
+        return ld_any<0, 4>(p);
+    } else {
+        const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 2;
+        const char* q = p - off;
+        const u32x4 v = ld_any<0, 4>(q);
+        const uint32_t last = *reinterpret_cast<const uint32_t*>(q + 12 + 2 * off);  // at a multiple of 4: v[3] again
+        return u32x4{__builtin_amdgcn_alignbit(v[1], v[0], 8 * off), __builtin_amdgcn_alignbit(v[2], v[1], 8 * off),
+                     __builtin_amdgcn_alignbit(v[3], v[2], 8 * off), __builtin_amdgcn_alignbit(last, v[3], 8 * off)};
+    }
+}
+
+// The 16 bytes of a row of K elements that start at byte kb, zeros behind its end; at any alignment.  Where the end cuts
+// 2-byte elements, the 16 bytes that end there are read and moved down: one load without a branch, so that many can be
+// under way ([801, 118] -> 384 4.7 -> 4.4 us; the three elements that f32 may have there come as fast one by one).
+template <int DT>
 __device__ __forceinline__ u32x4 row_piece(const char* row, int64_t kb, int K) {
     constexpr int S = DT == F32 ? 4 : 2, VE = 16 / S;
-    const int64_t left = (int64_t)K * S - kb;
-    if (left >= 16) {
-        if constexpr (ALIGNED) return *reinterpret_cast<const u32x4*>(row + kb);
-        else return ld_any<0, S>(row + kb);
+    const int64_t bytes = (int64_t)K * S;
+    if (S == 2 && bytes >= 16) {
+        const int64_t at = min(kb, bytes - 16);
+        const u32x4 v = ld_any<0, S>(row + at);
+        const int drop = (int)min<int64_t>(kb - at, 16);
+        uint64_t lo = v[0] | (uint64_t)v[1] << 32, hi = v[2] | (uint64_t)v[3] << 32;
+        if ((drop & 8) != 0) {
+            lo = hi;
+            hi = 0;
+        }
+        const int sh = 8 * (drop & 7);
+        lo = drop == 16 ? 0 : lo >> sh | (hi << 1) << (63 - sh);
+        hi = drop == 16 ? 0 : hi >> sh;
+        return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     }
+    if (bytes - kb >= 16) return ld_any<0, S>(row + kb);
     u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int j = 0; j < VE - 1; ++j) {
-        if (left > (int64_t)j * S) {
+        if (bytes - kb > (int64_t)j * S) {
             if constexpr (S == 4) v[j] = reinterpret_cast<const uint32_t*>(row + kb)[j];
             else v[j / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(row + kb)[j] << (16 * (j & 1));
         }
@@ -194,7 +226,16 @@ __device__ __forceinline__ void store_run(void* p, int dt, int64_t e, const floa
             for (int i = 0; i < 4; ++i)
                 t[i] = dt == BF16 ? pack_bf16x2(f[8 * q + 2 * i], f[8 * q + 2 * i + 1])
                                   : pack_f16x2(f[8 * q + 2 * i], f[8 * q + 2 * i + 1]);
-            st_any<NT, 2>(b + 16 * q, t);
+            char* d = b + 16 * q;
+            if (NT != 0 || (reinterpret_cast<uintptr_t>(b) & 2) == 0) {
+                st_any<NT, 4>(d, t);
+            } else {  // stores at odd multiples of 2 are as slow as loads: [48060, 384] -> 385 42.5 -> 35.5 us
+                *reinterpret_cast<uint16_t*>(d) = (uint16_t)t[0];
+                *reinterpret_cast<uint32_t*>(d + 2) = __builtin_amdgcn_alignbit(t[1], t[0], 16);
+                *reinterpret_cast<uint32_t*>(d + 6) = __builtin_amdgcn_alignbit(t[2], t[1], 16);
+                *reinterpret_cast<uint32_t*>(d + 10) = __builtin_amdgcn_alignbit(t[3], t[2], 16);
+                *reinterpret_cast<uint16_t*>(d + 14) = (uint16_t)(t[3] >> 16);
+            }
         }
     } else {
 #pragma unroll
@@ -337,10 +378,10 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < LX; ++u)
-            px[u] = row_piece<DT, DIRECT>(xb + xr[u] * a.xs, (int64_t)kt * SB + 16 * ((lane % 8) ^ key_x(8 * (LX * w + u) + lane / 8)), a.K);
+            px[u] = row_piece<DT>(xb + xr[u] * a.xs, (int64_t)kt * SB + 16 * ((lane % 8) ^ key_x(8 * (LX * w + u) + lane / 8)), a.K);
 #pragma unroll
         for (int u = 0; u < LW; ++u)
-            pw[u] = row_piece<DT, DIRECT>(wb + wr[u] * a.ws, (int64_t)kt * SB + 16 * ((lane % 8) ^ key_w(8 * (LW * w + u) + lane / 8)), a.K);
+            pw[u] = row_piece<DT>(wb + wr[u] * a.ws, (int64_t)kt * SB + 16 * ((lane % 8) ^ key_w(8 * (LW * w + u) + lane / 8)), a.K);
     };
     auto put_regs = [&](char* d) {
 #pragma unroll
@@ -438,7 +479,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
 // its stores.
 // WIDE: strips of w (16 columns of out) against groups of 16 R rows of x; else strips of x against groups of 16 R columns.
 // The groups of one strip are neighbours.
-template <int DT, int R, bool WIDE, bool ALIGNED>
+template <int DT, int R, bool WIDE, int A>
 __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
     constexpr int S = DT == F32 ? 4 : 2;
     extern __shared__ f32x4 part[];  // [strips of the block][split][R][64]
@@ -474,9 +515,9 @@ __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 const int64_t kb = (int64_t)(t0 + u * a.split) * 128 + 64 * s;
-                pf[u][s] = ALIGNED ? *reinterpret_cast<const u32x4*>(pb + kb) : ld_any<0, S>(pb + kb);
+                pf[u][s] = load_row<A>(pb + kb);
 #pragma unroll
-                for (int r = 0; r < R; ++r) qf[u][s][r] = ALIGNED ? *reinterpret_cast<const u32x4*>(qb[r] + kb) : ld_any<0, S>(qb[r] + kb);
+                for (int r = 0; r < R; ++r) qf[u][s][r] = load_row<A>(qb[r] + kb);
             }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -486,7 +527,7 @@ __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
                 for (int r = 0; r < R; ++r)
                     acc[r] = WIDE ? mma<DT>(pf[u][s], qf[u][s][r], acc[r]) : mma<DT>(qf[u][s][r], pf[u][s], acc[r]);
     };
-    constexpr int U = R >= 4 ? 2 : R == 2 ? 3 : 6;
+    constexpr int U = R >= 4 ? (A == 2 ? 1 : 2) : R == 2 ? 3 : 6;
     int t0 = ks;
     for (; t0 + (U - 1) * a.split < whole; t0 += U * a.split) pieces(std::integral_constant<int, U>(), t0);
     for (; t0 < whole; t0 += a.split) pieces(std::integral_constant<int, 1>(), t0);
@@ -494,10 +535,11 @@ __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int64_t kb = (int64_t)whole * 128 + 64 * s + 16 * g;
-            const u32x4 pf = row_piece<DT, ALIGNED>(pb - 16 * g, kb, a.K);
+            if (kb - 16 * g >= kbytes) break;
+            const u32x4 pf = row_piece<DT>(pb - 16 * g, kb, a.K);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const u32x4 qf = row_piece<DT, ALIGNED>(qb[r] - 16 * g, kb, a.K);
+                const u32x4 qf = row_piece<DT>(qb[r] - 16 * g, kb, a.K);
                 acc[r] = WIDE ? mma<DT>(pf, qf, acc[r]) : mma<DT>(qf, pf, acc[r]);
             }
         }
@@ -526,25 +568,18 @@ __global__ __launch_bounds__(1024) void linear_strip_kernel(LinArgs a) {
     }
 }
 
-// K of nothing: act(bias) + residual, one thread per element.
-__global__ __launch_bounds__(256) void linear_empty_kernel(LinArgs a) {
-    const int64_t total = a.M * a.N;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / a.N;
-        const int n = (int)(i - m * a.N);
-        float v[1] = {0.0f};
-        Bias<1> bias;
-        bias.load(a, n);
-        finish<true, 0, 1>(a, m, n, v, bias);
-    }
-}
-
 template <int DT, int R>
-void launch_strip(const LinArgs& a, bool wide, bool al, unsigned blocks, unsigned threads, size_t lds, hipStream_t st) {
-    if (wide && al) hipLaunchKernelGGL((linear_strip_kernel<DT, R, true, true>), dim3(blocks), dim3(threads), lds, st, a);
-    else if (wide) hipLaunchKernelGGL((linear_strip_kernel<DT, R, true, false>), dim3(blocks), dim3(threads), lds, st, a);
-    else if (al) hipLaunchKernelGGL((linear_strip_kernel<DT, R, false, true>), dim3(blocks), dim3(threads), lds, st, a);
-    else hipLaunchKernelGGL((linear_strip_kernel<DT, R, false, false>), dim3(blocks), dim3(threads), lds, st, a);
+void launch_strip(const LinArgs& a, bool wide, int align, unsigned blocks, unsigned threads, size_t lds, hipStream_t st) {
+    auto launch = [&](auto bytes) {
+        constexpr int A = decltype(bytes)::value;
+        if (wide) hipLaunchKernelGGL((linear_strip_kernel<DT, R, true, A>), dim3(blocks), dim3(threads), lds, st, a);
+        else hipLaunchKernelGGL((linear_strip_kernel<DT, R, false, A>), dim3(blocks), dim3(threads), lds, st, a);
+    };
+    if (align == 16) return launch(std::integral_constant<int, 16>());
+    if constexpr (DT != F32) {
+        if (align == 2) return launch(std::integral_constant<int, 2>());
+    }
+    launch(std::integral_constant<int, 4>());
 }
 
 template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, int NT>
@@ -562,19 +597,44 @@ int launch_tile(LinArgs& a, hipStream_t st) {
     return MBRT_OK;
 }
 
+// Tiles of 96 or 128 by 192, two workgroups to a CU: the height whose rounds over the CUs take fewer rows (the larger at a
+// tie, for its reuse).  bf16 us, 96 and 128 rows: [48060, 384] -> 1536, 8 and 6 rounds, 79 and 70; [48060, 1536] -> 384, 2
+// and 2 rounds, 93 and 95; [48060, 512] -> 384 43 and 51; [4096, 4096] -> 4096, 2 and 2, 127 and 137.
+template <int DT>
+int launch_large(LinArgs& a, bool direct, hipStream_t st) {
+    const int64_t cus = cu_count();
+    auto rounds = [&](int64_t bm, int64_t bn) { return ceil_div(ceil_div(a.M, bm) * ceil_div(a.N, bn), 2 * cus); };
+    // Past the caches where a wave's stores fill whole 64-byte pieces; cut ones need the cache to put them together: bf16
+    // [20000, 393] -> 500 40 -> 32 us through it, [48060, 385] -> 384 52 -> 37 past it.
+    const int64_t ob = dt_size(a.odt);
+    const bool nt = aligned(a.out, 64) && a.os * ob % 64 == 0;
+    if (!direct) return nt ? launch_tile<DT, 2, 2, 3, 6, false, 2>(a, st) : launch_tile<DT, 2, 2, 3, 6, false, 0>(a, st);
+    if (96 * rounds(96, 192) < 128 * rounds(128, 192))
+        return nt ? launch_tile<DT, 2, 2, 3, 6, true, 2>(a, st) : launch_tile<DT, 2, 2, 3, 6, true, 0>(a, st);
+    return nt ? launch_tile<DT, 2, 2, 4, 6, true, 2>(a, st) : launch_tile<DT, 2, 2, 4, 6, true, 0>(a, st);
+}
+
 }  // namespace
 
 template <int DT>
-int launch_linear(LinArgs& a, bool al, hipStream_t st) {
+int launch_linear(LinArgs& a, int align, hipStream_t st) {
+    const bool al = align == 16;
     const int64_t es = DT == F32 ? 4 : 2, cus = cu_count();
     const bool wide = a.M <= a.N;
     const int64_t shorter = wide ? a.M : a.N, longer = wide ? a.N : a.M;
     const int64_t strips = ceil_div(longer, 16);
-    // Strips, where one operand is short, or where tiles would leave CUs idle; of as few rows per wave as there are CUs
-    // for.  Rows at odd alignments, which tiles take through registers step by step, go in strips up to twice as
-    // far, spread eight times as wide.  us, tiles and strips: bf16 [200, 1536] -> 384 8.5 and 7.0, f32 31 and 11.3; [120,
-    // 1536] -> 384 9.0 and 5.8, f32 31 and 8.2; [801, 384] -> 384 4.6 and 7.0; [801, 118] -> 384 6.2 and 5.0, f32 7.0 and 5.2.
-    if (shorter <= 64 || strips * ceil_div(shorter, 64) <= (al ? 1 : 2) * cus) {
+    // Strips, where tiles would leave CUs idle, of as few rows per wave as there are CUs for; rows at odd alignments, which
+    // tiles take through registers step by step, go in strips up to twice as far, spread eight times as wide.  us,
+    // tiles and strips: bf16 [200, 1536] -> 384 8.5 and 7.0, f32 31 and 11.3; [120, 1536] -> 384 9.0 and 5.8, f32 31 and 8.2;
+    // [801, 384] -> 384 4.6 and 7.0; [801, 118] -> 384 6.2 and 4.3, f32 7.0 and 4.9.
+    // A short operand of up to 16 rows goes in strips too, which multiply no 16 rows in vain where tiles multiply 64: always
+    // for f32, whose products count ([48060, 384] -> 8 25 and 18; up to 32 rows while tiles are few, [5000, 1536] -> 24 31 and 18,
+    // but [48060, 1536] -> 24 81 and 93), and for 2-byte types where tiles of 64 are few or
+    // short ([10000, 384] -> 8 5.4 and 4.3, [48060, 130] -> 8 6.8 and 5.6, but [48060, 384] -> 16 8.4 and 10.5, [8, 384] ->
+    // 20000 4.4 and 6.5, [48060, 1536] -> 8 30 and 34).
+    if (strips * ceil_div(shorter, 64) <= (al ? 1 : 2) * cus ||
+        (shorter <= 16 && (DT == F32 || longer < 64 * cus || a.K * es < 768)) ||
+        (DT == F32 && shorter <= 32 && longer < 64 * cus)) {
         int R = shorter <= 16 ? 1 : shorter <= 32 ? 2 : 4;
         while (R > 1 && strips * ceil_div(shorter, 8 * R) <= (al ? 1 : 8) * cus) R /= 2;
         const int64_t groups = ceil_div(shorter, 16 * R), pairs = ceil_div(a.K * es, 128);
@@ -590,28 +650,21 @@ int launch_linear(LinArgs& a, bool al, hipStream_t st) {
         if (blocks >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many rows");
         const size_t lds = a.split == 1 ? 0 : (size_t)per_block * a.split * R * 1024;
         const unsigned threads = per_block * a.split * 64;
-        if (R == 1) launch_strip<DT, 1>(a, wide, al, (unsigned)blocks, threads, lds, st);
-        else if (R == 2) launch_strip<DT, 2>(a, wide, al, (unsigned)blocks, threads, lds, st);
-        else launch_strip<DT, 4>(a, wide, al, (unsigned)blocks, threads, lds, st);
+        if (R == 1) launch_strip<DT, 1>(a, wide, align, (unsigned)blocks, threads, lds, st);
+        else if (R == 2) launch_strip<DT, 2>(a, wide, align, (unsigned)blocks, threads, lds, st);
+        else launch_strip<DT, 4>(a, wide, align, (unsigned)blocks, threads, lds, st);
         return MBRT_OK;
     }
     // 32-bit offsets within a tile
     const bool direct = al && a.xs < (int64_t(1) << 22) && a.ws < (int64_t(1) << 22);
-    // Large tiles, two workgroups to a CU, once there are enough of them; of two heights the one whose rounds over the
-    // CUs take fewer rows (the larger at a tie, for its reuse).  bf16 us, 96 and 128 rows: [48060, 384] -> 1536, 8 and 6
-    // rounds, 79 and 70; [48060, 1536] -> 384, 2 and 2 rounds, 93 and 95; [48060, 512] -> 384 43 and 51; [4096, 4096]
-    // -> 4096, 2 and 2, 127 and 137.
-    auto rounds = [&](int64_t bm, int64_t bn) { return ceil_div(ceil_div(a.M, bm) * ceil_div(a.N, bn), 2 * cus); };
-    const bool big = ceil_div(a.M, 96) * ceil_div(a.N, 192) >= cus;
+    // Tiles of 64 x 64 until larger ones fill the CUs, and for a short operand that one of them holds (bf16 us, large
+    // and small: [48060, 384] -> 64 11.0 and 9.5, -> 128 12.0 and 14.1, [50, 384] -> 60000 12.7 and 10.8).  For f32 always: its
+    // products bound it either way, and small tiles compute fewer columns in vain ([48060, 384] -> 128 60 and 45, -> 384 119 and
+    // 117; [4096, 4096] -> 4096 1050 and 990, 139 TFLOP/s).
+    const bool big = DT != F32 && shorter > 64 && ceil_div(a.M, 96) * ceil_div(a.N, 192) >= cus;
     if (!big) return direct ? launch_tile<DT, 2, 2, 2, 2, true, 0>(a, st) : launch_tile<DT, 2, 2, 2, 2, false, 0>(a, st);
-    // Past the caches where a wave's stores fill whole 64-byte pieces; cut ones need the cache to put them together: bf16
-    // [20000, 393] -> 500 40 -> 32 us through it, [48060, 385] -> 384 52 -> 37 past it.
-    const int64_t ob = dt_size(a.odt);
-    const bool nt = aligned(a.out, 64) && a.os * ob % 64 == 0;
-    if (!direct) return nt ? launch_tile<DT, 2, 2, 3, 6, false, 2>(a, st) : launch_tile<DT, 2, 2, 3, 6, false, 0>(a, st);
-    if (96 * rounds(96, 192) < 128 * rounds(128, 192))
-        return nt ? launch_tile<DT, 2, 2, 3, 6, true, 2>(a, st) : launch_tile<DT, 2, 2, 3, 6, true, 0>(a, st);
-    return nt ? launch_tile<DT, 2, 2, 4, 6, true, 2>(a, st) : launch_tile<DT, 2, 2, 4, 6, true, 0>(a, st);
+    if constexpr (DT != F32) return launch_large<DT>(a, direct, st);
+    return MBRT_OK;
 }
 
 }  // namespace mbrt

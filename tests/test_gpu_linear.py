@@ -49,6 +49,21 @@ def test_large_tiles(dev, rows, k, n, dtype):
     _case(dev, rows, k, n, dtype, res=dtype, seed=3)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,k,n", [(16500, 384, 9), (16400, 96, 5), (6, 385, 16500), (5000, 130, 24), (5001, 66, 40),
+                                      (30, 131, 4200), (50, 129, 49200)])
+def test_short_operands(dev, rows, k, n, dtype):
+    """Many rows against few columns and the other way round: strips and small tiles, in rows at every alignment."""
+    _case(dev, rows, k, n, dtype, res=dtype, seed=rows)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("out", [F16, F32])
+@pytest.mark.parametrize("rows,k,n", [(33, 67, 41), (700, 129, 131), (2600, 64, 1537), (90, 7, 129)])
+def test_odd_rows_in_and_out(dev, rows, k, n, dtype, out):
+    _case(dev, rows, k, n, dtype, out, act=2, res=out, seed=9)
+
+
 @pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (F16, F32), (F32, F16), (BF16, F32)])
 @pytest.mark.parametrize("rows,k,n", [(3, 96, 70), (150, 96, 70), (90, 96, 8)])
