@@ -145,6 +145,14 @@ __device__ __forceinline__ float gelu_short(float x, float s) {
     return fmaf(-fabsf(x), p, fmaxf(x, 0.0f));
 }
 
+// tanh x = 1 - 2 / (e^2x + 1), and the first terms of its series where that cancels (relative error 3.3e-7 at 1/4).
+__device__ __forceinline__ float tanh_short(float x) {
+    const float x2 = x * x;
+    const float near = x * fmaf(x2, fmaf(x2, fmaf(x2, -0.0539682540f, 0.1333333333f), -0.3333333333f), 1.0f);
+    const float far = fmaf(-2.0f, fast_rcp(1.0f + __builtin_amdgcn_exp2f(fabsf(x) * 2.88539008177792681f)), 1.0f);
+    return fabsf(x) < 0.25f ? near : copysignf(far, x);
+}
+
 // f32 results take the library's erfc and tanh, 2-byte ones the short forms that bias_act uses for them (errors of
 // 1.5e-7 and less beside their half steps of 2^-9 and 2^-12).
 template <int NV>
@@ -163,8 +171,13 @@ __device__ __forceinline__ void activate(float (&v)[NV], int act, bool f32_out) 
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = sigmoidf(v[i]);
     } else if (act == MBRT_ACT_TANH) {
+        if (f32_out) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = tanhf(v[i]);
+            for (int i = 0; i < NV; ++i) v[i] = tanhf(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = tanh_short(v[i]);
+        }
     }
 }
 
@@ -311,22 +324,26 @@ __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int n, float
 // the A operand: a lane's four results of a block are four columns of one row of out, and two blocks 2 p, 2 p + 1 take
 // the columns 32 p + 8 q + 4 (ni % 2) + j (q = c / 4, j = c % 4) of the wave's, so that a lane ends with 8 columns in a
 // row, and a store of 16 bytes per lane fills 64 bytes in a row of out.
+// KS groups of such waves take the steps in turn and are added at the end.
 // DIRECT: rows are 16-byte aligned, and whole steps go from global memory straight into LDS.  NT: out is stored past the
 // caches: a large one would push x and w out of them.
 __device__ __forceinline__ int key_x(int r) { return r & 7; }
 __device__ __forceinline__ int key_w(int r) { return (r & 3) | (((r >> 3) & 1) << 2); }
 
-template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, int NT, bool ACT>
-__global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
+template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, int NT, int KS, bool ACT>
+__global__ __launch_bounds__(WM * WN * KS * 64) void linear_tile_kernel(LinArgs a) {
     constexpr int NW = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16;
     constexpr int S = DT == F32 ? 4 : 2;
     constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW;  // loads of 1 KB, 8 rows, per wave and step
     static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NI % 2 == 0, "whole loads per wave, blocks in pairs");
     constexpr int SB = kStepBytes, kBuf = (BM + BN) * SB;
-    __shared__ __attribute__((aligned(16))) char s0[kBuf];
-    __shared__ __attribute__((aligned(16))) char s1[kBuf];
+    __shared__ __attribute__((aligned(16))) char s0[KS * kBuf];
+    __shared__ __attribute__((aligned(16))) char s1[KS * kBuf];
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
-    const int w = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int kg = KS == 1 ? 0 : wave / NW, w = KS == 1 ? wave : wave % NW;
+    char* const mine0 = s0 + kg * kBuf;
+    char* const mine1 = s1 + kg * kBuf;
     const int wm = w / WN, wn = w % WN;
     // column tiles of one row tile are neighbours, on one XCD: x is read once into its L2
     const uint32_t tile = xcd_tile(blockIdx.x, gridDim.x);
@@ -420,25 +437,26 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
         // then costs reuse ([4096, 4096] -> 4096: 127 -> 146).
         const int first = a.ntiles <= 4 ? (int)(nt * (uint32_t)whole / a.ntiles) : 0;
         auto at = [&](int kt) { return kt + first < whole ? kt + first : kt + first - whole; };
-        // Step kt sits in d, the next one goes to dn, which held step kt - 1.  The buffers are separate objects and the
-        // loop is unrolled by two, so that the compiler sees that loads in flight into one do not touch the other.
+        // Step kt of this group sits in d, its next one goes to dn, which held the one before.  The buffers are separate
+        // objects and the loop is unrolled by two, so that the compiler sees that loads in flight into one do not touch the
+        // other.
         auto step = [&](int kt, const char* d, char* dn) {
             wait_loads();
             lds_barrier();  // every wave's loads have landed, and none still reads dn
-            if (kt + 1 < whole) load_direct(at(kt + 1), dn);
-            compute(d);
+            if (kt + KS < whole) load_direct(at(kt + KS), dn);
+            if (KS == 1 || kt < whole) compute(d);
         };
-        if (whole > 0) load_direct(at(0), s0);
-        for (int kt = 0; kt < whole; kt += 2) {
-            step(kt, s0, s1);
-            if (kt + 1 < whole) step(kt + 1, s1, s0);
+        if (kg < whole) load_direct(at(kg), mine0);
+        for (int kt = 0; kt < whole; kt += 2 * KS) {
+            step(kt + kg, mine0, mine1);
+            if (kt + KS < whole) step(kt + KS + kg, mine1, mine0);
         }
-        if (steps > whole) {
-            load_regs(whole);
+        if (steps > whole) {  // the first group takes what the rows' end cuts
+            if (kg == 0) load_regs(whole);
             __syncthreads();  // none still reads s0
-            put_regs(s0);
+            if (kg == 0) put_regs(s0);
             __syncthreads();
-            compute(s0);
+            if (kg == 0) compute(s0);
         }
     } else {
         // through registers: the next step's loads are issued before a step is computed and written to LDS after it
@@ -458,18 +476,38 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinArgs a) {
         }
     }
 
+    if constexpr (KS > 1) {  // the groups' sums, added in their order; group mi ends with the blocks mi
+        static_assert(BM * BN * 4 <= kBuf && MI <= KS, "room for the sums, a group for each");
+        __syncthreads();  // none still reads s0
+        f32x4* all = reinterpret_cast<f32x4*>(s0) + w * MI * NI * 64 + lane;
+        constexpr int kGroup = kBuf / 16;
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) all[kg * kGroup + (mi * NI + ni) * 64] = acc[mi][ni];
+        __syncthreads();
+        if (kg >= MI) return;
+#pragma unroll
+        for (int ni = 0; ni < NI; ++ni) {
+            f32x4 sum = all[(kg * NI + ni) * 64];
+#pragma unroll
+            for (int k = 1; k < KS; ++k) sum += all[k * kGroup + (kg * NI + ni) * 64];
+            acc[0][ni] = sum;
+        }
+    }
+
     const int n = n0 + wn * NI * 16 + 8 * g;
     Bias<8> bias[NI / 2];
 #pragma unroll
     for (int p = 0; p < NI / 2; ++p) bias[p].load(a, n + 32 * p);
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
+    for (int mi = 0; mi < (KS > 1 ? 1 : MI); ++mi)
 #pragma unroll
         for (int p = 0; p < NI / 2; ++p) {
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = acc[mi][2 * p + i / 4][i % 4];
-            finish<ACT, NT, 8>(a, m0 + wm * MI * 16 + mi * 16 + c, n + 32 * p, v, bias[p]);
+            finish<ACT, NT, 8>(a, m0 + wm * MI * 16 + (KS > 1 ? kg : mi) * 16 + c, n + 32 * p, v, bias[p]);
         }
 }
 
@@ -582,18 +620,18 @@ void launch_strip(const LinArgs& a, bool wide, int align, unsigned blocks, unsig
     launch(std::integral_constant<int, 4>());
 }
 
-template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, int NT>
+template <int DT, int WM, int WN, int MI, int NI, bool DIRECT, int NT, int KS = 1>
 int launch_tile(LinArgs& a, hipStream_t st) {
     constexpr int BM = WM * MI * 16, BN = WN * NI * 16;
     a.ntiles = (uint32_t)ceil_div(a.N, BN);
     a.groups = make_fastdiv(a.ntiles);
     const int64_t tiles = ceil_div(a.M, BM) * a.ntiles;
     if (tiles >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many tiles");
-    const dim3 grid((unsigned)tiles), block(WM * WN * 64);
+    const dim3 grid((unsigned)tiles), block(WM * WN * KS * 64);
     if (a.act != MBRT_ACT_NONE)
-        hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, DIRECT, NT, true>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, DIRECT, NT, KS, true>), grid, block, 0, st, a);
     else
-        hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, DIRECT, NT, false>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, DIRECT, NT, KS, false>), grid, block, 0, st, a);
     return MBRT_OK;
 }
 
@@ -623,16 +661,17 @@ int launch_linear(LinArgs& a, int align, hipStream_t st) {
     const bool wide = a.M <= a.N;
     const int64_t shorter = wide ? a.M : a.N, longer = wide ? a.N : a.M;
     const int64_t strips = ceil_div(longer, 16);
-    // Strips, where tiles would leave CUs idle, of as few rows per wave as there are CUs for; rows at odd alignments, which
-    // tiles take through registers step by step, go in strips up to twice as far, spread eight times as wide.  us,
-    // tiles and strips: bf16 [200, 1536] -> 384 8.5 and 7.0, f32 31 and 11.3; [120, 1536] -> 384 9.0 and 5.8, f32 31 and 8.2;
-    // [801, 384] -> 384 4.6 and 7.0; [801, 118] -> 384 6.2 and 4.3, f32 7.0 and 4.9.
+    // Strips, where tiles would leave most CUs idle (f32, bound by its products sooner: any), of as few rows per wave as there
+    // are CUs for; rows at odd alignments, which tiles take through registers step by step, go in strips up to twice as far,
+    // spread eight times as wide.  us, tiles and strips: bf16 [200, 1536] -> 384 8.5 and 6.7, [124, 1536] -> 1536 6.8 and
+    // 9.7, [120, 384] -> 1536 4.1 and 4.7; f32 17 at [124, 1536] -> 1536 and 26 in tiles, [200, 384] -> 1536 9.5 and 9.7,
+    // [1000, 1536] -> 384 26.5 and 31.3; [801, 118] -> 384 bf16 6.2 and 4.3, f32 7.0 and 4.9.
     // A short operand of up to 16 rows goes in strips too, which multiply no 16 rows in vain where tiles multiply 64: always
     // for f32, whose products count ([48060, 384] -> 8 25 and 18; up to 32 rows while tiles are few, [5000, 1536] -> 24 31 and 18,
     // but [48060, 1536] -> 24 81 and 93), and for 2-byte types where tiles of 64 are few or
     // short ([10000, 384] -> 8 5.4 and 4.3, [48060, 130] -> 8 6.8 and 5.6, but [48060, 384] -> 16 8.4 and 10.5, [8, 384] ->
     // 20000 4.4 and 6.5, [48060, 1536] -> 8 30 and 34).
-    if (strips * ceil_div(shorter, 64) <= (al ? 1 : 2) * cus ||
+    if (strips * ceil_div(shorter, 64) <= (DT == F32 ? (al ? 1 : 2) * cus : (al ? 1 : 4) * cus / 2) ||
         (shorter <= 16 && (DT == F32 || longer < 64 * cus || a.K * es < 768)) ||
         (DT == F32 && shorter <= 32 && longer < 64 * cus)) {
         int R = shorter <= 16 ? 1 : shorter <= 32 ? 2 : 4;
@@ -662,6 +701,16 @@ int launch_linear(LinArgs& a, int align, hipStream_t st) {
     // products bound it either way, and small tiles compute fewer columns in vain ([48060, 384] -> 128 60 and 45, -> 384 119 and
     // 117; [4096, 4096] -> 4096 1050 and 990, 139 TFLOP/s).
     const bool big = DT != F32 && shorter > 64 && ceil_div(a.M, 96) * ceil_div(a.N, 192) >= cus;
+    // Few tiles leave a CU with four waves, which wait for their loads and for each other step by step: 2 or 4 groups of them
+    // take the steps in turn, each in buffers of its own, and are added through LDS.  us with 1, 2 and 4 groups: bf16 [444,
+    // 1536] -> 1536 (168 tiles) 14.3, 11.3 and 9.9, [5000, 1536] -> 24 (79) 13.2, 9.7 and 8.3, [801, 384] -> 384 (91, six
+    // steps) 4.4, 4.1 and 4.3; [3000, 1536] -> 384 (282) 13.5, 10.9 and 15.8, [3000, 384] -> 384 4.8, 5.4 and 7.4; [1517, 1536] ->
+    // 1536 (576) 15.5, 20.3 and 24.8; f32 [444, 1536] -> 1536 33, 30 and 28.
+    if (!big && direct) {
+        const int64_t tiles = ceil_div(a.M, 64) * ceil_div(a.N, 64), steps = a.K * es / kStepBytes;
+        if (tiles <= cus && steps >= 12) return launch_tile<DT, 2, 2, 2, 2, true, 0, 4>(a, st);
+        if ((tiles <= cus && steps >= 4) || (2 * tiles <= 3 * cus && steps >= 24)) return launch_tile<DT, 2, 2, 2, 2, true, 0, 2>(a, st);
+    }
     if (!big) return direct ? launch_tile<DT, 2, 2, 2, 2, true, 0>(a, st) : launch_tile<DT, 2, 2, 2, 2, false, 0>(a, st);
     if constexpr (DT != F32) return launch_large<DT>(a, direct, st);
     return MBRT_OK;

@@ -57,6 +57,13 @@ def test_short_operands(dev, rows, k, n, dtype):
     _case(dev, rows, k, n, dtype, res=dtype, seed=rows)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,k,n", [(700, 840, 390), (700, 328, 390), (650, 256, 448), (1500, 1544, 900), (700, 768, 385)])
+def test_few_tiles(dev, rows, k, n, dtype):
+    """Tiles whose steps are shared out among groups of waves, whole and cut by the rows' end."""
+    _case(dev, rows, k, n, dtype, act=1, res=dtype, seed=n)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("out", [F16, F32])
 @pytest.mark.parametrize("rows,k,n", [(33, 67, 41), (700, 129, 131), (2600, 64, 1537), (90, 7, 129)])
