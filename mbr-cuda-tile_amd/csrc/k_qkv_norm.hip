@@ -6,7 +6,9 @@
 //
 // Bound by memory: each element is read and written once.  G lanes hold one head vector, 16 bytes each, and reduce
 // its sum of squares with DPP adds; a token has S such groups side by side (a wave, where it has the heads), which walk
-// its heads, so that a thread reads its cos, sin and gamma once for all of them.
+// its heads, so that a thread reads its cos, sin and gamma once for all of them.  MI355X: bf16 [60, 801] with 8 heads of
+// 64, 295 MB, 54.8 us (5.4 TB/s; a large copy 4.8); f32 [30, 801], 8 heads over 2 of 128, 25.7 us; a frame of 60 rows
+// 4.1 to 4.4, the launch.
 #include "abi_common.hpp"
 
 #include <algorithm>
@@ -59,7 +61,7 @@ __device__ __forceinline__ void* place(const QkvArgs& a, int64_t b, int64_t n, i
 }
 
 // LG: lanes per head vector, known here with f32 tables and gammas (every load of a thread is then issued before it waits
-// for one: a call for one frame 4.3 -> 3.4 us), or 0: all at run time.
+// for one: a call for one frame 4.4 -> 4.1 us), or 0: all at run time.
 template <int IDT, int ODT, int LG>
 __global__ __launch_bounds__(kThreads) void qkv_norm_vec_kernel(QkvArgs a) {
     constexpr int VE = (IDT == F32 || ODT == F32) ? 4 : 8;

@@ -6,7 +6,8 @@
 // Query rows: the H / H_kv query heads that share a key head are rows of one matrix, row r = (query r / G, head
 // r % G), so that each key and value is read once for all of them.
 // Keys: what the rows of a tile may see is one list, the sinks before the window and then the window's keys lo .. hi
-// of all its rows: t -> j = t < s ? t : lo + t - s, with s <= lo.  No key outside is read.  Whatever stands in keys that no row of the tile sees (NaN behind a sequence's end) is not read.
+// of all its rows: t -> j = t < s ? t : lo + t - s, with s <= lo.  No key outside is read, whatever stands there (NaN
+// behind a sequence's end).
 //
 // Per 32 keys, with v_mfma_f32_16x16x32 (lane l = (g, c): A[c][8 g + j], B[8 g + j][c], C[4 g + i][c]):
 //   S^T = K Q^T      A = K rows, B = the wave's 16 query rows: lane (g, c) holds S^T[key 16 kb + 4 g + i][row c].
@@ -17,15 +18,17 @@
 //                    2-byte type (split_p), so that only the inputs' and the output's own rounding is left.
 // Lane (g, c) ends with columns 16 db + 4 g .. + 3 of row c.
 //
-// What bounds it (MI355X, us; rocprofv3 counters in profiles/counters_window.md): bf16 [60, 801], 8 heads of 64 through 101
-// keys and 8 sinks, 57.8; its loads and stores alone take 43 (197 MB at 4.6 TB/s), the rest is the softmax's VALU work, which
-// hides behind them only in part (a wave's step of 64 keys: 24 MFMAs of 16 clocks, about 170 VALU instructions of 4 and 16
-// exponentials of 16, and 16 KB of LDS reads).  f16 [2, 16389], 8 heads over 2 of 128 through 1024 keys, 210: 134 GFLOP, half as
-// many again for the second part of p; 2052 workgroups on 512 places, so five rounds where four and a bit would do.
-// One step over 64 keys at a time, priorities around the MFMAs and row sums by the matrix unit gained nothing
-// over steps of 32, none and VALU sums; skipping steps that are hidden from a wave cost as much in register copies as it
-// saved; transpose reads by the compiler's builtin, which it can place early, 71 -> 64 at 32 rows per wave; addresses of a
-// tile from one scalar base and a layout without bank conflicts 290 -> 267 at f16 [2, 16389] with 16 rows per wave.
+// What bounds it (MI355X, us; counters by rocprofv3): bf16 [60, 801], 8 heads of 64 through 101 keys and 8 sinks, 57.5; its
+// loads and stores alone take 43 (197 MB at 4.6 TB/s), the rest is the softmax's VALU work, which hides behind them only in
+// part (a wave's tile of 64 keys: 24 MFMAs of 16 clocks, about 170 VALU instructions of 4 and 16 exponentials of 16, and 16 KB of
+// LDS reads).  f16 [2, 16389], 8 heads over 2 of 128 through 1024 keys, 210: 134 GFLOP, half as many again for the second
+// part of p (145 at a large library product's rate), on matrix units that are busy half the time; 2052 workgroups on 512
+// places, so five rounds where four and a bit would do.  One token: 60 caches of 1601 frames 20.4, 100 MB at 4.9 TB/s, as a
+// copy; [1, 200003] 22.7.
+// Not kept: steps of 64 keys, priorities around the MFMAs and row sums by the matrix unit (no gain); skipping steps that
+// are hidden from a wave, which cost as much in register copies as it saved.  Kept: transpose reads by the
+// compiler's builtin, which it can place early, 71 -> 64 at 32 rows per wave; addresses of a tile from one scalar base and a
+// layout without bank conflicts 290 -> 267 at f16 [2, 16389] with 16 rows per wave, 32 rows per wave 216.
 //
 // A value that a row does not see but another row of its tile does enters the product with weight 0.  Where that
 // value is infinite or NaN the product is NaN; a row that ends with anything not finite is computed again from the

@@ -9,8 +9,19 @@
 // contraction serves if both operands have the same.  Sums are f32; the epilogue works in f32 and rounds once,
 // on its store.
 //
-// Three forms, by shape (launch_linear below): tiles of 64 x 64 up to 128 x 192 through LDS, and strips of 16 rows of
-// the longer operand against all of a short one (few rows, or few output columns).
+// Forms, by shape (launch_linear below): tiles of 64 x 64 up to 128 x 192 through LDS, whose groups of waves share the
+// steps where tiles are few, and strips of 16 rows of the longer operand against all of a short one.
+//
+// What bounds it (MI355X, us; a large copy runs at 4.8 TB/s, a large library product at 1382 TFLOP/s, f32 153):
+//   [48060, 384] -> 1536 bf16 67 (184 MB: 41 at the copy's rate; 844 TFLOP/s).  Stores first: 8 bytes per lane and through the
+//   caches 99, 16 bytes 74, out past the caches 70; the matrix units are busy for 28 of it (counted), and a product's end and the
+//   next one's first loads overlap only between the two workgroups of a CU.
+//   [48060, 1536] -> 384 with residual 93 (221 MB: 46): 172 MB of reads arrive in the order in which tiles ask for them, and
+//   the loads alone take nearly as long.  The library's product alone 96 and, of the former, 122.
+//   f32 [4096, 4096] -> 4096 960: 143 TFLOP/s.  One row to some hundred: the launch, and the latency of one round of loads (4.1).
+// Not kept: steps of 64 bytes in four buffers or three of 192 x 192 (88 to 110), 256 x 256 (86 and 109), persistent
+// workgroups that store while the next tile loads (74 to 85), fragments fetched across the barrier (no gain), rows handed
+// round through LDS for stores of whole lines (67 -> 79).
 #pragma once
 
 #include "abi_common.hpp"
@@ -35,7 +46,8 @@ struct LinArgs {
     FastDiv groups, splits;  // ntiles and split
 };
 
-// The linear layer for operands of one dtype; align: all rows of x and w begin at multiples of it, 16, 4 or 2 bytes.  Instantiated in a source file per dtype.
+// The linear layer for operands of one dtype; align: all rows of x and w begin at multiples of it, 16, 4 or 2
+// bytes.  Instantiated in a source file per dtype.
 template <int DT>
 int launch_linear(LinArgs& a, int align, hipStream_t st);
 
@@ -709,7 +721,8 @@ int launch_linear(LinArgs& a, int align, hipStream_t st) {
     if (!big && direct) {
         const int64_t tiles = ceil_div(a.M, 64) * ceil_div(a.N, 64), steps = a.K * es / kStepBytes;
         if (tiles <= cus && steps >= 12) return launch_tile<DT, 2, 2, 2, 2, true, 0, 4>(a, st);
-        if ((tiles <= cus && steps >= 4) || (2 * tiles <= 3 * cus && steps >= 24)) return launch_tile<DT, 2, 2, 2, 2, true, 0, 2>(a, st);
+        if ((tiles <= cus && steps >= 4) || (2 * tiles <= 3 * cus && steps >= 24))
+            return launch_tile<DT, 2, 2, 2, 2, true, 0, 2>(a, st);
     }
     if (!big) return direct ? launch_tile<DT, 2, 2, 2, 2, true, 0>(a, st) : launch_tile<DT, 2, 2, 2, 2, false, 0>(a, st);
     if constexpr (DT != F32) return launch_large<DT>(a, direct, st);
