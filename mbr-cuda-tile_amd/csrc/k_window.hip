@@ -22,10 +22,12 @@
 // loads and stores alone take 43 (197 MB at 4.6 TB/s), the rest is the softmax's VALU work, which hides behind them only in
 // part (a wave's tile of 64 keys: 24 MFMAs of 16 clocks, about 170 VALU instructions of 4 and 16 exponentials of 16, and 16 KB of
 // LDS reads).  f16 [2, 16389], 8 heads over 2 of 128 through 1024 keys, 210: 134 GFLOP, half as many again for the second
-// part of p (145 at a large library product's rate), on matrix units that are busy half the time; 2052 workgroups on 512
-// places, so five rounds where four and a bit would do.  One token: 60 caches of 1601 frames 20.4, 100 MB at 4.9 TB/s, as a
+// part of p (145 at a large library product's rate), on matrix units that are busy half the time, the
+// VALU for about as long (9 operations and an exponential for each score), which two waves per SIMD overlap only in
+// part.  One token: 60 caches of 1601 frames 20.4, 100 MB at 4.9 TB/s, as a
 // copy; [1, 200003] 22.7.
-// Not kept: steps of 64 keys, priorities around the MFMAs and row sums by the matrix unit (no gain); skipping steps that
+// Not kept: steps of 64 keys, priorities around the MFMAs, row sums by the matrix unit (no gain), V fragments read two
+// blocks ahead (1 %); skipping steps that
 // are hidden from a wave, which cost as much in register copies as it saved.  Kept: transpose reads by the
 // compiler's builtin, which it can place early, 71 -> 64 at 32 rows per wave; addresses of a tile from one scalar base and a
 // layout without bank conflicts 290 -> 267 at f16 [2, 16389] with 16 rows per wave, 32 rows per wave 216.
