@@ -154,7 +154,7 @@ __device__ __forceinline__ float gelu_short(float x, float s) {
     p = fmaf(p, t, -0.142248368f);
     p = fmaf(p, t, 0.127414796f);
     p *= t * __builtin_amdgcn_exp2f(az * (az * -1.44269504088896341f));
-    return fmaf(-fabsf(x), p, fmaxf(x, 0.0f));
+    return fmaf(-fabsf(fminf(x, 64.0f)), p, fmaxf(x, 0.0f));  // p is 0 from 64 on: inf - 64 * 0, and -inf * 0 = NaN
 }
 
 // tanh x = 1 - 2 / (e^2x + 1), and the first terms of its series where that cancels (relative error 3.3e-7 at 1/4).

@@ -138,3 +138,43 @@ def window(q, k, v, out_dtype, left=None, right=None, sinks=0, q_start=None, key
         y = y * g[..., None]
         bound = bound * g.abs()[..., None] + y.abs() * (8 * U + 0.5 * U * (gate.cpu().double().abs()[..., None] if gate_is_logit else 0))
     return y, bound + half_step(out_dtype, y) + 1e-30
+
+
+def gelu_by_formula(x, s):
+    """x Phi by Abramowitz & Stegun 7.1.26 in 64 bits, erfc(z) = (a1 t + .. + a5 t^5) exp(-z^2), t = 1 / (1 + p z): the
+    form that 2-byte results take, its own error included."""
+    z = x.abs() * s
+    t = 1.0 / (1.0 + 0.3275911 * z)
+    p = t * (0.254829592 + t * (-0.284496736 + t * (1.421413741 + t * (-1.453152027 + t * 1.061405429))))
+    return torch.where(x > 0, x, 0.0 * x) - 0.5 * x.abs() * p * torch.exp(-z * z)
+
+
+def activation(x, act, out_dtype, short):
+    """(value, bound) of an activation of f32 arguments, relative to the value far into the tails too, infinities and
+    NaN included.  short: the forms that 2-byte results of 2-byte operands take."""
+    x = x.detach().cpu().double()
+    y, _ = act64(x, act)
+    tiny = 2.0 ** -126 * (1 + x.abs().clamp_max(1e38))   # results below the normal numbers may be flushed
+    if act in (1, 2):
+        s = 1.0 if act == 1 else math.sqrt(0.5)
+        z2 = (x * s).square().clamp_max(1e4)
+        if short:
+            # the formula's own error (at most 1.5e-7 |x| / 2), and f32: a dozen steps of erfc, three of z^2 through exp
+            own = (gelu_by_formula(x, s) - y).abs()
+            fine = torch.isfinite(x)
+            assert bool((own[fine] <= 0.75e-7 * x.abs()[fine] + 1e-12).all())
+            erfc = torch.special.erfc(x.abs() * s)
+            bound = own + 0.5 * x.abs() * erfc * (16 + 4 * z2) * U + 2 * U * y.abs()
+        else:
+            # erfc within OpenCL's 16 steps; its argument's rounding, d ln erfc / d ln z < 2 z^2 + 1
+            bound = y.abs() * (20 + 2 * (z2 + 1)) * U
+    elif act == 3:
+        bound = y.abs() * (8 + 3 * x.abs().clamp_max(200)) * U   # exp(-x): two roundings of its argument, rcp, add
+    elif act == 4:
+        # OpenCL's 5 steps of tanh; the short form's series (3.3e-7 at 1/4) and 1 - 2 / (exp + 1), which cancels to a quarter
+        bound = y.abs() * (4e-7 + 16 * U if short else 8 * U)
+    else:
+        bound = 0.0 * y.abs()
+    top = torch.finfo(out_dtype).max
+    y = torch.where(y.abs() > top * (1 + torch.finfo(out_dtype).eps / 4), torch.copysign(torch.full_like(y, math.inf), y), y)
+    return y, bound + half_step(out_dtype, y) + tiny

@@ -195,3 +195,36 @@ def test_same_result_every_time_captured_and_on_another_stream(dev):
         eager = mbrt.linear(x, w, b, act=2)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(outs, small) and torch.equal(eager, want), i
+
+
+def _arguments(dtype):
+    big = 6e4 if dtype == F16 else 1e30
+    inf = float("inf")
+    return torch.tensor([-inf, -big, -200.0, -12.0, -6.5, -5.0, -3.75, -1.0, -0.125, -1e-3, 0.0, 1e-3, 0.3125, 2.5, 6.0, 20.0,
+                         1000.0, big, inf, float("nan")], dtype=dtype)
+
+
+# one argument per row of x, in column 0, whose weights are 1: strips and tiles, whole pieces and cut ones, no features
+@pytest.mark.parametrize("rows,k,n", [(20, 64, 70), (20, 7, 70), (1500, 72, 200), (1500, 65, 200), (9, 0, 20)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("out", [F32, F16, BF16])
+@pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
+def test_activations_of_infinities_and_nan(dev, rows, k, n, dtype, out, act):
+    """Arguments that are infinite or NaN give what the functions' formulas give, for every type of operand and result."""
+    import mbrt
+
+    say(f"special arguments rows={rows} k={k} n={n} {dtype} -> {out} act={act}")
+    v = _arguments(dtype)
+    if k == 0:
+        x, w, b = torch.empty((rows, 0), dtype=dtype, device="cuda"), torch.empty((n, 0), dtype=dtype, device="cuda"), v.cuda()
+        arg = v.expand(rows, n)
+    else:
+        x, w, b = torch.zeros((rows, k), dtype=dtype), torch.zeros((n, k), dtype=dtype, device="cuda"), None
+        x[:, 0] = v.repeat(rows // v.numel() + 1)[:rows]
+        w[:, 0] = 1
+        arg, x = x[:, :1].expand(rows, n), x.cuda()
+    got = mbrt.linear(x, w, b, act=act, out_dtype=out).cpu().double()
+    want, _ = ref.activation(arg, act, out, False)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    special = torch.isinf(arg.double()) & ~torch.isnan(want)
+    assert torch.equal(got[special], want[special])
