@@ -130,6 +130,13 @@ __device__ __forceinline__ float elem(const uint16_t* p, int64_t i) {
     else return (float)__builtin_bit_cast(_Float16, p[i]);
 }
 
+// Whether query row r sees a key at all.  Where the weights of one that does add up to 0, every key that it sees scores
+// -infinity, and its softmax is NaN; zeros are for rows that see none.
+__device__ __forceinline__ bool sees_any(const WinArgs& a, int b, int r) {
+    const int qi = (int)fdiv((uint32_t)r, a.gdiv);
+    return make_span(a, b, qi, qi).count > 0;
+}
+
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
 
 // K and V tiles in LDS: rows of D 2-byte elements in 16-byte pieces, piece j of row r at j ^ swz(r).  The banks are 256
@@ -330,7 +337,7 @@ __device__ __forceinline__ float gate_of(const WinArgs& a, int b, int qi, int h)
 }
 
 // One row by the whole wave from the keys that it sees alone, element d = lane, lane + 64: for rows whose tile held
-// something not finite.  The gate is the caller's.
+// something not finite, and rows whose weights are all 0 (1 / 0 here, and so NaN).  The gate is the caller's.
 template <int DT, int D>
 __device__ __forceinline__ void row_alone(const WinArgs& a, int b, int kv, int r, float (&y)[2]) {
     const int lane = threadIdx.x % 64;
@@ -509,7 +516,7 @@ __global__ __launch_bounds__(256) void window_tile_kernel(WinArgs a) {
         const int r = r0 + 16 * x + c, qi = (int)fdiv((uint32_t)min(r, a.rows - 1), a.gdiv);
         const int h = kv * G + min(r, a.rows - 1) - qi * G;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-        bool bad = not_finite(l);
+        bool bad = not_finite(l) || (l == 0.0f && (rw.n[x] > 0 || min(sp.s, rw.jhi[x] + 1) > 0));  // as sees_any
 #pragma unroll
         for (int db = 0; db < D / 16; ++db)
 #pragma unroll
@@ -627,7 +634,8 @@ __global__ __launch_bounds__(kSplitWaves * 64) void window_split_kernel(WinArgs 
             }
             continue;
         }
-        if (__builtin_amdgcn_ballot_w64(not_finite(ls) || not_finite(o[0]) || not_finite(o[1])) != 0) {
+        if (__builtin_amdgcn_ballot_w64(not_finite(ls) || not_finite(o[0]) || not_finite(o[1])) != 0 ||
+            (ls == 0.0f && sees_any(a, b, r))) {
             store_row_alone<DT, D>(a, b, kv, r);
             continue;
         }
@@ -693,7 +701,8 @@ __global__ __launch_bounds__(kJoinWaves * 64) void window_join_kernel(WinArgs a)
         if (lane < D) o[0] += part[i][lane] * g;
         if (D > 64) o[1] += part[i][lane + 64] * g;
     }
-    if (__builtin_amdgcn_ballot_w64(not_finite(l) || not_finite(o[0]) || not_finite(o[1])) != 0) {
+    if (__builtin_amdgcn_ballot_w64(not_finite(l) || not_finite(o[0]) || not_finite(o[1])) != 0 ||
+        (l == 0.0f && sees_any(a, b, r))) {
         store_row_alone<DT, D>(a, b, kv, r);
         return;
     }

@@ -1,6 +1,8 @@
 """GPU tests of the windowed attention against its 64-bit form over the visible keys alone."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -272,3 +274,38 @@ def test_same_result_every_time_captured_and_on_other_streams(dev):
         eager = mbrt.attention_window(q, k, v, right=0)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(outs, wants) and torch.equal(eager, want)
+
+
+def test_scores_of_minus_infinity(dev):
+    """A query that sees keys, none of which scores above -infinity, is NaN, as the softmax is; zeros are for those that
+    see no key.  Where another key's score is finite the infinite ones have no weight."""
+    inf = float("inf")
+    import mbrt
+
+    for dtype in (BF16, F16):
+        for nq, nk in ((1, 90), (90, 90), (7, 90), (1, 5000), (2, 5000)):
+            say(f"scores of -inf nq={nq} nk={nk} {dtype}")
+            q, k, v = _qkv(5, 1, nq, nk, 2, 1, 64, dtype)
+            q[..., 0] = 1
+            k[:, nk - 1, 0, 0] = -inf
+            # each query sees its own key alone, the last one an infinite one
+            got = mbrt.attention_window(q, k, v, left=0, right=0).cpu()
+            want = v[:, nk - nq:].expand(1, nq, 2, 64).clone().cpu()
+            want[:, nq - 1] = float("nan")
+            assert torch.equal(torch.isnan(got), torch.isnan(want))
+            assert torch.equal(got[:, :nq - 1], want[:, :nq - 1])
+            # all keys but one
+            k[..., 0] = -inf
+            assert bool(torch.isnan(mbrt.attention_window(q, k, v)).all())
+            k[:, 3, 0, 0] = 0.5
+            got = mbrt.attention_window(q, k, v).cpu()
+            assert torch.equal(got, v[:, 3:4].expand(1, nq, 2, 64).cpu())
+            # queries behind every key: none is seen
+            assert bool((mbrt.attention_window(q, k, v, q_start=nk + 50, left=9) == 0).all())
+    q, k, v = _qkv(6, 1, 3, 200, 2, 2, 32, BF16)
+    k[..., 0] = -inf
+    q[..., 0] = 1
+    gate = torch.ones((1, 3, 2), device="cuda")
+    lens = torch.tensor([0], dtype=torch.int32, device="cuda")
+    assert bool(torch.isnan(mbrt.attention_window(q, k, v, gate=gate)).all())
+    assert bool((mbrt.attention_window(q, k, v, gate=gate, key_lens=lens) == 0).all())
