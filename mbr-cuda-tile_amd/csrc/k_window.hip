@@ -12,7 +12,7 @@
 // Per 32 keys, with v_mfma_f32_16x16x32 (lane l = (g, c): A[c][8 g + j], B[8 g + j][c], C[4 g + i][c]):
 //   S^T = K Q^T      A = K rows, B = the wave's 16 query rows: lane (g, c) holds S^T[key 16 kb + 4 g + i][row c].
 //   online softmax   per row c, as in the fused attention: the exponent's reference m moves only when a score
-//                    outgrows it by 2^8, each lane sums its own keys' p, the four lanes of a row are added at the end.
+//                    outgrows it by 2^kTop, each lane sums its own keys' p, the four lanes of a row are added at the end.
 //   O^T += V^T P^T   B = P^T from the S^T registers: slot j of lane group g is key 4 g + j, or 16 + 4 g + j - 4 from
 //                    j = 4 on; A = V^T by LDS transpose reads.  P enters as a sum of two or three values of the
 //                    2-byte type (split_p), so that only the inputs' and the output's own rounding is left.
@@ -48,7 +48,12 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr float kLazy = 8.0f;  // log2 units the running max may outgrow the exponent's reference
+// The weights are p = 2^(score - m) with a reference m that moves only when a score outgrows 2^kTop, and then to where the
+// score is 2^kBase: a row's largest weight lies between the two.  f16 has its smallest step at 2^-24, so its weights use the
+// top of its range.  A smaller distance loses less of small weights and moves m more often: f16 [2, 16389], 8 heads over 2 of
+// 128 through 1024 keys, with 2^13 220 us, 2^11 214, 2^10 210, 2^7 209 and 2^0 (to 2^8) 209.
+template <int DT> constexpr float kBase = DT == F16 ? 10.0f : 0.0f;
+template <int DT> constexpr float kTop = DT == F16 ? 15.0f : 8.0f;
 constexpr int kBufferDword3 = 0x00020000;  // raw buffer resource: 32-bit data format, no swizzle, no stride
 constexpr int kTile = 64;      // keys per LDS tile
 constexpr int kChunk = 32;     // keys per arithmetic step
@@ -100,8 +105,9 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
 }
 
 // Two values of P as NP 2-byte values each: bf16 truncated (exact difference) and the last part rounded, f16 rounded to
-// nearest each time (exact differences too; p <= 2^8, and parts below 2^-24 are lost beside a row sum of 1 or more).  Two
-// parts of bf16 hold 17 bits and of f16 22; an f32 output of bf16 heads takes three, 24 bits.
+// nearest each time (exact differences too).  Two parts of bf16 hold p to 2^-16 of itself; an f32 output of bf16 heads takes
+// three, 2^-24.  Two of f16 hold it to 2^-23, about what exp2 leaves of it, or to half of f16's smallest step where that is
+// more: 2^-25, which is 2^-35 of the row's largest weight or less.
 template <int DT, int NP>
 __device__ __forceinline__ void split_p(float p0, float p1, uint32_t (&w)[NP]) {
 #pragma unroll
@@ -277,14 +283,14 @@ __device__ __forceinline__ void attend(const WinArgs& a, const Span& sp, const R
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < 4; ++i) mx[x] = fmaxf(mx[x], s[x][kb][i]);
-        grown = grown || mx[x] * a.sl2 > st.m[x] + kLazy;
+        grown = grown || mx[x] * a.sl2 > st.m[x] + kTop<DT>;
     }
     if (__builtin_amdgcn_ballot_w64(grown) != 0) {
 #pragma unroll
         for (int x = 0; x < QS; ++x) {
             float top = fmaxf(mx[x], __shfl_xor(mx[x], 16));
             top = fmaxf(top, __shfl_xor(top, 32)) * a.sl2;
-            const float mn = top > st.m[x] + kLazy ? top : st.m[x];
+            const float mn = top > st.m[x] + kTop<DT> ? top - kBase<DT> : st.m[x];
             const float alpha = __builtin_amdgcn_exp2f(st.m[x] - mn);
             st.l[x] *= alpha;
 #pragma unroll

@@ -309,3 +309,41 @@ def test_scores_of_minus_infinity(dev):
     lens = torch.tensor([0], dtype=torch.int32, device="cuda")
     assert bool(torch.isnan(mbrt.attention_window(q, k, v, gate=gate)).all())
     assert bool((mbrt.attention_window(q, k, v, gate=gate, key_lens=lens) == 0).all())
+
+
+def _sink_case(B, nq, nk, D, dtype, gap, seed):
+    """Keys whose first scores `gap` above the others, which lie within half a unit, and whose first value is zero."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.zeros((B, nq, 2, D))
+    q[..., 0] = math.sqrt(D)
+    k = torch.zeros((B, nk, 2, D))
+    k[..., 0] = torch.rand((B, nk, 2), generator=g) - 0.5
+    k[:, 0, :, 0] = gap
+    v = 0.5 + torch.rand((B, nk, 2, D), generator=g)
+    v[:, 0] = 0
+    return q.to(dtype).cuda(), k.to(dtype).cuda(), v.to(dtype).cuda()
+
+
+@pytest.mark.parametrize("out", [F16, F32])
+@pytest.mark.parametrize("gap", [8.0, 12.0, 14.0, 16.0, 18.0])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_weights_far_below_a_sink(dev, D, gap, out):
+    """f16 heads whose output is made by weights far below the largest one: a sink of value zero."""
+    import mbrt
+
+    for B, nq, nk in ((1, 100, 1000), (1, 1, 1000), (1, 1, 20000), (128, 130, 600)):
+        say(f"sink D={D} gap={gap} B={B} nq={nq} nk={nk} {out}")
+        q, k, v = _sink_case(B, nq, nk, D, F16, gap, nk)
+        got = mbrt.attention_window(q, k, v, out_dtype=out)
+        s = k.cpu().double()[..., 0] * (float(q[0, 0, 0, 0]) / math.sqrt(D))   # [B, nk, 2]
+        e = torch.exp(s - s.amax(1, keepdim=True))
+        p = e / e.sum(1, keepdim=True)
+        vd = v.cpu().double()
+        y = (p[..., None] * vd).sum(1)
+        # scores: exact products but for the scale and exp2's argument, a few steps of `gap` each; the weights' two f16
+        # values: 2^-22 of each weight, and half the smallest f16 number beside a largest one of 2^10 or more, 2^-35 of the
+        # row's largest weight; sums: n steps
+        spread, lost = y.abs(), p.amax(1)[..., None] * vd.abs().sum(1)
+        bound = spread * (2.0 ** -22 + (6 * (gap + 1) + nk + 16) * ref.U) + 2.0 ** -35 * lost
+        y, bound = (t[:, None].expand(B, nq, 2, D) for t in (y, bound))
+        ref.check(got, y, bound + ref.half_step(out, y) + 1e-30, f"gap {gap}")
