@@ -456,8 +456,8 @@ MBRT_API int mbrt_split_qkv_norm_rotary(const void* qkv, int qkv_dtype, int64_t 
  * written only for the n_q queries.  scale > 0, or 0 for 1/sqrt(head_dim).  gate [B, n_q, H] (F32/F16/BF16, NULL for
  * none) multiplies each head's output by sigmoid(gate), or by gate itself when !gate_is_logit, before
  * the one rounding on the store.  f32 softmax and sums.  Probabilities enter the second product as sums of 2-byte values
- * of q's type: BF16 two, within 2^-16 of each probability (three, 2^-24, to an F32 out); F16 two, within 2^-23 of it or 2^-35 of its
- * row's largest probability, whichever is more.  A few queries against many keys are shared out over the keys and joined through
+ * of q's type: BF16 two or three, within 2^-17 of each probability (2^-24 to an F32 out); F16 two, within 2^-23 of it or 2^-35 of
+ * its row's largest probability, whichever is more.  A few queries against many keys are shared out over the keys and joined through
  * `workspace` (mbrt_attention_window_workspace_bytes of the same sizes; 0 bytes: may be NULL), in a fixed order:
  * results do not change from call to call.  Calls that overlap need workspaces of their own.
  * Beside mbrt_attention_ex, for songs longer than a chunk and for streaming. */

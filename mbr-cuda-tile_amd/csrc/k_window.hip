@@ -15,7 +15,7 @@
 //                    outgrows it by 2^kTop, each lane sums its own keys' p, the four lanes of a row are added at the end.
 //   O^T += V^T P^T   B = P^T from the S^T registers: slot j of lane group g is key 4 g + j, or 16 + 4 g + j - 4 from
 //                    j = 4 on; A = V^T by LDS transpose reads.  P enters as a sum of two or three values of the
-//                    2-byte type (split_p), so that only the inputs' and the output's own rounding is left.
+//                    2-byte type (split_p), so that little beside the inputs' and the output's own rounding is left.
 // Lane (g, c) ends with columns 16 db + 4 g .. + 3 of row c.
 //
 // What bounds it (MI355X, us; counters by rocprofv3): bf16 [60, 801], 8 heads of 64 through 101 keys and 8 sinks, 57.5; its
@@ -104,10 +104,13 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Two values of P as NP 2-byte values each: bf16 truncated (exact difference) and the last part rounded, f16 rounded to
-// nearest each time (exact differences too).  Two parts of bf16 hold p to 2^-16 of itself; an f32 output of bf16 heads takes
-// three, 2^-24.  Two of f16 hold it to 2^-23, about what exp2 leaves of it, or to half of f16's smallest step where that is
-// more: 2^-25, which is 2^-35 of the row's largest weight or less.
+// Two values of P as NP 2-byte values each, rounded to nearest each time (exact differences).  Two parts of bf16 hold p to
+// 2^-17 of itself, three to 2^-24.  Two of f16 hold it to 2^-23, about what exp2 leaves of it, or to half of f16's smallest step
+// where that is more: 2^-25, which is 2^-35 of the row's largest weight or less.
+// bf16 heads take three parts for f32 outputs, and where few queries share out their keys (window_split_kernel), which wait for
+// memory: one frame against 60 caches 22.0 us with two and with three, four against 20 caches of 1000 8.1 and 8.4.  The tiles of
+// query rows take two for 2-byte outputs: a third costs [60, 801] through 109 keys 57.5 -> 62, through all 155 -> 184, and
+// 2^-17 is below a hundredth of the output's own half step of 2^-9.
 template <int DT, int NP>
 __device__ __forceinline__ void split_p(float p0, float p1, uint32_t (&w)[NP]) {
 #pragma unroll
@@ -116,10 +119,9 @@ __device__ __forceinline__ void split_p(float p0, float p1, uint32_t (&w)[NP]) {
             if (i == NP - 1) {
                 w[i] = pack_bf16x2(p0, p1);
             } else {
-                const uint32_t b0 = __float_as_uint(p0) & 0xffff0000u, b1 = __float_as_uint(p1) & 0xffff0000u;
-                w[i] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-                p0 -= __uint_as_float(b0);
-                p1 -= __uint_as_float(b1);
+                w[i] = pack_bf16x2(p0, p1);
+                p0 -= bf16_lo(w[i]);
+                p1 -= bf16_hi(w[i]);
             }
         } else {
             w[i] = pack_f16x2(p0, p1);
@@ -868,7 +870,7 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
         }
         const size_t lds = (size_t)kSplitWaves * 16 * (Dv + 2) * 4;  // the joined rows; the V tiles need less
         static_assert(kChunk * 2 * Dv <= 16 * (Dv + 2) * 4, "V tile within the rows' space");
-        hipLaunchKernelGGL((window_split_kernel<DTv, Dv, NP>), dim3((unsigned)blocks), dim3(kSplitWaves * 64), lds, stm, a);
+        hipLaunchKernelGGL((window_split_kernel<DTv, Dv, DTv == BF16 ? 3 : 2>), dim3((unsigned)blocks), dim3(kSplitWaves * 64), lds, stm, a);
         if (plan.splits > 1)
             hipLaunchKernelGGL((window_join_kernel<DTv, Dv>), dim3((unsigned)(bkv * a.rows)), dim3(kJoinWaves * 64), 0, stm, a);
     };

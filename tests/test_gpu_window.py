@@ -347,3 +347,38 @@ def test_weights_far_below_a_sink(dev, D, gap, out):
         bound = spread * (2.0 ** -22 + (6 * (gap + 1) + nk + 16) * ref.U) + 2.0 ** -35 * lost
         y, bound = (t[:, None].expand(B, nq, 2, D) for t in (y, bound))
         ref.check(got, y, bound + ref.half_step(out, y) + 1e-30, f"gap {gap}")
+
+
+@pytest.mark.parametrize("dtype,out", [(BF16, F32), (F16, F32)])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_weights_add_up_to_one(dev, D, dtype, out):
+    """Values that are all 1 give 1: what is lost of each weight shows, whatever the scores' rounding."""
+    import mbrt
+
+    for B, nq, nk in ((4, 300, 300), (8, 1, 5), (8, 16, 7)):
+        say(f"weights D={D} {dtype} B={B} nq={nq} nk={nk}")
+        q, k, _ = _qkv(7, B, nq, nk, 2, 2, D, dtype)
+        v = torch.ones_like(k)
+        got = mbrt.attention_window(q, k, v, left=2, right=0, out_dtype=out).cpu().double()
+        # at most 3 weights, held to 2^-23 (f16 pairs; bf16 triples 2^-24); the same weights are summed in f32 on both sides:
+        # 2 additions each, the product's order, the quotient and the products with it.  Queries before the first key: 0.
+        want = (torch.arange(nk - nq, nk) >= 0).double()[None, :, None, None]
+        assert float((got - want).abs().max()) <= 2.0 ** -23 + 8 * ref.U
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_weights_of_bf16_behind_a_border(dev, D):
+    """2-byte outputs of values that are all 1, moved by their gate to just beside the border between 1 and 1 + 2^-7:
+    they fall on the gate's side of it if the weights add up to 1 within what is moved."""
+    import mbrt
+
+    # queries against caches: three parts, 2^-24, and f32's sums as in the test above; tiles: two parts, 2^-17
+    for B, nq, nk, off in ((64, 8, 40, 2.0 ** -24 + 10 * ref.U), (64, 1, 40, 2.0 ** -24 + 10 * ref.U),
+                           (8, 300, 300, 2.0 ** -17 + 10 * ref.U)):
+        say(f"border D={D} B={B} nq={nq} nk={nk}")
+        q, k, _ = _qkv(11, B, nq, nk, 4, 2, D, BF16)
+        v = torch.ones_like(k)
+        for side, want in ((1 + off, 1 + 2.0 ** -7), (1 - off, 1.0)):
+            gate = torch.full((B, nq, 4), (1 + 2.0 ** -8) * side, device="cuda")
+            got = mbrt.attention_window(q, k, v, left=2, right=0, gate=gate, gate_is_logit=False)
+            assert int((got != want).sum()) == 0
