@@ -411,8 +411,9 @@ MBRT_API int mbrt_attention_ex(const void* q, const void* k, const void* v, int 
  * [out_features] and residual [rows, out_features] of any of the three, each NULL for none, and out
  * [rows, out_features] of any.  Row strides in elements; x, weight and residual may have any from
  * 0 on, out at least out_features; rows at any alignment (16-byte ones are read faster).  Sums and
- * the epilogue are f32, with one rounding on the store; the activations are mbrt_bias_act's, and an
- * F32 operand's products are F32 products.  out may be residual (same dtype, same rows): the residual
+ * the epilogue are f32, with one rounding on the store; an F32 operand's products are F32 products.  The
+ * activations are mbrt_bias_act's functions; for 2-byte operands and out, GELU in its short form there (off by
+ * at most 0.75e-7 |x|), and tanh within 2^-19 of itself.  out may be residual (same dtype, same rows): the residual
  * stream updated in place.  in_features 0 leaves act(bias) + residual.  No workspace, no atomics.
  * The projections that the reference's model calls (linear*, src/mbr_cuda_tile.cu:712-3790,
  * 7586-7949), with the epilogues they end in and the residual add behind them. */

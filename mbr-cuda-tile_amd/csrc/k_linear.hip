@@ -69,6 +69,7 @@ int mbrt_linear(const void* x, int dtype, int64_t x_row_stride, const void* weig
     a.rdt = residual_dtype;
     a.odt = out_dtype;
     a.act = act;
+    a.short_act = dtype != F32 && out_dtype != F32;
     hipStream_t st = as_stream(stream);
     if (in_features == 0) {
         hipLaunchKernelGGL(linear_empty_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(rows * out_features, 256), 1 << 16)),

@@ -110,7 +110,7 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
 // bf16 heads take three parts for f32 outputs, and where few queries share out their keys (window_split_kernel), which wait for
 // memory: one frame against 60 caches 22.0 us with two and with three, four against 20 caches of 1000 8.1 and 8.4.  The tiles of
 // query rows take two for 2-byte outputs: a third costs [60, 801] through 109 keys 57.5 -> 62, through all 155 -> 184, and
-// 2^-17 is below a hundredth of the output's own half step of 2^-9.
+// 2^-17 is below a hundredth of the output's own half step of 2^-8.
 template <int DT, int NP>
 __device__ __forceinline__ void split_p(float p0, float p1, uint32_t (&w)[NP]) {
 #pragma unroll

@@ -40,6 +40,7 @@ struct LinArgs {
     int64_t M;
     int N, K;
     int bdt, rdt, odt, act;
+    int short_act;           // activations by their short forms
     uint32_t ntiles;         // tiles along N
     int split;               // strips: waves that share a strip's K
     int per_block;           // strips of a block
@@ -165,30 +166,32 @@ __device__ __forceinline__ float tanh_short(float x) {
     return fabsf(x) < 0.25f ? near : copysignf(far, x);
 }
 
-// f32 results take the library's erfc and tanh, 2-byte ones the short forms that bias_act uses for them (errors of
-// 1.5e-7 and less beside their half steps of 2^-9 and 2^-12).
+// f32 operands and f32 results take the library's erfc and tanh, 2-byte results of 2-byte operands the short forms: GELU's
+// is bias_act's in the same case, tanh's this layer's own.  tanh is within 2^-19 of itself.  GELU is within 0.75e-7 |x|, a
+// part of its value that grows into the negative tail: with z = x / sqrt 2 it passes half a step of bf16 (2^-8 of the value) below
+// x = -6.1, where GELU is -3e-9, and of f16 (2^-11) below -4.0, where it is -1.1e-4 and 5.5e-8 off; with z = x below -4.3 and -2.9.
 template <int NV>
-__device__ __forceinline__ void activate(float (&v)[NV], int act, bool f32_out) {
+__device__ __forceinline__ void activate(float (&v)[NV], int act, bool short_form) {
     if (act == MBRT_ACT_GELU_REF || act == MBRT_ACT_GELU_STD) {
         const bool ref = act == MBRT_ACT_GELU_REF;
         const float s = ref ? 1.0f : 0.70710678118654752440f;
-        if (f32_out) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = 0.5f * v[i] * erfcf(-v[i] * s);
-        } else {
+        if (short_form) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) v[i] = gelu_short(v[i], s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = 0.5f * v[i] * erfcf(-v[i] * s);
         }
     } else if (act == MBRT_ACT_SIGMOID) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = sigmoidf(v[i]);
     } else if (act == MBRT_ACT_TANH) {
-        if (f32_out) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = tanhf(v[i]);
-        } else {
+        if (short_form) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) v[i] = tanh_short(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = tanhf(v[i]);
         }
     }
 }
@@ -305,7 +308,7 @@ template <bool ACT, int NT, int NV>
 __device__ __forceinline__ void finish(const LinArgs& a, int64_t m, int n, float (&v)[NV], const Bias<NV>& bias) {
     if (m >= a.M || n >= a.N) return;
     bias.add_to(a, v);
-    if constexpr (ACT) activate<NV>(v, a.act, a.odt == F32);
+    if constexpr (ACT) activate<NV>(v, a.act, a.short_act != 0);
     const bool whole = n + NV <= a.N;
     if (a.res != nullptr) {
         float r[NV];

@@ -228,3 +228,18 @@ def test_activations_of_infinities_and_nan(dev, rows, k, n, dtype, out, act):
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     special = torch.isinf(arg.double()) & ~torch.isnan(want)
     assert torch.equal(got[special], want[special])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("out", [F32, F16, BF16])
+@pytest.mark.parametrize("act", [1, 2, 3, 4])
+def test_activations_in_their_tails(dev, dtype, out, act):
+    """Values relative to themselves, into the tails: the short forms are for 2-byte results of 2-byte operands alone."""
+    import mbrt
+
+    x = torch.cat((torch.linspace(-13, 13, 1301), torch.tensor([-6e4, -200.0, -30.0, 30.0, 200.0, 6e4])))[:, None].to(dtype)
+    for n in (5, 200):   # strips and tiles
+        say(f"tails {dtype} -> {out} act={act} n={n}")
+        w = torch.ones((n, 1), dtype=dtype, device="cuda")
+        want, bound = ref.activation(x.expand(-1, n), act, out, dtype != F32 and out != F32)
+        ref.check(mbrt.linear(x.cuda(), w, act=act, out_dtype=out), want, bound, f"act {act}")
