@@ -414,7 +414,8 @@ MBRT_API int mbrt_attention_ex(const void* q, const void* k, const void* v, int 
  * the epilogue are f32, with one rounding on the store; an F32 operand's products are F32 products.  The
  * activations are mbrt_bias_act's functions; for 2-byte operands and out, GELU in its short form there (off by
  * at most 0.75e-7 |x|), and tanh within 2^-19 of itself.  out may be residual (same dtype, same rows): the residual
- * stream updated in place.  in_features 0 leaves act(bias) + residual.  No workspace, no atomics.
+ * stream updated in place; it shares no other byte with an input, which is refused (columns of one wider
+ * matrix may be input and out).  in_features 0 leaves act(bias) + residual.  No workspace, no atomics.
  * The projections that the reference's model calls (linear*, src/mbr_cuda_tile.cu:712-3790,
  * 7586-7949), with the epilogues they end in and the residual add behind them. */
 MBRT_API int mbrt_linear(const void* x, int dtype, int64_t x_row_stride, const void* weight,

@@ -1,6 +1,8 @@
 // Entry point of the linear layer, and its kernels for f32 operands (linear.hpp).
 #include "linear.hpp"
 
+#include <utility>
+
 namespace mbrt {
 namespace {
 
@@ -15,6 +17,37 @@ __global__ __launch_bounds__(256) void linear_empty_kernel(LinArgs a) {
         bias.load(a, n);
         finish<true, 0, 1>(a, m, n, v, bias);
     }
+}
+
+// n rows of len bytes, one every step bytes.
+struct MemRows {
+    const void* at;
+    int64_t step, len, n;
+};
+
+// Whether two such sets share a byte.  Rows of one set between those of the other (columns of one wider matrix) do not.
+bool rows_meet(MemRows a, MemRows b) {
+    if (a.n <= 0 || b.n <= 0 || a.len <= 0 || b.len <= 0) return false;
+    typedef __int128 wide;
+    auto begin = [](const MemRows& r) { return (wide) reinterpret_cast<uintptr_t>(r.at); };
+    auto end = [&](const MemRows& r) { return begin(r) + (wide)(r.n - 1) * r.step + r.len; };
+    if (end(a) <= begin(b) || end(b) <= begin(a)) return false;
+    for (MemRows* r : {&a, &b})  // rows that touch or overlap: one row
+        if (r->step <= r->len) *r = MemRows{r->at, 0, (int64_t)(end(*r) - begin(*r)), 1};
+    if (a.n > b.n) std::swap(a, b);
+    // row i of a against the first row of b that ends behind its beginning
+    auto row_meets = [&](wide i) {
+        const wide lo = begin(a) + i * a.step, past = lo - begin(b) - b.len;
+        const wide j = past < 0 || b.n == 1 ? (past < 0 ? 0 : 1) : past / b.step + 1;
+        return j < b.n && begin(b) + j * b.step < lo + a.len;
+    };
+    if (b.n > 1 && a.step == b.step) {  // equal steps: a pair that meets can be moved until one of the two is its set's first row
+        const wide d = begin(b) - begin(a), i = d >= 0 ? d / a.step : -1;
+        return row_meets(0) || (i >= 0 && i < a.n && row_meets(i)) || (i + 1 >= 0 && i + 1 < a.n && row_meets(i + 1));
+    }
+    for (int64_t i = 0; i < a.n; ++i)
+        if (row_meets(i)) return true;
+    return false;
 }
 
 }  // namespace
@@ -52,6 +85,17 @@ int mbrt_linear(const void* x, int dtype, int64_t x_row_stride, const void* weig
                      (!bias || aligned(bias, dt_size(bias_dtype))) &&
                      (!residual || aligned(residual, dt_size(residual_dtype))),
                  MBRT_E_ALIGN, "%s: pointer not aligned to its elements", op);
+    const int64_t ob = dt_size(out_dtype);
+    const MemRows o{out, rows == 1 ? 0 : out_row_stride * ob, out_features * ob, rows};
+    auto apart = [&](const void* p, int dt, int64_t stride, int64_t n, int64_t cols) {
+        return p == nullptr || !rows_meet(o, MemRows{p, stride * dt_size(dt), cols * dt_size(dt), n});
+    };
+    const bool in_place = residual == out && residual_dtype == out_dtype && (rows == 1 || residual_row_stride == out_row_stride);
+    MBRT_REQUIRE(apart(x, dtype, x_row_stride, rows, in_features) &&
+                     apart(weight, dtype, weight_row_stride, out_features, in_features) &&
+                     apart(bias, bias_dtype, 0, 1, out_features) &&
+                     (in_place || apart(residual, residual_dtype, residual_row_stride, rows, out_features)),
+                 MBRT_E_INVALID_ARG, "%s: out overlaps an input (it may be the residual itself, in the same dtype and rows)", op);
     LinArgs a{};
     a.x = static_cast<const char*>(x);
     a.w = static_cast<const char*>(weight);

@@ -243,3 +243,29 @@ def test_activations_in_their_tails(dev, dtype, out, act):
         w = torch.ones((n, 1), dtype=dtype, device="cuda")
         want, bound = ref.activation(x.expand(-1, n), act, out, dtype != F32 and out != F32)
         ref.check(mbrt.linear(x.cuda(), w, act=act, out_dtype=out), want, bound, f"act {act}")
+
+
+def test_outputs_beside_their_inputs_and_within_them(dev):
+    """Columns of one wider matrix as input and out, and a residual beside out; what shares memory otherwise is refused."""
+    import mbrt
+
+    for rows, k, n in ((9, 64, 72), (700, 64, 72), (700, 72, 72)):
+        say(f"beside rows={rows} k={k} n={n}")
+        wide = _rand(1, (rows, k + 2 * n), BF16)
+        x, out, r = wide[:, :k], wide[:, k:k + n], wide[:, k + n:]
+        w = _rand(2, (n, k), BF16, 0.1)
+        want, bound = ref.linear(x, w, None, 0, r, BF16)
+        kept = wide.clone()
+        ref.check(mbrt.linear(x, w, out=out, residual=r), want, bound, "beside")
+        assert torch.equal(x, kept[:, :k]) and torch.equal(r, kept[:, k + n:])
+        with pytest.raises(mbrt.MbrtError, match="overlaps"):
+            mbrt.linear(x, w, out=wide[:, k - 1:k - 1 + n])
+        if rows == 700:
+            with pytest.raises(mbrt.MbrtError, match="overlaps"):
+                mbrt.linear(r, _rand(2, (n, n), BF16), out=r)
+    sq = _rand(3, (64, 64), BF16)
+    for kw in (dict(out=sq), dict(residual=sq[:, :1].expand(64, 64), out=sq)):
+        with pytest.raises(mbrt.MbrtError, match="overlaps"):
+            mbrt.linear(sq if len(kw) == 1 else _rand(4, (64, 64), BF16), _rand(5, (64, 64), BF16), **kw)
+    with pytest.raises(mbrt.MbrtError, match="overlaps"):
+        mbrt.linear(_rand(4, (64, 64), BF16), sq, out=sq)

@@ -161,3 +161,27 @@ def test_binding_refusals_without_the_extension_module(lib, monkeypatch):
 
     monkeypatch.setattr(mbrt, "_n", _calls)
     test_binding_refusals(lib)
+
+
+def test_linear_refuses_an_output_within_its_inputs(lib):
+    far = [(k + 1) << 32 for k in range(4)]
+
+    def call(x=far[0], w=far[1], b=None, r=None, out=far[2], xs=64, ws=64, rs=64, os=64, rows=100, dt=BF16, odt=BF16,
+             rdt=BF16):
+        return lib.mbrt_linear(x, dt, xs, w, ws, b, F32, r, rdt, rs, out, odt, os, rows, 64, 64, 0, None)
+
+    def refused(**kw):
+        return call(**kw) == ARG and "overlaps" in _err(lib)
+
+    size = 2 * 100 * 64
+    for at in (-size + 2, -2, 0, 2, size - 2):   # from one shared element at the front to one at the end
+        assert refused(out=far[0] + at) and refused(r=far[3], out=far[3] + (at or 2))
+    for at in (-size + 2, 0, 2 * 64 * 64 - 2):
+        assert refused(out=far[1] + at)
+    for at in (-size + 2, 0, 4 * 64 - 2):
+        assert refused(b=far[3], out=far[3] + at)
+    # the residual's place in another type or other rows
+    assert refused(r=far[2], rdt=F16) and refused(r=far[2], rs=0) and refused(r=far[2], rs=128)
+    # columns of one matrix of 128 of which x and out share one, or which meet at other strides; one row for all
+    assert refused(xs=128, os=128, out=far[0] + 2 * 63) and refused(xs=128, os=128, out=far[0] - 2 * 63)
+    assert refused(xs=100, os=128, out=far[0] + 2 * 64) and refused(xs=0, out=far[0] - 2 * 64 * 50)
