@@ -85,6 +85,8 @@ int mbrt_linear(const void* x, int dtype, int64_t x_row_stride, const void* weig
                      (!bias || aligned(bias, dt_size(bias_dtype))) &&
                      (!residual || aligned(residual, dt_size(residual_dtype))),
                  MBRT_E_ALIGN, "%s: pointer not aligned to its elements", op);
+    if (rows == 1) x_row_stride = residual_row_stride = 0;  // of a single row: not used
+    if (out_features == 1) weight_row_stride = 0;
     const int64_t ob = dt_size(out_dtype);
     const MemRows o{out, rows == 1 ? 0 : out_row_stride * ob, out_features * ob, rows};
     auto apart = [&](const void* p, int dt, int64_t stride, int64_t n, int64_t cols) {

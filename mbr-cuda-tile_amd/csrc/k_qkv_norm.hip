@@ -190,9 +190,13 @@ int mbrt_split_qkv_norm_rotary(const void* qkv, int qkv_dtype, int64_t qkv_batch
     MBRT_REQUIRE(pos0 >= 0 && pos0 <= n_pos && N <= n_pos - pos0, MBRT_E_SHAPE,
                  "%s: positions %lld .. %lld of a table of %lld", op, (long long)pos0, (long long)(pos0 + N),
                  (long long)n_pos);
-    const int64_t st[8] = {qkv_batch_stride, qkv_token_stride, q_batch_stride, q_head_stride, q_token_stride,
-                           kv_batch_stride, kv_head_stride, kv_token_stride};
-    for (int i = 0; i < 8; ++i) MBRT_REQUIRE(st[i] >= 0, MBRT_E_SHAPE, "%s: negative stride", op);
+    int64_t st[8] = {qkv_batch_stride, qkv_token_stride, q_batch_stride, q_head_stride, q_token_stride,
+                     kv_batch_stride, kv_head_stride, kv_token_stride};
+    const int64_t dim[8] = {B, N, B, H, N, B, H_kv, N};
+    for (int i = 0; i < 8; ++i) {
+        MBRT_REQUIRE(st[i] >= 0, MBRT_E_SHAPE, "%s: negative stride", op);
+        if (dim[i] <= 1) st[i] = 0;  // of a single index: not used
+    }
     MBRT_REQUIRE(B < (int64_t(1) << 31) && N < (int64_t(1) << 31), MBRT_E_SHAPE, "%s: dimension beyond 2^31", op);
     for (int i = 0; i < 2; ++i) {  // q, then k and v
         const int64_t* s = st + 2 + 3 * i;
@@ -219,14 +223,14 @@ int mbrt_split_qkv_norm_rotary(const void* qkv, int qkv_dtype, int64_t qkv_batch
     a.odt = out_dtype;
     a.gdt = gamma_dtype;
     a.tdt = trig_dtype;
-    a.in_bs = qkv_batch_stride;
-    a.in_ns = qkv_token_stride;
-    a.q_bs = q_batch_stride;
-    a.q_hs = q_head_stride;
-    a.q_ns = q_token_stride;
-    a.kv_bs = kv_batch_stride;
-    a.kv_hs = kv_head_stride;
-    a.kv_ns = kv_token_stride;
+    a.in_bs = st[0];
+    a.in_ns = st[1];
+    a.q_bs = st[2];
+    a.q_hs = st[3];
+    a.q_ns = st[4];
+    a.kv_bs = st[5];
+    a.kv_hs = st[6];
+    a.kv_ns = st[7];
     a.tokens = B * N;
     a.N = N;
     a.pos0 = pos0;

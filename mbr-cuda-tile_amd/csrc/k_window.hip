@@ -806,10 +806,13 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
     MBRT_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(key_lens, 4) &&
                      (!gate || aligned(gate, dt_size(gate_dtype))),
                  MBRT_E_ALIGN, "%s: q, k, v and out must be 16-byte aligned", op);
-    const int64_t st[9] = {q_batch_stride, q_head_stride, q_row_stride, kv_batch_stride, kv_head_stride,
-                           kv_row_stride, out_batch_stride, out_head_stride, out_row_stride};
-    for (int i = 0; i < 9; ++i)
+    int64_t st[9] = {q_batch_stride, q_head_stride, q_row_stride, kv_batch_stride, kv_head_stride,
+                     kv_row_stride, out_batch_stride, out_head_stride, out_row_stride};
+    const int64_t dim[9] = {B, H, n_q, B, H_kv, n_k, B, H, n_q};
+    for (int i = 0; i < 9; ++i) {
+        if (st[i] > 0 && dim[i] <= 1) st[i] = 0;  // of a single index: not used
         MBRT_REQUIRE(st[i] >= 0 && st[i] % 8 == 0, MBRT_E_ALIGN, "%s: strides must be non-negative multiples of 8", op);
+    }
     MBRT_REQUIRE((B == 1 || out_batch_stride > 0) && (H == 1 || out_head_stride > 0) && (n_q == 1 || out_row_stride > 0),
                  MBRT_E_SHAPE, "%s: rows of out overlap", op);
     const Plan plan = make_plan(B, H, H_kv, n_q, n_k, head_dim, left, right, std::min(sinks, n_k));
@@ -826,15 +829,15 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
     a.lens = key_lens;
     a.gate = gate;
     a.ws = static_cast<float*>(workspace);
-    a.q_bs = q_batch_stride;
-    a.q_hs = q_head_stride;
-    a.q_ns = q_row_stride;
-    a.kv_bs = kv_batch_stride;
-    a.kv_hs = kv_head_stride;
-    a.kv_ns = kv_row_stride;
-    a.o_bs = out_batch_stride;
-    a.o_hs = out_head_stride;
-    a.o_ns = out_row_stride;
+    a.q_bs = st[0];
+    a.q_hs = st[1];
+    a.q_ns = st[2];
+    a.kv_bs = st[3];
+    a.kv_hs = st[4];
+    a.kv_ns = st[5];
+    a.o_bs = st[6];
+    a.o_hs = st[7];
+    a.o_ns = st[8];
     a.nq = (int)n_q;
     a.nk = (int)n_k;
     a.rows = (int)(n_q * G);

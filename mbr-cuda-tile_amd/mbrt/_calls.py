@@ -188,6 +188,11 @@ def _unit_last(*ts):
             raise ValueError("mbrt: expected a contiguous last dim")
 
 
+def _alike(a, b):
+    """Strides that are used, the same in both (those of a single index are not)."""
+    return not a.numel() or all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n > 1)
+
+
 def _row_stride(t):
     """The one stride between the rows of [.., n] (0 where there is one row)."""
     span, stride = 1, 0
@@ -237,7 +242,7 @@ def split_qkv_norm_rotary(qkv, q_gamma, k_gamma, cos, sin, q, k, v, heads, kv_he
         raise ValueError("split_qkv_norm_rotary: expected q [B, H, N, D] and k, v [B, H_kv, N, D]")
     if q.dtype != k.dtype or v is not None and v.dtype != k.dtype:
         raise ValueError("split_qkv_norm_rotary: q, k and v differ in dtype")
-    if v is not None and v.stride() != k.stride():
+    if v is not None and not _alike(k, v):
         raise ValueError("split_qkv_norm_rotary: k and v must be strided alike")
     if q_gamma.shape != (D,) or k_gamma.shape != (D,) or q_gamma.dtype != k_gamma.dtype:
         raise ValueError("split_qkv_norm_rotary: expected gammas [D] of one dtype")
@@ -263,7 +268,7 @@ def attention_window(q, k, v, out, left, right, sinks, q_start, key_lens, gate, 
         raise ValueError("attention_window: expected q [B, N_q, H, D] and k, v [B, N_k, H_kv, D]")
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("attention_window: q, k and v differ in dtype")
-    if v.stride() != k.stride():
+    if not _alike(k, v):
         raise ValueError("attention_window: k and v must be strided alike")
     if out.shape != q.shape:
         raise ValueError("attention_window: expected out [B, N_q, H, D]")

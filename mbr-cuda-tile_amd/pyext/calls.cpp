@@ -379,6 +379,14 @@ void unit_last(std::initializer_list<const at::Tensor*> ts) {
             raise(PyExc_ValueError, "mbrt: expected a contiguous last dim");
 }
 
+// Strides that are used, the same in both (those of a single index are not).
+bool strided_alike(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0) return true;
+    for (int64_t d = 0; d < a.dim(); ++d)
+        if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+    return true;
+}
+
 // The one stride between the rows of [.., n] (0 where there is one row).
 int64_t row_stride(const at::Tensor& t) {
     int64_t span = 1, stride = 0;
@@ -444,7 +452,7 @@ MBRT_PY(split_qkv_norm_rotary) {
         raise(PyExc_ValueError, "split_qkv_norm_rotary: expected q [B, H, N, D] and k, v [B, H_kv, N, D]");
     if (q.scalar_type() != k.scalar_type() || (v.defined() && v.scalar_type() != k.scalar_type()))
         raise(PyExc_ValueError, "split_qkv_norm_rotary: q, k and v differ in dtype");
-    if (v.defined() && v.strides() != k.strides())
+    if (v.defined() && !strided_alike(k, v))
         raise(PyExc_ValueError, "split_qkv_norm_rotary: k and v must be strided alike");
     if (qg.dim() != 1 || qg.size(0) != D || kg.sizes() != qg.sizes() || kg.scalar_type() != qg.scalar_type())
         raise(PyExc_ValueError, "split_qkv_norm_rotary: expected gammas [D] of one dtype");
@@ -479,7 +487,7 @@ MBRT_PY(attention_window) {
     const int64_t B = q.size(0), nq = q.size(1), H = q.size(2), D = q.size(3), nk = k.size(1), KV = k.size(2);
     if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
         raise(PyExc_ValueError, "attention_window: q, k and v differ in dtype");
-    if (v.strides() != k.strides()) raise(PyExc_ValueError, "attention_window: k and v must be strided alike");
+    if (!strided_alike(k, v)) raise(PyExc_ValueError, "attention_window: k and v must be strided alike");
     if (out.sizes() != q.sizes()) raise(PyExc_ValueError, "attention_window: expected out [B, N_q, H, D]");
     if (lens.defined() && (lens.dim() != 1 || lens.size(0) != B || lens.scalar_type() != at::kInt))
         raise(PyExc_ValueError, "attention_window: expected key_lens [B] int32");

@@ -178,3 +178,28 @@ def test_captured_and_on_another_stream(dev):
         torch.cuda.synchronize()
         for a, b, c in zip(*outs):
             assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("path", ["native", "ctypes"])
+def test_strides_that_nothing_uses(dev, path, monkeypatch):
+    """Strides of dimensions of size 1 may be anything, and differ between keys and values."""
+    import mbrt
+    from mbrt import _calls
+
+    if path == "ctypes":
+        monkeypatch.setattr(mbrt, "_n", _calls)
+    for B, N, H, KV in ((1, 20, 2, 2), (3, 1, 2, 1), (1, 1, 1, 1)):
+        say(f"single indices B={B} N={N} {H}/{KV}")
+        qkv = _rand(1, (B, N, (H + 2 * KV) * 64), BF16)
+        gamma, (cos, sin) = torch.ones(64, device="cuda"), _tables(N, 64)
+        outs = []
+        for odd in (False, True):
+            views = []
+            for i, h in enumerate((H, KV, KV)):
+                t = _heads(B, h, N, 64, BF16, "bhnd")
+                st = [8 * t.numel() + 3 + i if odd and n == 1 else s for s, n in zip(t.stride(), t.shape)]
+                views.append(t.as_strided(t.shape, st))
+            mbrt.split_qkv_norm_rotary(qkv, gamma, gamma, cos, sin, *views, H, kv_heads=KV)
+            outs.append([t.clone() for t in views])
+        for a, b in zip(*outs):
+            assert torch.equal(a, b)

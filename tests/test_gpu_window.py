@@ -382,3 +382,31 @@ def test_weights_of_bf16_behind_a_border(dev, D):
             gate = torch.full((B, nq, 4), (1 + 2.0 ** -8) * side, device="cuda")
             got = mbrt.attention_window(q, k, v, left=2, right=0, gate=gate, gate_is_logit=False)
             assert int((got != want).sum()) == 0
+
+
+def _single_index_strides(t, dims):
+    """The same view with strides of `dims`, of one index each, that nothing uses."""
+    st = list(t.stride())
+    for d in dims:
+        assert t.shape[d] == 1
+        st[d] = 8 * t.numel() + 3
+    return t.as_strided(t.shape, st)
+
+
+@pytest.mark.parametrize("path", ["native", "ctypes"])
+def test_strides_that_nothing_uses(dev, path, monkeypatch):
+    """Strides of dimensions of size 1 may be anything, and differ between keys and values."""
+    import mbrt
+    from mbrt import _calls
+
+    if path == "ctypes":
+        monkeypatch.setattr(mbrt, "_n", _calls)
+    for B, nq, nk, H, KV, odd in ((1, 40, 60, 2, 2, (0,)), (3, 1, 60, 2, 1, (2,)), (1, 1, 1, 1, 1, (0, 1, 2)),
+                                  (2, 1, 60, 4, 4, ())):
+        say(f"single indices B={B} nq={nq} nk={nk} {H}/{KV}")
+        q, k, v = _qkv(3, B, nq, nk, H, KV, 64, BF16)
+        want = mbrt.attention_window(q, k, v, left=30, right=0)
+        qd = [d for d in range(3) if q.shape[d] == 1]
+        out = _single_index_strides(torch.empty_like(want), qd)
+        got = mbrt.attention_window(_single_index_strides(q, qd), k, _single_index_strides(v, odd), out, left=30, right=0)
+        assert torch.equal(got, want)
