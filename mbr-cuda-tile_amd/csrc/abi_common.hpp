@@ -44,6 +44,9 @@ inline int cold_input(int64_t bytes, int64_t limit = MBRT_HOT_BYTES) { return by
 // where kernels assume it).
 constexpr int64_t kMaxGridX = 0x7fffffffLL;
 
+// Whether a launch of so many blocks is within that and the 2^32 - 1 threads that a launch may have.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks < kMaxGridX && blocks <= 0xffffffffLL / threads; }
+
 }  // namespace mbrt
 
 #define MBRT_REQUIRE(cond, status, ...)                         \

@@ -257,7 +257,7 @@ int mbrt_split_qkv_norm_rotary(const void* qkv, int qkv_dtype, int64_t qkv_batch
         for (int i = 1; i < a.S; i *= 2) ++a.head_bits;
         a.ndiv = make_fastdiv((uint32_t)N);
         const int64_t blocks = ceil_div(a.tokens * a.G * a.S, kThreads);
-        vec = a.tokens < (int64_t(1) << 31) && blocks < kMaxGridX;  // 32-bit token numbers
+        vec = a.tokens < (int64_t(1) << 31) && grid_fits(blocks, kThreads);  // 32-bit token numbers
         if (vec)
             with_dt(qkv_dtype, [&](auto it) {
                 with_dt(out_dtype, [&](auto ot) {

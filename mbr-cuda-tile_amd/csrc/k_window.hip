@@ -858,7 +858,7 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
     const int64_t bkv = B * H_kv;
     a.qtiles = (uint32_t)ceil_div(a.rows, plan.few ? 16 : 64 * plan.qs);
     const int64_t blocks = bkv * a.qtiles * plan.splits;
-    MBRT_REQUIRE(blocks < kMaxGridX && bkv * a.rows < kMaxGridX, MBRT_E_SHAPE, "%s: too many tiles", op);
+    MBRT_REQUIRE(grid_fits(blocks, plan.few ? kSplitWaves * 64 : 256), MBRT_E_SHAPE, "%s: too many tiles", op);
     auto launch = [&](auto dt, auto dim, auto parts) {
         constexpr int DTv = decltype(dt)::value, Dv = decltype(dim)::value, NP = decltype(parts)::value;
         if (!plan.few) {

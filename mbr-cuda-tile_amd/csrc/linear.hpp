@@ -641,7 +641,7 @@ int launch_tile(LinArgs& a, hipStream_t st) {
     a.ntiles = (uint32_t)ceil_div(a.N, BN);
     a.groups = make_fastdiv(a.ntiles);
     const int64_t tiles = ceil_div(a.M, BM) * a.ntiles;
-    if (tiles >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many tiles");
+    if (!grid_fits(tiles, WM * WN * KS * 64)) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many tiles");
     const dim3 grid((unsigned)tiles), block(WM * WN * KS * 64);
     if (a.act != MBRT_ACT_NONE)
         hipLaunchKernelGGL((linear_tile_kernel<DT, WM, WN, MI, NI, DIRECT, NT, KS, true>), grid, block, 0, st, a);
@@ -701,9 +701,9 @@ int launch_linear(LinArgs& a, int align, hipStream_t st) {
         a.groups = make_fastdiv((uint32_t)groups);
         a.splits = make_fastdiv((uint32_t)a.split);
         const int64_t blocks = ceil_div(strips, per_block) * groups;
-        if (blocks >= kMaxGridX) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many rows");
         const size_t lds = a.split == 1 ? 0 : (size_t)per_block * a.split * R * 1024;
         const unsigned threads = per_block * a.split * 64;
+        if (!grid_fits(blocks, threads)) return set_error(MBRT_E_SHAPE, "mbrt_linear: too many rows");
         if (R == 1) launch_strip<DT, 1>(a, wide, align, (unsigned)blocks, threads, lds, st);
         else if (R == 2) launch_strip<DT, 2>(a, wide, align, (unsigned)blocks, threads, lds, st);
         else launch_strip<DT, 4>(a, wide, align, (unsigned)blocks, threads, lds, st);

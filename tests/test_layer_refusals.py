@@ -185,3 +185,15 @@ def test_linear_refuses_an_output_within_its_inputs(lib):
     # columns of one matrix of 128 of which x and out share one, or which meet at other strides; one row for all
     assert refused(xs=128, os=128, out=far[0] + 2 * 63) and refused(xs=128, os=128, out=far[0] - 2 * 63)
     assert refused(xs=100, os=128, out=far[0] + 2 * 64) and refused(xs=0, out=far[0] - 2 * 64 * 50)
+
+
+def test_calls_too_large_for_one_launch(lib):
+    """2^32 threads and more, which the hardware's launch cannot hold, are refused by size before the launch fails."""
+    far = [(k + 1) << 48 for k in range(4)]
+    for dt, rows, k, n in ((BF16, 1 << 32, 64, 64), (BF16, 1 << 33, 64, 8), (F32, 1 << 33, 64, 8), (F16, 1 << 32, 64, 1000)):
+        assert lib.mbrt_linear(far[0], dt, 0, far[1], k, None, F32, None, F32, 0, far[2], dt, n, rows, k, n, 0, None) == SHAPE
+        assert "too many" in _err(lib)
+    for B, nq, nk in ((1 << 24, 1, 16), (1 << 20, 2000, 16)):
+        assert lib.mbrt_attention_window(far[0], far[1], far[2], BF16, B, 1, 1, nq, nk, 64, nq * 64, 64, 64, 0, 0, 64, 5, 0, 0, -1,
+                                         None, None, F32, 1, far[3], BF16, nq * 64, 64, 64, 0.0, None, 0, None) == SHAPE
+        assert "too many" in _err(lib)
