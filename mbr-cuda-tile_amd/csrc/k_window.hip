@@ -800,7 +800,9 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
                  "%s: negative size, or a dimension beyond 2^28 (2^16 heads)", op);
     MBRT_REQUIRE(left >= -1 && right >= -1 && q_start >= -1 && q_start < (int64_t(1) << 28), MBRT_E_INVALID_ARG,
                  "%s: left, right and q_start are -1 or more, q_start below 2^28", op);
-    MBRT_REQUIRE(scale >= 0.0f && std::isfinite(scale), MBRT_E_INVALID_ARG, "%s: scale must be finite and >= 0", op);
+    const float sl2 = (scale == 0.0f ? 1.0f / std::sqrt((float)head_dim) : scale) * 1.44269504088896340736f;  // of powers of 2
+    MBRT_REQUIRE(scale >= 0.0f && std::isfinite(sl2), MBRT_E_INVALID_ARG,
+                 "%s: scale must be finite, as scale * log2(e) must, and >= 0", op);
     if (B == 0 || n_q == 0) return MBRT_OK;
     MBRT_REQUIRE(q && out && (n_k == 0 || (k && v)), MBRT_E_INVALID_ARG, "%s: NULL pointer", op);
     MBRT_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(key_lens, 4) &&
@@ -850,7 +852,7 @@ int mbrt_attention_window(const void* q, const void* k, const void* v, int dtype
     a.gdt = gate_dtype;
     a.glogit = gate_is_logit ? 1 : 0;
     a.odt = out_dtype;
-    a.sl2 = (scale == 0.0f ? 1.0f / std::sqrt((float)head_dim) : scale) * 1.44269504088896340736f;
+    a.sl2 = sl2;
     a.gdiv = make_fastdiv((uint32_t)G);
     a.kvdiv = make_fastdiv((uint32_t)H_kv);
     a.splits = (uint32_t)plan.splits;

@@ -187,6 +187,15 @@ def test_linear_refuses_an_output_within_its_inputs(lib):
     assert refused(xs=100, os=128, out=far[0] + 2 * 64) and refused(xs=0, out=far[0] - 2 * 64 * 50)
 
 
+def test_window_scale_beyond_float(lib):
+    def call(scale):
+        return lib.mbrt_attention_window(P, P, P, BF16, 1, 1, 1, 4, 4, 64, 256, 64, 64, 256, 64, 64, 5, 0, 0, -1, None, None, F32, 1,
+                                         None, BF16, 256, 64, 64, scale, None, 0, None)
+
+    assert call(3e38) == ARG and "scale" in _err(lib)      # in powers of 2 it is infinite
+    assert call(2e38) == ARG and "NULL" in _err(lib)       # accepted: the next refusal is out's
+
+
 def test_calls_too_large_for_one_launch(lib):
     """2^32 threads and more, which the hardware's launch cannot hold, are refused by size before the launch fails."""
     far = [(k + 1) << 48 for k in range(4)]
