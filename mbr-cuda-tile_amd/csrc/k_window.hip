@@ -524,7 +524,7 @@ __global__ __launch_bounds__(256) void window_tile_kernel(WinArgs a) {
         const int r = r0 + 16 * x + c, qi = (int)fdiv((uint32_t)min(r, a.rows - 1), a.gdiv);
         const int h = kv * G + min(r, a.rows - 1) - qi * G;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-        bool bad = not_finite(l) || (l == 0.0f && (rw.n[x] > 0 || min(sp.s, rw.jhi[x] + 1) > 0));  // as sees_any
+        bool bad = not_finite(l) || (l == 0.0f && sees_any(a, b, min(r, a.rows - 1)));
 #pragma unroll
         for (int db = 0; db < D / 16; ++db)
 #pragma unroll
