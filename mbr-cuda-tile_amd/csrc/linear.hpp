@@ -683,11 +683,16 @@ int launch_linear(LinArgs& a, int align, hipStream_t st) {
     // [1000, 1536] -> 384 26.5 and 31.3; [801, 118] -> 384 bf16 6.2 and 4.3, f32 7.0 and 4.9.
     // A short operand of up to 16 rows goes in strips too, which multiply no 16 rows in vain where tiles multiply 64: always
     // for f32, whose products count ([48060, 384] -> 8 25 and 18; up to 32 rows while tiles are few, [5000, 1536] -> 24 31 and 18,
-    // but [48060, 1536] -> 24 81 and 93), and for 2-byte types where tiles of 64 are few or
-    // short ([10000, 384] -> 8 5.4 and 4.3, [48060, 130] -> 8 6.8 and 5.6, but [48060, 384] -> 16 8.4 and 10.5, [8, 384] ->
-    // 20000 4.4 and 6.5, [48060, 1536] -> 8 30 and 34).
+    // but [48060, 1536] -> 24 81 and 93), and for 2-byte types where tiles of 64 are few ([10000, 384] -> 8 4.8 and 4.3, [16000,
+    // 1536] -> 8 12.4 and 12.3) or K is short.  How short goes by what a tile loses at its rows' end: whole pieces of 128 bytes
+    // up to one of them ([48060, 64] -> 8 4.3 and 4.1, [48060, 128] -> 16 4.8 and 5.2, [48060, 256] -> 16 6.3 and 7.6, [48060,
+    // 384] -> 8 8.0 and 8.6, -> 16 8.1 and 10.4), as rows at odd addresses ([48060, 65] -> 8 5.9 and 5.7, [48060, 193] -> 16 8.6 and 10.3,
+    // [48060, 385] -> 8 12.0 and 14.6); pieces that are cut up to six, where it turns with the other sizes (-> 8 from [48060, 200]
+    // 7.1 and 5.7, 386 10.6 and 9.7, 392 10.1 and 8.2, 456 11.6 and 10.5, 648 16.5 and 17.1; -> 16 376 9.7 and 9.4, 386 10.7 and
+    // 11.6, 392 10.5 and 9.4, 456 12.0 and 12.3; [16, 264] -> 20000 4.9 and 4.7, 386 6.7 and 8.3, 392 5.3 and 6.1).
+    const int64_t kb = a.K * es, short_k = kb % 128 != 0 && align >= 4 ? 6 * 128 : 2 * 128;
     if (strips * ceil_div(shorter, 64) <= (DT == F32 ? (al ? 1 : 2) * cus : (al ? 1 : 4) * cus / 2) ||
-        (shorter <= 16 && (DT == F32 || longer < 64 * cus || a.K * es < 768)) ||
+        (shorter <= 16 && (DT == F32 || longer < 64 * cus || kb < short_k)) ||
         (DT == F32 && shorter <= 32 && longer < 64 * cus)) {
         int R = shorter <= 16 ? 1 : shorter <= 32 ? 2 : 4;
         while (R > 1 && strips * ceil_div(shorter, 8 * R) <= (al ? 1 : 8) * cus) R /= 2;
