@@ -461,7 +461,8 @@ MBRT_API int mbrt_split_qkv_norm_rotary(const void* qkv, int qkv_dtype, int64_t 
  * of q's type: BF16 two or three, within 2^-17 of each probability (2^-24 to an F32 out); F16 two, within 2^-23 of it or 2^-35 of
  * its row's largest probability, whichever is more.  A few queries against many keys are shared out over the keys and joined through
  * `workspace` (mbrt_attention_window_workspace_bytes of the same sizes; 0 bytes: may be NULL), in a fixed order:
- * results do not change from call to call.  Calls that overlap need workspaces of their own.
+ * results do not change from call to call.  Calls that overlap need workspaces of their own; its size goes by the
+ * current device's compute units, too.  out may be q's own places (same dtype and strides); it must share no other byte with an input.
  * Beside mbrt_attention_ex, for songs longer than a chunk and for streaming. */
 MBRT_API int64_t mbrt_attention_window_workspace_bytes(int64_t B, int64_t H, int64_t H_kv, int64_t n_q, int64_t n_k,
                                                        int64_t head_dim, int64_t left, int64_t right,

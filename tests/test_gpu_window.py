@@ -410,3 +410,24 @@ def test_strides_that_nothing_uses(dev, path, monkeypatch):
         out = _single_index_strides(torch.empty_like(want), qd)
         got = mbrt.attention_window(_single_index_strides(q, qd), k, _single_index_strides(v, odd), out, left=30, right=0)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("nq,nk,H,KV", [(65, 3000, 8, 2), (257, 3000, 2, 2), (130, 2500, 4, 1)])
+def test_groups_of_queries_against_a_long_cache(dev, nq, nk, H, KV):
+    """More rows than are shared out over their keys, each list long."""
+    _case(1, nq, nk, H, KV, 64, BF16, right=0)
+    _case(2, nq, nk, H, KV, 32, F16, F32, lens=[nk, nk // 2 + 7], left=nk - 300, right=0, sinks=5)
+
+
+def test_output_in_the_place_of_the_queries(dev):
+    """Every form: a tile of rows, few rows, keys shared out; rows that are computed again read their query first."""
+    import mbrt
+
+    for nq, nk, kw in ((150, 150, dict(left=30, right=0)), (3, 60, dict()), (2, 6000, dict(right=0))):
+        say(f"in place nq={nq} nk={nk}")
+        q, k, v = _qkv(6, 2, nq, nk, 4, 2, 64, BF16)
+        v[0, nk - 2, 0, 5] = float("nan")
+        want = mbrt.attention_window(q, k, v, **kw)
+        got = mbrt.attention_window(q, k, v, q, **kw)
+        assert got is q and torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
