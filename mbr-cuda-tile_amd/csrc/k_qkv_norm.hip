@@ -7,8 +7,8 @@
 // Bound by memory: each element is read and written once.  G lanes hold one head vector, 16 bytes each, and reduce
 // its sum of squares with DPP adds; a token has S such groups side by side (a wave, where it has the heads), which walk
 // its heads, so that a thread reads its cos, sin and gamma once for all of them.  MI355X: bf16 [60, 801] with 8 heads of
-// 64, 295 MB, 54.8 us (5.4 TB/s; a large copy 4.8); f32 [30, 801], 8 heads over 2 of 128, 25.7 us; a frame of 60 rows
-// 4.1 to 4.4, the launch.
+// 64, 295 MB, 54.8 us (5.4 TB/s; a large copy 4.8 to 5.2); f32 [7, 1301], 8 heads over 2 of 128, heads outside tokens, 113 MB,
+// 25.7 us; a frame of 60 rows 4.1 to 4.4, the launch.
 #include "abi_common.hpp"
 
 #include <algorithm>
@@ -129,7 +129,9 @@ __global__ __launch_bounds__(kThreads) void qkv_norm_vec_kernel(QkvArgs a) {
     }
 }
 
-// Any even D, any alignment: a wave per head vector.
+// Any even D, any alignment: a wave per head vector, an element per lane and access.  One unaligned pointer or stride takes
+// the whole call here: the [60, 801] above with tokens 1537 elements apart 444 us, with heads of 66 497, the f32 one 50; a frame
+// of 60 rows 3.8, as the other kernel.
 __global__ __launch_bounds__(kThreads) void qkv_norm_any_kernel(QkvArgs a) {
     const int lane = threadIdx.x % 64;
     const int64_t vecs = a.tokens * a.heads, waves = (int64_t)gridDim.x * (kThreads / 64);

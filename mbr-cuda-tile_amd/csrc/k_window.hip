@@ -18,10 +18,11 @@
 //                    2-byte type (split_p), so that little beside the inputs' and the output's own rounding is left.
 // Lane (g, c) ends with columns 16 db + 4 g .. + 3 of row c.
 //
-// What bounds it (MI355X, us; counters by rocprofv3): bf16 [60, 801], 8 heads of 64 through 101 keys and 8 sinks, 57.5; its
+// What bounds it (MI355X, us; counters by rocprofv3): bf16 [60, 801], 8 heads of 64 through 101 keys and 8 sinks, 57.5 to 60; its
 // loads and stores alone take 43 (197 MB at 4.6 TB/s), the rest is the softmax's VALU work, which hides behind them only in
 // part (a wave's tile of 64 keys: 24 MFMAs of 16 clocks, about 170 VALU instructions of 4 and 16 exponentials of 16, and 16 KB of
-// LDS reads).  f16 [2, 16389], 8 heads over 2 of 128 through 1024 keys, 210: 134 GFLOP, half as many again for the second
+// LDS reads), a third of it for nothing: a wave's 16 rows see 124 keys, the list of its tile holds 172, and it works on 192.
+// f16 [2, 16389], 8 heads over 2 of 128 through 1024 keys, 210 to 215: 134 GFLOP, half as many again for the second
 // part of p (145 at a large library product's rate), on matrix units that are busy half the time, the
 // VALU for about as long (9 operations and an exponential for each score), which two waves per SIMD overlap only in
 // part.  One token: 60 caches of 1601 frames 20.4, 100 MB at 4.9 TB/s, as a
@@ -34,7 +35,8 @@
 //
 // A value that a row does not see but another row of its tile does enters the product with weight 0.  Where that
 // value is infinite or NaN the product is NaN; a row that ends with anything not finite is computed again from the
-// keys that it sees alone (row_alone), so that the definition holds for it too.
+// keys that it sees alone (row_alone), so that the definition holds for it too.  That takes its time, key by key, unless the row
+// turns out NaN: f16 [2, 16389] as above with one infinity in a value of one head 25 ms, in a sink's 102.
 #include "abi_common.hpp"
 
 #include <algorithm>
@@ -729,8 +731,9 @@ struct Plan {
     int64_t splits;  // window_split_kernel: shares of the key list
 };
 
-// Few rows (of one tile of 16, or of some while the tiles of 64 would leave CUs idle before long lists) go to the kernel that
-// shares out the keys, 8 waves to a share.  What bounds a share is what one CU can read (16 waves to it gain nothing: 805 keys
+// Few rows (of one tile of 16, or of up to 256 while the tiles of 64 would leave CUs idle before long lists) go to the kernel that
+// shares out the keys, 8 waves to a share.  Past 256 rows every tile of 64 walks its list alone, however few tiles there are:
+// [1, 100003] keys of 2 heads of 64, 64 queries of 8 heads 67 us and 65 1374; of 8 key heads 256 queries 238 and 257 1382.  What bounds a share is what one CU can read (16 waves to it gain nothing: 805 keys
 // of 64 columns 7.1 us with 8, 7.5 with 16); what a second one costs is the join's launch.  So a list is shared out from 32
 // pieces on, of 32 keys and 64 columns each (8 KB of keys and values), 5 to a share, over at most a workgroup per CU, and shorter ones
 // than 64 pieces only where there are 4 shares or more to it.  us, one share and shared out: 16 lists of 25 pieces 7.3 and

@@ -14,14 +14,17 @@
 //
 // What bounds it (MI355X, us; a large copy runs at 4.8 TB/s, a large library product at 1382 TFLOP/s, f32 153):
 //   [48060, 384] -> 1536 bf16 67 (184 MB: 41 at the copy's rate; 844 TFLOP/s).  Stores first: 8 bytes per lane and through the
-//   caches 99, 16 bytes 74, out past the caches 70; the matrix units are busy for 28 of it (counted), and a product's end and the
-//   next one's first loads overlap only between the two workgroups of a CU.
-//   [48060, 1536] -> 384 with residual 93 (221 MB: 46): 172 MB of reads arrive in the order in which tiles ask for them, and
-//   the loads alone take nearly as long.  The library's product alone 96 and, of the former, 122.
+//   caches 99, 16 bytes 74, out past the caches 70; 204 MB are written for 148 MB of out (counted).  The matrix units are busy for
+//   28 of it, and a product's end and the next one's first loads overlap only between the two workgroups of a CU.  With bias and
+//   GELU 104 to 109: the epilogue's 20 VALU operations an element have only the other workgroup to hide behind.
+//   [48060, 1536] -> 384 with residual 93 (221 MB: 46): 176 MB are read in the order in which tiles ask for them, two column tiles
+//   the same rows of x, and every step ends with no load under way; the loads alone take nearly as long.  The library's product
+//   alone 93 and, of the former, 120.
 //   f32 [4096, 4096] -> 4096 960: 143 TFLOP/s.  One row to some hundred: the launch, and the latency of one round of loads (4.1).
-// Not kept: steps of 64 bytes in four buffers or three of 192 x 192 (88 to 110), 256 x 256 (86 and 109), persistent
-// workgroups that store while the next tile loads (74 to 85), fragments fetched across the barrier (no gain), rows handed
-// round through LDS for stores of whole lines (67 -> 79).
+// Not kept, with the times of these two: steps of 64 bytes in four buffers (no gain), 192 x 192 in three buffers (110; 88 to 90,
+// less than the 93, but a form of its own for long K alone), 256 x 256 (86 and 109), persistent workgroups that store while the
+// next tile loads (74 to 85; 88), fragments fetched across the barrier (no gain), rows handed round through LDS for stores of whole
+// lines (67 -> 79).
 #pragma once
 
 #include "abi_common.hpp"
@@ -94,7 +97,7 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
 
 // 16 bytes of a row at a multiple of A bytes: 16, 4 or 2.  Loads at odd multiples of 2 are several times slower than others,
 // so with A = 2 they come as the 20 bytes around them, moved down: the dwords at both ends hold an element of the 16 bytes
-// each, and nothing outside these dwords is read ([48060, 385] -> 8 25.8 -> 14.4 us, [60, 385] -> 1536 7.9 -> 4.7; with A = 4
+// each, and nothing outside these dwords is read ([48060, 385] -> 8 in strips 25.8 -> 14.4 us, [60, 385] -> 1536 7.9 -> 4.7; with A = 4
 // the fifth dword costs: [20000, 500] -> 48 15.3 -> 25.7).
 template <int A>
 __device__ __forceinline__ u32x4 load_row(const char* p) {
