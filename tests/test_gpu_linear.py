@@ -269,3 +269,17 @@ def test_outputs_beside_their_inputs_and_within_them(dev):
             mbrt.linear(sq if len(kw) == 1 else _rand(4, (64, 64), BF16), _rand(5, (64, 64), BF16), **kw)
     with pytest.raises(mbrt.MbrtError, match="overlaps"):
         mbrt.linear(_rand(4, (64, 64), BF16), sq, out=sq)
+
+
+def test_calls_without_the_extension_module(dev, monkeypatch):
+    """The same results, and the same refusals on the GPU, through ctypes."""
+    import mbrt
+    from mbrt import _calls
+
+    wide = _rand(1, (3, 40, 100), BF16)
+    x, w, b, r = wide[..., :64], _rand(2, (36, 64), BF16, 0.1), _rand(3, (36,), F32), _rand(4, (3, 40, 36), F16)
+    want = mbrt.linear(x, w, b, wide[..., 64:].clone(), act=2, residual=r)
+    monkeypatch.setattr(mbrt, "_n", _calls)
+    assert torch.equal(mbrt.linear(x, w, b, wide[..., 64:], act=2, residual=r), want)
+    with pytest.raises(mbrt.MbrtError, match="overlaps"):
+        mbrt.linear(x, w, b, wide[..., 63:99])
