@@ -47,7 +47,8 @@ enum mbrt_dtype {
     MBRT_F16 = 1,
     MBRT_I64 = 2,
     MBRT_BF16 = 3,
-    MBRT_I32 = 4
+    MBRT_I32 = 4,
+    MBRT_MXFP4 = 5 /* microscaled 4-bit floats: only where an entry point names it (mbrt_mx_*, mbrt_block_norm) */
 };
 
 enum mbrt_status {
@@ -475,6 +476,67 @@ MBRT_API int mbrt_attention_window(const void* q, const void* k, const void* v, 
                                    int gate_dtype, int gate_is_logit, void* out, int out_dtype,
                                    int64_t out_batch_stride, int64_t out_head_stride, int64_t out_row_stride,
                                    float scale, void* workspace, int64_t workspace_bytes, mbrt_stream_t stream);
+
+/* ---- transformer layer in 4 bits: microscaled floats, their products, norms around a block ---- */
+
+/* MXFP4 (OCP Microscaling Formats specification v1.0): 32 consecutive features of a row share a scale 2^s, held as the
+ * byte s + 127 (E8M0; 255 is NaN), and each is held in 4 bits as E2M1: sign and 0, .5, 1, 1.5, 2, 3, 4 or 6 times 2^s.
+ * A row of n features is ceil(n / 32) scales and 16 ceil(n / 32) bytes of codes, feature 2 i in the low half of byte i; the last
+ * block is filled with zeros.  Rows of codes begin at multiples of 16 bytes (base and row stride, in bytes); scales may
+ * lie anywhere.
+ *
+ * mbrt_mx_quantize: rows of x (F32/F16/BF16, any row stride and alignment) into that format.  s = floor(log2 max|x|) - 2 over
+ * the block, at least -127; values are x 2^-s rounded to nearest, ties to the even code, past 6 to 6 (a block's largest
+ * value lies in [4, 8) before).  A block that holds an infinity or a NaN becomes NaN as a whole (its codes are unspecified);
+ * one of zeros has scale byte 0.
+ * mbrt_mx_dequantize: the values that codes and scales stand for, rounded once to out's type (F32/F16/BF16; exact in BF16
+ * and F32 as far as their exponents go: f32 overflows for scale bytes 253 and 254).  Any scale byte is taken, so other
+ * software's MXFP4 rows are, too.  Zeros that fill the last block are not written.
+ * Neither lets an output share a byte with another operand.  Beside mbrt_convert. */
+MBRT_API int mbrt_mx_quantize(const void* x, int dtype, int64_t x_row_stride, void* codes, int64_t codes_row_stride,
+                              void* scales, int64_t scales_row_stride, int64_t rows, int64_t features,
+                              mbrt_stream_t stream);
+MBRT_API int mbrt_mx_dequantize(const void* codes, int64_t codes_row_stride, const void* scales,
+                                int64_t scales_row_stride, void* out, int dtype, int64_t out_row_stride, int64_t rows,
+                                int64_t features, mbrt_stream_t stream);
+
+/* Linear layer of MXFP4 weights: out[r, n] = act(sum_k x[r, k] weight[n, k] + bias[n]) + residual[r, n] for weight
+ * [out_features, in_features] and x [rows, in_features] in MXFP4 (dtype MBRT_MXFP4, with x_scales) or F32/F16/BF16 (x_scales
+ * unused), bias and residual F32/F16/BF16 or NULL, out F32/F16/BF16 or MXFP4 (with out_scales; quantised from the f32
+ * results as by mbrt_mx_quantize).  Strides of codes in bytes, of other rows in elements; x, weight and residual may have
+ * any from 0 on.  Products are exact: 4-bit by 4-bit ones, and those of F32/F16/BF16 x, which is taken as a sum of bf16 values
+ * (what lies below 2^-133 of an F32 x is lost).  Sums and the epilogue are f32, with one rounding on the store; activations
+ * as mbrt_linear's, in their short forms unless x or out is F32.  out may be residual (same dtype, same rows); it shares no other byte
+ * with an operand.  in_features 0 leaves act(bias) + residual.  No workspace, no atomics.  Beside mbrt_linear, for layers
+ * whose weights, and where wanted activations, are held in 4 bits. */
+MBRT_API int mbrt_mx_linear(const void* x, int dtype, int64_t x_row_stride, const void* x_scales,
+                            int64_t x_scales_row_stride, const void* weight, int64_t weight_row_stride,
+                            const void* weight_scales, int64_t weight_scales_row_stride, const void* bias,
+                            int bias_dtype, const void* residual, int residual_dtype, int64_t residual_row_stride,
+                            void* out, int out_dtype, int64_t out_row_stride, void* out_scales,
+                            int64_t out_scales_row_stride, int64_t rows, int64_t in_features, int64_t out_features,
+                            int act, mbrt_stream_t stream);
+
+/* Norms before and after a block, with the gate and the scale of its residual, over rows of `dim`:
+ *   u = update                                                             post_gamma NULL
+ *     = update * post_scale * post_gamma / sqrt(sum update^2 + eps)        else
+ *   h = residual + alpha * layer_scale * gate * u                          rounded to residual's type
+ *   normed = h * scale * gamma / sqrt(sum h^2 + eps)                       of h as it is rounded
+ * residual, update and gate F32/F16/BF16, each of its own; gammas and layer_scale [dim] of any of these, layer_scale and gate NULL for 1.
+ * The gate has gate_cols = 1 value per row or dim of them, and row r has its row (r / gate_inner) % gate_period:
+ * one per row, per batch entry, per position, or one for all; gate_is_logit puts it through a sigmoid.  sum_out takes h
+ * in residual's type (NULL: not stored; it may be residual itself); normed F32/F16/BF16 or MXFP4 with normed_scales
+ * (quantised from the f32 results), none with gamma NULL.  normed may be update itself (same dtype and rows).  Outputs share
+ * no other byte with an operand.  Row strides in elements (codes and scales: bytes).  f32 throughout, one rounding of each
+ * output.  Beside mbrt_residual_add_rms_norm, for models that norm a block's output, gate it or scale it. */
+MBRT_API int mbrt_block_norm(const void* residual, int residual_dtype, int64_t residual_row_stride, const void* update,
+                             int update_dtype, int64_t update_row_stride, const void* post_gamma, int post_gamma_dtype,
+                             const void* gate, int gate_dtype, int64_t gate_cols, int64_t gate_row_stride,
+                             int64_t gate_inner, int64_t gate_period, int gate_is_logit, const void* layer_scale,
+                             int layer_scale_dtype, const void* gamma, int gamma_dtype, void* sum_out,
+                             int64_t sum_row_stride, void* normed, int normed_dtype, int64_t normed_row_stride,
+                             void* normed_scales, int64_t normed_scales_row_stride, int64_t rows, int64_t dim,
+                             float alpha, float post_scale, float scale, float eps, mbrt_stream_t stream);
 
 /* ---- STFT / iSTFT (n_fft = win_length = 2048) --------------------------------- */
 

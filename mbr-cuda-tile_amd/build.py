@@ -65,6 +65,12 @@ KERNEL_SOURCES = [
     "k_linear.hip",
     "k_linear_bf16.hip",
     "k_linear_f16.hip",
+    "k_mx_quant.hip",
+    "k_mx_linear.hip",
+    "k_mx_linear_f32.hip",
+    "k_mx_linear_f16.hip",
+    "k_mx_linear_bf16.hip",
+    "k_block_norm.hip",
     "k_qkv_norm.hip",
     "k_window.hip",
     "k_stft.hip",
@@ -81,6 +87,7 @@ EXTRA_FLAGS = {
     "k_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-Xarch_device", "-fno-honor-nans"],
     # accumulators in ordinary VGPRs here too
     **{f"k_linear{t}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for t in ("", "_bf16", "_f16")},
+    **{f"k_mx_linear{t}.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for t in ("", "_f32", "_bf16", "_f16")},
     "k_window.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

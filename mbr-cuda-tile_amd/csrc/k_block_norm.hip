@@ -1,0 +1,450 @@
+// The norms before and after a block, with the gate and the scale of its residual, in one pass over the rows:
+//
+//   u = update                                                                  (no post_gamma)
+//     = update * post_scale * post_gamma / sqrt(sum update^2 + eps)
+//   h = residual + alpha * layer_scale * gate * u                               rounded to residual's type
+//   normed = h * scale * gamma / sqrt(sum h^2 + eps)                            of h as it is rounded
+//
+// Every byte is read once and written once: a group of G lanes (16 or 64) holds a row in registers through both norms, lane
+// l its chunks l, l + G, ... of 16 bytes (VE elements: 8 where all operands have 2 bytes, else 4, f32 ones 16 bytes and
+// 2-byte ones 8).  The two sums of squares are butterflies within the group.  All loads are issued before the first use.
+// The vectors over the features are put into LDS once per block, multiplied as far as they go together.
+// A row whose last chunk is cut has it moved back to end at the row's end: its first elements are the chunk's before, left
+// out of the sums and stored twice with the same values, so that odd widths take the same loads as even ones.
+// normed may leave as microscaled 4-bit floats (mx.hpp): the lanes of a block of 32 stand side by side.
+#include "abi_common.hpp"
+#include "mx.hpp"
+#include "overlap.hpp"
+
+#include <algorithm>
+
+namespace mbrt {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct BlockNormArgs {
+    const char* res;
+    const char* upd;
+    const char* gate;        // NULL: 1
+    const void* gamma;       // NULL: no second norm
+    const void* post_gamma;  // NULL: no first norm
+    const void* ls;          // layer scale, NULL: 1
+    char* sum;               // NULL: not stored
+    char* out;               // normed, or its codes; NULL without gamma
+    uint8_t* oscales;
+    int64_t rs, us, gs, ss, os, oss;  // row strides in bytes
+    uint32_t rows;
+    int dim, chunks, padded; // chunks of VE of a row: those with elements, and with the zeros that fill a block of 32
+    int rdt, udt, gdt, odt, gadt, pdt, ldt;
+    int gate_vec, gate_logit;
+    FastDiv inner, period;   // gate row = (row / inner) % period
+    float alpha, scale, post_scale, eps;
+};
+
+// N elements of S bytes as they stand in memory, at any alignment of the elements.
+template <int S, int N>
+struct Chunk {
+    static constexpr int kWords = S * N / 4;
+    uint32_t w[kWords];
+    template <bool AL>
+    __device__ __forceinline__ void load(const char* p) {
+        if constexpr (kWords == 4) {
+            const u32x4 t = AL ? *reinterpret_cast<const u32x4*>(p) : ld_any<0, S>(p);
+            w[0] = t[0]; w[1] = t[1]; w[2] = t[2]; w[3] = t[3];
+        } else {
+            typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
+            const u32x2 t = AL ? *reinterpret_cast<const u32x2*>(p) : (u32x2)*reinterpret_cast<const any2*>(p);
+            w[0] = t[0]; w[1] = t[1];
+        }
+    }
+    template <bool AL>
+    __device__ __forceinline__ void store(char* p) const {
+        if constexpr (kWords == 4) {
+            const u32x4 t = {w[0], w[1], w[2], w[3]};
+            if constexpr (AL) *reinterpret_cast<u32x4*>(p) = t;
+            else st_any<0, S>(p, t);
+        } else {
+            typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
+            const u32x2 t = {w[0], w[1]};
+            if constexpr (AL) *reinterpret_cast<u32x2*>(p) = t;
+            else *reinterpret_cast<any2*>(p) = t;
+        }
+    }
+    __device__ __forceinline__ void to_f32(int dt, float (&f)[N]) const {
+        if constexpr (S == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = __uint_as_float(w[i]);
+        } else if (dt == BF16) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) f[2 * i] = bf16_lo(w[i]), f[2 * i + 1] = bf16_hi(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) {
+                const f32x2 t = unpack_f16x2(w[i]);
+                f[2 * i] = t.x;
+                f[2 * i + 1] = t.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void from_f32(int dt, const float (&f)[N]) {
+        if constexpr (S == 4) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = __float_as_uint(f[i]);
+        } else if (dt == BF16) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) w[i] = pack_f16x2(f[2 * i], f[2 * i + 1]);
+        }
+    }
+};
+
+__device__ __forceinline__ float gate_value(float g, int logit) { return logit ? sigmoidf(g) : g; }
+
+// RS, US: bytes of the residual's and the update's elements; GS: of a gate with a value per feature, 0 where there is one per
+// row or none.  AL: every row of every operand begins at a multiple of its chunk's bytes and is whole chunks long.
+template <int VE, int RS, int US, int GS, int G, int NC, bool AL>
+__global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
+    extern __shared__ float lds[];
+    float* const by = lds;            // alpha * layer_scale * post_scale * post_gamma
+    float* const gam = lds + a.dim;   // scale * gamma
+    const int lane = threadIdx.x % G;
+    const uint32_t row = blockIdx.x * (kThreads / G) + threadIdx.x / G;
+    const bool valid = row < a.rows;
+    const int64_t r = valid ? row : a.rows - 1;
+    Chunk<RS, VE> rv[NC];
+    Chunk<US, VE> uv[NC];
+    Chunk<GS ? GS : 2, VE> gv[NC];
+    int at[NC];  // first element of the chunk
+    const char* gp = a.gate;
+    if (a.gate != nullptr) {
+        uint32_t q, m, d;
+        q = fdiv((uint32_t)r, a.inner);
+        fdivmod(q, a.period, d, m);
+        gp += m * a.gs;
+    }
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+        const int c = min(lane + G * k, a.chunks - 1);
+        at[k] = AL ? c * VE : min(c * VE, a.dim - VE);
+        rv[k].template load<AL>(a.res + r * a.rs + (int64_t)at[k] * RS);
+        uv[k].template load<AL>(a.upd + r * a.us + (int64_t)at[k] * US);
+        if constexpr (GS != 0) gv[k].template load<AL>(gp + (int64_t)at[k] * GS);
+    }
+    float g = 1.0f;
+    if (GS == 0 && a.gate != nullptr) g = gate_value(load1(gp, a.gdt, 0), a.gate_logit);
+    for (int d = threadIdx.x; d < a.dim; d += kThreads) {
+        float b = a.alpha;
+        if (a.ls != nullptr) b *= load1(a.ls, a.ldt, d);
+        if (a.post_gamma != nullptr) b *= load1(a.post_gamma, a.pdt, d) * a.post_scale;
+        by[d] = b;
+        if (a.gamma != nullptr) gam[d] = load1(a.gamma, a.gadt, d) * a.scale;
+    }
+    float h[NC][VE];
+    if (a.post_gamma != nullptr) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            float u[VE];
+            uv[k].to_f32(a.udt, u);
+            const int first = AL ? (lane + G * k < a.chunks ? 0 : VE) : (lane + G * k) * VE - at[k];  // elements before: another chunk's
+#pragma unroll
+            for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(u[i], u[i], ss) : ss;
+        }
+        g *= rsqrtf(group_sum<G>(ss) + a.eps);
+    }
+    __syncthreads();
+    float ss = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+        float u[VE], x[VE];
+        uv[k].to_f32(a.udt, u);
+        rv[k].to_f32(a.rdt, x);
+        if constexpr (GS != 0) {
+            float w[VE];
+            gv[k].to_f32(a.gdt, w);
+            if (a.gate_logit) {
+#pragma unroll
+                for (int i = 0; i < VE; ++i) w[i] = sigmoidf(w[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) u[i] *= w[i];
+        }
+        const int first = AL ? (lane + G * k < a.chunks ? 0 : VE) : (lane + G * k) * VE - at[k];
+#pragma unroll
+        for (int i = 0; i < VE; ++i) h[k][i] = fmaf(u[i] * g, by[at[k] + i], x[i]);
+        Chunk<RS, VE> t;
+        t.from_f32(a.rdt, h[k]);
+        t.to_f32(a.rdt, h[k]);
+        if (a.sum != nullptr && valid && lane + G * k < a.chunks) t.template store<AL>(a.sum + r * a.ss + (int64_t)at[k] * RS);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(h[k][i], h[k][i], ss) : ss;
+    }
+    if (a.gamma == nullptr) return;
+    const float inv = rsqrtf(group_sum<G>(ss) + a.eps);
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+        float o[VE];
+#pragma unroll
+        for (int i = 0; i < VE; ++i) o[i] = h[k][i] * inv * gam[at[k] + i];
+        const bool mine = valid && lane + G * k < a.chunks;
+        if (a.odt == MXFP4) {
+            const int c = lane + G * k;
+            if constexpr (!AL) {  // a cut chunk back to its place, zeros behind it
+                const int move = c * VE - at[k];
+#pragma unroll
+                for (int s = VE / 2; s > 0; s /= 2) {
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) o[i] = (move & s) != 0 ? (i + s < VE ? o[i + s] : 0.0f) : o[i];
+                }
+            }
+            uint32_t size = 0;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                if (c >= a.chunks) o[i] = 0.0f;
+                size = max(size, mx_size(o[i]));
+            }
+            const uint32_t code = mx_scale_code(mx_group_size<32 / VE>(size));
+            if (valid && c < a.padded) {
+                if constexpr (VE == 8) *reinterpret_cast<uint32_t*>(a.out + r * a.os + c * 4) = mx_pack8(o, mx_scale_operand(code));
+                else *reinterpret_cast<uint16_t*>(a.out + r * a.os + c * 2) = (uint16_t)mx_pack4(o, mx_scale_operand(code));
+                if (c % (32 / VE) == 0) a.oscales[r * a.oss + c / (32 / VE)] = (uint8_t)code;
+            }
+        } else if (mine) {
+            if (VE == 4 && a.odt == F32) {
+                Chunk<4, 4> t;
+                float f[4] = {o[0], o[1], o[2], o[3]};
+                t.from_f32(F32, f);
+                t.template store<AL>(a.out + r * a.os + (int64_t)at[k] * 4);
+            } else {
+                Chunk<2, VE> t;
+                t.from_f32(a.odt, o);
+                t.template store<AL>(a.out + r * a.os + (int64_t)at[k] * 2);
+            }
+        }
+    }
+}
+
+// Rows too long for registers and too short for a chunk: a wave per row, element by element, three passes.
+__global__ __launch_bounds__(kThreads) void block_norm_loop_kernel(BlockNormArgs a) {
+    const int lane = threadIdx.x % 64;
+    const uint32_t row = blockIdx.x * (kThreads / 64) + threadIdx.x / 64;
+    if (row >= a.rows) return;  // the whole wave
+    const int64_t r = row;
+    const char *rp = a.res + r * a.rs, *up = a.upd + r * a.us, *gp = a.gate;
+    if (gp != nullptr) {
+        uint32_t d, m;
+        fdivmod(fdiv(row, a.inner), a.period, d, m);
+        gp += m * a.gs;
+    }
+    float post = 1.0f;
+    if (a.post_gamma != nullptr) {
+        float ss = 0.0f;
+        for (int d = lane; d < a.dim; d += 64) {
+            const float u = load1(up, a.udt, d);
+            ss = fmaf(u, u, ss);
+        }
+        post = rsqrtf(group_sum<64>(ss) + a.eps);
+    }
+    auto sum_at = [&](int d) {
+        float b = a.alpha, g = post;
+        if (a.ls != nullptr) b *= load1(a.ls, a.ldt, d);
+        if (a.post_gamma != nullptr) b *= load1(a.post_gamma, a.pdt, d) * a.post_scale;
+        if (gp != nullptr) g *= gate_value(load1(gp, a.gdt, a.gate_vec ? d : 0), a.gate_logit);
+        return round_through(fmaf(load1(up, a.udt, d) * g, b, load1(rp, a.rdt, d)), a.rdt);
+    };
+    float ss = 0.0f;
+    for (int d = lane; d < a.dim; d += 64) {
+        const float h = sum_at(d);
+        if (a.sum != nullptr) store1(a.sum + r * a.ss, a.rdt, d, h);
+        ss = fmaf(h, h, ss);
+    }
+    if (a.gamma == nullptr) return;
+    const float inv = rsqrtf(group_sum<64>(ss) + a.eps);
+    for (int d0 = 0; d0 < a.dim; d0 += 64) {
+        const int d = d0 + lane;
+        float o = 0.0f;
+        if (d < a.dim)  // the stored sum again: it may lie in the residual's place
+            o = (a.sum != nullptr ? load1(a.sum + r * a.ss, a.rdt, d) : sum_at(d)) * inv * (load1(a.gamma, a.gadt, d) * a.scale);
+        if (a.odt != MXFP4) {
+            if (d < a.dim) store1(a.out + r * a.os, a.odt, d, o);
+            continue;
+        }
+        uint32_t size = mx_size(o);
+#pragma unroll
+        for (int s = 1; s < 32; s *= 2) size = max(size, (uint32_t)__shfl_xor((int)size, s));
+        const uint32_t code = mx_scale_code(size);
+        const float next = __shfl_xor(o, 1);
+        if (d < 32 * ((a.dim + 31) / 32) && d % 2 == 0) {
+            const uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, o, next, mx_scale_operand(code), 0);
+            reinterpret_cast<uint8_t*>(a.out + r * a.os)[d / 2] = (uint8_t)w;
+            if (d % 32 == 0) a.oscales[r * a.oss + d / 32] = (uint8_t)code;
+        }
+    }
+}
+
+template <int VE, int RS, int US, int GS, bool AL>
+bool launch_shape(const BlockNormArgs& a, hipStream_t st) {
+    auto go = [&](auto g, auto nc) {
+        constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
+        hipLaunchKernelGGL((block_norm_kernel<VE, RS, US, GS, G, NC, AL>), dim3((unsigned)ceil_div(a.rows, kThreads / G)),
+                           dim3(kThreads), 2 * a.dim * sizeof(float), st, a);
+    };
+    typedef std::integral_constant<int, 16> G16;
+    typedef std::integral_constant<int, 64> G64;
+    const int n = a.odt == MXFP4 ? a.padded : a.chunks;
+    if (n <= 32) go(G16(), std::integral_constant<int, 2>());
+    else if (n <= 64) go(G16(), std::integral_constant<int, 4>());
+    else if (n <= 96) go(G16(), std::integral_constant<int, 6>());
+    else if (n <= 128) go(G64(), std::integral_constant<int, 2>());
+    else if (n <= 256) go(G64(), std::integral_constant<int, 4>());
+    else if (n <= 512) go(G64(), std::integral_constant<int, 8>());
+    else if (n <= 1024) go(G64(), std::integral_constant<int, 16>());
+    else return false;
+    return true;
+}
+
+template <int VE, bool AL>
+bool launch_sizes(const BlockNormArgs& a, int gate_bytes, hipStream_t st) {
+    if constexpr (VE == 8) {
+        return gate_bytes == 0 ? launch_shape<8, 2, 2, 0, AL>(a, st) : launch_shape<8, 2, 2, 2, AL>(a, st);
+    } else {
+        auto with_gate = [&](auto rs, auto us) {
+            constexpr int R = decltype(rs)::value, U = decltype(us)::value;
+            return gate_bytes == 0   ? launch_shape<4, R, U, 0, AL>(a, st)
+                   : gate_bytes == 2 ? launch_shape<4, R, U, 2, AL>(a, st)
+                                     : launch_shape<4, R, U, 4, AL>(a, st);
+        };
+        typedef std::integral_constant<int, 2> B2;
+        typedef std::integral_constant<int, 4> B4;
+        if (a.rdt == F32) return a.udt == F32 ? with_gate(B4(), B4()) : with_gate(B4(), B2());
+        return a.udt == F32 ? with_gate(B2(), B4()) : with_gate(B2(), B2());
+    }
+}
+
+int launch_block_norm(BlockNormArgs& a, hipStream_t st, const char* op) {
+    const bool wide = a.rdt == F32 || a.udt == F32 || (a.gate_vec && a.gdt == F32) || a.odt == F32;
+    const int ve = wide ? 4 : 8, gate_bytes = a.gate_vec ? dt_size(a.gdt) : 0;
+    a.chunks = (int)ceil_div(a.dim, ve);
+    a.padded = (int)ceil_div(a.dim, 32) * (32 / ve);
+    bool done = false;
+    if (a.dim >= ve && a.dim <= 8192) {
+        auto even = [&](const void* p, int64_t stride, int dt) {
+            const int64_t b = (int64_t)ve * dt_size(dt);
+            return p == nullptr || (aligned(p, b) && stride % b == 0);
+        };
+        const bool al = a.dim % ve == 0 && even(a.res, a.rs, a.rdt) && even(a.upd, a.us, a.udt) && even(a.sum, a.ss, a.rdt) &&
+                        (a.odt == MXFP4 || even(a.out, a.os, a.odt)) && (!a.gate_vec || even(a.gate, a.gs, a.gdt));
+        if (wide) done = al ? launch_sizes<4, true>(a, gate_bytes, st) : launch_sizes<4, false>(a, gate_bytes, st);
+        else done = al ? launch_sizes<8, true>(a, gate_bytes, st) : launch_sizes<8, false>(a, gate_bytes, st);
+    }
+    if (!done)
+        hipLaunchKernelGGL(block_norm_loop_kernel, dim3((unsigned)ceil_div(a.rows, kThreads / 64)), dim3(kThreads), 0, st, a);
+    return check_launch(op);
+}
+
+}  // namespace
+}  // namespace mbrt
+
+using namespace mbrt;
+
+extern "C" int mbrt_block_norm(const void* residual, int residual_dtype, int64_t residual_row_stride, const void* update,
+                               int update_dtype, int64_t update_row_stride, const void* post_gamma, int post_gamma_dtype,
+                               const void* gate, int gate_dtype, int64_t gate_cols, int64_t gate_row_stride,
+                               int64_t gate_inner, int64_t gate_period, int gate_is_logit, const void* layer_scale,
+                               int layer_scale_dtype, const void* gamma, int gamma_dtype, void* sum_out,
+                               int64_t sum_row_stride, void* normed, int normed_dtype, int64_t normed_row_stride,
+                               void* normed_scales, int64_t normed_scales_row_stride, int64_t rows, int64_t dim, float alpha,
+                               float post_scale, float scale, float eps, mbrt_stream_t stream) {
+    const char* op = "mbrt_block_norm";
+    MBRT_REQUIRE_FLOAT_DT(residual_dtype, op);
+    MBRT_REQUIRE_FLOAT_DT(update_dtype, op);
+    const bool mx = gamma != nullptr && normed_dtype == MXFP4;
+    if (gamma && !mx) MBRT_REQUIRE_FLOAT_DT(normed_dtype, op);
+    MBRT_REQUIRE((!post_gamma || is_float_dt(post_gamma_dtype)) && (!gate || is_float_dt(gate_dtype)) &&
+                     (!layer_scale || is_float_dt(layer_scale_dtype)) && (!gamma || is_float_dt(gamma_dtype)),
+                 MBRT_E_UNSUPPORTED_DTYPE, "%s: a gamma's, the gate's or the layer scale's dtype (expected F32/F16/BF16)", op);
+    MBRT_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) && dim >= 1 && dim < (int64_t(1) << 28), MBRT_E_SHAPE,
+                 "%s: bad shape rows=%lld dim=%lld (fewer than 2^31 rows, 1 to 2^28 - 1 features)", op, (long long)rows,
+                 (long long)dim);
+    MBRT_REQUIRE(!gate || ((gate_cols == 1 || gate_cols == dim) && gate_inner >= 1 && gate_period >= 1 && gate_row_stride >= 0),
+                 MBRT_E_SHAPE, "%s: gate of %lld columns, inner %lld, period %lld", op, (long long)gate_cols,
+                 (long long)gate_inner, (long long)gate_period);
+    if (rows == 0) return MBRT_OK;
+    const int64_t blocks = ceil_div(dim, kMxBlock);
+    const int64_t rb = dt_size(residual_dtype), ub = dt_size(update_dtype), ob = mx ? 1 : gamma ? dt_size(normed_dtype) : 1;
+    const int64_t ocols = mx ? 16 * blocks : dim;
+    if (rows == 1) {  // of a single row: not used
+        residual_row_stride = update_row_stride = sum_row_stride = dim;
+        normed_row_stride = ocols;
+        normed_scales_row_stride = blocks;
+    }
+    MBRT_REQUIRE(residual_row_stride >= 0 && update_row_stride >= 0 && (!sum_out || sum_row_stride >= dim) &&
+                     (!gamma || normed_row_stride >= ocols) && (!mx || normed_scales_row_stride >= blocks),
+                 MBRT_E_SHAPE, "%s: negative row stride, or output rows that overlap", op);
+    MBRT_REQUIRE(residual && update && (gamma ? normed != nullptr : sum_out != nullptr) && (!mx || normed_scales),
+                 MBRT_E_INVALID_ARG, "%s: NULL pointer", op);
+    MBRT_REQUIRE(aligned(residual, rb) && aligned(update, ub) && (!sum_out || aligned(sum_out, rb)) &&
+                     (!gamma || (mx ? aligned(normed, 16) && normed_row_stride % 16 == 0 : aligned(normed, ob))) &&
+                     (!gate || aligned(gate, dt_size(gate_dtype))) && (!gamma || aligned(gamma, dt_size(gamma_dtype))) &&
+                     (!post_gamma || aligned(post_gamma, dt_size(post_gamma_dtype))) &&
+                     (!layer_scale || aligned(layer_scale, dt_size(layer_scale_dtype))),
+                 MBRT_E_ALIGN, "%s: pointer not aligned to its elements, or rows of codes not to 16 bytes", op);
+    const int64_t gate_rows = gate ? std::min(gate_period, ceil_div(rows, gate_inner)) : 0;
+    if (gate_rows == 1) gate_row_stride = 0;
+    const MemRows R{residual, residual_row_stride * rb, dim * rb, rows}, U{update, update_row_stride * ub, dim * ub, rows};
+    const MemRows S{sum_out, sum_row_stride * rb, dim * rb, sum_out ? rows : 0};
+    const MemRows O{normed, normed_row_stride * ob, ocols * ob, gamma ? rows : 0};
+    const MemRows C{normed_scales, normed_scales_row_stride, blocks, mx ? rows : 0};
+    const MemRows Ga{gate, gate_row_stride * (gate ? dt_size(gate_dtype) : 0), gate_cols * (gate ? dt_size(gate_dtype) : 0), gate_rows};
+    const MemRows V[3] = {{gamma, 0, gamma ? dim * dt_size(gamma_dtype) : 0, 1},
+                          {post_gamma, 0, post_gamma ? dim * dt_size(post_gamma_dtype) : 0, 1},
+                          {layer_scale, 0, layer_scale ? dim * dt_size(layer_scale_dtype) : 0, 1}};
+    const bool sum_in_place = sum_out == residual && (rows == 1 || sum_row_stride == residual_row_stride);
+    const bool out_in_place = gamma && !mx && normed == update && normed_dtype == update_dtype &&
+                              (rows == 1 || normed_row_stride == update_row_stride);
+    bool clash = (!sum_in_place && rows_meet(S, R)) || rows_meet(S, U) || rows_meet(S, Ga) || rows_meet(S, O) || rows_meet(S, C) ||
+                 rows_meet(O, R) || (!out_in_place && rows_meet(O, U)) || rows_meet(O, Ga) || rows_meet(O, C) || rows_meet(C, R) ||
+                 rows_meet(C, U) || rows_meet(C, Ga);
+    for (const MemRows& v : V) clash = clash || rows_meet(v, S) || rows_meet(v, O) || rows_meet(v, C);
+    MBRT_REQUIRE(!clash, MBRT_E_INVALID_ARG,
+                 "%s: an output overlaps another operand (sum_out may be the residual, normed the update, in the same dtype and rows)",
+                 op);
+    BlockNormArgs a{};
+    a.res = static_cast<const char*>(residual);
+    a.upd = static_cast<const char*>(update);
+    a.gate = static_cast<const char*>(gate);
+    a.gamma = gamma;
+    a.post_gamma = post_gamma;
+    a.ls = layer_scale;
+    a.sum = static_cast<char*>(sum_out);
+    a.out = static_cast<char*>(normed);
+    a.oscales = static_cast<uint8_t*>(normed_scales);
+    a.rs = residual_row_stride * rb;
+    a.us = update_row_stride * ub;
+    a.gs = gate ? gate_row_stride * dt_size(gate_dtype) : 0;
+    a.ss = sum_row_stride * rb;
+    a.os = normed_row_stride * ob;
+    a.oss = normed_scales_row_stride;
+    a.rows = (uint32_t)rows;
+    a.dim = (int)dim;
+    a.rdt = residual_dtype;
+    a.udt = update_dtype;
+    a.gdt = gate_dtype;
+    a.odt = gamma ? normed_dtype : residual_dtype;
+    a.gadt = gamma_dtype;
+    a.pdt = post_gamma_dtype;
+    a.ldt = layer_scale_dtype;
+    a.gate_vec = gate && gate_cols > 1;
+    a.gate_logit = gate_is_logit != 0;
+    // rows / inner and the rows of a period stay below 2^31
+    a.inner = make_fastdiv((uint32_t)std::min<int64_t>(gate ? gate_inner : 1, rows));
+    a.period = make_fastdiv((uint32_t)std::min<int64_t>(gate ? gate_period : 1, rows));
+    a.alpha = alpha;
+    a.post_scale = post_scale;
+    a.scale = scale;
+    a.eps = eps;
+    return launch_block_norm(a, as_stream(stream), op);
+}

@@ -10,14 +10,14 @@ from __future__ import annotations
 
 import ctypes as C
 import warnings
-from typing import Sequence
+from typing import NamedTuple, Sequence
 
 import torch
 
 from . import _abi
 from ._abi import (  # noqa: F401
     ACT_GELU_REF, ACT_GELU_STD, ACT_NONE, ACT_SIGMOID, ACT_TANH, ADD, ARITH_BF16_INTERMEDIATES, BF16, DIV, F16, F32,
-    I32, I64,
+    I32, I64, MXFP4,
     LAYOUT_BHND, LAYOUT_BNHD, MUL, REDUCE_MAX, REDUCE_SUM, SCALAR_ADD, SCALAR_CLAMP, SCALAR_MUL, SUB,
     UNARY_GT, UNARY_NEG, MbrtError, lib, LIB_PATH,
 )
@@ -451,6 +451,120 @@ def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: tor
     _n.attention_window(q, k, v, out, -1 if left is None else left, -1 if right is None else right, sinks,
                         -1 if q_start is None else q_start, key_lens, gate, gate_is_logit, scale, workspace, _h(stream))
     return out
+
+
+# ---- transformer layer in 4 bits ------------------------------------------------------------
+
+class MxTensor(NamedTuple):
+    """Rows of microscaled 4-bit floats (MXFP4): codes [.., 16 ceil(n / 32)] and scales [.., ceil(n / 32)], both uint8, of n
+    features.  Rows of codes at multiples of 16 bytes."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    features: int
+
+    @property
+    def shape(self) -> torch.Size:
+        """Of what is held: [.., features]."""
+        return torch.Size((*self.codes.shape[:-1], self.features))
+
+
+def mx_empty(shape, device="cuda", stream=None) -> MxTensor:
+    """Memory for rows [.., n] in 4 bits."""
+    *lead, n = shape
+    blocks = -(-n // 32)
+    # codes first, so that their rows are aligned, in one allocation with the scales
+    rows = 1
+    for s in lead:
+        rows *= s
+    mem = _new(17 * rows * blocks, torch.uint8, device, stream)
+    return MxTensor(mem[:16 * rows * blocks].view(*lead, 16 * blocks), mem[16 * rows * blocks:].view(*lead, blocks), n)
+
+
+def mx_quantize(x: torch.Tensor, out: MxTensor | None = None, stream=None) -> MxTensor:
+    """Rows of x [.., n] f32, f16 or bf16 into 4 bits: a scale 2^s for each 32 features of a row, the largest of them in [4, 8)
+    of it, and each rounded to 0, .5, 1, 1.5, 2, 3, 4 or 6 of it, ties to even, the top to 6.  Blocks with an infinity or a NaN become
+    NaN.  x's rows at any stride and alignment, the last dim contiguous."""
+    if out is None:
+        out = mx_empty(x.shape, x.device, stream)
+    _n.mx_quantize(x, *out, _h(stream))
+    return out
+
+
+def mx_dequantize(x: MxTensor, out: torch.Tensor | None = None, out_dtype=None, stream=None) -> torch.Tensor:
+    """What x holds, as f32, f16 or bf16 (by default, and exact in the first and the last)."""
+    if out is None:
+        out = _new(x.shape, out_dtype or torch.bfloat16, x.codes.device, stream)
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("mx_dequantize: out and out_dtype disagree")
+    _n.mx_dequantize(*x, out, _h(stream))
+    return out
+
+
+def mx_linear(x, weight: MxTensor, bias: torch.Tensor | None = None, out=None, act: int = ACT_NONE,
+              residual: torch.Tensor | None = None, out_dtype=None, stream=None):
+    """act(x weight^T + bias) + residual for weight [N, K] in 4 bits and x [.., K] in 4 bits (MxTensor) or f32, f16 or bf16,
+    rounded once.  bias [N], residual and out [.., N], each f32, f16 or bf16; out may be an MxTensor, too, or residual itself.
+    out_dtype defaults to x's, bf16 for x in 4 bits; MxTensor gives results in 4 bits.  Rows at any stride (codes:
+    multiples of 16 bytes), the last dim contiguous."""
+    held = isinstance(x, MxTensor)
+    if not isinstance(weight, MxTensor) or not (held or isinstance(x, torch.Tensor)):
+        raise TypeError("mx_linear: expected weight an MxTensor, x a torch.Tensor or an MxTensor")
+    if len(weight.codes.shape) != 2 or not x.shape or x.shape[-1] != weight.features:
+        raise ValueError("mx_linear: expected x [.., K] and weight [N, K]")
+    if out is None:
+        shape = (*x.shape[:-1], weight.codes.shape[0])
+        dev = weight.codes.device
+        if out_dtype is MxTensor:
+            out = mx_empty(shape, dev, stream)
+        else:
+            out = _new(shape, out_dtype or (torch.bfloat16 if held else x.dtype), dev, stream)
+    elif out_dtype is not None and (out_dtype is MxTensor) != isinstance(out, MxTensor) or \
+            isinstance(out, torch.Tensor) and out_dtype not in (None, out.dtype):
+        raise ValueError("mx_linear: out and out_dtype disagree")
+    if isinstance(out, MxTensor) and out.features != weight.codes.shape[0]:
+        raise ValueError("mx_linear: expected out and residual [.., N]")
+    xc, xs = (x.codes, x.scales) if held else (x, None)
+    oc, os = (out.codes, out.scales) if isinstance(out, MxTensor) else (out, None)
+    _n.mx_linear(xc, xs, weight.codes, weight.scales, weight.features, bias, oc, os, act, residual, _h(stream))
+    return out
+
+
+def block_norm(residual: torch.Tensor, update: torch.Tensor, gamma: torch.Tensor | None = None,
+               post_gamma: torch.Tensor | None = None, gate: torch.Tensor | None = None, gate_is_logit: bool = False,
+               layer_scale: torch.Tensor | None = None, alpha: float = 1.0, sum_out: torch.Tensor | None = None, normed=None,
+               scale: float | None = None, post_scale: float | None = None, eps: float = 1e-12, store_sum: bool = True,
+               out_dtype=None, stream=None):
+    """(h, normed) around a block with output `update`, rows [.., D]:
+        u = update * post_scale * post_gamma / sqrt(sum update^2 + eps)   (update itself without post_gamma)
+        h = residual + alpha * layer_scale * gate * u                     in residual's dtype
+        normed = h * scale * gamma / sqrt(sum h^2 + eps)                  (None without gamma)
+    scale and post_scale are sqrt(D) by default.  gate [.., D] or [.., 1], with dims of 1 in front where rows share it (on one
+    side of the dims that do not), itself or a sigmoid's argument; layer_scale and gammas [D].  residual, update and gate f32, f16 or bf16 each,
+    rows at any stride.  sum_out may be residual itself; store_sum=False leaves h out.  normed: a tensor (it may be update
+    itself) or an MxTensor; out_dtype (update's dtype by default) may be MxTensor, too."""
+    if not isinstance(residual, torch.Tensor) or not isinstance(update, torch.Tensor):
+        raise TypeError("mbrt: expected a torch.Tensor")
+    if gamma is None and (normed is not None or out_dtype is not None or not store_sum):
+        raise ValueError("block_norm: without gamma there is only the sum")
+    if sum_out is not None and not store_sum:
+        raise ValueError("block_norm: sum_out and store_sum disagree")
+    if store_sum and sum_out is None:
+        sum_out = _new(residual.shape, residual.dtype, residual.device, stream)
+    if gamma is not None:
+        if normed is None and out_dtype is MxTensor:
+            normed = mx_empty(residual.shape, residual.device, stream)
+        elif normed is None:
+            normed = _new(residual.shape, out_dtype or update.dtype, residual.device, stream)
+        elif out_dtype is not None and (out_dtype is MxTensor) != isinstance(normed, MxTensor) or \
+                isinstance(normed, torch.Tensor) and out_dtype not in (None, normed.dtype):
+            raise ValueError("block_norm: normed and out_dtype disagree")
+        if isinstance(normed, MxTensor) and normed.features != residual.shape[-1]:
+            raise ValueError("block_norm: expected update, sum_out and normed [.., D]")
+    root = max(residual.shape[-1] if residual.dim() else 1, 1) ** 0.5
+    nc, ns = (normed.codes, normed.scales) if isinstance(normed, MxTensor) else (normed, None)
+    _n.block_norm(residual, update, post_gamma, gate, gate_is_logit, layer_scale, gamma, sum_out, nc, ns, alpha,
+                  root if post_scale is None else post_scale, root if scale is None else scale, eps, _h(stream))
+    return sum_out, normed
 
 
 N_FFT = 2048

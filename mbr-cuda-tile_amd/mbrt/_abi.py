@@ -17,6 +17,8 @@ MAX_DIMS = 8
 
 # dtype codes (src/tensor.h:17 values, plus I32)
 F32, F16, I64, BF16, I32 = 0, 1, 2, 3, 4
+# microscaled 4-bit floats, where a call names them
+MXFP4 = 5
 # binary ops
 ADD, SUB, MUL, DIV = 0, 1, 2, 3
 SCALAR_ADD, SCALAR_MUL, SCALAR_CLAMP = 0, 1, 2
@@ -108,6 +110,10 @@ SIGNATURES: dict[str, list] = {
     "mbrt_split_qkv_norm_rotary": [P, I, L, L, P, P, I, P, P, I, L, L, P, P, P, I, *[L] * 6, *[L] * 5, Fl, Fl, P],
     "mbrt_attention_window_workspace_bytes": [L] * 9,
     "mbrt_attention_window": [P, P, P, I, *[L] * 6, *[L] * 6, *[L] * 4, P, P, I, I, P, I, L, L, L, Fl, P, L, P],
+    "mbrt_mx_quantize": [P, I, L, P, L, P, L, L, L, P],
+    "mbrt_mx_dequantize": [P, L, P, L, P, I, L, L, L, P],
+    "mbrt_mx_linear": [P, I, L, P, L, P, L, P, L, P, I, P, I, L, P, I, L, P, L, L, L, L, I, P],
+    "mbrt_block_norm": [P, I, L, P, I, L, P, I, P, I, L, L, L, L, I, P, I, P, I, P, L, P, I, L, P, L, L, L, Fl, Fl, Fl, Fl, P],
     "mbrt_hann_window": [P, L, P],
     "mbrt_stft_num_frames": [L, L, I],
     "mbrt_stft": [P, P, P, L, L, L, L, L, L, I, I, P],

@@ -193,14 +193,14 @@ def _alike(a, b):
     return not a.numel() or all(x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n > 1)
 
 
-def _row_stride(t):
+def _row_stride(t, op="linear"):
     """The one stride between the rows of [.., n] (0 where there is one row)."""
     span, stride = 1, 0
     for d in range(t.dim() - 2, -1, -1):
         if t.shape[d] == 1:
             continue
         if t.numel() and span > 1 and t.stride(d) != span * stride:
-            raise ValueError("linear: the rows of a tensor lie at more than one stride")
+            raise ValueError(f"{op}: the rows of a tensor lie at more than one stride")
         if span == 1:
             stride = t.stride(d)
         span *= t.shape[d]
@@ -285,6 +285,129 @@ def attention_window(q, k, v, out, left, right, sinks, q_start, key_lens, gate, 
             0 if workspace is None else workspace.numel() * workspace.element_size())
     with _gpu(q, k, v, out, key_lens, gate, workspace):
         _abi.call("mbrt_attention_window", *args, _s(stream))
+
+
+def _mx(op, codes, scales, lead, features):
+    """Row strides of codes and scales that hold [*lead, features] in 4 bits."""
+    blocks = -(-features // 32)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError("mbrt: expected codes and scales of dtype torch.uint8")
+    if codes.shape != (*lead, 16 * blocks) or scales.shape != (*lead, blocks):
+        raise ValueError(f"{op}: expected codes [.., 16 ceil(n / 32)] and scales [.., ceil(n / 32)]")
+    _unit_last(codes, scales)
+    return _row_stride(codes, op), _row_stride(scales, op)
+
+
+def _rows(lead):
+    n = 1
+    for s in lead:
+        n *= s
+    return n
+
+
+def mx_quantize(x, codes, scales, features, stream):
+    _tensors(x, codes, scales)
+    if x.dim() < 1 or x.shape[-1] != features:
+        raise ValueError("mx_quantize: expected x [.., n]")
+    cs, ss = _mx("mx_quantize", codes, scales, x.shape[:-1], features)
+    _unit_last(x)
+    args = (_p(x), _dt(x), _row_stride(x, "mx_quantize"), _p(codes), cs, _p(scales), ss, _rows(x.shape[:-1]), features)
+    with _gpu(x, codes, scales):
+        _abi.call("mbrt_mx_quantize", *args, _s(stream))
+
+
+def mx_dequantize(codes, scales, features, out, stream):
+    _tensors(codes, scales, out)
+    if out.dim() < 1 or out.shape[-1] != features:
+        raise ValueError("mx_dequantize: expected out [.., n]")
+    cs, ss = _mx("mx_dequantize", codes, scales, out.shape[:-1], features)
+    _unit_last(out)
+    args = (_p(codes), cs, _p(scales), ss, _p(out), _dt(out), _row_stride(out, "mx_dequantize"), _rows(out.shape[:-1]), features)
+    with _gpu(codes, scales, out):
+        _abi.call("mbrt_mx_dequantize", *args, _s(stream))
+
+
+def mx_linear(x, x_scales, w, w_scales, K, bias, out, out_scales, act, residual, stream):
+    _tensors(x, w, w_scales, out, *(t for t in (x_scales, bias, out_scales, residual) if t is not None))
+    op = "mx_linear"
+    if x.dim() < 1 or w.dim() != 2 or x_scales is None and x.shape[-1] != K:
+        raise ValueError("mx_linear: expected x [.., K] and weight [N, K]")
+    N, lead = w.shape[0], x.shape[:-1]
+    ws, wss = _mx(op, w, w_scales, (N,), K)
+    xs, xss = (_row_stride(x, op), 0) if x_scales is None else _mx(op, x, x_scales, lead, K)
+    if out_scales is None and out.shape != (*lead, N) or residual is not None and residual.shape != (*lead, N):
+        raise ValueError("mx_linear: expected out and residual [.., N]")
+    os, oss = (_row_stride(out, op), 0) if out_scales is None else _mx(op, out, out_scales, lead, N)
+    if bias is not None and bias.shape != (N,):
+        raise ValueError("mx_linear: expected bias [N]")
+    _unit_last(x, out, residual, bias)
+    xdt = _dt(x) if x_scales is None else _abi.MXFP4
+    odt = _dt(out) if out_scales is None else _abi.MXFP4
+    args = (_p(x), xdt, xs, _p(x_scales), xss, _p(w), ws, _p(w_scales), wss, _p(bias), _dt(bias, _abi.F32), _p(residual),
+            _dt(residual, _abi.F32), 0 if residual is None else _row_stride(residual, op), _p(out), odt, os, _p(out_scales), oss,
+            _rows(lead), K, N, act)
+    with _gpu(x, x_scales, w, w_scales, bias, residual, out, out_scales):
+        _abi.call("mbrt_mx_linear", *args, _s(stream))
+
+
+def _gate_rows(gate, like):
+    """(columns, row stride, inner, period): row r of `like` [.., D] has the gate's row (r / inner) % period."""
+    if gate is None:
+        return 1, 0, 1, 1
+    D = like.shape[-1]
+    if not 1 <= gate.dim() <= like.dim() or gate.shape[-1] not in (1, D):
+        raise ValueError("block_norm: expected gate [.., D] or [.., 1]")
+    stride, inner, period, closed = 0, 1, 1, False
+    for d in range(2, like.dim() + 1):
+        n, m = like.shape[-d], gate.shape[-d] if d <= gate.dim() else 1
+        if m not in (1, n):
+            raise ValueError("block_norm: expected gate [.., D] or [.., 1]")
+        if n == 1:
+            continue
+        if m == 1:
+            if period == 1:
+                inner *= n
+            else:
+                closed = True
+            continue
+        if closed:
+            raise ValueError("block_norm: the gate's rows are shared on both sides of a dim that they do not share")
+        if period > 1 and like.numel() and gate.stride(-d) != period * stride:
+            raise ValueError("block_norm: the rows of a tensor lie at more than one stride")
+        if period == 1:
+            stride = gate.stride(-d)
+        period *= n
+    return gate.shape[-1], stride, max(inner, 1), max(period, 1)
+
+
+def block_norm(residual, update, post_gamma, gate, gate_is_logit, layer_scale, gamma, sum_out, normed, normed_scales, alpha,
+               post_scale, scale, eps, stream):
+    _tensors(residual, update, *(t for t in (post_gamma, gate, layer_scale, gamma, sum_out, normed, normed_scales) if t is not None))
+    op = "block_norm"
+    if residual.dim() < 1 or residual.shape[-1] < 1 or update.shape != residual.shape or \
+            sum_out is not None and sum_out.shape != residual.shape or \
+            normed is not None and normed_scales is None and normed.shape != residual.shape:
+        raise ValueError("block_norm: expected update, sum_out and normed [.., D]")
+    lead, D = residual.shape[:-1], residual.shape[-1]
+    if sum_out is not None and sum_out.dtype != residual.dtype:
+        raise ValueError("block_norm: sum_out and residual differ in dtype")
+    for t in (post_gamma, layer_scale, gamma):
+        if t is not None and t.shape != (D,):
+            raise ValueError("block_norm: expected gammas and layer_scale [D]")
+    _contig(post_gamma, layer_scale, gamma)
+    _unit_last(residual, update, sum_out, normed, gate)
+    os, oss = (0, 0) if normed is None else (_row_stride(normed, op), 0) if normed_scales is None else \
+        _mx(op, normed, normed_scales, lead, D)
+    odt = _abi.MXFP4 if normed_scales is not None else _dt(normed, _abi.F32)
+    cols, gs, inner, period = _gate_rows(gate, residual)
+    f = _abi.F32
+    args = (_p(residual), _dt(residual), _row_stride(residual, op), _p(update), _dt(update), _row_stride(update, op),
+            _p(post_gamma), _dt(post_gamma, f), _p(gate), _dt(gate, f), cols, gs, inner, period, int(bool(gate_is_logit)),
+            _p(layer_scale), _dt(layer_scale, f), _p(gamma), _dt(gamma, f), _p(sum_out),
+            0 if sum_out is None else _row_stride(sum_out, op), _p(normed), odt, os, _p(normed_scales), oss, _rows(lead), D,
+            _float(alpha), _float(post_scale), _float(scale), _float(eps))
+    with _gpu(residual, update, post_gamma, gate, layer_scale, gamma, sum_out, normed, normed_scales):
+        _abi.call("mbrt_block_norm", *args, _s(stream))
 
 
 def stft(x, window, hop, center, normalized, out, n_fft, win_length, stream):

@@ -387,13 +387,17 @@ bool strided_alike(const at::Tensor& a, const at::Tensor& b) {
     return true;
 }
 
+[[noreturn]] void raise_for(const char* op, const char* msg) {
+    raise(PyExc_ValueError, (std::string(op) + ": " + msg).c_str());
+}
+
 // The one stride between the rows of [.., n] (0 where there is one row).
-int64_t row_stride(const at::Tensor& t) {
+int64_t row_stride(const at::Tensor& t, const char* op = "linear") {
     int64_t span = 1, stride = 0;
     for (int64_t d = t.dim() - 2; d >= 0; --d) {
         if (t.size(d) == 1) continue;
         if (t.numel() && span > 1 && t.stride(d) != span * stride)
-            raise(PyExc_ValueError, "linear: the rows of a tensor lie at more than one stride");
+            raise_for(op, "the rows of a tensor lie at more than one stride");
         if (span == 1) stride = t.stride(d);
         span *= t.size(d);
     }
@@ -511,6 +515,172 @@ MBRT_PY(attention_window) {
     END_HANDLE_TH_ERRORS
 }
 
+// Whether t is [*lead of x, n].
+bool rows_like(const at::Tensor& t, const at::Tensor& x, int64_t n) {
+    if (t.dim() != x.dim() || t.size(-1) != n) return false;
+    for (int64_t d = 0; d < x.dim() - 1; ++d)
+        if (t.size(d) != x.size(d)) return false;
+    return true;
+}
+int64_t rows_of(const at::Tensor& x) {
+    int64_t rows = 1;
+    for (int64_t d = 0; d < x.dim() - 1; ++d) rows *= x.size(d);
+    return rows;
+}
+
+// Row strides of codes and scales that hold rows of n features in 4 bits, as many and shaped as x's.
+struct Mx {
+    int64_t codes, scales;
+};
+Mx mx_rows(const char* op, const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& x, int64_t n) {
+    if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte)
+        raise(PyExc_TypeError, "mbrt: expected codes and scales of dtype torch.uint8");
+    const int64_t blocks = (n + 31) / 32;
+    if (!rows_like(codes, x, 16 * blocks) || !rows_like(scales, x, blocks))
+        raise_for(op, "expected codes [.., 16 ceil(n / 32)] and scales [.., ceil(n / 32)]");
+    unit_last({&codes, &scales});
+    return Mx{row_stride(codes, op), row_stride(scales, op)};
+}
+
+// mx_quantize(x, codes, scales, features, stream)
+MBRT_PY(mx_quantize) {
+    HANDLE_TH_ERRORS
+    count(n, 5);
+    const at::Tensor &x = tensor(a[0]), &c = tensor(a[1]), &s = tensor(a[2]);
+    const int64_t features = integer(a[3]);
+    if (x.dim() < 1 || x.size(-1) != features) raise(PyExc_ValueError, "mx_quantize: expected x [.., n]");
+    const Mx m = mx_rows("mx_quantize", c, s, x, features);
+    unit_last({&x});
+    const int dt = dtype_code(x);
+    const int64_t xs = row_stride(x, "mx_quantize"), rows = rows_of(x);
+    void *xp = ptr(x), *cp = ptr(c), *sp = ptr(s);
+    const OnDevice on({&x, &c, &s});
+    const mbrt_stream_t st = on.stream(a[4]);
+    return call("mbrt_mx_quantize", [&] { return mbrt_mx_quantize(xp, dt, xs, cp, m.codes, sp, m.scales, rows, features, st); });
+    END_HANDLE_TH_ERRORS
+}
+
+// mx_dequantize(codes, scales, features, out, stream)
+MBRT_PY(mx_dequantize) {
+    HANDLE_TH_ERRORS
+    count(n, 5);
+    const at::Tensor &c = tensor(a[0]), &s = tensor(a[1]), &out = tensor(a[3]);
+    const int64_t features = integer(a[2]);
+    if (out.dim() < 1 || out.size(-1) != features) raise(PyExc_ValueError, "mx_dequantize: expected out [.., n]");
+    const Mx m = mx_rows("mx_dequantize", c, s, out, features);
+    unit_last({&out});
+    const int dt = dtype_code(out);
+    const int64_t os = row_stride(out, "mx_dequantize"), rows = rows_of(out);
+    void *cp = ptr(c), *sp = ptr(s), *op = ptr(out);
+    const OnDevice on({&c, &s, &out});
+    const mbrt_stream_t st = on.stream(a[4]);
+    return call("mbrt_mx_dequantize",
+                [&] { return mbrt_mx_dequantize(cp, m.codes, sp, m.scales, op, dt, os, rows, features, st); });
+    END_HANDLE_TH_ERRORS
+}
+
+// mx_linear(x, x_scales | None, weight codes, weight scales, K, bias | None, out, out_scales | None, act, residual | None,
+//           stream), with scales where x or out is in 4 bits
+MBRT_PY(mx_linear) {
+    HANDLE_TH_ERRORS
+    count(n, 11);
+    const char* name = "mx_linear";
+    const at::Tensor &x = tensor(a[0]), &w = tensor(a[2]), &wsc = tensor(a[3]), &out = tensor(a[6]);
+    const at::Tensor xsc = tensor_or_none(a[1]), b = tensor_or_none(a[5]), osc = tensor_or_none(a[7]), res = tensor_or_none(a[9]);
+    const int64_t K = integer(a[4]);
+    if (x.dim() < 1 || w.dim() != 2 || (!xsc.defined() && x.size(-1) != K))
+        raise(PyExc_ValueError, "mx_linear: expected x [.., K] and weight [N, K]");
+    const int64_t N = w.size(0), rows = rows_of(x);
+    const Mx wm = mx_rows(name, w, wsc, w, K);
+    const Mx xm = xsc.defined() ? mx_rows(name, x, xsc, x, K) : Mx{row_stride(x, name), 0};
+    if ((!osc.defined() && !rows_like(out, x, N)) || (res.defined() && !rows_like(res, x, N)))
+        raise(PyExc_ValueError, "mx_linear: expected out and residual [.., N]");
+    const Mx om = osc.defined() ? mx_rows(name, out, osc, x, N) : Mx{row_stride(out, name), 0};
+    if (b.defined() && (b.dim() != 1 || b.size(0) != N)) raise(PyExc_ValueError, "mx_linear: expected bias [N]");
+    unit_last({&x, &out, &res, &b});
+    const int xd = xsc.defined() ? MBRT_MXFP4 : dtype_code(x), od = osc.defined() ? MBRT_MXFP4 : dtype_code(out);
+    const int bd = dtype_or(b, MBRT_F32), rd = dtype_or(res, MBRT_F32), act = (int)integer(a[8]);
+    const int64_t rs = res.defined() ? row_stride(res, name) : 0;
+    void *xp = ptr(x), *xsp = ptr(xsc), *wp = ptr(w), *wsp = ptr(wsc), *bp = ptr(b), *rp = ptr(res), *op = ptr(out), *osp = ptr(osc);
+    const OnDevice on({&x, &xsc, &w, &wsc, &b, &res, &out, &osc});
+    const mbrt_stream_t st = on.stream(a[10]);
+    return call("mbrt_mx_linear", [&] {
+        return mbrt_mx_linear(xp, xd, xm.codes, xsp, xm.scales, wp, wm.codes, wsp, wm.scales, bp, bd, rp, rd, rs, op, od, om.codes,
+                              osp, om.scales, rows, K, N, act, st);
+    });
+    END_HANDLE_TH_ERRORS
+}
+
+// Row r of `like` [.., D] has the gate's row (r / inner) % period.
+struct GateRows {
+    int64_t cols = 1, stride = 0, inner = 1, period = 1;
+};
+GateRows gate_rows(const at::Tensor& gate, const at::Tensor& like) {
+    GateRows r;
+    if (!gate.defined()) return r;
+    const char* shape = "expected gate [.., D] or [.., 1]";
+    if (gate.dim() < 1 || gate.dim() > like.dim() || (gate.size(-1) != 1 && gate.size(-1) != like.size(-1)))
+        raise_for("block_norm", shape);
+    r.cols = gate.size(-1);
+    bool closed = false;
+    for (int64_t d = 2; d <= like.dim(); ++d) {
+        const int64_t n = like.size(-d), m = d <= gate.dim() ? gate.size(-d) : 1;
+        if (m != 1 && m != n) raise_for("block_norm", shape);
+        if (n == 1) continue;
+        if (m == 1) {
+            if (r.period == 1) r.inner *= n;
+            else closed = true;
+            continue;
+        }
+        if (closed) raise_for("block_norm", "the gate's rows are shared on both sides of a dim that they do not share");
+        if (r.period > 1 && like.numel() && gate.stride(-d) != r.period * r.stride)
+            raise_for("block_norm", "the rows of a tensor lie at more than one stride");
+        if (r.period == 1) r.stride = gate.stride(-d);
+        r.period *= n;
+    }
+    if (r.inner < 1) r.inner = 1;
+    if (r.period < 1) r.period = 1;
+    return r;
+}
+
+// block_norm(residual, update, post_gamma | None, gate | None, gate_is_logit, layer_scale | None, gamma | None, sum_out | None,
+//            normed | None, normed_scales | None, alpha, post_scale, scale, eps, stream)
+MBRT_PY(block_norm) {
+    HANDLE_TH_ERRORS
+    count(n, 15);
+    const char* name = "block_norm";
+    const at::Tensor &res = tensor(a[0]), &upd = tensor(a[1]);
+    const at::Tensor pg = tensor_or_none(a[2]), gate = tensor_or_none(a[3]), ls = tensor_or_none(a[5]), g = tensor_or_none(a[6]);
+    const at::Tensor sum = tensor_or_none(a[7]), out = tensor_or_none(a[8]), osc = tensor_or_none(a[9]);
+    auto fits = [&](const at::Tensor& t) { return !t.defined() || t.sizes() == res.sizes(); };
+    if (res.dim() < 1 || res.size(-1) < 1 || !fits(upd) || !fits(sum) || (!osc.defined() && !fits(out)))
+        raise(PyExc_ValueError, "block_norm: expected update, sum_out and normed [.., D]");
+    if (sum.defined() && sum.scalar_type() != res.scalar_type())
+        raise(PyExc_ValueError, "block_norm: sum_out and residual differ in dtype");
+    const int64_t D = res.size(-1), rows = rows_of(res);
+    for (const at::Tensor* t : {&pg, &ls, &g})
+        if (t->defined() && (t->dim() != 1 || t->size(0) != D))
+            raise(PyExc_ValueError, "block_norm: expected gammas and layer_scale [D]");
+    contig({&pg, &ls, &g});
+    unit_last({&res, &upd, &sum, &out, &gate});
+    const Mx om = !out.defined() ? Mx{0, 0} : osc.defined() ? mx_rows(name, out, osc, res, D) : Mx{row_stride(out, name), 0};
+    const int od = osc.defined() ? MBRT_MXFP4 : dtype_or(out, MBRT_F32);
+    const GateRows gr = gate_rows(gate, res);
+    const int rd = dtype_code(res), ud = dtype_code(upd), pd = dtype_or(pg, MBRT_F32), gd = dtype_or(gate, MBRT_F32);
+    const int ld = dtype_or(ls, MBRT_F32), gad = dtype_or(g, MBRT_F32), logit = truth(a[4]);
+    const int64_t rs = row_stride(res, name), us = row_stride(upd, name), ss = sum.defined() ? row_stride(sum, name) : 0;
+    const float alpha = (float)number(a[10]), ps = (float)number(a[11]), sc = (float)number(a[12]), eps = (float)number(a[13]);
+    void *rp = ptr(res), *up = ptr(upd), *pp = ptr(pg), *gp = ptr(gate), *lp = ptr(ls), *gap = ptr(g), *sp = ptr(sum),
+         *op = ptr(out), *osp = ptr(osc);
+    const OnDevice on({&res, &upd, &pg, &gate, &ls, &g, &sum, &out, &osc});
+    const mbrt_stream_t st = on.stream(a[14]);
+    return call("mbrt_block_norm", [&] {
+        return mbrt_block_norm(rp, rd, rs, up, ud, us, pp, pd, gp, gd, gr.cols, gr.stride, gr.inner, gr.period, logit, lp, ld,
+                               gap, gad, sp, ss, op, od, om.codes, osp, om.scales, rows, D, alpha, ps, sc, eps, st);
+    });
+    END_HANDLE_TH_ERRORS
+}
+
 // stft(x [B, L], window, hop, center, normalized, out, n_fft, win_length, stream)
 MBRT_PY(stft) {
     HANDLE_TH_ERRORS
@@ -581,6 +751,7 @@ PyMethodDef kMethods[] = {
     MBRT_DEF(residual_add_rms_norm), MBRT_DEF(bias_act), MBRT_DEF(glu), MBRT_DEF(gate_merge), MBRT_DEF(softmax),
     MBRT_DEF(split_qkv_rotary), MBRT_DEF(attention_ex), MBRT_DEF(stft), MBRT_DEF(istft), MBRT_DEF(chunk_accumulate),
     MBRT_DEF(linear), MBRT_DEF(split_qkv_norm_rotary), MBRT_DEF(attention_window),
+    MBRT_DEF(mx_quantize), MBRT_DEF(mx_dequantize), MBRT_DEF(mx_linear), MBRT_DEF(block_norm),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_mbrt_calls", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
