@@ -5,10 +5,12 @@
 //   h = residual + alpha * layer_scale * gate * u                               rounded to residual's type
 //   normed = h * scale * gamma / sqrt(sum h^2 + eps)                            of h as it is rounded
 //
-// Every byte is read once and written once: a group of G lanes (16 or 64) holds a row in registers through both norms, lane
-// l its chunks l, l + G, ... of 16 bytes (VE elements: 8 where all operands have 2 bytes, else 4, f32 ones 16 bytes and
-// 2-byte ones 8).  The two sums of squares are butterflies within the group.  All loads are issued before the first use.
-// The vectors over the features are put into LDS once per block, multiplied as far as they go together.
+// Every byte is read once and written once: a group of G lanes (16, 64, or the 256 of a block) holds a row in registers through
+// both norms, lane l its chunks l, l + G, ... of 16 bytes (VE elements: 8 where all operands have 2 bytes, else 4, f32 ones
+// 16 bytes and 2-byte ones 8).  The two sums of squares are butterflies within the group, and sums over four waves through
+// LDS where a block holds the row.  The vectors over the features are put into LDS once per block, multiplied as far as they go
+// together, or read where they are needed by a block that has one row.  All loads of rows, and those into LDS, are issued
+// before the first use: a call of few rows takes one round of them.
 // A row whose last chunk is cut has it moved back to end at the row's end: its first elements are the chunk's before, left
 // out of the sums and stored twice with the same values, so that odd widths take the same loads as even ones.
 // normed may leave as microscaled 4-bit floats (mx.hpp): the lanes of a block of 32 stand side by side.
@@ -103,15 +105,71 @@ struct Chunk {
 
 __device__ __forceinline__ float gate_value(float g, int logit) { return logit ? sigmoidf(g) : g; }
 
+// n elements p[d], d a thread's every kThreads-th, as they stand in memory (past the end: the last one).
+template <int E>
+struct Staged {
+    uint32_t w[E];
+    __device__ __forceinline__ void load(const void* p, int dt, int dim) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = 0;
+        if (p == nullptr) return;
+        if (dt == F32) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = reinterpret_cast<const uint32_t*>(p)[min((int)threadIdx.x + e * kThreads, dim - 1)];
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) w[e] = reinterpret_cast<const uint16_t*>(p)[min((int)threadIdx.x + e * kThreads, dim - 1)];
+        }
+    }
+    __device__ __forceinline__ float value(int e, int dt) const {
+        return dt == F32 ? __uint_as_float(w[e]) : dt == BF16 ? bf16_lo(w[e]) : (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+    }
+};
+
+// N features from d on, at any place; p NULL: ones.
+template <int N>
+__device__ __forceinline__ void features(const void* p, int dt, int d, float (&f)[N]) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = 1.0f;
+    } else if (dt == F32) {
+#pragma unroll
+        for (int q = 0; q < N / 4; ++q) {
+            const u32x4 t = ld_any<0, 4>(reinterpret_cast<const float*>(p) + d + 4 * q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[4 * q + i] = __uint_as_float(t[i]);
+        }
+    } else {
+        Chunk<2, N> t;
+        t.template load<false>(reinterpret_cast<const char*>(p) + 2 * d);
+        t.to_f32(dt, f);
+    }
+}
+
+// The sum over a group's lanes, in each of them.  turn: another place in LDS for each sum of a row.
+template <int G>
+__device__ __forceinline__ float row_sum(float v, float* turn) {
+    if constexpr (G <= 64) {
+        return group_sum<G>(v);
+    } else {
+        v = group_sum<64>(v);
+        if (threadIdx.x % 64 == 0) turn[threadIdx.x / 64] = v;
+        __syncthreads();
+        return (turn[0] + turn[1]) + (turn[2] + turn[3]);
+    }
+}
+
 // RS, US: bytes of the residual's and the update's elements; GS: of a gate with a value per feature, 0 where there is one per
 // row or none.  AL: every row of every operand begins at a multiple of its chunk's bytes and is whole chunks long.
 template <int VE, int RS, int US, int GS, int G, int NC, bool AL>
 __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
+    constexpr bool IN_LDS = G < kThreads;
+    constexpr int E = (NC * G * VE + kThreads - 1) / kThreads;  // features of a thread as it fills LDS
     extern __shared__ float lds[];
-    float* const by = lds;            // alpha * layer_scale * post_scale * post_gamma
-    float* const gam = lds + a.dim;   // scale * gamma
+    float* const by = lds;            // IN_LDS: alpha * layer_scale * post_scale * post_gamma
+    float* const gam = lds + a.dim;   // and scale * gamma
     const int lane = threadIdx.x % G;
-    const uint32_t row = blockIdx.x * (kThreads / G) + threadIdx.x / G;
+    const int64_t row = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
     const bool valid = row < a.rows;
     const int64_t r = valid ? row : a.rows - 1;
     Chunk<RS, VE> rv[NC];
@@ -120,9 +178,8 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
     int at[NC];  // first element of the chunk
     const char* gp = a.gate;
     if (a.gate != nullptr) {
-        uint32_t q, m, d;
-        q = fdiv((uint32_t)r, a.inner);
-        fdivmod(q, a.period, d, m);
+        uint32_t d, m;
+        fdivmod(fdiv((uint32_t)r, a.inner), a.period, d, m);
         gp += m * a.gs;
     }
 #pragma unroll
@@ -133,15 +190,33 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
         uv[k].template load<AL>(a.upd + r * a.us + (int64_t)at[k] * US);
         if constexpr (GS != 0) gv[k].template load<AL>(gp + (int64_t)at[k] * GS);
     }
-    float g = 1.0f;
-    if (GS == 0 && a.gate != nullptr) g = gate_value(load1(gp, a.gdt, 0), a.gate_logit);
-    for (int d = threadIdx.x; d < a.dim; d += kThreads) {
-        float b = a.alpha;
-        if (a.ls != nullptr) b *= load1(a.ls, a.ldt, d);
-        if (a.post_gamma != nullptr) b *= load1(a.post_gamma, a.pdt, d) * a.post_scale;
-        by[d] = b;
-        if (a.gamma != nullptr) gam[d] = load1(a.gamma, a.gadt, d) * a.scale;
+    uint32_t gw = 0;
+    if (GS == 0 && a.gate != nullptr)
+        gw = a.gdt == F32 ? *reinterpret_cast<const uint32_t*>(gp) : *reinterpret_cast<const uint16_t*>(gp);
+    if constexpr (IN_LDS) {
+        Staged<E> ls, pg, ga;
+        ls.load(a.ls, a.ldt, a.dim);
+        pg.load(a.post_gamma, a.pdt, a.dim);
+        ga.load(a.gamma, a.gadt, a.dim);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            float b = a.alpha;
+            if (a.ls != nullptr) b *= ls.value(e, a.ldt);
+            if (a.post_gamma != nullptr) b *= pg.value(e, a.pdt) * a.post_scale;
+            const int d = threadIdx.x + e * kThreads;
+            if (d < a.dim) {
+                by[d] = b;
+                gam[d] = ga.value(e, a.gadt) * a.scale;
+            }
+        }
+        __syncthreads();
     }
+    float g = 1.0f;
+    if (GS == 0 && a.gate != nullptr)
+        g = gate_value(a.gdt == F32    ? __uint_as_float(gw)
+                       : a.gdt == BF16 ? bf16_lo(gw)
+                                       : (float)__builtin_bit_cast(_Float16, (uint16_t)gw),
+                       a.gate_logit);
     float h[NC][VE];
     if (a.post_gamma != nullptr) {
         float ss = 0.0f;
@@ -149,13 +224,12 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
         for (int k = 0; k < NC; ++k) {
             float u[VE];
             uv[k].to_f32(a.udt, u);
-            const int first = AL ? (lane + G * k < a.chunks ? 0 : VE) : (lane + G * k) * VE - at[k];  // elements before: another chunk's
+            const int first = AL ? (lane + G * k < a.chunks ? 0 : VE) : (lane + G * k) * VE - at[k];  // before it: another chunk's
 #pragma unroll
             for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(u[i], u[i], ss) : ss;
         }
-        g *= rsqrtf(group_sum<G>(ss) + a.eps);
+        g *= rsqrtf(row_sum<G>(ss, lds) + a.eps);
     }
-    __syncthreads();
     float ss = 0.0f;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
@@ -173,22 +247,50 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
             for (int i = 0; i < VE; ++i) u[i] *= w[i];
         }
         const int first = AL ? (lane + G * k < a.chunks ? 0 : VE) : (lane + G * k) * VE - at[k];
+        float f[VE];
+        if constexpr (IN_LDS) {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) h[k][i] = fmaf(u[i] * g, by[at[k] + i], x[i]);
+            for (int i = 0; i < VE; ++i) f[i] = by[at[k] + i];
+        } else {
+            float p[VE];
+            features<VE>(a.ls, a.ldt, at[k], f);
+            features<VE>(a.post_gamma, a.pdt, at[k], p);
+            const float b = a.post_gamma != nullptr ? a.alpha * a.post_scale : a.alpha;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) f[i] *= p[i] * b;
+        }
+#pragma unroll
+        for (int i = 0; i < VE; ++i) h[k][i] = fmaf(u[i] * g, f[i], x[i]);
         Chunk<RS, VE> t;
         t.from_f32(a.rdt, h[k]);
         t.to_f32(a.rdt, h[k]);
-        if (a.sum != nullptr && valid && lane + G * k < a.chunks) t.template store<AL>(a.sum + r * a.ss + (int64_t)at[k] * RS);
+        if (G <= 64 && a.sum != nullptr && valid && lane + G * k < a.chunks) t.template store<AL>(a.sum + r * a.ss + (int64_t)at[k] * RS);
 #pragma unroll
         for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(h[k][i], h[k][i], ss) : ss;
     }
+    const float inv = rsqrtf(row_sum<G>(ss, lds + 4) + a.eps);
+    if (G > 64 && a.sum != nullptr) {  // not before every wave has its part of a row that it may replace, a cut chunk's first elements too
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+            Chunk<RS, VE> t;
+            t.from_f32(a.rdt, h[k]);
+            if (lane + G * k < a.chunks) t.template store<AL>(a.sum + r * a.ss + (int64_t)at[k] * RS);
+        }
+    }
     if (a.gamma == nullptr) return;
-    const float inv = rsqrtf(group_sum<G>(ss) + a.eps);
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
         float o[VE];
+        if constexpr (IN_LDS) {
 #pragma unroll
-        for (int i = 0; i < VE; ++i) o[i] = h[k][i] * inv * gam[at[k] + i];
+            for (int i = 0; i < VE; ++i) o[i] = gam[at[k] + i];
+        } else {
+            features<VE>(a.gamma, a.gadt, at[k], o);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) o[i] *= a.scale;
+        }
+#pragma unroll
+        for (int i = 0; i < VE; ++i) o[i] *= h[k][i] * inv;
         const bool mine = valid && lane + G * k < a.chunks;
         if (a.odt == MXFP4) {
             const int c = lane + G * k;
@@ -290,19 +392,30 @@ bool launch_shape(const BlockNormArgs& a, hipStream_t st) {
     auto go = [&](auto g, auto nc) {
         constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
         hipLaunchKernelGGL((block_norm_kernel<VE, RS, US, GS, G, NC, AL>), dim3((unsigned)ceil_div(a.rows, kThreads / G)),
-                           dim3(kThreads), 2 * a.dim * sizeof(float), st, a);
+                           dim3(kThreads), (G < kThreads ? 2 * a.dim : 8) * sizeof(float), st, a);
     };
     typedef std::integral_constant<int, 16> G16;
     typedef std::integral_constant<int, 64> G64;
+    typedef std::integral_constant<int, 256> G256;
     const int n = a.odt == MXFP4 ? a.padded : a.chunks;
     if (n <= 32) go(G16(), std::integral_constant<int, 2>());
     else if (n <= 64) go(G16(), std::integral_constant<int, 4>());
     else if (n <= 96) go(G16(), std::integral_constant<int, 6>());
     else if (n <= 128) go(G64(), std::integral_constant<int, 2>());
-    else if (n <= 256) go(G64(), std::integral_constant<int, 4>());
-    else if (n <= 512) go(G64(), std::integral_constant<int, 8>());
-    else if (n <= 1024) go(G64(), std::integral_constant<int, 16>());
-    else return false;
+    else if (n <= 256) {
+#ifdef BN_G64
+        go(G64(), std::integral_constant<int, 4>());
+#else
+        go(G256(), std::integral_constant<int, 1>());
+#endif
+    } else if (n <= 512) go(G256(), std::integral_constant<int, 2>());
+    else if (n <= 1024) go(G256(), std::integral_constant<int, 4>());
+    else if constexpr (VE == 4) {
+        if (n > 2048) return false;
+        go(G256(), std::integral_constant<int, 8>());
+    } else {
+        return false;
+    }
     return true;
 }
 

@@ -76,11 +76,43 @@ __device__ __forceinline__ void to_parts(const u32x4 (&raw)[XT == F32 ? 2 : 1], 
     }
 }
 
+// x Phi(x) = x / (1 + exp(-p(x))) with p the odd polynomial of degree 13 that comes nearest to log(Phi(x) / Phi(-x)) up to 6.5,
+// weighted so that a value is off by at most 5.4e-6, and by at most 2^-7 of itself down to x = -6.3, where it is -9e-10: far within
+// the two significant bits of results in 4 bits, at 11 operations for gelu_short's 16.
+__device__ __forceinline__ float gelu_logistic(float x) {
+    constexpr float L = -1.44269504088896341f;
+    const float x2 = x * x;
+    float p = fmaf(7.40792158e-10f * L, x2, -9.01705128e-08f * L);
+    p = fmaf(p, x2, 4.01454603e-06f * L);
+    p = fmaf(p, x2, -7.20723898e-05f * L);
+    p = fmaf(p, x2, -2.37610013e-04f * L);
+    p = fmaf(p, x2, 0.0729833124f * L);
+    p = fmaf(p, x2, 1.59560622f * L);
+    return x * fast_rcp(1.0f + __builtin_amdgcn_exp2f(x * p));
+}
+
+// activate for results in 4 bits.  The reference's GELU, x Phi(sqrt 2 x), is the other's at sqrt 2 x by 1 / sqrt 2.
+template <int NV>
+__device__ __forceinline__ void activate_mx(float (&v)[NV], const MxLinArgs& a) {
+    if ((a.act == MBRT_ACT_GELU_REF || a.act == MBRT_ACT_GELU_STD) && a.short_act != 0) {
+        const float s = a.act == MBRT_ACT_GELU_REF ? 1.41421356237309505f : 1.0f, r = a.act == MBRT_ACT_GELU_REF ? 0.70710678118654752f : 1.0f;
+        if (a.act == MBRT_ACT_GELU_STD) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = gelu_logistic(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = r * gelu_logistic(s * v[i]);
+        }
+    } else {
+        activate<NV>(v, a.act, a.short_act != 0);
+    }
+}
+
 // bias, activation and residual of NV consecutive columns n .. of row m, for results that leave in 4 bits: zeros past N.
 template <bool ACT, int NV>
 __device__ __forceinline__ void finish_values(const MxLinArgs& a, int64_t m, int n, float (&v)[NV], const Bias<NV>& bias) {
     bias.add_to(a, v);
-    if constexpr (ACT) activate<NV>(v, a.act, a.short_act != 0);
+    if constexpr (ACT) activate_mx<NV>(v, a);
     if (a.res != nullptr) {
         const int64_t e = min(m, a.M - 1) * a.rs + n;
         if (n + NV <= a.N) {
@@ -122,24 +154,152 @@ __device__ __forceinline__ void finish8(const MxLinArgs& a, int64_t m, int n, fl
     }
 }
 
-// ---- tiles, x in 4 bits ------------------------------------------------------------------------
-// As linear_tile_kernel: WM x WN waves of MI x NI blocks of 16 x 16, K in steps of 128 bytes (8 blocks, two matrix
-// instructions) of every row through two LDS buffers filled straight from global memory, LDS rows of 8 pieces at j ^ key(row),
-// w the A operand with columns dealt so that a lane ends with 8 in a row.  The scales of a step, 8 bytes per row, come
-// through registers and are written to LDS by the thread that has the row, in front of the barrier that the step has anyway.
-template <int WM, int WN, int MI, int NI, int NT, bool ACT, bool OMX>
-__global__ __launch_bounds__(WM * WN * 64) void mx_tile_kernel(MxLinArgs a) {
-    constexpr int NW = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16, NTH = NW * 64;
-    constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW, SL = (BM + BN + NTH - 1) / NTH;
-    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NI % 2 == 0, "whole loads per wave, blocks in pairs");
-    constexpr int SB = kStepBytes, kBuf = (BM + BN) * SB;
+// ---- tiles -------------------------------------------------------------------------------------
+// WM x WN waves of MI x NI blocks of 16 x 16, w the A operand: lane (g, c) ends with four columns of row c of each block.
+// Which columns a block has is free: where results go out in 4 bits (OMX, NI = 8), block ni deals column 32 q + 4 ni + j to its
+// row 4 q + j, so that lane (g, c) ends with the 32 columns 32 g .. of its row, a whole block of the format; else 32 (ni / 2) +
+// 8 q + 4 (ni % 2) + j, 8 columns in a row for every two blocks.
+template <bool OMX>
+__device__ __forceinline__ constexpr int tile_col(int ni, int i) {
+    return OMX ? 32 * (i >> 2) + 4 * ni + (i & 3) : 32 * (ni / 2) + 8 * (i >> 2) + 4 * (ni % 2) + (i & 3);
+}
+
+// LDS rows of SB bytes: piece j of a row stands at j ^ key(row), so that eight neighbouring lanes, which read the same piece of
+// eight rows, find them in different banks.  key_c: the key of the row that lane c reads, of x or w.
+template <int SB>
+__device__ __forceinline__ int tile_key_x(int r) { return SB == 128 ? r & 7 : (r >> 1) & 3; }
+template <int SB, bool OMX>
+__device__ __forceinline__ int tile_key_w(int r) {
+    const int hi = OMX ? (r >> 5) & 1 : (r >> 3) & 1;
+    return SB == 128 ? (r & 3) | hi << 2 : ((r >> 1) & 1) | hi << 1;
+}
+template <int SB>
+__device__ __forceinline__ int tile_key_c(int c) { return SB == 128 ? c & 7 : (c >> 1) & 3; }
+
+// The bias is where the sums begin.
+template <int MI, int NI, bool OMX>
+__device__ __forceinline__ void tile_begin(const MxLinArgs& a, int n, int g, f32x4 (&acc)[MI][NI]) {
+    Bias<4> bias[NI];
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) bias[ni].load(a, n + tile_col<OMX>(ni, 4 * g));
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni) {
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        bias[ni].add_to(a, v);
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) acc[mi][ni] = f32x4{v[0], v[1], v[2], v[3]};
+    }
+}
+
+// Results in 4 bits of a wave's tile at row m, column n.
+template <int MI, bool ACT, int NI>
+__device__ __forceinline__ void tile_finish_mx(const MxLinArgs& a, int64_t m0, int n0, int g, int c, f32x4 (&acc)[MI][NI]) {
+    static_assert(NI == 8, "a lane has a whole block");
+    const int n = n0 + 32 * g;
+    const bool whole = n0 + 128 <= a.N;
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+        const int64_t m = m0 + mi * 16 + c;
+        float v[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = acc[mi][i / 4][i % 4];
+        if constexpr (ACT) activate_mx<32>(v, a);
+        if (a.res != nullptr && n < a.N) {
+            const int64_t e = min(m, a.M - 1) * a.rs + n;
+            if (n + 32 <= a.N) {
+                float r[32];
+                load_run<32>(a.res, a.rdt, e, r);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] += r[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (n + i < a.N) v[i] += load1(a.res, a.rdt, e + i);
+            }
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = n + i < a.N ? v[i] : 0.0f;
+        }
+        // the largest of them, and whether one is NaN: an operation each for two values
+        float top = 0.0f;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            top = fmaxf(fmaxf(top, __builtin_fabsf(v[i])), __builtin_fabsf(v[i + 1]));
+            nan |= __builtin_isunordered(v[i], v[i + 1]);
+        }
+        const uint32_t code = mx_scale_code(nan ? 0x7fc00000u : __float_as_uint(top));
+        if (m < a.M && n < a.N) {
+            u32x4 q;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float t[8] = {v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3], v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]};
+                q[i] = mx_pack8(t, mx_scale_operand(code));
+            }
+            *reinterpret_cast<u32x4*>(static_cast<char*>(a.out) + m * a.os + n / 2) = q;
+            a.osc[m * a.oss + n / 32] = (uint8_t)code;
+        }
+    }
+}
+
+// Other results: 16 rows at a time through the wave's own part of LDS (stage: 1 KB per block of 16 columns), from where a
+// row's columns go out side by side, whole 128-byte lines at once.  Units of four columns are dealt to even and odd
+// halves of an LDS row, and then by its key, so that neither side of the exchange meets a bank twice.
+template <int MI, int NI, bool ACT, int NT>
+__device__ __forceinline__ void tile_finish(const MxLinArgs& a, int64_t m0, int n0, int lane, char* stage, f32x4 (&acc)[MI][NI]) {
+    constexpr int RB = NI * 64;  // bytes of a staged row
+    static_assert(NI == 2 || NI == 4 || NI == 8, "whole rows per access");
+    const int g = lane / 16, c = lane % 16;
+    auto place = [&](int row, int unit) { return stage + row * RB + 16 * (((unit >> 1) + 2 * NI * (unit & 1)) ^ (row & (2 * NI - 1) & 7)); };
+    const bool wide = a.odt == F32;
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+        asm volatile("" ::: "memory");  // a wave's LDS accesses keep their order, as long as the compiler does
+#pragma unroll
+        for (int ni = 0; ni < NI; ++ni) *reinterpret_cast<f32x4*>(place(c, tile_col<false>(ni, 4 * g) / 4)) = acc[mi][ni];
+        asm volatile("" ::: "memory");
+        if (wide) {
+            constexpr int LPR = NI * 4, RPI = 64 / LPR;
+#pragma unroll
+            for (int k = 0; k < 16 / RPI; ++k) {
+                const int r = k * RPI + lane / LPR, u = lane % LPR;
+                const f32x4 t = *reinterpret_cast<const f32x4*>(place(r, u));
+                float v[4] = {t[0], t[1], t[2], t[3]};
+                finish<ACT, NT, 4>(a, m0 + mi * 16 + r, n0 + 4 * u, v, Bias<4>());
+            }
+        } else {
+            constexpr int LPR = NI * 2, RPI = 64 / LPR;
+#pragma unroll
+            for (int k = 0; k < (16 + RPI - 1) / RPI; ++k) {
+                const int r = k * RPI + lane / LPR, u = lane % LPR;
+                const f32x4 t = *reinterpret_cast<const f32x4*>(place(r, 2 * u)), s = *reinterpret_cast<const f32x4*>(place(r, 2 * u + 1));
+                float v[8] = {t[0], t[1], t[2], t[3], s[0], s[1], s[2], s[3]};
+                finish<ACT, NT, 8>(a, m0 + mi * 16 + r, n0 + 8 * u, v, Bias<8>());
+            }
+        }
+    }
+}
+
+// x in 4 bits: K in steps of SB bytes (2 or 4 blocks of each row for one matrix instruction, or two) through two LDS buffers filled
+// straight from global memory.  The scales of a step, 4 bytes per row and instruction, come through registers and
+// are written to LDS by the thread that has the row, in front of the barrier that the step has anyway.
+template <int WM, int WN, int MI, int NI, int SB, int OCC, int NT, bool ACT, bool OMX>
+__global__ __launch_bounds__(WM * WN * 64, OCC) void mx_tile_kernel(MxLinArgs a) {
+    constexpr int NW = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16, NTH = NW * 64, R = BM + BN;
+    constexpr int PB = SB / 16, RPL = 1024 / SB, KI = SB / 64;  // pieces of a row, rows of a load, instructions of a step
+    constexpr int LX = BM / RPL / NW, LW = BN / RPL / NW, SL = (R + NTH - 1) / NTH;
+    static_assert(BM % (RPL * NW) == 0 && BN % (RPL * NW) == 0 && NI % 2 == 0, "whole loads per wave, blocks in pairs");
+    constexpr int kBuf = R * SB;
+    static_assert(OMX || NW * NI * 1024 <= kBuf, "room for the rows on their way out");
     __shared__ __attribute__((aligned(16))) char s0[kBuf];
     __shared__ __attribute__((aligned(16))) char s1[kBuf];
-    __shared__ __attribute__((aligned(8))) uint8_t c0[(BM + BN) * 8];
-    __shared__ __attribute__((aligned(8))) uint8_t c1[(BM + BN) * 8];
+    __shared__ uint32_t c0[R * KI];
+    __shared__ uint32_t c1[R * KI];
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int w = __builtin_amdgcn_readfirstlane(tid / 64);
     const int wm = w / WN, wn = w % WN;
+    // column tiles of one row tile are neighbours, on one XCD
     const uint32_t tile = xcd_tile(blockIdx.x, gridDim.x);
     uint32_t mt, nt;
     fdivmod(tile, a.groups, mt, nt);
@@ -148,76 +308,90 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile_kernel(MxLinArgs a) {
     const char* xb = a.x + m0 * a.xs;
     const char* wb = a.w + (int64_t)n0 * a.ws;
     const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
-    const int steps = (a.nb + 7) / 8;
+    const int steps = (a.nb + PB - 1) / PB;
 
-    int xr[LX], wr[LW];
+    // lane i of load u covers LDS row RPL (LX w + u) + i / PB, place i % PB; rows past the end repeat the last one, pieces
+    // behind a row's end its last one
+    uint32_t xo[LX], wo[LW];
+    int xp[LX], wp[LW];
 #pragma unroll
-    for (int u = 0; u < LX; ++u) xr[u] = min(8 * (LX * w + u) + lane / 8, mrows - 1);
+    for (int u = 0; u < LX; ++u) {
+        const int r = RPL * (LX * w + u) + lane / PB;
+        xp[u] = (lane % PB) ^ tile_key_x<SB>(r);
+        xo[u] = (uint32_t)min(r, mrows - 1) * (uint32_t)a.xs;
+    }
 #pragma unroll
-    for (int u = 0; u < LW; ++u) wr[u] = min(8 * (LW * w + u) + lane / 8, nrows - 1);
+    for (int u = 0; u < LW; ++u) {
+        const int r = RPL * (LW * w + u) + lane / PB;
+        wp[u] = (lane % PB) ^ tile_key_w<SB, OMX>(r);
+        wo[u] = (uint32_t)min(r, nrows - 1) * (uint32_t)a.ws;
+    }
     const __amdgpu_buffer_rsrc_t xres = __builtin_amdgcn_make_buffer_rsrc((void*)xb, (short)0, -1, kBufferDword3);
     const __amdgpu_buffer_rsrc_t wres = __builtin_amdgcn_make_buffer_rsrc((void*)wb, (short)0, -1, kBufferDword3);
-    // pieces behind a row's end: its last one
     auto load = [&](int kt, char* d) {
-        const int last = a.nb - 1 - 8 * kt;
+        const int last = a.nb - 1 - PB * kt;
 #pragma unroll
-        for (int u = 0; u < LX; ++u)
-            load_to_lds(xres, d + 1024 * (LX * w + u),
-                        (uint32_t)xr[u] * (uint32_t)a.xs + 16u * min((lane % 8) ^ key_x(8 * (LX * w + u) + lane / 8), last), kt * SB);
+        for (int u = 0; u < LX; ++u) load_to_lds(xres, d + 1024 * (LX * w + u), xo[u] + 16u * min(xp[u], last), kt * SB);
 #pragma unroll
-        for (int u = 0; u < LW; ++u)
-            load_to_lds(wres, d + BM * SB + 1024 * (LW * w + u),
-                        (uint32_t)wr[u] * (uint32_t)a.ws + 16u * min((lane % 8) ^ key_w(8 * (LW * w + u) + lane / 8), last), kt * SB);
+        for (int u = 0; u < LW; ++u) load_to_lds(wres, d + BM * SB + 1024 * (LW * w + u), wo[u] + 16u * min(wp[u], last), kt * SB);
     };
     const uint8_t* sp[SL];
 #pragma unroll
     for (int u = 0; u < SL; ++u) {
-        const int r = min(tid + u * NTH, BM + BN - 1);
+        const int r = min(tid + u * NTH, R - 1);
         sp[u] = r < BM ? a.xsc + (m0 + min(r, mrows - 1)) * a.xss : a.wsc + (int64_t)(n0 + min(r - BM, nrows - 1)) * a.wss;
     }
-    typedef uint32_t any8 __attribute__((ext_vector_type(2), aligned(1)));
-    u32x2 sv[SL];
-    auto load_scales = [&](int kt) {
-        const int left = a.nb - 8 * kt;
-#pragma unroll
-        for (int u = 0; u < SL; ++u) {
-            if (left >= 8) {
-                sv[u] = *reinterpret_cast<const any8*>(sp[u] + 8 * kt);
-            } else {
-                sv[u] = u32x2{0u, 0u};
-#pragma unroll
-                for (int j = 0; j < 7; ++j)
-                    if (j < left) sv[u][j / 4] |= (uint32_t)sp[u][8 * kt + j] << (8 * (j % 4));
-            }
-        }
-    };
-    auto put_scales = [&](uint8_t* d) {
+    typedef uint32_t any4 __attribute__((aligned(1)));
+    uint32_t sv[SL][KI];
+    auto load_scales = [&](int kt) {  // zeros behind a row's end
 #pragma unroll
         for (int u = 0; u < SL; ++u)
-            if (tid + u * NTH < BM + BN) *reinterpret_cast<u32x2*>(d + 8 * (tid + u * NTH)) = sv[u];
+#pragma unroll
+            for (int s = 0; s < KI; ++s) {
+                const int b = PB * kt + 4 * s;
+                if (b + 4 <= a.nb) {
+                    sv[u][s] = *reinterpret_cast<const any4*>(sp[u] + b);
+                } else {
+                    sv[u][s] = 0;
+#pragma unroll
+                    for (int j = 0; j < 3; ++j)
+                        if (b + j < a.nb) sv[u][s] |= (uint32_t)sp[u][b + j] << (8 * j);
+                }
+            }
+    };
+    auto put_scales = [&](uint32_t* d) {
+#pragma unroll
+        for (int u = 0; u < SL; ++u)
+            if (tid + u * NTH < R) {
+#pragma unroll
+                for (int s = 0; s < KI; ++s) d[s * R + tid + u * NTH] = sv[u][s];
+            }
     };
 
+    load(0, s0);
+    load_scales(0);
     f32x4 acc[MI][NI];
+    tile_begin<MI, NI, OMX>(a, n0 + wn * NI * 16, g, acc);
+    const int xrow = wm * MI * 16 + c, wrow = BM + wn * NI * 16;
+    auto compute = [&](const char* d, const uint32_t* ds) {
+        const uint8_t* sc = reinterpret_cast<const uint8_t*>(ds);
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-        for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int xrow = wm * MI * 16 + c, wrow = BM + wn * NI * 16 + 8 * (c >> 2) + (c & 3);
-    auto compute = [&](const char* d, const uint8_t* ds) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int piece = 16 * ((4 * s + g) ^ (c & 7));
+        for (int s = 0; s < KI; ++s) {
+            if (s > 0) __builtin_amdgcn_sched_barrier(0);  // the second instruction's operands not beside the first's
             u32x4 xf[MI], wf[NI];
             uint32_t xs[MI], ws[NI];
+            const int piece = 16 * ((4 * s + g) ^ tile_key_c<SB>(c));
 #pragma unroll
             for (int mi = 0; mi < MI; ++mi) {
-                xf[mi] = *reinterpret_cast<const u32x4*>(d + (xrow + mi * 16) * SB + piece);
-                xs[mi] = ds[(xrow + mi * 16) * 8 + 4 * s + g];
+                const int r = xrow + mi * 16;
+                xf[mi] = *reinterpret_cast<const u32x4*>(d + r * SB + piece);
+                xs[mi] = sc[(s * R + r) * 4 + g];
             }
 #pragma unroll
             for (int ni = 0; ni < NI; ++ni) {
-                wf[ni] = *reinterpret_cast<const u32x4*>(d + (wrow + 32 * (ni / 2) + 4 * (ni % 2)) * SB + piece);
-                ws[ni] = ds[(wrow + 32 * (ni / 2) + 4 * (ni % 2)) * 8 + 4 * s + g];
+                const int r = wrow + tile_col<OMX>(ni, c);
+                wf[ni] = *reinterpret_cast<const u32x4*>(d + r * SB + piece);
+                ws[ni] = sc[(s * R + r) * 4 + g];
             }
 #pragma unroll
             for (int mi = 0; mi < MI; ++mi)
@@ -225,7 +399,9 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile_kernel(MxLinArgs a) {
                 for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = mx_mma(wf[ni], ws[ni], xf[mi], xs[mi], acc[mi][ni]);
         }
     };
-    auto step = [&](int kt, char* d, uint8_t* ds, char* dn) {
+    // Step kt sits in d, the next one goes to dn, which held the one before; separate objects, and the loop unrolled by two, so that
+    // the compiler sees that loads in flight into one do not touch the other.
+    auto step = [&](int kt, char* d, uint32_t* ds, char* dn) {
         put_scales(ds);  // waits for them; the buffer was last read two steps ago
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         wait_loads();
@@ -236,37 +412,32 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_tile_kernel(MxLinArgs a) {
         }
         compute(d, ds);
     };
-    load(0, s0);
-    load_scales(0);
     for (int kt = 0; kt < steps; kt += 2) {
         step(kt, s0, c0, s1);
         if (kt + 1 < steps) step(kt + 1, s1, c1, s0);
     }
 
-    const int n = n0 + wn * NI * 16 + 8 * g;
-    Bias<8> bias[NI / 2];
-#pragma unroll
-    for (int p = 0; p < NI / 2; ++p) bias[p].load(a, n + 32 * p);
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-        for (int p = 0; p < NI / 2; ++p) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = acc[mi][2 * p + i / 4][i % 4];
-            finish8<ACT, OMX, NT>(a, m0 + wm * MI * 16 + mi * 16 + c, n + 32 * p, v, bias[p]);
-        }
+    const int64_t m = m0 + wm * MI * 16;
+    const int n = n0 + wn * NI * 16;
+    if constexpr (OMX) {
+        tile_finish_mx<MI, ACT>(a, m, n, g, c, acc);
+    } else {
+        // the buffer that the last step did not use: no wave reads it any more
+        MxLinArgs rest = a;
+        rest.bias = nullptr;
+        tile_finish<MI, NI, ACT, NT>(rest, m, n, lane, ((steps & 1) != 0 ? s1 : s0) + w * NI * 1024, acc);
+    }
 }
 
-// ---- tiles, x in 16 or 32 bits -------------------------------------------------------------------
-// Steps of 64 features: w becomes bf16 and x its parts on their way through registers into LDS, one plane of 128-byte rows
-// per part.  The next step's loads are under way while one is computed.  The parts of x meet the same weights.
+// x in 16 or 32 bits: steps of 64 features; w becomes bf16 and x its parts on their way through registers into LDS, one plane of
+// 128-byte rows per part.  Loads of three steps are under way while one is computed.  The parts of x meet the same weights.
 template <int XT, int WM, int WN, int MI, int NI, int NT, bool ACT, bool OMX>
 __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a) {
     constexpr int NW = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16, P = mx_parts(XT), Q = XT == F32 ? 2 : 1;
     constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW, S = XT == F32 ? 4 : 2;
     static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NI % 2 == 0, "whole loads per wave, blocks in pairs");
     constexpr int SB = 128, kBuf = (BM * P + BN) * SB;
+    static_assert(OMX || NW * NI * 1024 <= kBuf, "room for the rows on their way out");
     __shared__ __attribute__((aligned(16))) char lds[2][kBuf];
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int w = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -289,54 +460,62 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
         wp[u] = a.w + r * a.ws;
         sp[u] = a.wsc + r * a.wss;
     }
-    u32x4 px[LX][Q];
-    uint32_t pw[LW], ps[LW];
-    const int64_t kbytes = (int64_t)a.K * S;
-    auto load = [&](int kt) {
+    // three steps are on their way at once, each in registers of its own
+    struct Regs {
+        u32x4 x[LX][Q];
+        uint32_t w[LW], scale[LW];
+    };
+    Regs r0, r1, r2;
+    auto load = [&](int kt, Regs& d, auto cut) __attribute__((always_inline)) {
         // lane's piece: features 64 kt + 8 j of its row, j = lane % 8 (placed at j ^ key in LDS)
         const int j = lane % 8;
         const int64_t kb = ((int64_t)kt * 64 + 8 * j) * S;
-        const bool whole = ((int64_t)kt + 1) * 64 * S <= kbytes;
 #pragma unroll
         for (int u = 0; u < LX; ++u)
 #pragma unroll
-            for (int q = 0; q < Q; ++q) px[u][q] = whole ? ld_any<0, S>(xp[u] + kb + 16 * q) : row_piece<XT>(xp[u], kb + 16 * q, a.K);
+            for (int q = 0; q < Q; ++q) d.x[u][q] = cut ? row_piece<XT>(xp[u], kb + 16 * q, a.K) : ld_any<0, S>(xp[u] + kb + 16 * q);
         const int b = min(2 * kt + j / 4, a.nb - 1);  // past the last block, where x is zeros: its codes again
 #pragma unroll
         for (int u = 0; u < LW; ++u) {
-            pw[u] = *reinterpret_cast<const uint32_t*>(wp[u] + 16 * (int64_t)b + 4 * (j % 4));
-            ps[u] = 2 * kt + j / 4 < a.nb ? sp[u][b] : 0u;
+            d.w[u] = *reinterpret_cast<const uint32_t*>(wp[u] + 16 * (int64_t)b + 4 * (j % 4));
+            d.scale[u] = cut && 2 * kt + j / 4 >= a.nb ? 0u : sp[u][b];
         }
     };
-    auto put = [&](char* d) {
+    auto put = [&](const Regs& from, char* d) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < LX; ++u) {
             const int r = 8 * (LX * w + u) + lane / 8;
             u32x4 f[P];
-            to_parts<XT>(px[u], f);
+            to_parts<XT>(from.x[u], f);
 #pragma unroll
-            for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(d + (p * BM + r) * SB + 16 * ((lane % 8) ^ key_x(r))) = f[p];
+            for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(d + (p * BM + r) * SB + 16 * ((lane % 8) ^ tile_key_x<SB>(r))) = f[p];
         }
 #pragma unroll
         for (int u = 0; u < LW; ++u) {
             const int r = 8 * (LW * w + u) + lane / 8;
-            *reinterpret_cast<u32x4*>(d + (P * BM + r) * SB + 16 * ((lane % 8) ^ key_w(r))) =
-                mx_unpack8_bf16(pw[u], mx_scale_operand(ps[u]));
+            *reinterpret_cast<u32x4*>(d + (P * BM + r) * SB + 16 * ((lane % 8) ^ tile_key_w<SB, OMX>(r))) =
+                mx_unpack8_bf16(from.w[u], mx_scale_operand(from.scale[u]));
         }
     };
+    auto ready = [&]() {  // the step is in LDS, and none still reads the other buffer; loads may be under way
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        lds_barrier();
+    };
+    typedef std::integral_constant<bool, false> Whole;
+    const int whole = a.K / 64;
+    if (whole > 0) load(0, r0, Whole());
+    if (whole > 1) load(1, r1, Whole());
+    if (whole > 2) load(2, r2, Whole());
     f32x4 acc[MI][NI];
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-        for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int xrow = wm * MI * 16 + c, wrow = P * BM + wn * NI * 16 + 8 * (c >> 2) + (c & 3);
-    auto compute = [&](const char* d) {
+    tile_begin<MI, NI, OMX>(a, n0 + wn * NI * 16, g, acc);
+    const int xrow = wm * MI * 16 + c, wrow = P * BM + wn * NI * 16;
+    auto compute = [&](const char* d) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int piece = 16 * ((4 * s + g) ^ (c & 7));
+            const int piece = 16 * ((4 * s + g) ^ tile_key_c<SB>(c));
             u32x4 wf[NI];
 #pragma unroll
-            for (int ni = 0; ni < NI; ++ni) wf[ni] = *reinterpret_cast<const u32x4*>(d + (wrow + 32 * (ni / 2) + 4 * (ni % 2)) * SB + piece);
+            for (int ni = 0; ni < NI; ++ni) wf[ni] = *reinterpret_cast<const u32x4*>(d + (wrow + tile_col<OMX>(ni, c)) * SB + piece);
 #pragma unroll
             for (int p = P - 1; p >= 0; --p) {
                 u32x4 xf[MI];
@@ -349,28 +528,36 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
             }
         }
     };
-    load(0);
-    put(lds[0]);
-    for (int kt = 0; kt < steps; ++kt) {
-        __syncthreads();  // the step is in LDS, and none still reads the other buffer
-        if (kt + 1 < steps) load(kt + 1);
+    // step kt, whose registers `mine` are free; the next one's are `next`
+    auto step = [&](int kt, Regs& mine, const Regs& next) __attribute__((always_inline)) {
+        if (kt >= whole) return;
+        ready();
+        if (kt + 3 < whole) load(kt + 3, mine, Whole());
         compute(lds[kt & 1]);
-        if (kt + 1 < steps) put(lds[(kt + 1) & 1]);
+        if (kt + 1 < whole) put(next, lds[(kt + 1) & 1]);
+    };
+    if (whole > 0) put(r0, lds[0]);
+    for (int kt = 0; kt < whole; kt += 3) {
+        step(kt, r0, r1);
+        step(kt + 1, r1, r2);
+        step(kt + 2, r2, r0);
+    }
+    if (steps > whole) {  // the step that the rows' end cuts
+        load(whole, r0, std::integral_constant<bool, true>());
+        put(r0, lds[whole & 1]);
+        ready();
+        compute(lds[whole & 1]);
     }
 
-    const int n = n0 + wn * NI * 16 + 8 * g;
-    Bias<8> bias[NI / 2];
-#pragma unroll
-    for (int p = 0; p < NI / 2; ++p) bias[p].load(a, n + 32 * p);
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-        for (int p = 0; p < NI / 2; ++p) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = acc[mi][2 * p + i / 4][i % 4];
-            finish8<ACT, OMX, NT>(a, m0 + wm * MI * 16 + mi * 16 + c, n + 32 * p, v, bias[p]);
-        }
+    const int64_t m = m0 + wm * MI * 16;
+    const int n = n0 + wn * NI * 16;
+    if constexpr (OMX) {
+        tile_finish_mx<MI, ACT>(a, m, n, g, c, acc);
+    } else {
+        MxLinArgs rest = a;
+        rest.bias = nullptr;
+        tile_finish<MI, NI, ACT, NT>(rest, m, n, lane, lds[steps & 1] + w * NI * 1024, acc);
+    }
 }
 
 // ---- strips ------------------------------------------------------------------------------------
@@ -535,6 +722,154 @@ __global__ __launch_bounds__(1024) void mx_strip_kernel(MxLinArgs a) {
     }
 }
 
+// ---- few rows against many weights -----------------------------------------------------------------
+// At most 16 rows of x: what takes time is reading w.  A wave takes 32 columns, columns dealt so that a lane ends with 8 in a
+// row; `split` waves share the K of one such strip, 16 blocks at a time in turn, the scales of a row's 16 in one load.  x stands in LDS, as bf16 parts or as its codes, zeros up to
+// whole turns, so that w alone waits for memory: 8 KB a wave, and the next turn's as many while one is computed.
+// [1, 4096] bf16 -> 16384: 13.3 us in strips, which read x again for every 16 columns.
+#ifndef MX_TOKEN_BLOCKS
+#define MX_TOKEN_BLOCKS 65536
+#define MX_TOKEN_WAVES 8
+#endif
+#ifndef MX_TOKEN_NT
+#define MX_TOKEN_NT 0
+#endif
+template <int XT>
+struct TokenX {  // bytes of a row of x in LDS, for a number of blocks
+    static constexpr int kBlock = XT == MXFP4 ? 16 : 64;  // a block's codes, or one part of its values
+    static __host__ __device__ int64_t row(int64_t blocks) {
+        return XT == MXFP4 ? 17 * blocks + 16 - blocks % 16 : 64 * blocks * mx_parts(XT) + 16;
+    }
+};
+
+template <int XT, bool OMX>
+__global__ __launch_bounds__(1024) void mx_token_kernel(MxLinArgs a) {
+    constexpr int P = mx_parts(XT), Q = XT == F32 ? 2 : 1, S = XT == F32 ? 4 : 2, PW = 2;
+    extern __shared__ __attribute__((aligned(16))) char xl[];
+    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
+    const int ks = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int turns = (a.nb + 15) / 16, padded = 16 * turns, M = (int)a.M;
+    const int rb = (int)TokenX<XT>::row(padded);
+    const int64_t p0 = (int64_t)blockIdx.x * 32;
+    const char* wb[PW];
+    const uint8_t* ws[PW];
+#pragma unroll
+    for (int p = 0; p < PW; ++p) {
+        const int64_t r = min(p0 + tile_col<false>(p, c), (int64_t)a.N - 1);
+        wb[p] = a.w + r * a.ws;
+        ws[p] = a.wsc + r * a.wss;
+    }
+    typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
+    struct Turn {
+        u32x4 w[PW][4];
+        u32x4 scales[PW];  // byte g of each
+    };
+    auto load = [&](int t, Turn& d) {  // blocks behind a row's end: its last one, scale 0 (x is zeros there)
+#pragma unroll
+        for (int p = 0; p < PW; ++p) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                d.w[p][s] = gld<MX_TOKEN_NT>(reinterpret_cast<const u32x4*>(wb[p] + 16 * (int64_t)min(16 * t + 4 * s + g, a.nb - 1)));
+            if (16 * t + 16 <= a.nb) {
+                d.scales[p] = *reinterpret_cast<const any16*>(ws[p] + 16 * t);
+            } else {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int b = 16 * t + 4 * s + g;
+                    d.scales[p][s] = b < a.nb ? (uint32_t)ws[p][b] << (8 * g) : 0u;
+                }
+            }
+        }
+    };
+    Turn one, two;
+    if (ks < turns) load(ks, one);
+
+    if constexpr (XT == MXFP4) {
+        for (int i = tid; i < M * padded; i += blockDim.x) {
+            const int m = i / padded, b = i - m * padded;
+            u32x4 v = {0u, 0u, 0u, 0u};
+            uint32_t sc = 0;
+            if (b < a.nb) {
+                v = *reinterpret_cast<const u32x4*>(a.x + m * a.xs + 16 * (int64_t)b);
+                sc = a.xsc[m * a.xss + b];
+            }
+            *reinterpret_cast<u32x4*>(xl + m * rb + 16 * b) = v;
+            xl[m * rb + 16 * padded + b] = (char)sc;
+        }
+    } else {
+        for (int i = tid; i < M * padded * 4; i += blockDim.x) {  // 8 features each
+            const int m = i / (4 * padded), e = i - m * 4 * padded;
+            const char* row = a.x + m * a.xs;
+            u32x4 raw[Q], f[P];
+#pragma unroll
+            for (int q = 0; q < Q; ++q) raw[q] = row_piece<XT>(row, (int64_t)e * 8 * S + 16 * q, a.K);
+            to_parts<XT>(raw, f);
+#pragma unroll
+            for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(xl + m * rb + p * 64 * padded + 16 * e) = f[p];
+        }
+    }
+    __syncthreads();
+
+    f32x4 acc[PW];
+#pragma unroll
+    for (int p = 0; p < PW; ++p) acc[p] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const char* xr = xl + min(c, M - 1) * rb;
+    auto compute = [&](int t, const Turn& d) {
+        const int b = 16 * t + g;
+        if constexpr (XT == MXFP4) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const u32x4 xf = *reinterpret_cast<const u32x4*>(xr + 16 * (b + 4 * s));
+                const uint32_t xsc = *reinterpret_cast<const uint8_t*>(xr + 16 * padded + b + 4 * s);
+#pragma unroll
+                for (int p = 0; p < PW; ++p) acc[p] = mx_mma(d.w[p][s], d.scales[p][s] >> (8 * g), xf, xsc, acc[p]);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    u32x4 wf[PW];
+#pragma unroll
+                    for (int p = 0; p < PW; ++p) wf[p] = mx_unpack8_bf16(d.w[p][s][q], mx_scale_operand(d.scales[p][s] >> (8 * g) & 255u));
+#pragma unroll
+                    for (int i = P - 1; i >= 0; --i) {
+                        const u32x4 xf = *reinterpret_cast<const u32x4*>(xr + i * 64 * padded + 64 * (b + 4 * s) + 16 * q);
+#pragma unroll
+                        for (int p = 0; p < PW; ++p) acc[p] = mma<BF16>(wf[p], xf, acc[p]);
+                    }
+                }
+        }
+    };
+    for (int t = ks; t < turns; t += 2 * a.split) {
+        if (t + a.split < turns) load(t + a.split, two);
+        compute(t, one);
+        if (t + a.split < turns) {
+            if (t + 2 * a.split < turns) load(t + 2 * a.split, one);
+            compute(t + a.split, two);
+        }
+    }
+
+    f32x4* part = reinterpret_cast<f32x4*>(xl) + lane;
+    if (a.split > 1) {
+        __syncthreads();  // x is not read any more
+#pragma unroll
+        for (int p = 0; p < PW; ++p) part[(ks * PW + p) * 64] = acc[p];
+        __syncthreads();
+        if (ks > 0) return;
+#pragma unroll
+        for (int p = 0; p < PW; ++p)
+            for (int k = 1; k < a.split; ++k) acc[p] += part[(k * PW + p) * 64];
+    }
+    const int n = (int)min<int64_t>(p0 + 8 * g, (int64_t)a.N + 32);
+    Bias<8> bias;
+    bias.load(a, n);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = acc[i / 4][i % 4];
+    finish8<true, OMX, 0>(a, c, n, v, bias);
+}
+
 template <int XT, int PW, int R, bool OMX>
 void launch_mx_strip(const MxLinArgs& a, int align, unsigned blocks, unsigned threads, size_t lds, hipStream_t st) {
     if constexpr (XT == MXFP4) {
@@ -548,7 +883,8 @@ void launch_mx_strip(const MxLinArgs& a, int align, unsigned blocks, unsigned th
     }
 }
 
-template <int XT, int WM, int WN, int MI, int NI, int NT, bool OMX>
+// SB, OCC: of x in 4 bits
+template <int XT, int WM, int WN, int MI, int NI, int SB, int OCC, int NT, bool OMX>
 int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
     constexpr int BM = WM * MI * 16, BN = WN * NI * 16;
     a.ntiles = (uint32_t)ceil_div(a.N, BN);
@@ -559,7 +895,7 @@ int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
     auto launch = [&](auto act) {
         constexpr bool ACT = decltype(act)::value;
         if constexpr (XT == MXFP4)
-            hipLaunchKernelGGL((mx_tile_kernel<WM, WN, MI, NI, NT, ACT, OMX>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((mx_tile_kernel<WM, WN, MI, NI, SB, OCC, NT, ACT, OMX>), grid, block, 0, st, a);
         else
             hipLaunchKernelGGL((mx_wide_tile_kernel<XT, WM, WN, MI, NI, NT, ACT, OMX>), grid, block, 0, st, a);
     };
@@ -571,14 +907,22 @@ int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
 template <int XT, bool OMX>
 int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
     const int64_t cus = cu_count();
-    const int64_t cols = ceil_div(a.N, 16), rows = ceil_div(a.M, 16);
+    const int64_t cols = ceil_div(a.N, 16);
+    const int64_t turns = ceil_div(a.nb, 16), token_lds = std::max(a.M * TokenX<XT>::row(16 * turns), int64_t(0));
+    if (a.M <= 16 && (int64_t)a.N * a.nb >= MX_TOKEN_BLOCKS && token_lds <= (int64_t(1) << 16)) {
+        const int64_t strips = ceil_div(a.N, 32), room = std::max<int64_t>(1, std::min<int64_t>(16, MX_TOKEN_WAVES * cus / strips));
+        a.split = (int)ceil_div(turns, ceil_div(turns, room));
+        const size_t lds = (size_t)std::max<int64_t>(token_lds, a.split > 1 ? a.split * 2048 : 0);
+        hipLaunchKernelGGL((mx_token_kernel<XT, OMX>), dim3((unsigned)strips), dim3(64 * a.split), lds, st, a);
+        return MBRT_OK;
+    }
     // 32-bit offsets within a tile
     const bool far = XT == MXFP4 && (a.xs >= (int64_t(1) << 22) || a.ws >= (int64_t(1) << 22));
     if (far || ceil_div(std::max(a.M, (int64_t)a.N), 16) * ceil_div(std::min(a.M, (int64_t)a.N), 64) <= cus ||
         std::min(a.M, (int64_t)a.N) <= 16) {
         constexpr int PW = OMX ? 2 : 1;
         const int64_t strips = ceil_div(cols, PW);
-        int R = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+        int R = a.M <= 16 ? 1 : a.M <= 32 || XT == F32 ? 2 : 4;  // (f32 rows in three parts: no registers for more)
         while (R > 1 && strips * ceil_div(a.M, 8 * R) <= cus) R /= 2;
         const int64_t groups = ceil_div(a.M, 16 * R), turns = ceil_div(a.nb, 4);
         const int64_t room = std::max<int64_t>(1, std::min<int64_t>({16, 64 / (R * PW), 8 * cus / (strips * groups)}));
@@ -593,17 +937,24 @@ int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
         if (!grid_fits(blocks, threads) || groups >= (int64_t(1) << 31)) return set_error(MBRT_E_SHAPE, "mbrt_mx_linear: too many rows");
         if (R == 1) launch_mx_strip<XT, PW, 1, OMX>(a, align, (unsigned)blocks, threads, lds, st);
         else if (R == 2) launch_mx_strip<XT, PW, 2, OMX>(a, align, (unsigned)blocks, threads, lds, st);
-        else launch_mx_strip<XT, PW, 4, OMX>(a, align, (unsigned)blocks, threads, lds, st);
+        else if constexpr (XT != F32) launch_mx_strip<XT, PW, 4, OMX>(a, align, (unsigned)blocks, threads, lds, st);
         return MBRT_OK;
     }
     const bool big = XT != F32 && std::min(a.M, (int64_t)a.N) > 64 && ceil_div(a.M, 128) * ceil_div(a.N, 128) >= cus;
-    if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, 0, OMX>(a, st);
-    if constexpr (XT != F32) {
-        const bool nt = !OMX && aligned(a.out, 64) && a.os * dt_size(a.odt) % 64 == 0;
-        if constexpr (!OMX) {
-            if (nt) return launch_mx_tile<XT, 2, 2, 4, 4, 2, OMX>(a, st);
+    // short K in steps of 64 bytes, whose buffers leave room for three workgroups to a CU
+    const bool small_steps = a.nb <= 32;
+    if constexpr (OMX) {
+        if (!big) return launch_mx_tile<XT, 4, 1, 1, 8, 64, 3, 0, true>(a, st);
+        if constexpr (XT != F32)
+            return small_steps ? launch_mx_tile<XT, 4, 1, 2, 8, 64, 3, 0, true>(a, st) : launch_mx_tile<XT, 4, 1, 2, 8, 128, 2, 0, true>(a, st);
+    } else {
+        if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, 128, 4, 0, false>(a, st);
+        if constexpr (XT != F32) {
+            const bool nt = aligned(a.out, 64) && a.os * dt_size(a.odt) % 64 == 0;
+            if (small_steps)
+                return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 0, false>(a, st);
+            return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 128, 2, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 128, 2, 0, false>(a, st);
         }
-        return launch_mx_tile<XT, 2, 2, 4, 4, 0, OMX>(a, st);
     }
     return MBRT_OK;
 }
