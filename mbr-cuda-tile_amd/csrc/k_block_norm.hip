@@ -398,17 +398,16 @@ bool launch_shape(const BlockNormArgs& a, hipStream_t st) {
     typedef std::integral_constant<int, 64> G64;
     typedef std::integral_constant<int, 256> G256;
     const int n = a.odt == MXFP4 ? a.padded : a.chunks;
+    // A block per row from 129 chunks on, whose loads are spread over more lanes: us, a wave and a block per row, [1800, 1536] bf16
+    // 9.5 and 7.6, [100, 1024] f32 3.7 and 2.7, [12, 2000] bf16 5.8 and 3.0, [12000, 1536] 36.7 and 34.5; but of many short rows
+    // half a block's lanes would have nothing: [18786, 526] f32 29 and 37, [24000, 768] 44.7 and 46.8.
     if (n <= 32) go(G16(), std::integral_constant<int, 2>());
     else if (n <= 64) go(G16(), std::integral_constant<int, 4>());
     else if (n <= 96) go(G16(), std::integral_constant<int, 6>());
     else if (n <= 128) go(G64(), std::integral_constant<int, 2>());
-    else if (n <= 256) {
-#ifdef BN_G64
-        go(G64(), std::integral_constant<int, 4>());
-#else
-        go(G256(), std::integral_constant<int, 1>());
-#endif
-    } else if (n <= 512) go(G256(), std::integral_constant<int, 2>());
+    else if (n <= 192 && a.rows >= 16 * cu_count()) go(G64(), std::integral_constant<int, 3>());
+    else if (n <= 256) go(G256(), std::integral_constant<int, 1>());
+    else if (n <= 512) go(G256(), std::integral_constant<int, 2>());
     else if (n <= 1024) go(G256(), std::integral_constant<int, 4>());
     else if constexpr (VE == 4) {
         if (n > 2048) return false;

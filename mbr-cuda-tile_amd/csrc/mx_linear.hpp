@@ -167,14 +167,14 @@ __device__ __forceinline__ constexpr int tile_col(int ni, int i) {
 // LDS rows of SB bytes: piece j of a row stands at j ^ key(row), so that eight neighbouring lanes, which read the same piece of
 // eight rows, find them in different banks.  key_c: the key of the row that lane c reads, of x or w.
 template <int SB>
-__device__ __forceinline__ int tile_key_x(int r) { return SB == 128 ? r & 7 : (r >> 1) & 3; }
+__device__ __forceinline__ int tile_key_x(int r) { return SB >= 128 ? r & 7 : (r >> 1) & 3; }
 template <int SB, bool OMX>
 __device__ __forceinline__ int tile_key_w(int r) {
     const int hi = OMX ? (r >> 5) & 1 : (r >> 3) & 1;
-    return SB == 128 ? (r & 3) | hi << 2 : ((r >> 1) & 1) | hi << 1;
+    return SB >= 128 ? (r & 3) | hi << 2 : ((r >> 1) & 1) | hi << 1;
 }
 template <int SB>
-__device__ __forceinline__ int tile_key_c(int c) { return SB == 128 ? c & 7 : (c >> 1) & 3; }
+__device__ __forceinline__ int tile_key_c(int c) { return SB >= 128 ? c & 7 : (c >> 1) & 3; }
 
 // The bias is where the sums begin.
 template <int MI, int NI, bool OMX>
@@ -429,14 +429,29 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void mx_tile_kernel(MxLinArgs a)
     }
 }
 
-// x in 16 or 32 bits: steps of 64 features; w becomes bf16 and x its parts on their way through registers into LDS, one plane of
-// 128-byte rows per part.  Loads of three steps are under way while one is computed.  The parts of x meet the same weights.
-template <int XT, int WM, int WN, int MI, int NI, int NT, bool ACT, bool OMX>
+// x in 16 or 32 bits: steps of FS features; w becomes bf16 and x its parts on their way through registers into LDS, one plane of
+// rows per part.  Every load costs the same whatever its width, so a thread takes whole blocks of w, 16 bytes and a scale. Loads of
+// three steps are under way while one is computed.  The parts of x meet the same weights.  LDS rows of x: piece j (8 features) at
+// j ^ key(row).  Of w: piece 4 b + q of block b at (b + FS / 32 q) ^ key(row), so that the lanes that hold a row's blocks
+// write side by side, and rows that are read together, or written, differ in their keys.
+template <int FS, bool OMX>
+__device__ __forceinline__ int wide_key_w(int r) {
+    const int hi = OMX ? (r >> 5) & 1 : (r >> 3) & 1;
+    return FS == 128 ? (r & 1) << 2 | hi << 1 | ((r >> 1) & 1) : ((r >> 1) & 1) << 2 | (r & 1) << 1 | hi;
+}
+template <int FS>
+__device__ __forceinline__ int wide_key_c(int c) {  // of the row of w that lane c reads
+    return FS == 128 ? (c & 1) << 2 | ((c >> 2) & 1) << 1 | ((c >> 1) & 1) : ((c >> 1) & 1) << 2 | (c & 1) << 1 | ((c >> 2) & 1);
+}
+
+template <int XT, int WM, int WN, int MI, int NI, int FS, int NT, bool ACT, bool OMX>
 __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a) {
-    constexpr int NW = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16, P = mx_parts(XT), Q = XT == F32 ? 2 : 1;
-    constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW, S = XT == F32 ? 4 : 2;
-    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && NI % 2 == 0, "whole loads per wave, blocks in pairs");
-    constexpr int SB = 128, kBuf = (BM * P + BN) * SB;
+    constexpr int NW = WM * WN, NTH = NW * 64, BM = WM * MI * 16, BN = WN * NI * 16, P = mx_parts(XT), Q = XT == F32 ? 2 : 1;
+    constexpr int S = XT == F32 ? 4 : 2, PR = FS / 8, BR = FS / 32;     // pieces and blocks of a row's step
+    constexpr int LX = BM * PR / NTH, WB = BN * BR, LW = (WB + NTH - 1) / NTH;  // pieces of x and blocks of w for a thread
+    static_assert(FS == 64 || FS == 128, "one or two banks' round of a row");
+    static_assert(BM * PR % NTH == 0 && NI % 2 == 0, "as much of x for every thread, blocks in pairs");
+    constexpr int SB = 2 * FS, kBuf = (BM * P + BN) * SB;
     static_assert(OMX || NW * NI * 1024 <= kBuf, "room for the rows on their way out");
     __shared__ __attribute__((aligned(16))) char lds[2][kBuf];
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
@@ -448,79 +463,88 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
     const int64_t m0 = (int64_t)mt * BM;
     const int n0 = (int)nt * BN;
     const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
-    const int steps = (a.K + 63) / 64;
+    const int steps = (a.K + FS - 1) / FS, whole = a.K / FS;
     const char* xp[LX];
     const char* wp[LW];
     const uint8_t* sp[LW];
 #pragma unroll
-    for (int u = 0; u < LX; ++u) xp[u] = a.x + (m0 + min(8 * (LX * w + u) + lane / 8, mrows - 1)) * a.xs;
+    for (int u = 0; u < LX; ++u) xp[u] = a.x + (m0 + min((tid + u * NTH) / PR, mrows - 1)) * a.xs;
 #pragma unroll
     for (int u = 0; u < LW; ++u) {
-        const int64_t r = n0 + min(8 * (LW * w + u) + lane / 8, nrows - 1);
+        const int64_t r = n0 + min(min(tid + u * NTH, WB - 1) / BR, nrows - 1);
         wp[u] = a.w + r * a.ws;
         sp[u] = a.wsc + r * a.wss;
     }
     // three steps are on their way at once, each in registers of its own
     struct Regs {
-        u32x4 x[LX][Q];
-        uint32_t w[LW], scale[LW];
+        u32x4 x[LX][Q], w[LW];
+        uint32_t scale[LW];
     };
     Regs r0, r1, r2;
     auto load = [&](int kt, Regs& d, auto cut) __attribute__((always_inline)) {
-        // lane's piece: features 64 kt + 8 j of its row, j = lane % 8 (placed at j ^ key in LDS)
-        const int j = lane % 8;
-        const int64_t kb = ((int64_t)kt * 64 + 8 * j) * S;
+        const int64_t kb = ((int64_t)kt * FS + 8 * (tid % PR)) * S;
 #pragma unroll
         for (int u = 0; u < LX; ++u)
 #pragma unroll
             for (int q = 0; q < Q; ++q) d.x[u][q] = cut ? row_piece<XT>(xp[u], kb + 16 * q, a.K) : ld_any<0, S>(xp[u] + kb + 16 * q);
-        const int b = min(2 * kt + j / 4, a.nb - 1);  // past the last block, where x is zeros: its codes again
+        const int b = kt * BR + tid % BR, at = cut ? min(b, a.nb - 1) : b;  // past the last block, where x is zeros: its codes again
 #pragma unroll
         for (int u = 0; u < LW; ++u) {
-            d.w[u] = *reinterpret_cast<const uint32_t*>(wp[u] + 16 * (int64_t)b + 4 * (j % 4));
-            d.scale[u] = cut && 2 * kt + j / 4 >= a.nb ? 0u : sp[u][b];
+            d.w[u] = *reinterpret_cast<const u32x4*>(wp[u] + 16 * (int64_t)at);
+            d.scale[u] = cut && b >= a.nb ? 0u : sp[u][at];
         }
     };
-    auto put = [&](const Regs& from, char* d) __attribute__((always_inline)) {
+    auto put = [&](Regs& from, char* d) __attribute__((always_inline)) {
+        // nothing is computed from these registers, and so waits for their loads, before this place
+#pragma unroll
+        for (int u = 0; u < LX; ++u)
+#pragma unroll
+            for (int q = 0; q < Q; ++q) asm volatile("" : "+v"(from.x[u][q]));
+#pragma unroll
+        for (int u = 0; u < LW; ++u) asm volatile("" : "+v"(from.w[u]), "+v"(from.scale[u]));
 #pragma unroll
         for (int u = 0; u < LX; ++u) {
-            const int r = 8 * (LX * w + u) + lane / 8;
+            const int r = (tid + u * NTH) / PR;
             u32x4 f[P];
             to_parts<XT>(from.x[u], f);
 #pragma unroll
-            for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(d + (p * BM + r) * SB + 16 * ((lane % 8) ^ tile_key_x<SB>(r))) = f[p];
+            for (int p = 0; p < P; ++p) *reinterpret_cast<u32x4*>(d + (p * BM + r) * SB + 16 * ((tid % PR) ^ (r & 7))) = f[p];
         }
 #pragma unroll
         for (int u = 0; u < LW; ++u) {
-            const int r = 8 * (LW * w + u) + lane / 8;
-            *reinterpret_cast<u32x4*>(d + (P * BM + r) * SB + 16 * ((lane % 8) ^ tile_key_w<SB, OMX>(r))) =
-                mx_unpack8_bf16(from.w[u], mx_scale_operand(from.scale[u]));
+            const int r = (tid + u * NTH) / BR, b = tid % BR;
+            if (WB % NTH != 0 && r >= BN) break;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<u32x4*>(d + (P * BM + r) * SB + 16 * ((b + BR * q) ^ wide_key_w<FS, OMX>(r))) =
+                    mx_unpack8_bf16(from.w[u][q], mx_scale_operand(from.scale[u]));
         }
     };
     auto ready = [&]() {  // the step is in LDS, and none still reads the other buffer; loads may be under way
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         lds_barrier();
     };
-    typedef std::integral_constant<bool, false> Whole;
-    const int whole = a.K / 64;
-    if (whole > 0) load(0, r0, Whole());
-    if (whole > 1) load(1, r1, Whole());
-    if (whole > 2) load(2, r2, Whole());
+    typedef std::integral_constant<bool, false> No;
+    typedef std::integral_constant<bool, true> Yes;
+    if (whole > 0) load(0, r0, No());
+    if (whole > 1) load(1, r1, No());
+    if (whole > 2) load(2, r2, No());
     f32x4 acc[MI][NI];
     tile_begin<MI, NI, OMX>(a, n0 + wn * NI * 16, g, acc);
     const int xrow = wm * MI * 16 + c, wrow = P * BM + wn * NI * 16;
     auto compute = [&](const char* d) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int piece = 16 * ((4 * s + g) ^ tile_key_c<SB>(c));
+        for (int s = 0; s < FS / 32; ++s) {
             u32x4 wf[NI];
 #pragma unroll
-            for (int ni = 0; ni < NI; ++ni) wf[ni] = *reinterpret_cast<const u32x4*>(d + (wrow + tile_col<OMX>(ni, c)) * SB + piece);
+            for (int ni = 0; ni < NI; ++ni)
+                wf[ni] = *reinterpret_cast<const u32x4*>(d + (wrow + tile_col<OMX>(ni, c)) * SB + 16 * ((s + BR * g) ^ wide_key_c<FS>(c)));
 #pragma unroll
             for (int p = P - 1; p >= 0; --p) {
                 u32x4 xf[MI];
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi) xf[mi] = *reinterpret_cast<const u32x4*>(d + (p * BM + xrow + mi * 16) * SB + piece);
+                for (int mi = 0; mi < MI; ++mi)
+                    xf[mi] = *reinterpret_cast<const u32x4*>(d + (p * BM + xrow + mi * 16) * SB + 16 * ((4 * s + g) ^ (c & 7)));
 #pragma unroll
                 for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
@@ -528,22 +552,26 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
             }
         }
     };
-    // step kt, whose registers `mine` are free; the next one's are `next`
-    auto step = [&](int kt, Regs& mine, const Regs& next) __attribute__((always_inline)) {
-        if (kt >= whole) return;
+    // Step kt, whose registers `mine` are free for step kt + 3; the next one's are `next`.  No condition stands between the loads
+    // (the last ones load the last whole step again), so that each wait is for the oldest of them alone.
+    auto step = [&](int kt, Regs& mine, Regs& next, auto on) __attribute__((always_inline)) {
         ready();
-        if (kt + 3 < whole) load(kt + 3, mine, Whole());
+        if (on) load(min(kt + 3, whole - 1), mine, No());
         compute(lds[kt & 1]);
-        if (kt + 1 < whole) put(next, lds[(kt + 1) & 1]);
+        put(next, lds[(kt + 1) & 1]);
     };
     if (whole > 0) put(r0, lds[0]);
-    for (int kt = 0; kt < whole; kt += 3) {
-        step(kt, r0, r1);
-        step(kt + 1, r1, r2);
-        step(kt + 2, r2, r0);
+    int kt = 0;
+    for (; kt + 3 <= whole; kt += 3) {
+        step(kt, r0, r1, Yes());
+        step(kt + 1, r1, r2, Yes());
+        step(kt + 2, r2, r0, Yes());
     }
+    if (kt < whole) step(kt, r0, r1, No());
+    if (kt + 1 < whole) step(kt + 1, r1, r2, No());
     if (steps > whole) {  // the step that the rows' end cuts
-        load(whole, r0, std::integral_constant<bool, true>());
+        load(whole, r0, Yes());
+        ready();  // (what the last step put there in vain is read by none)
         put(r0, lds[whole & 1]);
         ready();
         compute(lds[whole & 1]);
@@ -554,8 +582,10 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
     if constexpr (OMX) {
         tile_finish_mx<MI, ACT>(a, m, n, g, c, acc);
     } else {
+        // a wave's own part of a buffer: the last step's other one, which nothing reads or, behind a cut step, writes any more
         MxLinArgs rest = a;
         rest.bias = nullptr;
+        ready();
         tile_finish<MI, NI, ACT, NT>(rest, m, n, lane, lds[steps & 1] + w * NI * 1024, acc);
     }
 }
@@ -883,7 +913,7 @@ void launch_mx_strip(const MxLinArgs& a, int align, unsigned blocks, unsigned th
     }
 }
 
-// SB, OCC: of x in 4 bits
+// SB, OCC: of x in 4 bits (else SB is the features of a step)
 template <int XT, int WM, int WN, int MI, int NI, int SB, int OCC, int NT, bool OMX>
 int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
     constexpr int BM = WM * MI * 16, BN = WN * NI * 16;
@@ -897,7 +927,7 @@ int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
         if constexpr (XT == MXFP4)
             hipLaunchKernelGGL((mx_tile_kernel<WM, WN, MI, NI, SB, OCC, NT, ACT, OMX>), grid, block, 0, st, a);
         else
-            hipLaunchKernelGGL((mx_wide_tile_kernel<XT, WM, WN, MI, NI, NT, ACT, OMX>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((mx_wide_tile_kernel<XT, WM, WN, MI, NI, SB, NT, ACT, OMX>), grid, block, 0, st, a);
     };
     if (a.act != MBRT_ACT_NONE) launch(std::integral_constant<bool, true>());
     else launch(std::integral_constant<bool, false>());
@@ -941,22 +971,33 @@ int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
         return MBRT_OK;
     }
     const bool big = XT != F32 && std::min(a.M, (int64_t)a.N) > 64 && ceil_div(a.M, 128) * ceil_div(a.N, 128) >= cus;
-    // short K in steps of 64 bytes, whose buffers leave room for three workgroups to a CU
-    const bool small_steps = a.nb <= 32;
-    if constexpr (OMX) {
-        if (!big) return launch_mx_tile<XT, 4, 1, 1, 8, 64, 3, 0, true>(a, st);
-        if constexpr (XT != F32)
-            return small_steps ? launch_mx_tile<XT, 4, 1, 2, 8, 64, 3, 0, true>(a, st) : launch_mx_tile<XT, 4, 1, 2, 8, 128, 2, 0, true>(a, st);
+    if constexpr (XT != MXFP4) {
+        constexpr int FS = XT == BF16 ? 128 : 64;
+        if constexpr (OMX) {
+            if (!big) return launch_mx_tile<XT, 4, 1, 1, 8, FS, 1, 0, true>(a, st);
+            if constexpr (XT != F32) return launch_mx_tile<XT, 4, 1, 2, 8, 64, 1, 0, true>(a, st);
+        } else {
+            if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, FS, 1, 0, false>(a, st);
+            if constexpr (XT != F32) {
+                const bool nt = aligned(a.out, 64) && a.os * dt_size(a.odt) % 64 == 0;
+                return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 1, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 1, 0, false>(a, st);
+            }
+        }
+        return MBRT_OK;
     } else {
-        if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, 128, 4, 0, false>(a, st);
-        if constexpr (XT != F32) {
+        // short K in steps of 64 bytes, whose buffers leave room for three workgroups to a CU
+        const bool small_steps = a.nb <= 32;
+        if constexpr (OMX) {
+            if (!big) return launch_mx_tile<XT, 4, 1, 1, 8, 64, 3, 0, true>(a, st);
+            return small_steps ? launch_mx_tile<XT, 4, 1, 2, 8, 64, 3, 0, true>(a, st) : launch_mx_tile<XT, 4, 1, 2, 8, 128, 2, 0, true>(a, st);
+        } else {
+            if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, 128, 4, 0, false>(a, st);
             const bool nt = aligned(a.out, 64) && a.os * dt_size(a.odt) % 64 == 0;
             if (small_steps)
                 return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 0, false>(a, st);
             return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 128, 2, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 128, 2, 0, false>(a, st);
         }
     }
-    return MBRT_OK;
 }
 
 }  // namespace
