@@ -16,8 +16,9 @@ __global__ __launch_bounds__(64) void mx_empty_kernel(MxLinArgs a) {
     float v[8] = {};
     Bias<8> bias;
     bias.load(a, at);
-    if (a.odt == MXFP4) finish8<true, true, 0>(a, row, at, v, bias);
-    else finish8<true, false, 0>(a, row, at, v, bias);
+    if (a.odt != MXFP4) finish8<true, false>(a, row, at, v, bias);
+    else if (a.short_act != 0) finish8<true, true>(a, row, at, v, bias);
+    else finish8<false, true>(a, row, at, v, bias);
 }
 
 }  // namespace

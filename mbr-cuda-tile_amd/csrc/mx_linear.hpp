@@ -91,28 +91,41 @@ __device__ __forceinline__ float gelu_logistic(float x) {
     return x * fast_rcp(1.0f + __builtin_amdgcn_exp2f(x * p));
 }
 
-// activate for results in 4 bits.  The reference's GELU, x Phi(sqrt 2 x), is the other's at sqrt 2 x by 1 / sqrt 2.
-template <int NV>
-__device__ __forceinline__ void activate_mx(float (&v)[NV], const MxLinArgs& a) {
-    if ((a.act == MBRT_ACT_GELU_REF || a.act == MBRT_ACT_GELU_STD) && a.short_act != 0) {
-        const float s = a.act == MBRT_ACT_GELU_REF ? 1.41421356237309505f : 1.0f, r = a.act == MBRT_ACT_GELU_REF ? 0.70710678118654752f : 1.0f;
-        if (a.act == MBRT_ACT_GELU_STD) {
+// What a kernel applies to its sums: nothing, GELU in a form for short results, or any function.  What stands behind the sums of a
+// tile runs once in a workgroup's life, so that code costs as much to fetch as to run: one that holds every function for all of a lane's
+// values takes [17916, 1536] -> 384 from 12.8 to 28.6 us with GELU.
+enum MxAct { kActNone = 0, kActGelu = 1, kActAny = 2 };
+
+// The reference's GELU, x Phi(sqrt 2 x), is the other's at sqrt 2 x by 1 / sqrt 2.  OMX: for results in 4 bits.  SHORT: the short
+// forms of the others.
+template <int KIND, bool OMX, bool SHORT, int NV>
+__device__ __forceinline__ void activate_mx(const MxLinArgs& a, float (&v)[NV]) {
+    if constexpr (KIND == kActGelu) {
+        const bool ref = a.act == MBRT_ACT_GELU_REF;
+        if constexpr (OMX) {
+            if (ref) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = gelu_logistic(v[i]);
+                for (int i = 0; i < NV; ++i) v[i] = 0.70710678118654752f * gelu_logistic(1.41421356237309505f * v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) v[i] = gelu_logistic(v[i]);
+            }
         } else {
+            const float s = ref ? 1.0f : 0.70710678118654752440f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = r * gelu_logistic(s * v[i]);
+            for (int i = 0; i < NV; ++i) v[i] = gelu_short(v[i], s);
         }
-    } else {
-        activate<NV>(v, a.act, a.short_act != 0);
+    } else if constexpr (KIND == kActAny) {
+        if (OMX && SHORT && (a.act == MBRT_ACT_GELU_REF || a.act == MBRT_ACT_GELU_STD)) activate_mx<kActGelu, true, true>(a, v);
+        else activate<NV>(v, a.act, SHORT || a.short_act != 0);
     }
 }
 
 // bias, activation and residual of NV consecutive columns n .. of row m, for results that leave in 4 bits: zeros past N.
-template <bool ACT, int NV>
+template <bool SHORT, int NV>
 __device__ __forceinline__ void finish_values(const MxLinArgs& a, int64_t m, int n, float (&v)[NV], const Bias<NV>& bias) {
     bias.add_to(a, v);
-    if constexpr (ACT) activate_mx<NV>(v, a);
+    activate_mx<kActAny, true, SHORT>(a, v);
     if (a.res != nullptr) {
         const int64_t e = min(m, a.M - 1) * a.rs + n;
         if (n + NV <= a.N) {
@@ -144,13 +157,13 @@ __device__ __forceinline__ void store_mx(const MxLinArgs& a, int64_t m, int n, c
     }
 }
 
-template <bool ACT, bool OMX, int NT>
+template <bool SHORT, bool OMX>
 __device__ __forceinline__ void finish8(const MxLinArgs& a, int64_t m, int n, float (&v)[8], const Bias<8>& bias) {
     if constexpr (OMX) {
-        finish_values<ACT, 8>(a, m, n, v, bias);
+        finish_values<SHORT, 8>(a, m, n, v, bias);
         store_mx(a, m, n, v);
     } else {
-        finish<ACT, NT, 8>(a, m, n, v, bias);
+        finish<true, 0, 8>(a, m, n, v, bias);
     }
 }
 
@@ -176,23 +189,32 @@ __device__ __forceinline__ int tile_key_w(int r) {
 template <int SB>
 __device__ __forceinline__ int tile_key_c(int c) { return SB >= 128 ? c & 7 : (c >> 1) & 3; }
 
-// The bias is where the sums begin.
+// The bias is where the sums begin: four columns in one load where all columns of the tile are there (a load for each column
+// took [48060, 384] -> 1536 from 40 to 53 us).
 template <int MI, int NI, bool OMX>
-__device__ __forceinline__ void tile_begin(const MxLinArgs& a, int n, int g, f32x4 (&acc)[MI][NI]) {
-    Bias<4> bias[NI];
+__device__ __forceinline__ void tile_begin(const MxLinArgs& a, int n0, int g, f32x4 (&acc)[MI][NI]) {
+    f32x4 b[NI];
+    if (a.bias == nullptr) {
 #pragma unroll
-    for (int ni = 0; ni < NI; ++ni) bias[ni].load(a, n + tile_col<OMX>(ni, 4 * g));
+        for (int ni = 0; ni < NI; ++ni) b[ni] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    } else if (n0 + NI * 16 <= a.N && a.bdt == F32) {
 #pragma unroll
-    for (int ni = 0; ni < NI; ++ni) {
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        bias[ni].add_to(a, v);
+        for (int ni = 0; ni < NI; ++ni)
+            b[ni] = __builtin_bit_cast(f32x4, ld_any<0, 4>(static_cast<const float*>(a.bias) + n0 + tile_col<OMX>(ni, 4 * g)));
+    } else {
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi) acc[mi][ni] = f32x4{v[0], v[1], v[2], v[3]};
+        for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[ni][j] = load1(a.bias, a.bdt, min(n0 + tile_col<OMX>(ni, 4 * g) + j, a.N - 1));
     }
+#pragma unroll
+    for (int ni = 0; ni < NI; ++ni)
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) acc[mi][ni] = b[ni];
 }
 
 // Results in 4 bits of a wave's tile at row m, column n.
-template <int MI, bool ACT, int NI>
+template <int MI, int KIND, bool SHORT, int NI>
 __device__ __forceinline__ void tile_finish_mx(const MxLinArgs& a, int64_t m0, int n0, int g, int c, f32x4 (&acc)[MI][NI]) {
     static_assert(NI == 8, "a lane has a whole block");
     const int n = n0 + 32 * g;
@@ -203,7 +225,7 @@ __device__ __forceinline__ void tile_finish_mx(const MxLinArgs& a, int64_t m0, i
         float v[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = acc[mi][i / 4][i % 4];
-        if constexpr (ACT) activate_mx<32>(v, a);
+        activate_mx<KIND, true, SHORT>(a, v);
         if (a.res != nullptr && n < a.N) {
             const int64_t e = min(m, a.M - 1) * a.rs + n;
             if (n + 32 <= a.N) {
@@ -246,56 +268,63 @@ __device__ __forceinline__ void tile_finish_mx(const MxLinArgs& a, int64_t m0, i
 // Other results: 16 rows at a time through the wave's own part of LDS (stage: 1 KB per block of 16 columns), from where a
 // row's columns go out side by side, whole 128-byte lines at once.  Units of four columns are dealt to even and odd
 // halves of an LDS row, and then by its key, so that neither side of the exchange meets a bank twice.
-template <int MI, int NI, bool ACT, int NT>
+template <int MI, int NI, int KIND, int NT>
 __device__ __forceinline__ void tile_finish(const MxLinArgs& a, int64_t m0, int n0, int lane, char* stage, f32x4 (&acc)[MI][NI]) {
     constexpr int RB = NI * 64;  // bytes of a staged row
+    constexpr int kTurns = KIND == kActNone ? 16 : 1;  // one copy of an activation for all rows of a block
     static_assert(NI == 2 || NI == 4 || NI == 8, "whole rows per access");
     const int g = lane / 16, c = lane % 16;
     auto place = [&](int row, int unit) { return stage + row * RB + 16 * (((unit >> 1) + 2 * NI * (unit & 1)) ^ (row & (2 * NI - 1) & 7)); };
-    const bool wide = a.odt == F32;
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
         asm volatile("" ::: "memory");  // a wave's LDS accesses keep their order, as long as the compiler does
 #pragma unroll
         for (int ni = 0; ni < NI; ++ni) *reinterpret_cast<f32x4*>(place(c, tile_col<false>(ni, 4 * g) / 4)) = acc[mi][ni];
         asm volatile("" ::: "memory");
-        if (wide) {
+        if (KIND != kActGelu && a.odt == F32) {
             constexpr int LPR = NI * 4, RPI = 64 / LPR;
-#pragma unroll
+#pragma unroll kTurns
             for (int k = 0; k < 16 / RPI; ++k) {
                 const int r = k * RPI + lane / LPR, u = lane % LPR;
                 const f32x4 t = *reinterpret_cast<const f32x4*>(place(r, u));
                 float v[4] = {t[0], t[1], t[2], t[3]};
-                finish<ACT, NT, 4>(a, m0 + mi * 16 + r, n0 + 4 * u, v, Bias<4>());
+                activate_mx<KIND, false, false>(a, v);
+                finish<false, NT, 4>(a, m0 + mi * 16 + r, n0 + 4 * u, v, Bias<4>());
             }
         } else {
             constexpr int LPR = NI * 2, RPI = 64 / LPR;
-#pragma unroll
+#pragma unroll kTurns
             for (int k = 0; k < (16 + RPI - 1) / RPI; ++k) {
                 const int r = k * RPI + lane / LPR, u = lane % LPR;
                 const f32x4 t = *reinterpret_cast<const f32x4*>(place(r, 2 * u)), s = *reinterpret_cast<const f32x4*>(place(r, 2 * u + 1));
                 float v[8] = {t[0], t[1], t[2], t[3], s[0], s[1], s[2], s[3]};
-                finish<ACT, NT, 8>(a, m0 + mi * 16 + r, n0 + 8 * u, v, Bias<8>());
+                activate_mx<KIND, false, false>(a, v);
+                finish<false, NT, 8>(a, m0 + mi * 16 + r, n0 + 8 * u, v, Bias<8>());
             }
         }
     }
 }
 
 // x in 4 bits: K in steps of SB bytes (2 or 4 blocks of each row for one matrix instruction, or two) through two LDS buffers filled
-// straight from global memory.  The scales of a step, 4 bytes per row and instruction, come through registers and
-// are written to LDS by the thread that has the row, in front of the barrier that the step has anyway.
-template <int WM, int WN, int MI, int NI, int SB, int OCC, int NT, bool ACT, bool OMX>
+// straight from global memory.  Scales come 16 blocks at a time, 16 bytes per row, through registers, and are written to LDS by
+// the thread that has the row, in front of the barrier that the step has anyway: of rows that lie 128 bytes apart every load
+// fetches a line, and 4 or 8 bytes of it at a time cost as much as the codes ([4096, 4096] -> 4096 64 us).
+template <int WM, int WN, int MI, int NI, int SB, int OCC, int NT, int KIND, bool OMX>
 __global__ __launch_bounds__(WM * WN * 64, OCC) void mx_tile_kernel(MxLinArgs a) {
     constexpr int NW = WM * WN, BM = WM * MI * 16, BN = WN * NI * 16, NTH = NW * 64, R = BM + BN;
     constexpr int PB = SB / 16, RPL = 1024 / SB, KI = SB / 64;  // pieces of a row, rows of a load, instructions of a step
     constexpr int LX = BM / RPL / NW, LW = BN / RPL / NW, SL = (R + NTH - 1) / NTH;
     static_assert(BM % (RPL * NW) == 0 && BN % (RPL * NW) == 0 && NI % 2 == 0, "whole loads per wave, blocks in pairs");
+    static_assert(SB == 64 || SB == 128, "a group of scales is four or two steps");
     constexpr int kBuf = R * SB;
     static_assert(OMX || NW * NI * 1024 <= kBuf, "room for the rows on their way out");
     __shared__ __attribute__((aligned(16))) char s0[kBuf];
     __shared__ __attribute__((aligned(16))) char s1[kBuf];
-    __shared__ uint32_t c0[R * KI];
-    __shared__ uint32_t c1[R * KI];
+    // [instruction of a group of four][row], the next group's in the other half; four words between 32 rows and the next, so that
+    // lanes that read rows 32 apart do not meet
+    constexpr int RS = R + R / 8;
+    __shared__ uint32_t sc[2][4 * RS];
+    auto scale_at = [](int r) { return r + 4 * (r >> 5); };
     const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int w = __builtin_amdgcn_readfirstlane(tid / 64);
     const int wm = w / WN, wn = w % WN;
@@ -342,29 +371,35 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void mx_tile_kernel(MxLinArgs a)
         sp[u] = r < BM ? a.xsc + (m0 + min(r, mrows - 1)) * a.xss : a.wsc + (int64_t)(n0 + min(r - BM, nrows - 1)) * a.wss;
     }
     typedef uint32_t any4 __attribute__((aligned(1)));
-    uint32_t sv[SL][KI];
-    auto load_scales = [&](int kt) {  // zeros behind a row's end
+    typedef uint32_t any16 __attribute__((ext_vector_type(4), aligned(1)));
+    u32x4 sv[SL];
+    auto load_scales = [&](int b0) {  // of 16 blocks, zeros behind a row's end
 #pragma unroll
-        for (int u = 0; u < SL; ++u)
+        for (int u = 0; u < SL; ++u) {
+            if (b0 + 16 <= a.nb) {
+                sv[u] = *reinterpret_cast<const any16*>(sp[u] + b0);
+                continue;
+            }
 #pragma unroll
-            for (int s = 0; s < KI; ++s) {
-                const int b = PB * kt + 4 * s;
+            for (int s = 0; s < 4; ++s) {
+                const int b = b0 + 4 * s;
+                sv[u][s] = 0;
                 if (b + 4 <= a.nb) {
                     sv[u][s] = *reinterpret_cast<const any4*>(sp[u] + b);
                 } else {
-                    sv[u][s] = 0;
 #pragma unroll
                     for (int j = 0; j < 3; ++j)
                         if (b + j < a.nb) sv[u][s] |= (uint32_t)sp[u][b + j] << (8 * j);
                 }
             }
+        }
     };
     auto put_scales = [&](uint32_t* d) {
 #pragma unroll
         for (int u = 0; u < SL; ++u)
             if (tid + u * NTH < R) {
 #pragma unroll
-                for (int s = 0; s < KI; ++s) d[s * R + tid + u * NTH] = sv[u][s];
+                for (int s = 0; s < 4; ++s) d[s * RS + scale_at(tid + u * NTH)] = sv[u][s];
             }
     };
 
@@ -374,7 +409,7 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void mx_tile_kernel(MxLinArgs a)
     tile_begin<MI, NI, OMX>(a, n0 + wn * NI * 16, g, acc);
     const int xrow = wm * MI * 16 + c, wrow = BM + wn * NI * 16;
     auto compute = [&](const char* d, const uint32_t* ds) {
-        const uint8_t* sc = reinterpret_cast<const uint8_t*>(ds);
+        const uint8_t* scale = reinterpret_cast<const uint8_t*>(ds) + g;
 #pragma unroll
         for (int s = 0; s < KI; ++s) {
             if (s > 0) __builtin_amdgcn_sched_barrier(0);  // the second instruction's operands not beside the first's
@@ -385,13 +420,13 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void mx_tile_kernel(MxLinArgs a)
             for (int mi = 0; mi < MI; ++mi) {
                 const int r = xrow + mi * 16;
                 xf[mi] = *reinterpret_cast<const u32x4*>(d + r * SB + piece);
-                xs[mi] = sc[(s * R + r) * 4 + g];
+                xs[mi] = scale[(s * RS + scale_at(r)) * 4];
             }
 #pragma unroll
             for (int ni = 0; ni < NI; ++ni) {
                 const int r = wrow + tile_col<OMX>(ni, c);
                 wf[ni] = *reinterpret_cast<const u32x4*>(d + r * SB + piece);
-                ws[ni] = sc[(s * R + r) * 4 + g];
+                ws[ni] = scale[(s * RS + scale_at(r)) * 4];
             }
 #pragma unroll
             for (int mi = 0; mi < MI; ++mi)
@@ -399,33 +434,41 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void mx_tile_kernel(MxLinArgs a)
                 for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = mx_mma(wf[ni], ws[ni], xf[mi], xs[mi], acc[mi][ni]);
         }
     };
-    // Step kt sits in d, the next one goes to dn, which held the one before; separate objects, and the loop unrolled by two, so that
-    // the compiler sees that loads in flight into one do not touch the other.
-    auto step = [&](int kt, char* d, uint32_t* ds, char* dn) {
-        put_scales(ds);  // waits for them; the buffer was last read two steps ago
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        wait_loads();
-        lds_barrier();   // every wave's loads and scales are there, and none still reads dn
-        if (kt + 1 < steps) {
-            load(kt + 1, dn);
-            load_scales(kt + 1);
+    // Step kt sits in d, the next one goes to dn, which held the one before; separate objects, and the loop unrolled, so that
+    // the compiler sees that loads in flight into one do not touch the other.  I: the step's place in its group of scales, whose
+    // first step puts them there and sends for the next ones.
+    constexpr int GS = 4 / KI;  // steps of a group
+    auto step = [&](int kt, auto place, char* d, char* dn) {
+        constexpr int I = decltype(place)::value;
+        uint32_t* const ds = sc[(kt / GS) & 1];
+        if constexpr (I == 0) {
+            put_scales(ds);  // waits for them; this half was last read a group ago
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        compute(d, ds);
+        wait_loads();
+        lds_barrier();  // every wave's loads and scales are there, and none still reads dn
+        if (kt + 1 < steps) load(kt + 1, dn);
+        if (I == 0 && kt + GS < steps) load_scales((kt + GS) * PB);
+        compute(d, ds + I * KI * RS);
     };
-    for (int kt = 0; kt < steps; kt += 2) {
-        step(kt, s0, c0, s1);
-        if (kt + 1 < steps) step(kt + 1, s1, c1, s0);
+    for (int kt = 0; kt < steps; kt += GS) {
+        step(kt, std::integral_constant<int, 0>(), s0, s1);
+        if (kt + 1 < steps) step(kt + 1, std::integral_constant<int, 1>(), s1, s0);
+        if constexpr (GS == 4) {
+            if (kt + 2 < steps) step(kt + 2, std::integral_constant<int, 2>(), s0, s1);
+            if (kt + 3 < steps) step(kt + 3, std::integral_constant<int, 3>(), s1, s0);
+        }
     }
 
     const int64_t m = m0 + wm * MI * 16;
     const int n = n0 + wn * NI * 16;
     if constexpr (OMX) {
-        tile_finish_mx<MI, ACT>(a, m, n, g, c, acc);
+        tile_finish_mx<MI, KIND, true>(a, m, n, g, c, acc);
     } else {
         // the buffer that the last step did not use: no wave reads it any more
         MxLinArgs rest = a;
         rest.bias = nullptr;
-        tile_finish<MI, NI, ACT, NT>(rest, m, n, lane, ((steps & 1) != 0 ? s1 : s0) + w * NI * 1024, acc);
+        tile_finish<MI, NI, KIND, NT>(rest, m, n, lane, ((steps & 1) != 0 ? s1 : s0) + w * NI * 1024, acc);
     }
 }
 
@@ -444,7 +487,7 @@ __device__ __forceinline__ int wide_key_c(int c) {  // of the row of w that lane
     return FS == 128 ? (c & 1) << 2 | ((c >> 2) & 1) << 1 | ((c >> 1) & 1) : ((c >> 1) & 1) << 2 | (c & 1) << 1 | ((c >> 2) & 1);
 }
 
-template <int XT, int WM, int WN, int MI, int NI, int FS, int NT, bool ACT, bool OMX>
+template <int XT, int WM, int WN, int MI, int NI, int FS, int NT, int KIND, bool OMX>
 __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a) {
     constexpr int NW = WM * WN, NTH = NW * 64, BM = WM * MI * 16, BN = WN * NI * 16, P = mx_parts(XT), Q = XT == F32 ? 2 : 1;
     constexpr int S = XT == F32 ? 4 : 2, PR = FS / 8, BR = FS / 32;     // pieces and blocks of a row's step
@@ -580,13 +623,13 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
     const int64_t m = m0 + wm * MI * 16;
     const int n = n0 + wn * NI * 16;
     if constexpr (OMX) {
-        tile_finish_mx<MI, ACT>(a, m, n, g, c, acc);
+        tile_finish_mx<MI, KIND, XT != F32>(a, m, n, g, c, acc);
     } else {
         // a wave's own part of a buffer: the last step's other one, which nothing reads or, behind a cut step, writes any more
         MxLinArgs rest = a;
         rest.bias = nullptr;
         ready();
-        tile_finish<MI, NI, ACT, NT>(rest, m, n, lane, lds[steps & 1] + w * NI * 1024, acc);
+        tile_finish<MI, NI, KIND, NT>(rest, m, n, lane, lds[steps & 1] + w * NI * 1024, acc);
     }
 }
 
@@ -716,7 +759,7 @@ __global__ __launch_bounds__(1024) void mx_strip_kernel(MxLinArgs a) {
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = s[i / 4][i % 4];
-            finish8<true, OMX, 0>(a, m, n, v, bias);
+            finish8<XT != F32, OMX>(a, m, n, v, bias);
         } else {
             const int n = (int)min<int64_t>(p0 + 4 * g, a.N);
             Bias<4> bias;
@@ -897,7 +940,7 @@ __global__ __launch_bounds__(1024) void mx_token_kernel(MxLinArgs a) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = acc[i / 4][i % 4];
-    finish8<true, OMX, 0>(a, c, n, v, bias);
+    finish8<XT != F32, OMX>(a, c, n, v, bias);
 }
 
 template <int XT, int PW, int R, bool OMX>
@@ -922,15 +965,17 @@ int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
     const int64_t tiles = ceil_div(a.M, BM) * a.ntiles;
     if (!grid_fits(tiles, WM * WN * 64)) return set_error(MBRT_E_SHAPE, "mbrt_mx_linear: too many tiles");
     const dim3 grid((unsigned)tiles), block(WM * WN * 64);
-    auto launch = [&](auto act) {
-        constexpr bool ACT = decltype(act)::value;
+    auto launch = [&](auto kind) {
+        constexpr int KIND = decltype(kind)::value;
         if constexpr (XT == MXFP4)
-            hipLaunchKernelGGL((mx_tile_kernel<WM, WN, MI, NI, SB, OCC, NT, ACT, OMX>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((mx_tile_kernel<WM, WN, MI, NI, SB, OCC, NT, KIND, OMX>), grid, block, 0, st, a);
         else
-            hipLaunchKernelGGL((mx_wide_tile_kernel<XT, WM, WN, MI, NI, SB, NT, ACT, OMX>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((mx_wide_tile_kernel<XT, WM, WN, MI, NI, SB, NT, KIND, OMX>), grid, block, 0, st, a);
     };
-    if (a.act != MBRT_ACT_NONE) launch(std::integral_constant<bool, true>());
-    else launch(std::integral_constant<bool, false>());
+    const bool gelu = a.act == MBRT_ACT_GELU_REF || a.act == MBRT_ACT_GELU_STD;
+    if (a.act == MBRT_ACT_NONE) launch(std::integral_constant<int, kActNone>());
+    else if (XT != F32 && gelu && a.short_act != 0) launch(std::integral_constant<int, XT != F32 ? kActGelu : kActAny>());
+    else launch(std::integral_constant<int, kActAny>());
     return MBRT_OK;
 }
 
@@ -993,6 +1038,10 @@ int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
         } else {
             if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, 128, 4, 0, false>(a, st);
             const bool nt = aligned(a.out, 64) && a.os * dt_size(a.odt) % 64 == 0;
+            // Long K: 256 x 256, which asks L2 and LDS for half as much per product, where there are nearly enough of them for the
+            // CUs ([4096, 4096] -> 4096 50.5 and 39.9 us; [6055, 1536] -> 1536, 144 tiles, 18.9 and 18.0; [48060, 1536] -> 384 29 and 34).
+            if (a.nb >= 64 && 4 * ceil_div(a.M, 256) * ceil_div(a.N, 256) >= 3 * cus)
+                return nt ? launch_mx_tile<XT, 2, 4, 8, 4, 128, 2, 2, false>(a, st) : launch_mx_tile<XT, 2, 4, 8, 4, 128, 2, 0, false>(a, st);
             if (small_steps)
                 return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 0, false>(a, st);
             return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 128, 2, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 128, 2, 0, false>(a, st);
