@@ -2,7 +2,11 @@
 //
 // A lane has 8 features of a row: 16 bytes of a 2-byte type, two loads of an f32.  The four lanes of a block agree on its
 // scale by two DPP steps, each writes a dword of codes and the first of them the scale.  Both directions move 2.5 (or 4.5)
-// bytes per feature and compute next to nothing: memory bounds them, so every lane has kUnits pieces under way.
+// bytes per feature and compute next to nothing: memory bounds them.  bf16 [48060, 1536], 187 MB each way, in us with 2, 4
+// and 8 pieces under way per lane: quantise 34, 36 and 39, back 36, 37 and 37 (a copy of as many bytes: 37).  A large x is
+// read past the caches: quantise 31, and there and back 62 rather than 72, since the codes are still in a cache for the
+// second call.  Rows that are not whole 16-byte pieces lose alone what they win in a row of calls: bf16 [12421, 2013]
+// 14.7 -> 17.5 alone, 32.6 -> 29.2 there and back.
 #include "abi_common.hpp"
 #include "mx.hpp"
 #include "overlap.hpp"
@@ -12,7 +16,7 @@
 namespace mbrt {
 namespace {
 
-constexpr int kThreads = 256, kUnits = 4;
+constexpr int kThreads = 256, kUnits = 2;
 
 struct MxRows {
     char* codes;
@@ -32,12 +36,12 @@ struct Raw8 {
 #pragma unroll
         for (auto& q : w) q = u32x4{0u, 0u, 0u, 0u};
     }
-    template <int A>
+    template <int A, int NT>
     __device__ __forceinline__ void load(const char* p) {
 #pragma unroll
         for (int q = 0; q < (DT == F32 ? 2 : 1); ++q) {
-            if constexpr (A == 16) w[q] = *reinterpret_cast<const u32x4*>(p + 16 * q);
-            else w[q] = ld_any<0, A>(p + 16 * q);
+            if constexpr (A == 16) w[q] = gld<NT>(reinterpret_cast<const u32x4*>(p + 16 * q));
+            else w[q] = ld_any<NT, A>(p + 16 * q);
         }
     }
     // n < 8 features, zeros behind them
@@ -69,8 +73,8 @@ struct Raw8 {
     }
 };
 
-// A: 16 where every piece of x is aligned to 16 bytes and whole, else x's elements.
-template <int DT, int A>
+// A: 16 where every piece of x is aligned to 16 bytes and whole, else x's elements.  NT: x is read past the caches.
+template <int DT, int A, int NT>
 __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(MxRows a) {
     constexpr int S = DT == F32 ? 4 : 2;
     Raw8<DT> v[kUnits];
@@ -81,7 +85,7 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(MxRows a) {
         fdivmod(min(i, (uint32_t)a.total - 1), a.per_row, row[u], place[u]);
         const char* p = a.x + row[u] * a.xs + (int64_t)place[u] * (8 * S);
         const int left = a.K - 8 * (int)place[u];
-        if (left >= 8) v[u].template load<A>(p);
+        if (left >= 8) v[u].template load<A, NT>(p);
         else if (A == 16) v[u].clear();
         else v[u].load_some(p, left);
     }
@@ -183,12 +187,15 @@ int mx_convert(const char* op, bool to_codes, char* x, int dt, int64_t xs, char*
     a.pieces = (int)(4 * blocks);
     a.per_row = make_fastdiv((uint32_t)a.pieces);
     const bool al = aligned(x, 16) && a.xs % 16 == 0 && K % 8 == 0;
+    const bool cold = cold_input(rows * K * es) != 0;
     with_dt(dt, [&](auto t) {
         constexpr int DT = decltype(t)::value, S = DT == F32 ? 4 : 2;
         for_row_ranges(a, es, [&](const MxRows& r, dim3 grid) {
             if (to_codes) {
-                if (al) hipLaunchKernelGGL((mx_quantize_kernel<DT, 16>), grid, dim3(kThreads), 0, st, r);
-                else hipLaunchKernelGGL((mx_quantize_kernel<DT, S>), grid, dim3(kThreads), 0, st, r);
+                if (al && cold) hipLaunchKernelGGL((mx_quantize_kernel<DT, 16, 1>), grid, dim3(kThreads), 0, st, r);
+                else if (al) hipLaunchKernelGGL((mx_quantize_kernel<DT, 16, 0>), grid, dim3(kThreads), 0, st, r);
+                else if (cold) hipLaunchKernelGGL((mx_quantize_kernel<DT, S, 1>), grid, dim3(kThreads), 0, st, r);
+                else hipLaunchKernelGGL((mx_quantize_kernel<DT, S, 0>), grid, dim3(kThreads), 0, st, r);
             } else {
                 if (al) hipLaunchKernelGGL((mx_dequantize_kernel<DT, 16>), grid, dim3(kThreads), 0, st, r);
                 else hipLaunchKernelGGL((mx_dequantize_kernel<DT, S>), grid, dim3(kThreads), 0, st, r);
