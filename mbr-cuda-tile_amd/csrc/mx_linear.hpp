@@ -22,7 +22,6 @@ struct MxLinArgs : LinArgs {  // w, and x and out where they are in 4 bits: code
     uint8_t* osc;
     int64_t wss, xss, oss;    // row strides of the scales
     int nb;                   // blocks of a row of w
-    int rows_outer;           // strips: groups of x rows are the slower index
 };
 
 // x of dtype XT (MXFP4, F32, F16, BF16).  Instantiated in a source file per dtype.
@@ -76,9 +75,9 @@ __device__ __forceinline__ void to_parts(const u32x4 (&raw)[XT == F32 ? 2 : 1], 
     }
 }
 
-// x Phi(x) = x / (1 + exp(-p(x))) with p the odd polynomial of degree 13 that comes nearest to log(Phi(x) / Phi(-x)) up to 6.5,
-// weighted so that a value is off by at most 5.4e-6, and by at most 2^-7 of itself down to x = -6.3, where it is -9e-10: far within
-// the two significant bits of results in 4 bits, at 11 operations for gelu_short's 16.
+// x Phi(x) = x / (1 + exp(-p(x))) with p the odd polynomial of degree 13 that comes nearest to log(Phi(x) / Phi(-x)) up to 6.5: a
+// value is off by at most 5.5e-6, and by at most 2^-6.9 of itself down to x = -5 (2^-5.6 down to -6.5, where it is -3e-10): far
+// within the two significant bits of results in 4 bits, at 11 operations for gelu_short's 16.
 __device__ __forceinline__ float gelu_logistic(float x) {
     constexpr float L = -1.44269504088896341f;
     const float x2 = x * x;
@@ -652,14 +651,7 @@ __global__ __launch_bounds__(1024) void mx_strip_kernel(MxLinArgs a) {
     uint32_t piece, kw, sb, group;
     fdivmod((uint32_t)wv, a.splits, piece, kw);
     const int ks = (int)kw;
-    // strips (of columns) of a block are neighbours; a.groups counts the faster index
-    if (a.rows_outer) {
-        uint32_t s;
-        fdivmod(blockIdx.x, a.groups, group, s);
-        sb = s;
-    } else {
-        fdivmod(blockIdx.x, a.groups, sb, group);
-    }
+    fdivmod(blockIdx.x, a.groups, sb, group);  // the strips of a block are neighbours
     const int64_t p0 = ((int64_t)sb * a.per_block + piece) * 16 * PW, q0 = (int64_t)group * 16 * R;
     const char* wb[PW];
     const uint8_t* ws[PW];
@@ -796,17 +788,10 @@ __global__ __launch_bounds__(1024) void mx_strip_kernel(MxLinArgs a) {
 }
 
 // ---- few rows against many weights -----------------------------------------------------------------
-// At most 16 rows of x: what takes time is reading w.  A wave takes 32 columns, columns dealt so that a lane ends with 8 in a
-// row; `split` waves share the K of one such strip, 16 blocks at a time in turn, the scales of a row's 16 in one load.  x stands in LDS, as bf16 parts or as its codes, zeros up to
-// whole turns, so that w alone waits for memory: 8 KB a wave, and the next turn's as many while one is computed.
-// [1, 4096] bf16 -> 16384: 13.3 us in strips, which read x again for every 16 columns.
-#ifndef MX_TOKEN_BLOCKS
-#define MX_TOKEN_BLOCKS 65536
-#define MX_TOKEN_WAVES 8
-#endif
-#ifndef MX_TOKEN_NT
-#define MX_TOKEN_NT 0
-#endif
+// At most 16 rows of x: what takes time is reading w.  A wave takes 32 columns, dealt so that a lane ends with 8 in a row;
+// `split` waves share the K of one such strip, 16 blocks at a time in turn, the scales of a row's 16 in one load.  x stands in
+// LDS, as bf16 parts or as its codes, zeros up to whole turns, so that w alone waits for memory: 8 KB a wave, and the next
+// turn's as many while one is computed.  Past the caches w comes no faster ([1, 4096] bf16 -> 16384: 10.6 us either way).
 template <int XT>
 struct TokenX {  // bytes of a row of x in LDS, for a number of blocks
     static constexpr int kBlock = XT == MXFP4 ? 16 : 64;  // a block's codes, or one part of its values
@@ -842,7 +827,7 @@ __global__ __launch_bounds__(1024) void mx_token_kernel(MxLinArgs a) {
         for (int p = 0; p < PW; ++p) {
 #pragma unroll
             for (int s = 0; s < 4; ++s)
-                d.w[p][s] = gld<MX_TOKEN_NT>(reinterpret_cast<const u32x4*>(wb[p] + 16 * (int64_t)min(16 * t + 4 * s + g, a.nb - 1)));
+                d.w[p][s] = *reinterpret_cast<const u32x4*>(wb[p] + 16 * (int64_t)min(16 * t + 4 * s + g, a.nb - 1));
             if (16 * t + 16 <= a.nb) {
                 d.scales[p] = *reinterpret_cast<const any16*>(ws[p] + 16 * t);
             } else {
@@ -982,40 +967,52 @@ int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
 template <int XT, bool OMX>
 int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
     const int64_t cus = cu_count();
-    const int64_t cols = ceil_div(a.N, 16);
-    const int64_t turns = ceil_div(a.nb, 16), token_lds = std::max(a.M * TokenX<XT>::row(16 * turns), int64_t(0));
-    if (a.M <= 16 && (int64_t)a.N * a.nb >= MX_TOKEN_BLOCKS && token_lds <= (int64_t(1) << 16)) {
-        const int64_t strips = ceil_div(a.N, 32), room = std::max<int64_t>(1, std::min<int64_t>(16, MX_TOKEN_WAVES * cus / strips));
-        a.split = (int)ceil_div(turns, ceil_div(turns, room));
-        const size_t lds = (size_t)std::max<int64_t>(token_lds, a.split > 1 ? a.split * 2048 : 0);
-        hipLaunchKernelGGL((mx_token_kernel<XT, OMX>), dim3((unsigned)strips), dim3(64 * a.split), lds, st, a);
+    const int64_t cols = ceil_div(a.N, 16), M = a.M, N = a.N;
+    // A few rows of x and a strip of 32 columns or more for every CU: x through LDS.  us of this and of strips, 16 waves a CU (8: up to
+    // 1.6 more), K -> N: bf16 [1, 4096] -> 16384 10.6 and 13.9, [1, 1536] -> 8192 5.1 and 4.9, [4, 1536] -> 8192 6.3 and 5.3, [4, 4096]
+    // -> 16384 12.6 and 16.3; f32 [1, 1536] -> 8192 6.2 and 8.2, [4, 1024] -> 32768 10.5 and 15.9, [8, 1024] -> 32768 19.3 and 16.4;
+    // 4 bits [1, 1536] -> 8192 4.4 and 4.9, [16, 4096] -> 16384 10.6 and 17.3.  With half as many strips as CUs it loses: bf16 and 4
+    // bits [1, 4096] -> 4096 7.2 and 6.2, 6.0 and 5.7.
+    const int64_t strips32 = ceil_div(N, 32), turns16 = ceil_div(a.nb, 16);
+    if (M <= (XT == MXFP4 ? 16 : 4) && strips32 >= cus * (XT == BF16 ? std::min<int64_t>(M, 2) : 1) &&
+        M * TokenX<XT>::row(16 * turns16) <= (int64_t(1) << 16)) {
+        const int64_t room = std::max<int64_t>(1, std::min<int64_t>(16, 16 * cus / strips32));
+        a.split = (int)ceil_div(turns16, ceil_div(turns16, room));
+        const size_t lds = (size_t)std::max<int64_t>(M * TokenX<XT>::row(16 * turns16), a.split > 1 ? a.split * 2048 : 0);
+        hipLaunchKernelGGL((mx_token_kernel<XT, OMX>), dim3((unsigned)strips32), dim3(64 * a.split), lds, st, a);
         return MBRT_OK;
     }
-    // 32-bit offsets within a tile
-    const bool far = XT == MXFP4 && (a.xs >= (int64_t(1) << 22) || a.ws >= (int64_t(1) << 22));
-    if (far || ceil_div(std::max(a.M, (int64_t)a.N), 16) * ceil_div(std::min(a.M, (int64_t)a.N), 64) <= cus ||
-        std::min(a.M, (int64_t)a.N) <= 16) {
+    // Strips for what gives the CUs no work as tiles, and for 16 rows (a tile has four times as many).  us of strips and of 64 x 64
+    // tiles for bf16 and for 4 bits: [256, 1536] -> 384 6.3 and 10.6, 4.5 and 4.8; [32, 4096] -> 4096 13.1 and 21.9, 9.3 and 10.7;
+    // [256, 384] -> 1536 6.0 and 5.2, 4.0 and 3.8; [512, 384] -> 1536 7.9 and 5.5, 5.1 and 3.9; [1, 8192] -> 8192 13.8 and 40, 12.7
+    // and 18.1.  Two blocks of rows to a wave where that leaves a wave for every CU ([64, 1536] -> 1536 7.0 and 6.6, 5.5 and 5.1;
+    // [24, 384] -> 1536 3.0 and 3.3, 2.9 and 3.0); not f32, whose parts fill the registers (10.1 and 12.5).
+    const bool far = XT == MXFP4 && (a.xs >= (int64_t(1) << 22) || a.ws >= (int64_t(1) << 22));  // 32-bit offsets in a tile
+    if (far || M <= 16 || ceil_div(std::max(M, N), 16) * ceil_div(std::min(M, N), 64) <= cus) {
         constexpr int PW = OMX ? 2 : 1;
         const int64_t strips = ceil_div(cols, PW);
-        int R = a.M <= 16 ? 1 : a.M <= 32 || XT == F32 ? 2 : 4;  // (f32 rows in three parts: no registers for more)
-        while (R > 1 && strips * ceil_div(a.M, 8 * R) <= cus) R /= 2;
-        const int64_t groups = ceil_div(a.M, 16 * R), turns = ceil_div(a.nb, 4);
+        const int R = XT != F32 && strips * ceil_div(M, 16) > cus && M > 16 ? 2 : 1;
+        const int64_t groups = ceil_div(M, 16 * R), turns = ceil_div(a.nb, 4);
         const int64_t room = std::max<int64_t>(1, std::min<int64_t>({16, 64 / (R * PW), 8 * cus / (strips * groups)}));
         a.split = (int)std::max<int64_t>(1, ceil_div(turns, ceil_div(turns, room)));
         a.splits = make_fastdiv((uint32_t)a.split);
         a.per_block = std::max(1, 4 / a.split);
-        const int64_t sblocks = ceil_div(strips, a.per_block), blocks = sblocks * groups;
-        a.rows_outer = a.M > a.N;
-        a.groups = make_fastdiv((uint32_t)(a.rows_outer ? sblocks : groups));
+        const int64_t blocks = ceil_div(strips, a.per_block) * groups;
+        a.groups = make_fastdiv((uint32_t)groups);
         const unsigned threads = a.per_block * a.split * 64;
         const size_t lds = a.split == 1 ? 0 : (size_t)a.per_block * a.split * R * PW * 1024;
         if (!grid_fits(blocks, threads) || groups >= (int64_t(1) << 31)) return set_error(MBRT_E_SHAPE, "mbrt_mx_linear: too many rows");
         if (R == 1) launch_mx_strip<XT, PW, 1, OMX>(a, align, (unsigned)blocks, threads, lds, st);
-        else if (R == 2) launch_mx_strip<XT, PW, 2, OMX>(a, align, (unsigned)blocks, threads, lds, st);
-        else if constexpr (XT != F32) launch_mx_strip<XT, PW, 4, OMX>(a, align, (unsigned)blocks, threads, lds, st);
+        else if constexpr (XT != F32) launch_mx_strip<XT, PW, 2, OMX>(a, align, (unsigned)blocks, threads, lds, st);
         return MBRT_OK;
     }
-    const bool big = XT != F32 && std::min(a.M, (int64_t)a.N) > 64 && ceil_div(a.M, 128) * ceil_div(a.N, 128) >= cus;
+    // Tiles of 64 x 64 (4-bit results: 64 x 128) or 128 x 128.  us of both: 16- and 32-bit x, where two small ones fill a CU's LDS, bf16
+    // [2048, 1536] -> 1536, 192 large tiles, 24.7 and 20.7, [4096, 1536] -> 384, 96, 15.9 and 19.4; 4-bit x [2048, 1536] -> 1536 8.7
+    // and 10.9, [4096, 384] -> 1536, 384 tiles, 9.8 and 7.8; both in 4 bits [4096, 384] -> 1536 8.0 and 9.6, [4096, 1536] -> 1536, 384,
+    // 14.6 and 14.4, [6144, 1536] -> 1536, 576, 22.9 and 19.7.
+    const int64_t tiles = ceil_div(M, 128) * ceil_div(N, 128);
+    const bool big = XT != F32 && std::min(M, N) > 64 && (XT != MXFP4 ? 2 * tiles >= cus : OMX ? tiles >= 2 * cus : tiles >= cus);
+    const bool nt = !OMX && aligned(a.out, 64) && a.os * dt_size(a.odt) % 64 == 0;
     if constexpr (XT != MXFP4) {
         constexpr int FS = XT == BF16 ? 128 : 64;
         if constexpr (OMX) {
@@ -1023,29 +1020,23 @@ int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
             if constexpr (XT != F32) return launch_mx_tile<XT, 4, 1, 2, 8, 64, 1, 0, true>(a, st);
         } else {
             if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, FS, 1, 0, false>(a, st);
-            if constexpr (XT != F32) {
-                const bool nt = aligned(a.out, 64) && a.os * dt_size(a.odt) % 64 == 0;
+            if constexpr (XT != F32)
                 return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 1, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 1, 0, false>(a, st);
-            }
         }
         return MBRT_OK;
+    } else if constexpr (OMX) {
+        // steps of 64 bytes leave room for three workgroups to a CU, of 128 for two ([24000, 1536] -> 1536 55 and 57 us)
+        return big ? launch_mx_tile<XT, 4, 1, 2, 8, 64, 3, 0, true>(a, st) : launch_mx_tile<XT, 4, 1, 1, 8, 64, 3, 0, true>(a, st);
     } else {
-        // short K in steps of 64 bytes, whose buffers leave room for three workgroups to a CU
-        const bool small_steps = a.nb <= 32;
-        if constexpr (OMX) {
-            if (!big) return launch_mx_tile<XT, 4, 1, 1, 8, 64, 3, 0, true>(a, st);
-            return small_steps ? launch_mx_tile<XT, 4, 1, 2, 8, 64, 3, 0, true>(a, st) : launch_mx_tile<XT, 4, 1, 2, 8, 128, 2, 0, true>(a, st);
-        } else {
-            if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, 128, 4, 0, false>(a, st);
-            const bool nt = aligned(a.out, 64) && a.os * dt_size(a.odt) % 64 == 0;
-            // Long K: 256 x 256, which asks L2 and LDS for half as much per product, where there are nearly enough of them for the
-            // CUs ([4096, 4096] -> 4096 50.5 and 39.9 us; [6055, 1536] -> 1536, 144 tiles, 18.9 and 18.0; [48060, 1536] -> 384 29 and 34).
-            if (a.nb >= 64 && 4 * ceil_div(a.M, 256) * ceil_div(a.N, 256) >= 3 * cus)
-                return nt ? launch_mx_tile<XT, 2, 4, 8, 4, 128, 2, 2, false>(a, st) : launch_mx_tile<XT, 2, 4, 8, 4, 128, 2, 0, false>(a, st);
-            if (small_steps)
-                return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 0, false>(a, st);
-            return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 128, 2, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 128, 2, 0, false>(a, st);
-        }
+        if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, 128, 4, 0, false>(a, st);
+        // Long K: 256 x 256, which asks L2 and LDS for half as much per product, if four fifths of what the CUs then compute is wanted.  us
+        // of 128 x 128 and of these: [4096, 4096] -> 4096, all of it wanted, 62 and 42; [24000, 1536] -> 1152, 83 %, 41 and 37, -> 1536,
+        // 73 %, 48 and 55; [48060, 1536] -> 1536, 87 %, 92 and 93, -> 384, 55 %, 29 and 36; [48060, 384] -> 1536 41 and 54.
+        const int64_t tiles256 = ceil_div(M, 256) * ceil_div(N, 256);
+        if (a.nb >= 48 && 5.0 * (double)M * (double)N >= 4.0 * 65536.0 * (double)(ceil_div(tiles256, cus) * cus))
+            return nt ? launch_mx_tile<XT, 2, 4, 8, 4, 128, 2, 2, false>(a, st) : launch_mx_tile<XT, 2, 4, 8, 4, 128, 2, 0, false>(a, st);
+        // (steps of 128 bytes: [48060, 384] -> 1536 53 for 41, [24000, 4096] -> 1536 105 for 114)
+        return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 3, 0, false>(a, st);
     }
 }
 

@@ -88,6 +88,19 @@ def test_short_operands(dev, rows, k, n, x):
     _case(dev, rows, k, n, x, res=BF16, seed=rows)
 
 
+@pytest.mark.parametrize("x", [MX, F16, BF16, F32])
+@pytest.mark.parametrize("rows,k,n", [(1, 100, 16400), (2, 545, 16390), (4, 1290, 16411), (16, 513, 8200), (1, 9, 40001)])
+def test_few_rows_against_many_weights(dev, rows, k, n, x):
+    _case(dev, rows, k, n, x, bias=F16, res=F32, seed=n)
+    _case(dev, rows, k, n, x, MX, act=1, seed=n + 9)
+
+
+@pytest.mark.parametrize("out,res", [(BF16, BF16), (F32, None)])
+@pytest.mark.parametrize("rows,k,n", [(4090, 1540, 4001), (3900, 1633, 4096)])
+def test_long_k(dev, rows, k, n, out, res):
+    _case(dev, rows, k, n, MX, out, act=2 if res else 0, res=res, seed=k)
+
+
 @pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("x,out", [(MX, BF16), (MX, F32), (F32, F32), (BF16, F16), (F16, F32)])
 @pytest.mark.parametrize("rows,k,n", [(3, 96, 70), (150, 96, 70), (90, 96, 8)])
