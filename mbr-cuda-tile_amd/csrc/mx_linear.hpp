@@ -75,19 +75,19 @@ __device__ __forceinline__ void to_parts(const u32x4 (&raw)[XT == F32 ? 2 : 1], 
     }
 }
 
-// x Phi(x) = x / (1 + exp(-p(x))) with p the odd polynomial of degree 13 that comes nearest to log(Phi(x) / Phi(-x)) up to 6.5: a
-// value is off by at most 5.5e-6, and by at most 2^-6.9 of itself down to x = -5 (2^-5.6 down to -6.5, where it is -3e-10): far
-// within the two significant bits of results in 4 bits, at 11 operations for gelu_short's 16.
-__device__ __forceinline__ float gelu_logistic(float x) {
-    constexpr float L = -1.44269504088896341f;
-    const float x2 = x * x;
-    float p = fmaf(7.40792158e-10f * L, x2, -9.01705128e-08f * L);
-    p = fmaf(p, x2, 4.01454603e-06f * L);
-    p = fmaf(p, x2, -7.20723898e-05f * L);
-    p = fmaf(p, x2, -2.37610013e-04f * L);
-    p = fmaf(p, x2, 0.0729833124f * L);
-    p = fmaf(p, x2, 1.59560622f * L);
-    return x * fast_rcp(1.0f + __builtin_amdgcn_exp2f(x * p));
+// x Phi(s x) = max(x, 0) - |x| 2^p(|x|), with p the polynomial of degree 5 that comes nearest to log2 Phi(-s |x|) up to 6.5 / s, where
+// 2^p is 4e-11 and beyond which p keeps falling: a value is off by at most 4.7e-6, and by at most 2^-7.1 of itself down to there,
+// far within the two significant bits of results in 4 bits, at 7 operations and an exp2 for gelu_short's 16 and two.
+// s: sqrt 2 in the reference's form (REF), 1 in the other.
+template <bool REF>
+__device__ __forceinline__ float gelu_tail(float x) {
+    const float t = __builtin_fabsf(x);
+    float p = REF ? fmaf(-0.00161456782f, t, 0.0223558452f) : fmaf(-0.000285417947f, t, 0.0055889613f);
+    p = fmaf(p, t, REF ? -0.135041833f : -0.0477444939f);
+    p = fmaf(p, t, REF ? -0.929357886f : -0.464678943f);
+    p = fmaf(p, t, REF ? -1.62438309f : -1.14861226f);
+    p = fmaf(p, t, -1.00034082f);
+    return fmaf(-t, __builtin_amdgcn_exp2f(p), fmaxf(x, 0.0f));
 }
 
 // What a kernel applies to its sums: nothing, GELU in a form for short results, or any function.  What stands behind the sums of a
@@ -95,8 +95,7 @@ __device__ __forceinline__ float gelu_logistic(float x) {
 // values takes [17916, 1536] -> 384 from 12.8 to 28.6 us with GELU.
 enum MxAct { kActNone = 0, kActGelu = 1, kActAny = 2 };
 
-// The reference's GELU, x Phi(sqrt 2 x), is the other's at sqrt 2 x by 1 / sqrt 2.  OMX: for results in 4 bits.  SHORT: the short
-// forms of the others.
+// OMX: for results in 4 bits.  SHORT: the short forms of the others.
 template <int KIND, bool OMX, bool SHORT, int NV>
 __device__ __forceinline__ void activate_mx(const MxLinArgs& a, float (&v)[NV]) {
     if constexpr (KIND == kActGelu) {
@@ -104,10 +103,10 @@ __device__ __forceinline__ void activate_mx(const MxLinArgs& a, float (&v)[NV]) 
         if constexpr (OMX) {
             if (ref) {
 #pragma unroll
-                for (int i = 0; i < NV; ++i) v[i] = 0.70710678118654752f * gelu_logistic(1.41421356237309505f * v[i]);
+                for (int i = 0; i < NV; ++i) v[i] = gelu_tail<true>(v[i]);
             } else {
 #pragma unroll
-                for (int i = 0; i < NV; ++i) v[i] = gelu_logistic(v[i]);
+                for (int i = 0; i < NV; ++i) v[i] = gelu_tail<false>(v[i]);
             }
         } else {
             const float s = ref ? 1.0f : 0.70710678118654752440f;
