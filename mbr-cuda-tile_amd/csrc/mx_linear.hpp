@@ -87,7 +87,7 @@ __device__ __forceinline__ float gelu_tail(float x) {
     p = fmaf(p, t, REF ? -0.929357886f : -0.464678943f);
     p = fmaf(p, t, REF ? -1.62438309f : -1.14861226f);
     p = fmaf(p, t, -1.00034082f);
-    return fmaf(-t, __builtin_amdgcn_exp2f(p), fmaxf(x, 0.0f));
+    return fmaf(-t, __builtin_amdgcn_exp2f(p), __builtin_amdgcn_fmed3f(x, 0.0f, __builtin_inff()));  // fmaxf would quiet x first
 }
 
 // What a kernel applies to its sums: nothing, GELU in a form for short results, or any function.  What stands behind the sums of a
@@ -241,15 +241,12 @@ __device__ __forceinline__ void tile_finish_mx(const MxLinArgs& a, int64_t m0, i
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = n + i < a.N ? v[i] : 0.0f;
         }
-        // the largest of them, and whether one is NaN: an operation each for two values
+        // the largest of them, or NaN if one is: an operation for two values
         float top = 0.0f;
-        bool nan = false;
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-            top = fmaxf(fmaxf(top, __builtin_fabsf(v[i])), __builtin_fabsf(v[i + 1]));
-            nan |= __builtin_isunordered(v[i], v[i + 1]);
-        }
-        const uint32_t code = mx_scale_code(nan ? 0x7fc00000u : __float_as_uint(top));
+        for (int i = 0; i < 32; i += 2)
+            top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, __builtin_fabsf(v[i])), __builtin_fabsf(v[i + 1]));
+        const uint32_t code = mx_scale_code(__float_as_uint(__builtin_fabsf(top)));
         if (m < a.M && n < a.N) {
             u32x4 q;
 #pragma unroll

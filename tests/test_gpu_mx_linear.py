@@ -204,6 +204,26 @@ def test_specials_stay_in_their_row_and_column(dev, rows, n, x):
     assert torch.equal(torch.isnan(got), bad)
 
 
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("x", [MX, BF16, F16, F32])
+@pytest.mark.parametrize("rows,n", [(7, 90), (200, 160), (600, 400), (5000, 1024)])
+def test_specials_in_4_bits(dev, rows, n, x, act):
+    """A NaN takes its block along, its scale 255, and no other; so does an infinity that act leaves one, or makes NaN."""
+    import mbrt
+
+    v, w = _rand(1, (rows, 80), F32), _rand(2, (n, 80), F32, 0.1)
+    b = _rand(3, (n,), F32)
+    v[3, 7], b[33], b[70] = math.nan, math.inf, -math.inf
+    xs = mbrt.mx_quantize(v) if x == MX else v.to(x)
+    w = mbrt.mx_quantize(w)
+    got = mbrt.mx_linear(xs, w, b, act=act, out_dtype=mbrt.MxTensor).scales.cpu()
+    bad = torch.zeros((rows, -(-n // 32)), dtype=torch.bool)
+    bad[3] = True
+    if act < 3:
+        bad[:, 1] = bad[:, 2] = True
+    assert torch.equal(got == 255, bad)
+
+
 @pytest.mark.parametrize("x", [BF16, F16, F32])
 @pytest.mark.parametrize("rows,n", [(3, 40), (300, 200)])
 def test_infinities_of_x(dev, rows, n, x):
