@@ -36,7 +36,7 @@ struct BlockNormArgs {
     char* out;               // normed, or its codes; NULL without gamma
     uint8_t* oscales;
     int64_t rs, us, gs, ss, os, oss;  // row strides in bytes
-    uint32_t rows;
+    uint32_t rows, row0;  // of this launch; the first one's number among all
     int dim, chunks, padded; // chunks of VE of a row: those with elements, and with the zeros that fill a block of 32
     int rdt, udt, gdt, odt, gadt, pdt, ldt;
     int gate_vec, gate_logit;
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
     const char* gp = a.gate;
     if (a.gate != nullptr) {
         uint32_t d, m;
-        fdivmod(fdiv((uint32_t)r, a.inner), a.period, d, m);
+        fdivmod(fdiv(a.row0 + (uint32_t)r, a.inner), a.period, d, m);
         gp += m * a.gs;
     }
 #pragma unroll
@@ -338,7 +338,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_loop_kernel(BlockNormArgs
     const char *rp = a.res + r * a.rs, *up = a.upd + r * a.us, *gp = a.gate;
     if (gp != nullptr) {
         uint32_t d, m;
-        fdivmod(fdiv(row, a.inner), a.period, d, m);
+        fdivmod(fdiv(a.row0 + row, a.inner), a.period, d, m);
         gp += m * a.gs;
     }
     float post = 1.0f;
@@ -436,24 +436,38 @@ bool launch_sizes(const BlockNormArgs& a, int gate_bytes, hipStream_t st) {
     }
 }
 
-int launch_block_norm(BlockNormArgs& a, hipStream_t st, const char* op) {
+int launch_block_norm(BlockNormArgs a, hipStream_t st, const char* op) {
     const bool wide = a.rdt == F32 || a.udt == F32 || (a.gate_vec && a.gdt == F32) || a.odt == F32;
     const int ve = wide ? 4 : 8, gate_bytes = a.gate_vec ? dt_size(a.gdt) : 0;
     a.chunks = (int)ceil_div(a.dim, ve);
     a.padded = (int)ceil_div(a.dim, 32) * (32 / ve);
-    bool done = false;
+    bool vec = false, al = false;
     if (a.dim >= ve && a.dim <= 8192) {
         auto even = [&](const void* p, int64_t stride, int dt) {
             const int64_t b = (int64_t)ve * dt_size(dt);
             return p == nullptr || (aligned(p, b) && stride % b == 0);
         };
-        const bool al = a.dim % ve == 0 && even(a.res, a.rs, a.rdt) && even(a.upd, a.us, a.udt) && even(a.sum, a.ss, a.rdt) &&
-                        (a.odt == MXFP4 || even(a.out, a.os, a.odt)) && (!a.gate_vec || even(a.gate, a.gs, a.gdt));
-        if (wide) done = al ? launch_sizes<4, true>(a, gate_bytes, st) : launch_sizes<4, false>(a, gate_bytes, st);
-        else done = al ? launch_sizes<8, true>(a, gate_bytes, st) : launch_sizes<8, false>(a, gate_bytes, st);
+        al = a.dim % ve == 0 && even(a.res, a.rs, a.rdt) && even(a.upd, a.us, a.udt) && even(a.sum, a.ss, a.rdt) &&
+             (a.odt == MXFP4 || even(a.out, a.os, a.odt)) && (!a.gate_vec || even(a.gate, a.gs, a.gdt));
+        vec = true;
     }
-    if (!done)
-        hipLaunchKernelGGL(block_norm_loop_kernel, dim3((unsigned)ceil_div(a.rows, kThreads / 64)), dim3(kThreads), 0, st, a);
+    // a launch has fewer than 2^32 threads, up to 256 of them to a row
+    const int64_t rows = a.rows, step = int64_t(1) << 23;
+    for (int64_t r0 = 0; r0 < rows; r0 += step) {
+        BlockNormArgs p = a;
+        p.row0 = (uint32_t)r0;
+        p.rows = (uint32_t)std::min(step, rows - r0);
+        p.res += r0 * a.rs;
+        p.upd += r0 * a.us;
+        if (a.sum != nullptr) p.sum += r0 * a.ss;
+        if (a.out != nullptr) p.out += r0 * a.os;
+        if (a.oscales != nullptr) p.oscales += r0 * a.oss;
+        bool done = false;
+        if (vec && wide) done = al ? launch_sizes<4, true>(p, gate_bytes, st) : launch_sizes<4, false>(p, gate_bytes, st);
+        else if (vec) done = al ? launch_sizes<8, true>(p, gate_bytes, st) : launch_sizes<8, false>(p, gate_bytes, st);
+        if (!done)
+            hipLaunchKernelGGL(block_norm_loop_kernel, dim3((unsigned)ceil_div(p.rows, kThreads / 64)), dim3(kThreads), 0, st, p);
+    }
     return check_launch(op);
 }
 

@@ -969,12 +969,11 @@ int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
     // -> 16384 12.6 and 16.3; f32 [1, 1536] -> 8192 6.2 and 8.2, [4, 1024] -> 32768 10.5 and 15.9, [8, 1024] -> 32768 19.3 and 16.4;
     // 4 bits [1, 1536] -> 8192 4.4 and 4.9, [16, 4096] -> 16384 10.6 and 17.3.  With half as many strips as CUs it loses: bf16 and 4
     // bits [1, 4096] -> 4096 7.2 and 6.2, 6.0 and 5.7.
-    const int64_t strips32 = ceil_div(N, 32), turns16 = ceil_div(a.nb, 16);
-    if (M <= (XT == MXFP4 ? 16 : 4) && strips32 >= cus * (XT == BF16 ? std::min<int64_t>(M, 2) : 1) &&
-        M * TokenX<XT>::row(16 * turns16) <= (int64_t(1) << 16)) {
+    const int64_t strips32 = ceil_div(N, 32), turns16 = ceil_div(a.nb, 16), x_row = TokenX<XT>::row(16 * turns16);
+    if (M <= (XT == MXFP4 ? 16 : 4) && strips32 >= cus * (XT == BF16 ? std::min<int64_t>(M, 2) : 1) && M * x_row <= (int64_t(1) << 16)) {
         const int64_t room = std::max<int64_t>(1, std::min<int64_t>(16, 16 * cus / strips32));
         a.split = (int)ceil_div(turns16, ceil_div(turns16, room));
-        const size_t lds = (size_t)std::max<int64_t>(M * TokenX<XT>::row(16 * turns16), a.split > 1 ? a.split * 2048 : 0);
+        const size_t lds = (size_t)std::max<int64_t>(M * x_row, a.split > 1 ? a.split * 2048 : 0);
         hipLaunchKernelGGL((mx_token_kernel<XT, OMX>), dim3((unsigned)strips32), dim3(64 * a.split), lds, st, a);
         return MBRT_OK;
     }

@@ -181,6 +181,26 @@ def test_rows_far_apart(dev):
     _verify(got, r, u, gamma, None, None, False, None, 1.0, BF16, 1.0, D ** 0.5, EPS, before=(before, u))
 
 
+@pytest.mark.parametrize("D", [3, 8])
+def test_more_rows_than_a_launch_has(dev, D):
+    """The rows around 2^23, and the last ones, as in a call of their own."""
+    import mbrt
+
+    rows = (1 << 24) + 77
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r, u = (torch.randn((rows, D), generator=g, device="cuda").to(BF16) for _ in range(2))
+    gate = torch.randn((rows, 1), generator=g, device="cuda")
+    gamma, post = _rand(3, (D,), F32, 0.1, 1.0), _rand(4, (D,), F32, 0.1, 1.0)
+    h, n = mbrt.block_norm(r, u, gamma, post_gamma=post, gate=gate, gate_is_logit=True)
+    held = mbrt.block_norm(r, u, gamma, gate=gate, store_sum=False, out_dtype=mbrt.MxTensor)[1]
+    for a, b in ((0, 9), ((1 << 23) - 9, (1 << 23) + 9), (rows - 99, rows)):
+        part = r[a:b], u[a:b], gamma
+        h2, n2 = mbrt.block_norm(*part, post_gamma=post, gate=gate[a:b], gate_is_logit=True)
+        held2 = mbrt.block_norm(*part, gate=gate[a:b], store_sum=False, out_dtype=mbrt.MxTensor)[1]
+        assert torch.equal(h[a:b], h2) and torch.equal(n[a:b], n2)
+        assert torch.equal(held.codes[a:b], held2.codes) and torch.equal(held.scales[a:b], held2.scales)
+
+
 def test_captured_on_another_stream_and_without_the_extension_module(dev, monkeypatch):
     import mbrt
     from mbrt import _calls
