@@ -8,9 +8,13 @@
 // Every byte is read once and written once: a group of G lanes (16, 64, or the 256 of a block) holds a row in registers through
 // both norms, lane l its chunks l, l + G, ... of 16 bytes (VE elements: 8 where all operands have 2 bytes, else 4, f32 ones
 // 16 bytes and 2-byte ones 8).  The two sums of squares are butterflies within the group, and sums over four waves through
-// LDS where a block holds the row.  The vectors over the features are put into LDS once per block, multiplied as far as they go
-// together, or read where they are needed by a block that has one row.  All loads of rows, and those into LDS, are issued
-// before the first use: a call of few rows takes one round of them.
+// LDS where a block holds the row.  The vectors over the features are put into LDS once per block, or read where they are
+// needed by a block that has one row.  All loads of rows, and those into LDS, are issued before the first use: a call of few
+// rows takes one round of them.
+// An h of 2 bytes is formed in the formula's order, one f32 rounding per operation and a division among them (IN_ORDER): of
+// bf16 elements 2 in 10^7 are then rounded to another side than the formula in f32 rounds them, and normed follows them; factors
+// multiplied together first leave 3 in 10^5.  It costs a vector in LDS and five operations an element (f16 [4, 4003, 512] 14.1 ->
+// 14.9 us, bf16 [60, 384] 4.4 -> 5.0); an f32 h, which has no such sides, takes the product (f32 [60, 801, 384] 46.9 for 49.8).
 // A row whose last chunk is cut has it moved back to end at the row's end: its first elements are the chunk's before, left
 // out of the sums and stored twice with the same values, so that odd widths take the same loads as even ones.
 // normed may leave as microscaled 4-bit floats (mx.hpp): the lanes of a block of 32 stand side by side.
@@ -103,7 +107,14 @@ struct Chunk {
     }
 };
 
-__device__ __forceinline__ float gate_value(float g, int logit) { return logit ? sigmoidf(g) : g; }
+// A gate for a whole row: one exp and one division each.
+__device__ __forceinline__ float gate_value(float g, int logit) { return logit ? 1.0f / (1.0f + expf(-g)) : g; }
+
+// v / root, correctly rounded but for results below f32's normal ones.
+__device__ __forceinline__ float over(float v, float root, float inv_root) {
+    const float q = v * inv_root;
+    return fmaf(fmaf(-q, root, v), inv_root, q);
+}
 
 // n elements p[d], d a thread's every kThreads-th, as they stand in memory (past the end: the last one).
 template <int E>
@@ -163,11 +174,13 @@ __device__ __forceinline__ float row_sum(float v, float* turn) {
 // row or none.  AL: every row of every operand begins at a multiple of its chunk's bytes and is whole chunks long.
 template <int VE, int RS, int US, int GS, int G, int NC, bool AL>
 __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
-    constexpr bool IN_LDS = G < kThreads;
+    constexpr bool IN_LDS = G < kThreads, IN_ORDER = RS == 2;
     constexpr int E = (NC * G * VE + kThreads - 1) / kThreads;  // features of a thread as it fills LDS
     extern __shared__ float lds[];
-    float* const by = lds;            // IN_LDS: alpha * layer_scale * post_scale * post_gamma
-    float* const gam = lds + a.dim;   // and scale * gamma
+    // IN_LDS: post_scale * post_gamma, layer_scale (IN_ORDER) or the product of both with alpha, and scale * gamma
+    float* const post = lds;
+    float* const by = lds + (IN_ORDER ? a.dim : 0);
+    float* const gam = by + a.dim;
     const int lane = threadIdx.x % G;
     const int64_t row = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
     const bool valid = row < a.rows;
@@ -200,11 +213,15 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
         ga.load(a.gamma, a.gadt, a.dim);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            float b = a.alpha;
-            if (a.ls != nullptr) b *= ls.value(e, a.ldt);
-            if (a.post_gamma != nullptr) b *= pg.value(e, a.pdt) * a.post_scale;
             const int d = threadIdx.x + e * kThreads;
             if (d < a.dim) {
+                float b = IN_ORDER ? 1.0f : a.alpha;
+                if (a.ls != nullptr) b *= ls.value(e, a.ldt);
+                if (a.post_gamma != nullptr) {
+                    const float p = pg.value(e, a.pdt) * a.post_scale;
+                    if constexpr (IN_ORDER) post[d] = p;
+                    else b *= p;
+                }
                 by[d] = b;
                 gam[d] = ga.value(e, a.gadt) * a.scale;
             }
@@ -218,6 +235,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
                                        : (float)__builtin_bit_cast(_Float16, (uint16_t)gw),
                        a.gate_logit);
     float h[NC][VE];
+    float root = 0.0f, inv_root = 0.0f;
     if (a.post_gamma != nullptr) {
         float ss = 0.0f;
 #pragma unroll
@@ -228,7 +246,14 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
 #pragma unroll
             for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(u[i], u[i], ss) : ss;
         }
-        g *= rsqrtf(row_sum<G>(ss, lds) + a.eps);
+        ss = row_sum<G>(ss, lds) + a.eps;
+        if constexpr (IN_ORDER) {
+            root = sqrtf(ss);
+            inv_root = 1.0f / root;
+            if (root == __builtin_inff()) root = 0.0f;  // (then the quotient below stays 0)
+        } else {
+            g *= rsqrtf(ss);
+        }
     }
     float ss = 0.0f;
 #pragma unroll
@@ -236,31 +261,55 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
         float u[VE], x[VE];
         uv[k].to_f32(a.udt, u);
         rv[k].to_f32(a.rdt, x);
+        const int first = AL ? (lane + G * k < a.chunks ? 0 : VE) : (lane + G * k) * VE - at[k];
+        float f[VE], w[VE];
         if constexpr (GS != 0) {
-            float w[VE];
             gv[k].to_f32(a.gdt, w);
             if (a.gate_logit) {
 #pragma unroll
                 for (int i = 0; i < VE; ++i) w[i] = sigmoidf(w[i]);
             }
-#pragma unroll
-            for (int i = 0; i < VE; ++i) u[i] *= w[i];
         }
-        const int first = AL ? (lane + G * k < a.chunks ? 0 : VE) : (lane + G * k) * VE - at[k];
-        float f[VE];
-        if constexpr (IN_LDS) {
+        if constexpr (IN_ORDER) {
+            if (a.post_gamma != nullptr) {
+                if constexpr (IN_LDS) {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) f[i] = by[at[k] + i];
+                    for (int i = 0; i < VE; ++i) f[i] = post[at[k] + i];
+                } else {
+                    features<VE>(a.post_gamma, a.pdt, at[k], f);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) f[i] *= a.post_scale;
+                }
+#pragma unroll
+                for (int i = 0; i < VE; ++i) u[i] = over(u[i] * f[i], root, inv_root);
+            }
+            if (a.ls != nullptr) {
+                if constexpr (IN_LDS) {
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) f[i] = by[at[k] + i];
+                } else {
+                    features<VE>(a.ls, a.ldt, at[k], f);
+                }
+#pragma unroll
+                for (int i = 0; i < VE; ++i) u[i] *= f[i];
+            }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) h[k][i] = fmaf(u[i] * (GS != 0 ? w[i] : g), a.alpha, x[i]);
         } else {
-            float p[VE];
-            features<VE>(a.ls, a.ldt, at[k], f);
-            features<VE>(a.post_gamma, a.pdt, at[k], p);
-            const float b = a.post_gamma != nullptr ? a.alpha * a.post_scale : a.alpha;
+            if constexpr (IN_LDS) {
 #pragma unroll
-            for (int i = 0; i < VE; ++i) f[i] *= p[i] * b;
+                for (int i = 0; i < VE; ++i) f[i] = by[at[k] + i];
+            } else {
+                float p[VE];
+                features<VE>(a.ls, a.ldt, at[k], f);
+                features<VE>(a.post_gamma, a.pdt, at[k], p);
+                const float b = a.post_gamma != nullptr ? a.alpha * a.post_scale : a.alpha;
+#pragma unroll
+                for (int i = 0; i < VE; ++i) f[i] *= p[i] * b;
+            }
+#pragma unroll
+            for (int i = 0; i < VE; ++i) h[k][i] = fmaf(GS != 0 ? u[i] * w[i] * g : u[i] * g, f[i], x[i]);
         }
-#pragma unroll
-        for (int i = 0; i < VE; ++i) h[k][i] = fmaf(u[i] * g, f[i], x[i]);
         Chunk<RS, VE> t;
         t.from_f32(a.rdt, h[k]);
         t.to_f32(a.rdt, h[k]);
@@ -341,21 +390,22 @@ __global__ __launch_bounds__(kThreads) void block_norm_loop_kernel(BlockNormArgs
         fdivmod(fdiv(a.row0 + row, a.inner), a.period, d, m);
         gp += m * a.gs;
     }
-    float post = 1.0f;
+    float root = 1.0f;
     if (a.post_gamma != nullptr) {
         float ss = 0.0f;
         for (int d = lane; d < a.dim; d += 64) {
             const float u = load1(up, a.udt, d);
             ss = fmaf(u, u, ss);
         }
-        post = rsqrtf(group_sum<64>(ss) + a.eps);
+        root = sqrtf(group_sum<64>(ss) + a.eps);
     }
+    const float row_gate = gp != nullptr && !a.gate_vec ? gate_value(load1(gp, a.gdt, 0), a.gate_logit) : 1.0f;
     auto sum_at = [&](int d) {
-        float b = a.alpha, g = post;
-        if (a.ls != nullptr) b *= load1(a.ls, a.ldt, d);
-        if (a.post_gamma != nullptr) b *= load1(a.post_gamma, a.pdt, d) * a.post_scale;
-        if (gp != nullptr) g *= gate_value(load1(gp, a.gdt, a.gate_vec ? d : 0), a.gate_logit);
-        return round_through(fmaf(load1(up, a.udt, d) * g, b, load1(rp, a.rdt, d)), a.rdt);
+        float u = load1(up, a.udt, d);
+        if (a.post_gamma != nullptr) u = u * (load1(a.post_gamma, a.pdt, d) * a.post_scale) / root;
+        if (a.ls != nullptr) u *= load1(a.ls, a.ldt, d);
+        u *= a.gate_vec ? gate_value(load1(gp, a.gdt, d), a.gate_logit) : row_gate;
+        return round_through(fmaf(u, a.alpha, load1(rp, a.rdt, d)), a.rdt);
     };
     float ss = 0.0f;
     for (int d = lane; d < a.dim; d += 64) {
@@ -392,7 +442,7 @@ bool launch_shape(const BlockNormArgs& a, hipStream_t st) {
     auto go = [&](auto g, auto nc) {
         constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
         hipLaunchKernelGGL((block_norm_kernel<VE, RS, US, GS, G, NC, AL>), dim3((unsigned)ceil_div(a.rows, kThreads / G)),
-                           dim3(kThreads), (G < kThreads ? 2 * a.dim : 8) * sizeof(float), st, a);
+                           dim3(kThreads), (G < kThreads ? (RS == 2 ? 3 : 2) * a.dim : 8) * sizeof(float), st, a);
     };
     typedef std::integral_constant<int, 16> G16;
     typedef std::integral_constant<int, 64> G64;
