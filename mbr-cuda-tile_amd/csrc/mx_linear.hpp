@@ -469,7 +469,8 @@ __global__ __launch_bounds__(WM * WN * 64, OCC) void mx_tile_kernel(MxLinArgs a)
 
 // x in 16 or 32 bits: steps of FS features; w becomes bf16 and x its parts on their way through registers into LDS, one plane of
 // rows per part.  Every load costs the same whatever its width, so a thread takes whole blocks of w, 16 bytes and a scale. Loads of
-// three steps are under way while one is computed.  The parts of x meet the same weights.  LDS rows of x: piece j (8 features) at
+// three steps are under way while one is computed.  KG groups of waves each take a part of the steps, with buffers of their own, and
+// are added in order at the end.  The parts of x meet the same weights.  LDS rows of x: piece j (8 features) at
 // j ^ key(row).  Of w: piece 4 b + q of block b at (b + FS / 32 q) ^ key(row), so that the lanes that hold a row's blocks
 // write side by side, and rows that are read together, or written, differ in their keys.
 template <int FS, bool OMX>
@@ -482,8 +483,8 @@ __device__ __forceinline__ int wide_key_c(int c) {  // of the row of w that lane
     return FS == 128 ? (c & 1) << 2 | ((c >> 2) & 1) << 1 | ((c >> 1) & 1) : ((c >> 1) & 1) << 2 | (c & 1) << 1 | ((c >> 2) & 1);
 }
 
-template <int XT, int WM, int WN, int MI, int NI, int FS, int NT, int KIND, bool OMX>
-__global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a) {
+template <int XT, int WM, int WN, int MI, int NI, int FS, int KG, int NT, int KIND, bool OMX>
+__global__ __launch_bounds__(KG * WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a) {
     constexpr int NW = WM * WN, NTH = NW * 64, BM = WM * MI * 16, BN = WN * NI * 16, P = mx_parts(XT), Q = XT == F32 ? 2 : 1;
     constexpr int S = XT == F32 ? 4 : 2, PR = FS / 8, BR = FS / 32;     // pieces and blocks of a row's step
     constexpr int LX = BM * PR / NTH, WB = BN * BR, LW = (WB + NTH - 1) / NTH;  // pieces of x and blocks of w for a thread
@@ -491,9 +492,12 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
     static_assert(BM * PR % NTH == 0 && NI % 2 == 0, "as much of x for every thread, blocks in pairs");
     constexpr int SB = 2 * FS, kBuf = (BM * P + BN) * SB;
     static_assert(OMX || NW * NI * 1024 <= kBuf, "room for the rows on their way out");
-    __shared__ __attribute__((aligned(16))) char lds[2][kBuf];
-    const int tid = threadIdx.x, lane = tid % 64, g = lane / 16, c = lane % 16;
+    static_assert(KG == 1 || MI * NI * NW * 1024 <= kBuf, "room for a group's sums");
+    __shared__ __attribute__((aligned(16))) char all_lds[KG][2][kBuf];
+    const int tid = threadIdx.x % NTH, lane = tid % 64, g = lane / 16, c = lane % 16;
     const int w = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int kg = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / NTH);
+    auto& lds = all_lds[kg];
     const int wm = w / WN, wn = w % WN;
     const uint32_t tile = xcd_tile(blockIdx.x, gridDim.x);
     uint32_t mt, nt;
@@ -501,7 +505,9 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
     const int64_t m0 = (int64_t)mt * BM;
     const int n0 = (int)nt * BN;
     const int mrows = (int)min((int64_t)BM, a.M - m0), nrows = min(BN, a.N - n0);
-    const int steps = (a.K + FS - 1) / FS, whole = a.K / FS;
+    // a group's whole steps are first .. whole - 1; a step that the rows' end cuts is the last group's
+    const int all_whole = a.K / FS, share = (all_whole + KG - 1) / KG, first = min(kg * share, all_whole), whole = min(first + share, all_whole);
+    const bool cut = a.K % FS != 0;
     const char* xp[LX];
     const char* wp[LW];
     const uint8_t* sp[LW];
@@ -564,11 +570,17 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
     };
     typedef std::integral_constant<bool, false> No;
     typedef std::integral_constant<bool, true> Yes;
-    if (whole > 0) load(0, r0, No());
-    if (whole > 1) load(1, r1, No());
-    if (whole > 2) load(2, r2, No());
+    if (first < whole) load(first, r0, No());
+    if (first + 1 < whole) load(first + 1, r1, No());
+    if (first + 2 < whole) load(first + 2, r2, No());
     f32x4 acc[MI][NI];
     tile_begin<MI, NI, OMX>(a, n0 + wn * NI * 16, g, acc);
+    if (KG > 1 && kg > 0) {
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < NI; ++ni) acc[mi][ni] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     const int xrow = wm * MI * 16 + c, wrow = P * BM + wn * NI * 16;
     auto compute = [&](const char* d) __attribute__((always_inline)) {
 #pragma unroll
@@ -595,11 +607,11 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
     auto step = [&](int kt, Regs& mine, Regs& next, auto on) __attribute__((always_inline)) {
         ready();
         if (on) load(min(kt + 3, whole - 1), mine, No());
-        compute(lds[kt & 1]);
-        put(next, lds[(kt + 1) & 1]);
+        compute(lds[(kt - first) & 1]);
+        put(next, lds[(kt - first + 1) & 1]);
     };
-    if (whole > 0) put(r0, lds[0]);
-    int kt = 0;
+    if (first < whole) put(r0, lds[0]);
+    int kt = first;
     for (; kt + 3 <= whole; kt += 3) {
         step(kt, r0, r1, Yes());
         step(kt + 1, r1, r2, Yes());
@@ -607,24 +619,45 @@ __global__ __launch_bounds__(WM * WN * 64) void mx_wide_tile_kernel(MxLinArgs a)
     }
     if (kt < whole) step(kt, r0, r1, No());
     if (kt + 1 < whole) step(kt + 1, r1, r2, No());
-    if (steps > whole) {  // the step that the rows' end cuts
+    if (cut && kg == KG - 1) {
         load(whole, r0, Yes());
         ready();  // (what the last step put there in vain is read by none)
-        put(r0, lds[whole & 1]);
+        put(r0, lds[(whole - first) & 1]);
         ready();
-        compute(lds[whole & 1]);
+        compute(lds[(whole - first) & 1]);
     }
 
+    char* stage = lds[(whole - first + (cut ? 1 : 0)) & 1];  // the last step's other buffer: nothing reads it or, behind a cut step, writes it
+    if constexpr (KG > 1) {
+        // as many barriers for every group; then the other groups' sums, in their order
+        for (int i = whole - first + (cut && kg == KG - 1 ? 2 : 0); i < share + (cut ? 2 : 0); ++i) ready();
+        ready();
+        f32x4* const sums = reinterpret_cast<f32x4*>(all_lds[kg][0]) + w * 64 + lane;
+        if (kg > 0) {
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni) sums[(mi * NI + ni) * NW * 64] = acc[mi][ni];
+        }
+        ready();
+        if (kg > 0) return;
+#pragma unroll
+        for (int k = 1; k < KG; ++k)
+#pragma unroll
+            for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+                for (int ni = 0; ni < NI; ++ni) acc[mi][ni] += sums[k * (2 * kBuf / 16) + (mi * NI + ni) * NW * 64];
+        stage = all_lds[0][0];
+    }
     const int64_t m = m0 + wm * MI * 16;
     const int n = n0 + wn * NI * 16;
     if constexpr (OMX) {
         tile_finish_mx<MI, KIND, XT != F32>(a, m, n, g, c, acc);
     } else {
-        // a wave's own part of a buffer: the last step's other one, which nothing reads or, behind a cut step, writes any more
         MxLinArgs rest = a;
         rest.bias = nullptr;
-        ready();
-        tile_finish<MI, NI, KIND, NT>(rest, m, n, lane, lds[steps & 1] + w * NI * 1024, acc);
+        if constexpr (KG == 1) ready();
+        tile_finish<MI, NI, KIND, NT>(rest, m, n, lane, stage + w * NI * 1024, acc);  // a wave's own part
     }
 }
 
@@ -937,7 +970,7 @@ void launch_mx_strip(const MxLinArgs& a, int align, unsigned blocks, unsigned th
     }
 }
 
-// SB, OCC: of x in 4 bits (else SB is the features of a step)
+// SB, OCC: of x in 4 bits (else SB is the features of a step, OCC the groups of waves that share the steps)
 template <int XT, int WM, int WN, int MI, int NI, int SB, int OCC, int NT, bool OMX>
 int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
     constexpr int BM = WM * MI * 16, BN = WN * NI * 16;
@@ -945,13 +978,13 @@ int launch_mx_tile(MxLinArgs& a, hipStream_t st) {
     a.groups = make_fastdiv(a.ntiles);
     const int64_t tiles = ceil_div(a.M, BM) * a.ntiles;
     if (!grid_fits(tiles, WM * WN * 64)) return set_error(MBRT_E_SHAPE, "mbrt_mx_linear: too many tiles");
-    const dim3 grid((unsigned)tiles), block(WM * WN * 64);
+    const dim3 grid((unsigned)tiles), block((XT == MXFP4 ? 1 : OCC) * WM * WN * 64);
     auto launch = [&](auto kind) {
         constexpr int KIND = decltype(kind)::value;
         if constexpr (XT == MXFP4)
             hipLaunchKernelGGL((mx_tile_kernel<WM, WN, MI, NI, SB, OCC, NT, KIND, OMX>), grid, block, 0, st, a);
         else
-            hipLaunchKernelGGL((mx_wide_tile_kernel<XT, WM, WN, MI, NI, SB, NT, KIND, OMX>), grid, block, 0, st, a);
+            hipLaunchKernelGGL((mx_wide_tile_kernel<XT, WM, WN, MI, NI, SB, OCC, NT, KIND, OMX>), grid, block, 0, st, a);
     };
     const bool gelu = a.act == MBRT_ACT_GELU_REF || a.act == MBRT_ACT_GELU_STD;
     if (a.act == MBRT_ACT_NONE) launch(std::integral_constant<int, kActNone>());
@@ -1014,6 +1047,10 @@ int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
             if (!big) return launch_mx_tile<XT, 4, 1, 1, 8, FS, 1, 0, true>(a, st);
             if constexpr (XT != F32) return launch_mx_tile<XT, 4, 1, 2, 8, 64, 1, 0, true>(a, st);
         } else {
+            // At most a tile for every CU: two groups of waves share its steps.  us, one and two groups: bf16, f16 and f32 [700, 4096] -> 1024
+            // 23.6 and 20.0, 41.9 and 33.1, 60 and 45; [512, 1536] -> 1536 11.3 and 11.3, 17.9 and 16.2, 24.9 and 20.8; [512, 384] ->
+            // 1536 5.5 and 5.7, 7.6 and 7.2, 9.4 and 8.9.
+            if (!big && ceil_div(M, 64) * ceil_div(N, 64) <= cus) return launch_mx_tile<XT, 2, 2, 2, 2, FS, 2, 0, false>(a, st);
             if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, FS, 1, 0, false>(a, st);
             if constexpr (XT != F32)
                 return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 1, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 1, 0, false>(a, st);

@@ -101,6 +101,12 @@ def test_long_k(dev, rows, k, n, out, res):
     _case(dev, rows, k, n, MX, out, act=2 if res else 0, res=res, seed=k)
 
 
+@pytest.mark.parametrize("x", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,k,n", [(520, 63, 640), (520, 64, 640), (500, 129, 650), (513, 384, 900), (400, 1152, 1100), (700, 1007, 530)])
+def test_steps_shared_by_groups_of_waves(dev, rows, k, n, x):
+    _case(dev, rows, k, n, x, act=2, res=F16, seed=k)
+
+
 @pytest.mark.parametrize("act", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("x,out", [(MX, BF16), (MX, F32), (F32, F32), (BF16, F16), (F16, F32)])
 @pytest.mark.parametrize("rows,k,n", [(3, 96, 70), (150, 96, 70), (90, 96, 8)])
