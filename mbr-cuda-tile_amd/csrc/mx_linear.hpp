@@ -1047,10 +1047,10 @@ int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
             if (!big) return launch_mx_tile<XT, 4, 1, 1, 8, FS, 1, 0, true>(a, st);
             if constexpr (XT != F32) return launch_mx_tile<XT, 4, 1, 2, 8, 64, 1, 0, true>(a, st);
         } else {
-            // At most a tile for every CU: two groups of waves share its steps.  us, one and two groups: bf16, f16 and f32 [700, 4096] -> 1024
-            // 23.6 and 20.0, 41.9 and 33.1, 60 and 45; [512, 1536] -> 1536 11.3 and 11.3, 17.9 and 16.2, 24.9 and 20.8; [512, 384] ->
-            // 1536 5.5 and 5.7, 7.6 and 7.2, 9.4 and 8.9.
-            if (!big && ceil_div(M, 64) * ceil_div(N, 64) <= cus) return launch_mx_tile<XT, 2, 2, 2, 2, FS, 2, 0, false>(a, st);
+            // At most a tile for every CU, and steps to share: two groups of waves.  us, one and two groups: bf16, f16 and f32 [700, 4096]
+            // -> 1024 22.4 and 20.0, 41.9 and 33.1, 58.6 and 45.0; [512, 1536] -> 1536 11.5 and 11.3, 18.7 and 16.2, 25.0 and 20.8; [512,
+            // 384] -> 1536, 3 steps of bf16 and 6 of the others, 5.5 and 5.7, 7.4 and 7.2, 9.4 and 8.9.
+            if (!big && a.K >= 6 * FS && ceil_div(M, 64) * ceil_div(N, 64) <= cus) return launch_mx_tile<XT, 2, 2, 2, 2, FS, 2, 0, false>(a, st);
             if (!big) return launch_mx_tile<XT, 2, 2, 2, 2, FS, 1, 0, false>(a, st);
             if constexpr (XT != F32)
                 return nt ? launch_mx_tile<XT, 2, 2, 4, 4, 64, 1, 2, false>(a, st) : launch_mx_tile<XT, 2, 2, 4, 4, 64, 1, 0, false>(a, st);
