@@ -78,7 +78,7 @@ __device__ __forceinline__ void to_parts(const u32x4 (&raw)[XT == F32 ? 2 : 1], 
 // x Phi(s x) = max(x, 0) - |x| 2^p(|x|), with p the polynomial of degree 7 that comes nearest to log2 Phi(-s |x|) up to 6.5 / s, where
 // 2^p is 4e-11 and beyond which p keeps falling: a value is off by at most 1.1e-7, and by at most 2^-12.4 of itself down to there, at
 // 9 operations and an exp2 for gelu_short's 16 and two.  Results in 4 bits are far coarser, but each of them that falls to another
-// side of a code is off by a quarter: a form of degree 5, 4.7e-6 off, saves 3 us of feed_chunk's 114 and puts 5 in 10^5 there.
+// side of a code is off by a quarter: a form of degree 5, 4.7e-6 off, saves 3 us of feed_chunk's 117 and puts 5 in 10^5 there.
 // s: sqrt 2 in the reference's form (REF), 1 in the other.
 template <bool REF>
 __device__ __forceinline__ float gelu_tail(float x) {
