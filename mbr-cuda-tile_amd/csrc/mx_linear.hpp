@@ -75,22 +75,30 @@ __device__ __forceinline__ void to_parts(const u32x4 (&raw)[XT == F32 ? 2 : 1], 
     }
 }
 
-// x Phi(s x) = max(x, 0) - |x| 2^p(|x|), with p the polynomial of degree 7 that comes nearest to log2 Phi(-s |x|) up to 6.5 / s, where
-// 2^p is 4e-11 and beyond which p keeps falling: a value is off by at most 1.1e-7, and by at most 2^-12.4 of itself down to there, at
-// 9 operations and an exp2 for gelu_short's 16 and two.  Results in 4 bits are far coarser, but each of them that falls to another
-// side of a code is off by a quarter: a form of degree 5, 4.7e-6 off, saves 3 us of feed_chunk's 117 and puts 5 in 10^5 there.
-// s: sqrt 2 in the reference's form (REF), 1 in the other.
-template <bool REF>
-__device__ __forceinline__ float gelu_tail(float x) {
+// x Phi(s x) = max(x, 0) - t Phi(-s t), t = |x|, for results in 4 bits.  With r = 1 / (1 + c t), Phi(-s t) is r P(r) 2^(-k t^2): P, of
+// degree 7, comes within 2.3e-8 of the scaled function up to s t = 13.2, where Phi leaves f32's normal numbers (and the product is 0
+// from there).  In f32 a value is off by at most 2^-23 (0.75 (s x)^2 + 6) of itself, as f32 rounds the argument of an erfc, so a
+// block that lies wholly in the tail has the codes that the formula gives it.  12 operations and two transcendental ones ([48060, 384]
+// -> 1536 and back 122 us).  A polynomial for log2 Phi alone, 9 and one (117 us), is off by 1.1e-7 at most, but by 2^-12 of the value at
+// s x = -5 and by a third of it at -11: of values around -5, 2 in 10^4 then have other codes, and around -11 one in ten.
+struct GeluTail {
+    float c, k;
+};
+__device__ __forceinline__ GeluTail gelu_tail_of(int act) {  // s: sqrt 2 in the reference's form, 1 in the other
+    return act == MBRT_ACT_GELU_REF ? GeluTail{0.42426407f, 1.44269504f} : GeluTail{0.3f, 0.72134752f};
+}
+__device__ __forceinline__ float gelu_tail(float x, GeluTail f) {
     const float t = __builtin_fabsf(x);
-    float p = REF ? fmaf(-1.51317709e-05f, t, 0.000422811223f) : fmaf(-1.33747221e-06f, t, 5.28514029e-05f);
-    p = fmaf(p, t, REF ? -0.00494488003f : -0.000874139543f);
-    p = fmaf(p, t, REF ? 0.0333767533f : 0.00834418833f);
-    p = fmaf(p, t, REF ? -0.152023286f : -0.0537483469f);
-    p = fmaf(p, t, REF ? -0.917114735f : -0.458557367f);
-    p = fmaf(p, t, REF ? -1.62812996f : -1.15126169f);
-    p = fmaf(p, t, -0.999987721f);
-    return fmaf(-t, __builtin_amdgcn_exp2f(p), __builtin_amdgcn_fmed3f(x, 0.0f, __builtin_inff()));  // fmaxf would quiet x first
+    const float r = fast_rcp(fmaf(f.c, t, 1.0f));
+    float p = fmaf(0.0366180278f, r, -0.161052659f);
+    p = fmaf(p, r, 0.212840408f);
+    p = fmaf(p, r, -0.0595139973f);
+    p = fmaf(p, r, 0.131569877f);
+    p = fmaf(p, r, 0.0990252048f);
+    p = fmaf(p, r, 0.120892622f);
+    p = fmaf(p, r, 0.119620487f);
+    const float e = __builtin_amdgcn_exp2f(-(t * f.k) * t);
+    return fmaf(-(t * r * p), e, __builtin_amdgcn_fmed3f(x, 0.0f, __builtin_inff()));  // fmaxf would quiet x first
 }
 
 // What a kernel applies to its sums: nothing, GELU in a form for short results, or any function.  What stands behind the sums of a
@@ -102,17 +110,12 @@ enum MxAct { kActNone = 0, kActGelu = 1, kActAny = 2 };
 template <int KIND, bool OMX, bool SHORT, int NV>
 __device__ __forceinline__ void activate_mx(const MxLinArgs& a, float (&v)[NV]) {
     if constexpr (KIND == kActGelu) {
-        const bool ref = a.act == MBRT_ACT_GELU_REF;
         if constexpr (OMX) {
-            if (ref) {
+            const GeluTail f = gelu_tail_of(a.act);
 #pragma unroll
-                for (int i = 0; i < NV; ++i) v[i] = gelu_tail<true>(v[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < NV; ++i) v[i] = gelu_tail<false>(v[i]);
-            }
+            for (int i = 0; i < NV; ++i) v[i] = gelu_tail(v[i], f);
         } else {
-            const float s = ref ? 1.0f : 0.70710678118654752440f;
+            const float s = a.act == MBRT_ACT_GELU_REF ? 1.0f : 0.70710678118654752440f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) v[i] = gelu_short(v[i], s);
         }
