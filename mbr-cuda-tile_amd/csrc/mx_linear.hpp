@@ -77,7 +77,7 @@ __device__ __forceinline__ void to_parts(const u32x4 (&raw)[XT == F32 ? 2 : 1], 
 
 // x Phi(s x) = max(x, 0) - t Phi(-s t), t = |x|, for results in 4 bits.  With r = 1 / (1 + c t), Phi(-s t) is r P(r) 2^(-k t^2): P, of
 // degree 7, comes within 2.3e-8 of the scaled function up to s t = 13.2, where Phi leaves f32's normal numbers (and the product is 0
-// from there).  In f32 a value is off by at most 2^-23 (0.75 (s x)^2 + 6) of itself, as f32 rounds the argument of an erfc, so a
+// from there).  In f32 a value is off by at most 2^-23 (0.75 (s x)^2 + 16) of itself, as f32 rounds the argument of an erfc, so a
 // block that lies wholly in the tail has the codes that the formula gives it.  12 operations and two transcendental ones ([48060, 384]
 // -> 1536 and back 122 us).  A polynomial for log2 Phi alone, 9 and one (117 us), is off by 1.1e-7 at most, but by 2^-12 of the value at
 // s x = -5 and by a third of it at -11: of values around -5, 2 in 10^4 then have other codes, and around -11 one in ten.

@@ -23,7 +23,7 @@ def _gelu(pre, act):
     Roundings, in halves of U = 2^-23: k, its product with |x| and that with |x| each move the exponent, (s x)^2 / 2 as a natural
     one, by one of its size: 0.75 (s x)^2 U.  The argument 1 + c |x| (1), its reciprocal (2, and as much again in the polynomial),
     the polynomial of degree 7 with a sum of magnitudes of at most twice its value (7 steps: 14 at most), what it differs from the
-    function by (2.3e-8 of 0.12 and more: 4), exp2 (2), three products and the last sum (4): 29 halves, so 16.  What lies below
+    function by (2.3e-8 of 0.12 and more: 4), exp2 (2), three products and the last sum (4): 29 halves, taken as 32.  What lies below
     f32's normal numbers may be 0."""
     y, _ = layer_ref.act64(pre, act)
     z2 = (2.0 if act == 1 else 1.0) * pre * pre
