@@ -505,7 +505,8 @@ MBRT_API int mbrt_mx_dequantize(const void* codes, int64_t codes_row_stride, con
  * unused), bias and residual F32/F16/BF16 or NULL, out F32/F16/BF16 or MXFP4 (with out_scales; quantised from the f32
  * results as by mbrt_mx_quantize).  Strides of codes in bytes, of other rows in elements; x, weight and residual may have
  * any from 0 on.  Products are exact: 4-bit by 4-bit ones, and those of F32/F16/BF16 x, which is taken as a sum of bf16 values
- * (what lies below 2^-133 of an F32 x is lost).  Sums and the epilogue are f32, with one rounding on the store; activations
+ * (what lies below 2^-133 of an F32 x is lost) and meets the weights in bf16: one of 2^128 or more, which scale bytes 253 and 254 can
+ * express and mbrt_mx_quantize writes for no finite f32, leaves its out feature infinite or NaN there; x in MXFP4 takes it as it is.  Sums and the epilogue are f32, with one rounding on the store; activations
  * as mbrt_linear's, in their short forms unless x or out is F32; GELU in front of results in 4 bits, whose scale follows a block's
  * largest value however small, in full f32: x Phi(s x) is off by 2^-23 (0.75 (s x)^2 + 16) of itself at most in the negative tail (s: sqrt 2
  * in the reference's form, else 1), and may be 0 where Phi is below 2^-126.  out may be residual (same dtype, same rows); it shares no other

@@ -6,7 +6,8 @@
 // sums f32.  Blocks behind a row's last one are whatever the row's last block holds, with scales of 2^-127 on both sides:
 // 2^-254 times 36 at most, which leaves an f32 as it is.
 //
-// x in 16 or 32 bits: a weight has two significant bits and a power of two, so it is exactly a bf16, and x is exactly the sum of
+// x in 16 or 32 bits: a weight below 2^128 (all but the largest under scale bytes 253 and 254, which become infinities) has two
+// significant bits and a power of two, so it is exactly a bf16, and x is exactly the sum of
 // one (bf16), two (f16) or three (f32) bf16 values, each the leading bits of what the ones before leave.  All of them go
 // through the bf16 matrix instructions: nothing is rounded but the f32 sums.
 #pragma once

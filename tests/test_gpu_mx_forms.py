@@ -1,13 +1,15 @@
 """GPU tests of the forms that only large calls of the 4-bit layer and the norms around a block take, with row counts derived
-from the device's compute units, so that the forms stay covered."""
+from the device's compute units, so that the forms stay covered; and of the largest and smallest scales."""
 from __future__ import annotations
 
 import pytest
 import torch
 
+import layer_ref
+import mx_ref as ref
 from gpu_util import say
 from test_gpu_block_norm import _case as norm_case
-from test_gpu_mx_linear import BF16, F16, F32, MX, _case, _rand
+from test_gpu_mx_linear import BF16, F16, F32, MX, _case, _operand, _rand
 
 pytestmark = pytest.mark.gpu
 
@@ -62,7 +64,7 @@ def test_three_chunks_to_a_lane(dev, D, rdt, udt, out):
     norm_case((5, rows // 4), D, rdt, udt, out, gate="batch", post=False, scaled=False, seed=D + 1)
 
 
-@pytest.mark.parametrize("D,dtype", [(769, F32), (700, F32), (1535, BF16), (1536, F16)])
+@pytest.mark.parametrize("D,dtype", [(767, F32), (700, F32), (1535, BF16), (1536, F16)])
 def test_three_chunks_to_a_lane_in_place(dev, D, dtype):
     import mbrt
 
@@ -72,3 +74,41 @@ def test_three_chunks_to_a_lane_in_place(dev, D, dtype):
     want = mbrt.block_norm(r, u, gamma, post_gamma=gamma, alpha=0.5)
     h, n = mbrt.block_norm(r, u, gamma, post_gamma=gamma, alpha=0.5, sum_out=r, normed=u)
     assert h is r and n is u and torch.equal(r, want[0]) and torch.equal(u, want[1])
+
+
+# ---- scales at their ends ---------------------------------------------------------------------------
+
+def _weights(n, blocks, byte, top, seed):
+    """Rows of blocks under one scale byte, with codes 0 .. top of either sign; their values in 64 bits."""
+    import mbrt
+
+    g = torch.Generator().manual_seed(seed)
+    c = torch.randint(0, top + 1, (n, 32 * blocks), generator=g) + 8 * torch.randint(0, 2, (n, 32 * blocks), generator=g)
+    w = mbrt.MxTensor((c[:, 0::2] | c[:, 1::2] << 4).to(torch.uint8).cuda(), torch.full((n, blocks), byte, dtype=torch.uint8, device="cuda"), 32 * blocks)
+    return w, ref.values(c, torch.full((n, blocks), byte), 32 * blocks)
+
+
+@pytest.mark.parametrize("x", [MX, BF16, F16, F32])
+@pytest.mark.parametrize("byte,top,e", [(0, 7, 60), (1, 7, 60), (252, 7, -60), (253, 5, -60), (254, 3, -60), (253, 7, -60), (254, 7, -60)])
+@pytest.mark.parametrize("rows,n", [(3, 8200), (20, 40), (300, 200)])
+def test_weights_under_the_smallest_and_largest_scales(dev, rows, n, x, byte, top, e):
+    """x of a size that leaves the products f32's normal numbers (f16, which is not that wide, meets scale bytes 20 and 21).  A weight of 2^128 or more (codes 6 and 7 under byte 253, 4 to 7
+    under 254) is beyond bf16: with x in 16 or 32 bits its output feature is not finite; with x in 4 bits it counts as it is."""
+    import mbrt
+
+    say(f"scale byte {byte} top {top} rows={rows} n={n} x={x}")
+    if x == F16:
+        byte, e = (byte + 20, 10) if byte < 2 else (byte, -20)
+    w, w64 = _weights(n, 2, byte, top, 3)
+    v = _rand(1, (rows, 64), F32).double().cpu()
+    v = torch.where(v == 0, torch.ones_like(v), v) * 2.0 ** e
+    xs = mbrt.mx_quantize(v.float().cuda()) if x == MX else v.to(x).cuda()
+    x64 = ref.held(xs) if x == MX else xs.cpu().double()
+    got = mbrt.mx_linear(xs, w, out_dtype=F32)
+    want, bound = ref.linear(x64, w64, None, 0, None, F32)
+    if x != MX:
+        beyond = (w64.abs() >= 2.0 ** 128).any(-1)
+        assert bool(beyond.any()) == ((byte, top) in ((253, 7), (254, 7)))
+        assert not bool(torch.isfinite(got.cpu()[:, beyond]).any())
+        got, want, bound = got[:, (~beyond).cuda()], want[:, ~beyond], bound[:, ~beyond]
+    layer_ref.check(got, want, bound, f"scale byte {byte}")
