@@ -530,8 +530,9 @@ MBRT_API int mbrt_mx_linear(const void* x, int dtype, int64_t x_row_stride, cons
  * one per row, per batch entry, per position, or one for all; gate_is_logit puts it through a sigmoid.  sum_out takes h
  * in residual's type (NULL: not stored; it may be residual itself); normed F32/F16/BF16 or MXFP4 with normed_scales
  * (quantised from the f32 results), none with gamma NULL.  normed may be update itself (same dtype and rows).  Outputs share
- * no other byte with an operand.  Row strides in elements (codes and scales: bytes).  f32 throughout, one rounding of each
- * output.  Beside mbrt_residual_add_rms_norm, for models that norm a block's output, gate it or scale it. */
+ * no other byte with an operand.  Row strides in elements (codes and scales: bytes).  f32 throughout, in the formula's order, one
+ * rounding of each output: what differs from the formula in f32 is the order of the sums, a step of f32 or so, and so now and then the
+ * side to which a 2-byte h on a tie of its rounding falls, which normed follows.  Beside mbrt_residual_add_rms_norm, for models that norm a block's output, gate it or scale it. */
 MBRT_API int mbrt_block_norm(const void* residual, int residual_dtype, int64_t residual_row_stride, const void* update,
                              int update_dtype, int64_t update_row_stride, const void* post_gamma, int post_gamma_dtype,
                              const void* gate, int gate_dtype, int64_t gate_cols, int64_t gate_row_stride,

@@ -11,10 +11,10 @@
 // LDS where a block holds the row.  The vectors over the features are put into LDS once per block, or read where they are
 // needed by a block that has one row.  All loads of rows, and those into LDS, are issued before the first use: a call of few
 // rows takes one round of them.
-// An h of 2 bytes is formed in the formula's order, one f32 rounding per operation and a division among them (IN_ORDER): of
-// bf16 elements 2 in 10^7 are then rounded to another side than the formula in f32 rounds them, and normed follows them; factors
-// multiplied together first leave 3 in 10^5.  It costs a vector in LDS and five operations an element (f16 [4, 4003, 512] 14.1 ->
-// 14.9 us, bf16 [60, 384] 4.4 -> 5.0); an f32 h, which has no such sides, takes the product (f32 [60, 801, 384] 46.9 for 49.8).
+// Both results are formed in the formula's order, one f32 rounding per operation and quotients by the roots, so that they differ from
+// the formula in f32 calls by the order of the two sums alone, and 4-bit values behind them seldom do.  An h of 2 bytes that lies on
+// a tie of its rounding can still fall to the other side, and normed follows it as it is stored: of [48060, 384] 154 elements in bf16
+// and 949 in f16, where the formula in f32 itself differs from 64 bits in 709 and 3193.
 // A row whose last chunk is cut has it moved back to end at the row's end: its first elements are the chunk's before, left
 // out of the sums and stored twice with the same values, so that odd widths take the same loads as even ones.
 // normed may leave as microscaled 4-bit floats (mx.hpp): the lanes of a block of 32 stand side by side.
@@ -110,10 +110,17 @@ struct Chunk {
 // A gate for a whole row: one exp and one division each.
 __device__ __forceinline__ float gate_value(float g, int logit) { return logit ? 1.0f / (1.0f + expf(-g)) : g; }
 
-// v / root, correctly rounded but for results below f32's normal ones.
-__device__ __forceinline__ float over(float v, float root, float inv_root) {
-    const float q = v * inv_root;
-    return fmaf(fmaf(-q, root, v), inv_root, q);
+// v / sqrt(ss): the device's square root and a quotient correctly rounded (but below f32's normal numbers), by one division per row.
+struct Root {
+    float value, inv;
+};
+__device__ __forceinline__ Root root_of(float ss) {
+    const float r = sqrtf(ss);
+    return {r == __builtin_inff() ? 0.0f : r, 1.0f / r};  // (of an infinite sum the quotients are 0: so they stay)
+}
+__device__ __forceinline__ float over(float v, Root r) {
+    const float q = v * r.inv;
+    return fmaf(fmaf(-q, r.value, v), r.inv, q);
 }
 
 // n elements p[d], d a thread's every kThreads-th, as they stand in memory (past the end: the last one).
@@ -174,12 +181,12 @@ __device__ __forceinline__ float row_sum(float v, float* turn) {
 // row or none.  AL: every row of every operand begins at a multiple of its chunk's bytes and is whole chunks long.
 template <int VE, int RS, int US, int GS, int G, int NC, bool AL>
 __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
-    constexpr bool IN_LDS = G < kThreads, IN_ORDER = RS == 2;
+    constexpr bool IN_LDS = G < kThreads;
     constexpr int E = (NC * G * VE + kThreads - 1) / kThreads;  // features of a thread as it fills LDS
     extern __shared__ float lds[];
-    // IN_LDS: post_scale * post_gamma, layer_scale (IN_ORDER) or the product of both with alpha, and scale * gamma
+    // IN_LDS: post_scale * post_gamma, layer_scale and scale * gamma
     float* const post = lds;
-    float* const by = lds + (IN_ORDER ? a.dim : 0);
+    float* const by = lds + a.dim;
     float* const gam = by + a.dim;
     const int lane = threadIdx.x % G;
     const int64_t row = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G;
@@ -215,14 +222,8 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
         for (int e = 0; e < E; ++e) {
             const int d = threadIdx.x + e * kThreads;
             if (d < a.dim) {
-                float b = IN_ORDER ? 1.0f : a.alpha;
-                if (a.ls != nullptr) b *= ls.value(e, a.ldt);
-                if (a.post_gamma != nullptr) {
-                    const float p = pg.value(e, a.pdt) * a.post_scale;
-                    if constexpr (IN_ORDER) post[d] = p;
-                    else b *= p;
-                }
-                by[d] = b;
+                post[d] = pg.value(e, a.pdt) * a.post_scale;
+                by[d] = ls.value(e, a.ldt);
                 gam[d] = ga.value(e, a.gadt) * a.scale;
             }
         }
@@ -235,7 +236,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
                                        : (float)__builtin_bit_cast(_Float16, (uint16_t)gw),
                        a.gate_logit);
     float h[NC][VE];
-    float root = 0.0f, inv_root = 0.0f;
+    Root root{};
     if (a.post_gamma != nullptr) {
         float ss = 0.0f;
 #pragma unroll
@@ -246,14 +247,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
 #pragma unroll
             for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(u[i], u[i], ss) : ss;
         }
-        ss = row_sum<G>(ss, lds) + a.eps;
-        if constexpr (IN_ORDER) {
-            root = sqrtf(ss);
-            inv_root = 1.0f / root;
-            if (root == __builtin_inff()) root = 0.0f;  // (then the quotient below stays 0)
-        } else {
-            g *= rsqrtf(ss);
-        }
+        root = root_of(row_sum<G>(ss, lds) + a.eps);
     }
     float ss = 0.0f;
 #pragma unroll
@@ -270,46 +264,30 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
                 for (int i = 0; i < VE; ++i) w[i] = sigmoidf(w[i]);
             }
         }
-        if constexpr (IN_ORDER) {
-            if (a.post_gamma != nullptr) {
-                if constexpr (IN_LDS) {
+        if (a.post_gamma != nullptr) {
+            if constexpr (IN_LDS) {
 #pragma unroll
-                    for (int i = 0; i < VE; ++i) f[i] = post[at[k] + i];
-                } else {
-                    features<VE>(a.post_gamma, a.pdt, at[k], f);
+                for (int i = 0; i < VE; ++i) f[i] = post[at[k] + i];
+            } else {
+                features<VE>(a.post_gamma, a.pdt, at[k], f);
 #pragma unroll
-                    for (int i = 0; i < VE; ++i) f[i] *= a.post_scale;
-                }
-#pragma unroll
-                for (int i = 0; i < VE; ++i) u[i] = over(u[i] * f[i], root, inv_root);
-            }
-            if (a.ls != nullptr) {
-                if constexpr (IN_LDS) {
-#pragma unroll
-                    for (int i = 0; i < VE; ++i) f[i] = by[at[k] + i];
-                } else {
-                    features<VE>(a.ls, a.ldt, at[k], f);
-                }
-#pragma unroll
-                for (int i = 0; i < VE; ++i) u[i] *= f[i];
+                for (int i = 0; i < VE; ++i) f[i] *= a.post_scale;
             }
 #pragma unroll
-            for (int i = 0; i < VE; ++i) h[k][i] = fmaf(u[i] * (GS != 0 ? w[i] : g), a.alpha, x[i]);
-        } else {
+            for (int i = 0; i < VE; ++i) u[i] = over(u[i] * f[i], root);
+        }
+        if (a.ls != nullptr) {
             if constexpr (IN_LDS) {
 #pragma unroll
                 for (int i = 0; i < VE; ++i) f[i] = by[at[k] + i];
             } else {
-                float p[VE];
                 features<VE>(a.ls, a.ldt, at[k], f);
-                features<VE>(a.post_gamma, a.pdt, at[k], p);
-                const float b = a.post_gamma != nullptr ? a.alpha * a.post_scale : a.alpha;
-#pragma unroll
-                for (int i = 0; i < VE; ++i) f[i] *= p[i] * b;
             }
 #pragma unroll
-            for (int i = 0; i < VE; ++i) h[k][i] = fmaf(GS != 0 ? u[i] * w[i] * g : u[i] * g, f[i], x[i]);
+            for (int i = 0; i < VE; ++i) u[i] *= f[i];
         }
+#pragma unroll
+        for (int i = 0; i < VE; ++i) h[k][i] = fmaf(u[i] * (GS != 0 ? w[i] : g), a.alpha, x[i]);
         Chunk<RS, VE> t;
         t.from_f32(a.rdt, h[k]);
         t.to_f32(a.rdt, h[k]);
@@ -317,7 +295,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
 #pragma unroll
         for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(h[k][i], h[k][i], ss) : ss;
     }
-    const float inv = rsqrtf(row_sum<G>(ss, lds + 4) + a.eps);
+    root = root_of(row_sum<G>(ss, lds + 4) + a.eps);
     if (G > 64 && a.sum != nullptr) {  // not before every wave has its part of a row that it may replace, a cut chunk's first elements too
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
@@ -339,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
             for (int i = 0; i < VE; ++i) o[i] *= a.scale;
         }
 #pragma unroll
-        for (int i = 0; i < VE; ++i) o[i] *= h[k][i] * inv;
+        for (int i = 0; i < VE; ++i) o[i] = over(h[k][i] * o[i], root);
         const bool mine = valid && lane + G * k < a.chunks;
         if (a.odt == MXFP4) {
             const int c = lane + G * k;
@@ -414,12 +392,12 @@ __global__ __launch_bounds__(kThreads) void block_norm_loop_kernel(BlockNormArgs
         ss = fmaf(h, h, ss);
     }
     if (a.gamma == nullptr) return;
-    const float inv = rsqrtf(group_sum<64>(ss) + a.eps);
+    const float sum_root = sqrtf(group_sum<64>(ss) + a.eps);
     for (int d0 = 0; d0 < a.dim; d0 += 64) {
         const int d = d0 + lane;
         float o = 0.0f;
         if (d < a.dim)  // the stored sum again: it may lie in the residual's place
-            o = (a.sum != nullptr ? load1(a.sum + r * a.ss, a.rdt, d) : sum_at(d)) * inv * (load1(a.gamma, a.gadt, d) * a.scale);
+            o = (a.sum != nullptr ? load1(a.sum + r * a.ss, a.rdt, d) : sum_at(d)) * (load1(a.gamma, a.gadt, d) * a.scale) / sum_root;
         if (a.odt != MXFP4) {
             if (d < a.dim) store1(a.out + r * a.os, a.odt, d, o);
             continue;
@@ -442,7 +420,7 @@ bool launch_shape(const BlockNormArgs& a, hipStream_t st) {
     auto go = [&](auto g, auto nc) {
         constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
         hipLaunchKernelGGL((block_norm_kernel<VE, RS, US, GS, G, NC, AL>), dim3((unsigned)ceil_div(a.rows, kThreads / G)),
-                           dim3(kThreads), (G < kThreads ? (RS == 2 ? 3 : 2) * a.dim : 8) * sizeof(float), st, a);
+                           dim3(kThreads), (G < kThreads ? 3 * a.dim : 8) * sizeof(float), st, a);
     };
     typedef std::integral_constant<int, 16> G16;
     typedef std::integral_constant<int, 64> G64;
