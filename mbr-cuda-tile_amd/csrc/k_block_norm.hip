@@ -14,7 +14,8 @@
 // Both results are formed in the formula's order, one f32 rounding per operation and quotients by the roots, so that they differ from
 // the formula in f32 calls by the order of the two sums alone, and 4-bit values behind them seldom do.  An h of 2 bytes that lies on
 // a tie of its rounding can still fall to the other side, and normed follows it as it is stored: of [48060, 384] 154 elements in bf16
-// and 949 in f16, where the formula in f32 itself differs from 64 bits in 709 and 3193.
+// and 949 in f16, where the formula in f32 itself differs from 64 bits in 709 and 3193.  Quotients cost 0.3 us of 13.4 (f16
+// [4, 4003, 512]) against products with the reciprocal root.
 // A row whose last chunk is cut has it moved back to end at the row's end: its first elements are the chunk's before, left
 // out of the sums and stored twice with the same values, so that odd widths take the same loads as even ones.
 // normed may leave as microscaled 4-bit floats (mx.hpp): the lanes of a block of 32 stand side by side.
@@ -123,24 +124,27 @@ __device__ __forceinline__ float over(float v, Root r) {
     return fmaf(fmaf(-q, r.value, v), r.inv, q);
 }
 
-// n elements p[d], d a thread's every kThreads-th, as they stand in memory (past the end: the last one).
+// Elements p[d] of a vector of dim >= 4, d a thread's every kThreads-th (past the end: any), as they stand in memory: a dword each, for
+// two bytes the element and the next, the last two at the end.  A load per type in branches of its own would wait for the one
+// before, since either could still be on its way into its register.
 template <int E>
 struct Staged {
     uint32_t w[E];
     __device__ __forceinline__ void load(const void* p, int dt, int dim) {
+        typedef uint32_t any1 __attribute__((aligned(2)));
+        const int64_t size = dt == F32 ? 4 : 2;
+        const int last = dt == F32 ? dim - 1 : dim - 2;
 #pragma unroll
         for (int e = 0; e < E; ++e) w[e] = 0;
         if (p == nullptr) return;
-        if (dt == F32) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) w[e] = reinterpret_cast<const uint32_t*>(p)[min((int)threadIdx.x + e * kThreads, dim - 1)];
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) w[e] = reinterpret_cast<const uint16_t*>(p)[min((int)threadIdx.x + e * kThreads, dim - 1)];
-        }
+        for (int e = 0; e < E; ++e)
+            w[e] = *reinterpret_cast<const any1*>(static_cast<const char*>(p) + min((int)threadIdx.x + e * kThreads, last) * size);
     }
-    __device__ __forceinline__ float value(int e, int dt) const {
-        return dt == F32 ? __uint_as_float(w[e]) : dt == BF16 ? bf16_lo(w[e]) : (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+    __device__ __forceinline__ float value(int e, int dt, int dim) const {
+        if (dt == F32) return __uint_as_float(w[e]);
+        const uint32_t v = (int)threadIdx.x + e * kThreads > dim - 2 ? w[e] >> 16 : w[e];
+        return dt == BF16 ? bf16_lo(v) : (float)__builtin_bit_cast(_Float16, (uint16_t)v);
     }
 };
 
@@ -222,9 +226,9 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
         for (int e = 0; e < E; ++e) {
             const int d = threadIdx.x + e * kThreads;
             if (d < a.dim) {
-                post[d] = pg.value(e, a.pdt) * a.post_scale;
-                by[d] = ls.value(e, a.ldt);
-                gam[d] = ga.value(e, a.gadt) * a.scale;
+                post[d] = pg.value(e, a.pdt, a.dim) * a.post_scale;
+                by[d] = ls.value(e, a.ldt, a.dim);
+                gam[d] = ga.value(e, a.gadt, a.dim) * a.scale;
             }
         }
         __syncthreads();
