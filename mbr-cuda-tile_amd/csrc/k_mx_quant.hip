@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(MxRows a) {
 
 // Calls of more pieces than a launch counts in 32 bits go in several launches of whole rows.
 template <class F>
-void for_row_ranges(MxRows a, int64_t es, F launch) {
+void for_row_ranges(MxRows a, F launch) {
     const int64_t step = std::max<int64_t>(1, (int64_t(1) << 31) / a.pieces);
     for (int64_t r0 = 0, n = a.rows; r0 < n; r0 += step) {
         a.rows = std::min(step, n - r0);
@@ -190,7 +190,7 @@ int mx_convert(const char* op, bool to_codes, char* x, int dt, int64_t xs, char*
     const bool cold = cold_input(rows * K * es) != 0;
     with_dt(dt, [&](auto t) {
         constexpr int DT = decltype(t)::value, S = DT == F32 ? 4 : 2;
-        for_row_ranges(a, es, [&](const MxRows& r, dim3 grid) {
+        for_row_ranges(a, [&](const MxRows& r, dim3 grid) {
             if (to_codes) {
                 if (al && cold) hipLaunchKernelGGL((mx_quantize_kernel<DT, 16, 1>), grid, dim3(kThreads), 0, st, r);
                 else if (al) hipLaunchKernelGGL((mx_quantize_kernel<DT, 16, 0>), grid, dim3(kThreads), 0, st, r);

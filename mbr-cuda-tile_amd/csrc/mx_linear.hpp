@@ -269,7 +269,8 @@ __device__ __forceinline__ void tile_finish_mx(const MxLinArgs& a, int64_t m0, i
 
 // Other results: 16 rows at a time through the wave's own part of LDS (stage: 1 KB per block of 16 columns), from where a
 // row's columns go out side by side, whole 128-byte lines at once.  Units of four columns are dealt to even and odd
-// halves of an LDS row, and then by its key, so that neither side of the exchange meets a bank twice.
+// halves of an LDS row, and then by its key, which parts neighbouring units; rows eight apart on the way in, and two neighbours on the
+// way out, still share their banks (1.15e6 of 7.4e6 LDS cycles of [48060, 384] -> 1536 are conflicts).
 template <int MI, int NI, int KIND, int NT>
 __device__ __forceinline__ void tile_finish(const MxLinArgs& a, int64_t m0, int n0, int lane, char* stage, f32x4 (&acc)[MI][NI]) {
     constexpr int RB = NI * 64;  // bytes of a staged row
@@ -307,7 +308,7 @@ __device__ __forceinline__ void tile_finish(const MxLinArgs& a, int64_t m0, int 
     }
 }
 
-// x in 4 bits: K in steps of SB bytes (2 or 4 blocks of each row for one matrix instruction, or two) through two LDS buffers filled
+// x in 4 bits: K in steps of SB bytes (4 or 8 blocks of each row, for one matrix instruction or two) through two LDS buffers filled
 // straight from global memory.  Scales come 16 blocks at a time, 16 bytes per row, through registers, and are written to LDS by
 // the thread that has the row, in front of the barrier that the step has anyway: of rows that lie 128 bytes apart every load
 // fetches a line, and 4 or 8 bytes of it at a time cost as much as the codes ([4096, 4096] -> 4096 64 us).
@@ -827,7 +828,7 @@ __global__ __launch_bounds__(1024) void mx_strip_kernel(MxLinArgs a) {
 // At most 16 rows of x: what takes time is reading w.  A wave takes 32 columns, dealt so that a lane ends with 8 in a row;
 // `split` waves share the K of one such strip, 16 blocks at a time in turn, the scales of a row's 16 in one load.  x stands in
 // LDS, as bf16 parts or as its codes, zeros up to whole turns, so that w alone waits for memory: 8 KB a wave, and the next
-// turn's as many while one is computed.  Past the caches w comes no faster ([1, 4096] bf16 -> 16384: 10.6 us either way).
+// turn's as many while one is computed.  Every workgroup has an x of its own, so that a large one leaves a CU room for fewer waves.  Past the caches w comes no faster ([1, 4096] bf16 -> 16384: 10.6 us either way).
 template <int XT>
 struct TokenX {  // bytes of a row of x in LDS, for a number of blocks
     static constexpr int kBlock = XT == MXFP4 ? 16 : 64;  // a block's codes, or one part of its values
@@ -1007,8 +1008,9 @@ int launch_mx_shapes(MxLinArgs& a, int align, hipStream_t st) {
     // A few rows of x and a strip of 32 columns or more for every CU: x through LDS.  us of this and of strips, 16 waves a CU (8: up to
     // 1.6 more), K -> N: bf16 [1, 4096] -> 16384 10.6 and 13.9, [1, 1536] -> 8192 5.1 and 4.9, [4, 1536] -> 8192 6.3 and 5.3, [4, 4096]
     // -> 16384 12.6 and 16.3; f32 [1, 1536] -> 8192 6.2 and 8.2, [4, 1024] -> 32768 10.5 and 15.9, [8, 1024] -> 32768 19.3 and 16.4;
-    // 4 bits [1, 1536] -> 8192 4.4 and 4.9, [16, 4096] -> 16384 10.6 and 17.3.  With half as many strips as CUs it loses: bf16 and 4
-    // bits [1, 4096] -> 4096 7.2 and 6.2, 6.0 and 5.7.
+    // 4 bits [1, 1536] -> 8192 4.4 and 4.9, [16, 4096] -> 16384 10.6 and 17.3.  Where strips are many, a workgroup is one wave, and LDS has
+    // room for only four with an x of 33 KB: bf16 [2, 8192] -> 131072 180 and 189, [4, 4096] -> 131072 113 and 108, 4 bits [16, 4096] ->
+    // 131072 99 and 118.  With half as many strips as CUs it loses: bf16 and 4 bits [1, 4096] -> 4096 7.2 and 6.2, 6.0 and 5.7.
     const int64_t strips32 = ceil_div(N, 32), turns16 = ceil_div(a.nb, 16), x_row = TokenX<XT>::row(16 * turns16);
     if (M <= (XT == MXFP4 ? 16 : 4) && strips32 >= cus * (XT == BF16 ? std::min<int64_t>(M, 2) : 1) && M * x_row <= (int64_t(1) << 16)) {
         const int64_t room = std::max<int64_t>(1, std::min<int64_t>(16, 16 * cus / strips32));
