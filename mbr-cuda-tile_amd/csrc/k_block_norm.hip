@@ -430,9 +430,9 @@ bool launch_shape(const BlockNormArgs& a, hipStream_t st) {
     typedef std::integral_constant<int, 64> G64;
     typedef std::integral_constant<int, 256> G256;
     const int n = a.odt == MXFP4 ? a.padded : a.chunks;
-    // A block per row from 129 chunks on, whose loads are spread over more lanes: us, a wave and a block per row, [1800, 1536] bf16
-    // 9.5 and 7.6, [100, 1024] f32 3.7 and 2.7, [12, 2000] bf16 5.8 and 3.0, [12000, 1536] 36.7 and 34.5; but of many short rows
-    // half a block's lanes would have nothing: [18786, 526] f32 29 and 37, [24000, 768] 44.7 and 46.8.
+    // A block per row from 129 chunks on, whose loads are spread over more lanes: us, a wave and a block per row, bf16 [12, 1500] 5.6
+    // and 4.6, [1800, 1536] 8.7 and 8.5, [3000, 1536] 11.8 and 11.3.  But of many rows of up to 192 half a block's lanes would have
+    // next to nothing: bf16 [5000, 1536] 15.5 and 15.7, [12000, 1536] 29 and 36; f32 [6000, 768] 12.0 and 14.0, [18786, 526] 27.6 and 37.
     if (n <= 32) go(G16(), std::integral_constant<int, 2>());
     else if (n <= 64) go(G16(), std::integral_constant<int, 4>());
     else if (n <= 96) go(G16(), std::integral_constant<int, 6>());
