@@ -13,8 +13,8 @@
 // rows takes one round of them.
 // Both results are formed in the formula's order, one f32 rounding per operation and quotients by the roots, so that they differ from
 // the formula in f32 calls by the order of the two sums alone, and 4-bit values behind them seldom do.  An h of 2 bytes that lies on
-// a tie of its rounding can still fall to the other side, and normed follows it as it is stored: of [48060, 384] 154 elements in bf16
-// and 949 in f16, where the formula in f32 itself differs from 64 bits in 709 and 3193.  Quotients cost 0.3 us of 13.4 (f16
+// a tie of its rounding can still fall to the other side, and normed follows it as it is stored: of [48060, 384] 146 elements in bf16
+// and 754 in f16, where the formula in f32 itself differs from 64 bits in 709 and 3193.  Quotients cost 0.3 us of 13.2 (f16
 // [4, 4003, 512]) against products with the reciprocal root.
 // A row whose last chunk is cut has it moved back to end at the row's end: its first elements are the chunk's before, left
 // out of the sums and stored twice with the same values, so that odd widths take the same loads as even ones.
@@ -168,6 +168,16 @@ __device__ __forceinline__ void features(const void* p, int dt, int d, float (&f
     }
 }
 
+// The sum of a chunk's squares from its element `first` on (AL: of all, or with first VE of none).  Lanes add chunk by chunk: shorter chains
+// of roundings than element by element, and half the operations where nothing is left out inside a chunk.
+template <bool AL, int VE>
+__device__ __forceinline__ float chunk_squares(const float (&v)[VE], int first) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) t = AL || i >= first ? fmaf(v[i], v[i], t) : t;
+    return AL && first != 0 ? 0.0f : t;
+}
+
 // The sum over a group's lanes, in each of them.  turn: another place in LDS for each sum of a row.
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float* turn) {
@@ -248,8 +258,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
             float u[VE];
             uv[k].to_f32(a.udt, u);
             const int first = AL ? (lane + G * k < a.chunks ? 0 : VE) : (lane + G * k) * VE - at[k];  // before it: another chunk's
-#pragma unroll
-            for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(u[i], u[i], ss) : ss;
+            ss += chunk_squares<AL>(u, first);
         }
         root = root_of(row_sum<G>(ss, lds) + a.eps);
     }
@@ -296,8 +305,7 @@ __global__ __launch_bounds__(kThreads) void block_norm_kernel(BlockNormArgs a) {
         t.from_f32(a.rdt, h[k]);
         t.to_f32(a.rdt, h[k]);
         if (G <= 64 && a.sum != nullptr && valid && lane + G * k < a.chunks) t.template store<AL>(a.sum + r * a.ss + (int64_t)at[k] * RS);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) ss = i >= first ? fmaf(h[k][i], h[k][i], ss) : ss;
+        ss += chunk_squares<AL>(h[k], first);
     }
     root = root_of(row_sum<G>(ss, lds + 4) + a.eps);
     if (G > 64 && a.sum != nullptr) {  // not before every wave has its part of a row that it may replace, a cut chunk's first elements too
