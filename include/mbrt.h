@@ -505,13 +505,14 @@ MBRT_API int mbrt_mx_dequantize(const void* codes, int64_t codes_row_stride, con
  * unused), bias and residual F32/F16/BF16 or NULL, out F32/F16/BF16 or MXFP4 (with out_scales; quantised from the f32
  * results as by mbrt_mx_quantize).  Strides of codes in bytes, of other rows in elements; x, weight and residual may have
  * any from 0 on.  Products are exact: 4-bit by 4-bit ones, and those of F32/F16/BF16 x, which is taken as a sum of bf16 values
- * (what lies below 2^-133 of an F32 x is lost) and meets the weights in bf16: one of 2^128 or more, which scale bytes 253 and 254 can
- * express and mbrt_mx_quantize writes for no finite f32, leaves its out feature infinite or NaN there; x in MXFP4 takes it as it is.  Sums and the epilogue are f32, with one rounding on the store; activations
- * as mbrt_linear's, in their short forms unless x or out is F32; GELU in front of results in 4 bits, whose scale follows a block's
- * largest value however small, in full f32: x Phi(s x) is off by 2^-23 (0.75 (s x)^2 + 16) of itself at most in the negative tail (s: sqrt 2
- * in the reference's form, else 1), and may be 0 where Phi is below 2^-126.  out may be residual (same dtype, same rows); it shares no other
- * byte with an operand.  in_features 0 leaves act(bias) + residual.  No workspace, no atomics.  Beside mbrt_linear, for layers
- * whose weights, and where wanted activations, are held in 4 bits. */
+ * (what lies below 2^-133 of an F32 x is lost) and meets the weights in bf16: one of 2^128 or more, which scale bytes 253 and
+ * 254 can express and mbrt_mx_quantize writes for no finite f32, leaves its out feature infinite or NaN there; x in MXFP4
+ * takes it as it is.  Sums and the epilogue are f32, with one rounding on the store; activations as mbrt_linear's, in their
+ * short forms unless x or out is F32; GELU in front of results in 4 bits, whose scale follows a block's largest value however
+ * small, in full f32: x Phi(s x) is off by 2^-23 (0.75 (s x)^2 + 16) of itself at most in the negative tail (s: sqrt 2 in the
+ * reference's form, else 1), and may be 0 where Phi is below 2^-126.  out may be residual (same dtype, same rows); it shares
+ * no other byte with an operand.  in_features 0 leaves act(bias) + residual.  No workspace, no atomics.  Beside mbrt_linear,
+ * for layers whose weights, and where wanted activations, are held in 4 bits. */
 MBRT_API int mbrt_mx_linear(const void* x, int dtype, int64_t x_row_stride, const void* x_scales,
                             int64_t x_scales_row_stride, const void* weight, int64_t weight_row_stride,
                             const void* weight_scales, int64_t weight_scales_row_stride, const void* bias,
@@ -530,9 +531,10 @@ MBRT_API int mbrt_mx_linear(const void* x, int dtype, int64_t x_row_stride, cons
  * one per row, per batch entry, per position, or one for all; gate_is_logit puts it through a sigmoid.  sum_out takes h
  * in residual's type (NULL: not stored; it may be residual itself); normed F32/F16/BF16 or MXFP4 with normed_scales
  * (quantised from the f32 results), none with gamma NULL.  normed may be update itself (same dtype and rows).  Outputs share
- * no other byte with an operand.  Row strides in elements (codes and scales: bytes).  f32 throughout, in the formula's order, one
- * rounding of each output: what differs from the formula in f32 is the order of the sums, a step of f32 or so, and so now and then the
- * side to which a 2-byte h on a tie of its rounding falls, which normed follows.  Beside mbrt_residual_add_rms_norm, for models that norm a block's output, gate it or scale it. */
+ * no other byte with an operand.  Row strides in elements (codes and scales: bytes).  f32 throughout, in the formula's order,
+ * one rounding of each output: what differs from the formula in f32 is the order of the sums, a step of f32 or so, and so now
+ * and then the side to which a 2-byte h on a tie of its rounding falls, which normed follows.  Beside
+ * mbrt_residual_add_rms_norm, for models that norm a block's output, gate it or scale it. */
 MBRT_API int mbrt_block_norm(const void* residual, int residual_dtype, int64_t residual_row_stride, const void* update,
                              int update_dtype, int64_t update_row_stride, const void* post_gamma, int post_gamma_dtype,
                              const void* gate, int gate_dtype, int64_t gate_cols, int64_t gate_row_stride,

@@ -505,8 +505,7 @@ def mx_linear(x, weight: MxTensor, bias: torch.Tensor | None = None, out=None, a
     """act(x weight^T + bias) + residual for weight [N, K] in 4 bits and x [.., K] in 4 bits (MxTensor) or f32, f16 or bf16,
     rounded once.  bias [N], residual and out [.., N], each f32, f16 or bf16; out may be an MxTensor, too, or residual itself.
     out_dtype defaults to x's, bf16 for x in 4 bits; MxTensor gives results in 4 bits.  Weights of 2^128 and more (scale bytes 253 and 254)
-    count as infinities unless x is in 4 bits.  Rows at any stride (codes:
-    multiples of 16 bytes), the last dim contiguous."""
+    count as infinities unless x is in 4 bits.  Rows at any stride (codes: multiples of 16 bytes), the last dim contiguous."""
     held = isinstance(x, MxTensor)
     if not isinstance(weight, MxTensor) or not (held or isinstance(x, torch.Tensor)):
         raise TypeError("mx_linear: expected weight an MxTensor, x a torch.Tensor or an MxTensor")
